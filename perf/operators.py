@@ -9,10 +9,10 @@
 With ``own`` false ``run`` computes the same from elementary torch operations.
 
 The 8-bit moments: blocks of 32 consecutive elements of a tensor share a power of two, 2^(X - 127), the binade of the
-largest magnitude after it is rounded up to the code's mantissa.  A code is a float of 4 exponent and M mantissa bits
-below that binade, without subnormals (M = 3 and a sign for the first moment, M = 4 for the square root of the second).
-Roundings to fewer bits are stochastic with 16 random bits a value; the bits come from an integer mix of the seed, the
-step and the element's position, where every tensor starts at a multiple of 32.
+largest magnitude after it is rounded up to three mantissa bits.  A code is a float with three mantissa bits in the
+binades down from there, without subnormals: a sign and 16 binades for the first moment, 32 for the second.  Roundings to
+fewer bits are stochastic with 16 random bits a value; the bits come from an integer mix of the seed, the step and the
+element's position, where every tensor starts at a multiple of 32.
 """
 from __future__ import annotations
 
@@ -214,8 +214,7 @@ def prepare(case, seed):
         v.mul_(size[k] * size[k])
     if case["bits"] == 8:
         half = torch.full((total,), 0x8000, dtype=torch.int64, device="cuda")
-        first = _coded(first, half, 3)
-        second = _coded(second.sqrt(), half, 4).square()
+        first, second = _coded(first, half, True), _coded(second, half, False)
     state.update(first_flat=first, second_flat=second, step=1000, seed=seed)
     state["factor"] = torch.full((), 0.37, device="cuda") if case["factor"] else None
     state["params"] = _views(state["param_flat"], shapes)
@@ -310,18 +309,13 @@ def _plain_adamw(state, case):
     if state["factor"] is not None:
         g = g * state["factor"]
     m = state["first_flat"] * beta1 + g * (1.0 - beta1)
-    old = state["second_flat"]
-    if case["bits"] == 8:
-        old = old.sqrt().square()    # the square root is what is held
-    v = old * beta2 + (g * g) * (1.0 - beta2)
-    r = v.sqrt()
-    denominator = r * (1.0 / math.sqrt(1.0 - beta2 ** t)) + EPS
+    v = state["second_flat"] * beta2 + (g * g) * (1.0 - beta2)
+    denominator = v.sqrt() * (1.0 / math.sqrt(1.0 - beta2 ** t)) + EPS
     p = p * (1.0 - LR * DECAY) - (m / denominator) * (LR / (1.0 - beta1 ** t))
     if case["bits"] == 8 or case["dtype"] == "bfloat16":
         bits = _random_bits(state["seed"], t, p.numel())
     if case["bits"] == 8:
-        m = _coded(m, bits & 0xFFFF, 3)
-        v = _coded(r, bits >> 16, 4).square()
+        m, v = _coded(m, bits & 0xFFFF, True), _coded(v, bits >> 16, False)
     if case["dtype"] == "bfloat16":
         word = p.view(torch.int32) + (_mix(bits + 0x9E3779B1) & 0xFFFF).int()
         p = (word & -65536).view(torch.float32).bfloat16()
@@ -349,21 +343,21 @@ def _random_bits(seed, t, count):
     return _mix(torch.arange(count, device="cuda") ^ key)
 
 
-def _coded(x, random16, mantissa):
+def _coded(x, random16, signed):
     """The values that the 8-bit codes of `x` stand for."""
     word = x.abs().view(torch.int32).long()
-    drop = 23 - mantissa
-    top = ((word + ((1 << drop) - 1)) >> 23).view(-1, 32).amax(1).clamp(min=16)
-    low = ((top - 15) << mantissa).repeat_interleave(32)
-    code = ((word + (random16 << (drop - 16))) >> drop) - low
-    least = ((low + 1) << drop).int().view(torch.float32)
-    if mantissa == 4:    # a square root that is not 0 never becomes 0
-        under = (word > 0).long()
-    else:
+    binades = 16 if signed else 32
+    top = ((word + 0xFFFFF) >> 23).view(-1, 32).amax(1).clamp(min=binades)
+    low = ((top - (binades - 1)) << 3).repeat_interleave(32)
+    code = ((word + (random16 << 4)) >> 20) - low
+    if signed:    # below the least code: up to it as often as the value's share of it
+        least = ((low + 1) << 20).int().view(torch.float32)
         under = (x.abs() > least * (random16.float() * 2.0 ** -16)).long()
+    else:         # a second moment that is not 0 never becomes 0
+        under = (word > 0).long()
     code = torch.where(code < 1, under, code)
-    value = torch.where(code > 0, ((code + low) << drop).int().view(torch.float32), torch.zeros_like(x))
-    return torch.copysign(value, x) if mantissa == 3 else value
+    value = torch.where(code > 0, ((code + low) << 20).int().view(torch.float32), torch.zeros_like(x))
+    return torch.copysign(value, x) if signed else value
 
 
 def _run_grad_norm(state):
