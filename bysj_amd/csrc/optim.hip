@@ -1,0 +1,711 @@
+// The optimiser step over all tensors of a model (no counterpart in the reference, which has no training):
+//
+//   grad_norm   norm = sqrt(sum g^2) over every gradient, factor = min(1, max_norm / (norm + 1e-6))
+//   adamw_step  g' = g * factor
+//               m = m * b1 + g' * (1 - b1),   v = v * b2 + (g' * g') * (1 - b2)
+//               p = p * (1 - lr wd) - (m / (sqrt(v) * (1 / sqrt(1 - b2^t)) + eps)) * (lr / (1 - b1^t))
+//
+// A model of this kind is hundreds of tensors, most of them small, so the work
+// is cut into chunks of kChunk elements over all tensors, one workgroup each:
+// two launches a step whatever the number of tensors.  A plan (built once on
+// the host) lists the tensors and the chunks; the gradients, which move from
+// step to step, are passed by value to the first launch, which writes them and
+// the step's scalars (bias corrections in 64 bits) into the plan.  Both kernels
+// are bound by their streams: 28 bytes per float32 element with moments in 32
+// bits, 16 with moments in 8 bits.
+//
+// Every product and sum of the update is rounded to float32 as written above
+// (square root and division are the correctly rounded ones), so a step equals
+// the same chain of elementwise operations bit for bit.
+//
+// Moments in 8 bits: 32 consecutive elements share a power of two, 2^(X - 127),
+// kept as the byte X.  X is the largest exponent after the magnitude is rounded
+// up to three mantissa bits, so no value of the block overflows and scaling is
+// exact.  A code is a float with three mantissa bits in the B binades down from
+// there: code c > 0 stands for the float32 with the bits (c + ((X - B + 1) << 3)) << 20,
+// with B = 16 and a sign bit for the first moment and B = 32 for the second.
+// Since the scale is a power of two, a block's grid stays the same when its
+// largest value changes, and an average that stands on it moves only by what
+// the step adds.  A nonzero second moment never becomes 0: the next step would
+// divide a first moment by eps.
+//
+// Roundings to codes, and to bfloat16 parameters, are stochastic (16 random
+// bits): b2 = 0.999 moves v by a thousandth a step, far below half a step of
+// any 8-bit code, and a nearest rounding would freeze the average (a bfloat16
+// weight likewise).  The mean of the rounded average then follows the exact
+// one.  The bits come from an integer mix of (seed, step, position in the plan).
+#include <cmath>
+#include <cstring>
+
+#include "common.h"
+
+namespace dpa4k {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kChunk = 4096;           // elements of a workgroup: 4 vectors of 4 per thread
+constexpr int kVectors = kChunk / (kBlock * 4);
+constexpr int kSpan = 32;              // elements that share a scale
+constexpr int kPointers = 440;         // gradients passed by value: kernel arguments below 4 KB
+
+// One tensor of a plan.  The first eight fields are set when the plan is built.
+struct alignas(128) Record {
+  void* param;
+  void* exp_avg;
+  void* exp_avg_sq;
+  uint8_t* exp_avg_scale;
+  uint8_t* exp_avg_sq_scale;
+  int64_t count;
+  uint64_t position;      // of its first element, every tensor padded to kSpan
+  int64_t step;           // steps taken
+  const void* grad;       // of this step; null where the tensor takes none
+  float factor, decay, step_size, inverse_root;
+  uint64_t reserved;
+  float* values[2];       // float32 moments to read or write
+};
+static_assert(sizeof(Record) == 128, "records are 128 bytes");
+static_assert(offsetof(Record, step) == DPA4K_ADAMW_STEP_OFFSET, "the header's offset of the step count");
+
+struct Chunk {
+  int32_t tensor, index;
+};
+
+struct PointerList {
+  const void* p[kPointers];
+};
+
+__host__ __device__ inline uint32_t mix(uint32_t x) {
+  // the constants are odd words of the fractions of sqrt(2) and sqrt(3)
+  x = (x ^ (x >> 16)) * 0x6A09E667u;
+  x = (x ^ (x >> 15)) * 0xBB67AE85u;
+  return x ^ (x >> 16);
+}
+
+// ---------------------------------------------------------------------------
+// four elements
+// ---------------------------------------------------------------------------
+
+// Vectors of any element alignment: one access each.
+template <typename T>
+struct vec4_of {
+  typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(uint16_t bf16) { return __uint_as_float(static_cast<uint32_t>(bf16) << 16); }
+
+// Elements [at, at + 4) of a stream of `count` as float32, zeros past its end.
+template <bool kWhole, typename T>
+__device__ __forceinline__ fvec<4> load4(const T* __restrict__ p, int64_t at, int64_t count) {
+  fvec<4> out;
+  if (kWhole) {
+    const auto raw = *reinterpret_cast<const typename vec4_of<T>::type*>(p + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out.v[i] = to_float(raw[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out.v[i] = at + i < count ? to_float(p[at + i]) : 0.0f;
+  }
+  return out;
+}
+
+template <bool kWhole, typename T>
+__device__ __forceinline__ void store4(T* __restrict__ p, int64_t at, int64_t count, const T (&value)[4]) {
+  if (kWhole) {
+    typename vec4_of<T>::type raw;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = value[i];
+    *reinterpret_cast<typename vec4_of<T>::type*>(p + at) = raw;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + i < count) p[at + i] = value[i];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// codes of 8 bits
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t group8_max(uint32_t value) {
+  int x = static_cast<int>(value);
+  int y = xor_lane<1>(x);
+  x = x > y ? x : y;
+  y = xor_lane<2>(x);
+  x = x > y ? x : y;
+  y = xor_lane<4>(x);
+  return static_cast<uint32_t>(x > y ? x : y);
+}
+
+// A signed code has a sign bit and 16 binades, an unsigned one 32.
+template <bool kSigned>
+constexpr uint32_t kBinades = kSigned ? 16u : 32u;
+
+template <bool kSigned>
+__device__ __forceinline__ float decode(uint32_t code, uint32_t top) {
+  const uint32_t c = kSigned ? code & 0x7Fu : code;
+  uint32_t word = c == 0 ? 0u : (c + ((top - kBinades<kSigned> + 1u) << 3)) << 20;
+  if (kSigned) word |= (code & 0x80u) << 24;
+  return top == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(word);
+}
+
+// The shared exponent of the 32 values held by 8 consecutive lanes, and this
+// lane's four codes.  A block with an infinity or NaN takes X = 255 and stands
+// for NaN.  `random16`: 16 bits a value, compared with the 20 bits cut off.
+template <bool kSigned>
+__device__ __forceinline__ uint32_t encode4(const float (&value)[4], const uint32_t (&random16)[4], uint32_t& top) {
+  uint32_t word[4], most = kBinades<kSigned>;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    word[i] = __float_as_uint(value[i]) & 0x7FFFFFFFu;
+    const uint32_t exponent = (word[i] + 0xFFFFFu) >> 23;
+    most = exponent > most ? exponent : most;
+  }
+  most = group8_max(most);
+  top = most < 255u ? most : 255u;
+  const uint32_t low = (top - kBinades<kSigned> + 1u) << 3;
+  const float least = __uint_as_float((low + 1u) << 20);
+  uint32_t packed = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    int code = static_cast<int>((word[i] + (random16[i] << 4)) >> 20) - static_cast<int>(low);
+    if (kSigned) {
+      // below the least code: up to it as often as the value's share of it
+      const float share = least * (static_cast<float>(random16[i]) * 1.52587890625e-5f);
+      if (code < 1) code = __uint_as_float(word[i]) > share ? 1 : 0;
+      code = (code & 0x7F) | static_cast<int>((__float_as_uint(value[i]) >> 24) & 0x80u);
+    } else if (code < 1) {
+      code = word[i] != 0u ? 1 : 0;
+    }
+    packed |= (static_cast<uint32_t>(code) & 0xFFu) << (8 * i);
+  }
+  return packed;
+}
+
+// ---------------------------------------------------------------------------
+// AdamW
+// ---------------------------------------------------------------------------
+
+struct StepScalars {
+  double lr, beta1, beta2, weight_decay;
+  const float* lr_device;
+  const float* factor;
+};
+
+// One thread per tensor: its gradient's address and this step's scalars.  A
+// factor that is NaN (the norm was not finite) takes no step anywhere.
+__global__ __launch_bounds__(kBlock) void adamw_begin_kernel(PointerList grads, Record* __restrict__ records,
+                                                             int first, int count, StepScalars s) {
+  const int i = blockIdx.x * kBlock + threadIdx.x;
+  if (i >= count) return;
+  Record& r = records[first + i];
+  const float factor = s.factor != nullptr ? *s.factor : 1.0f;
+  const void* grad = factor == factor ? grads.p[i] : nullptr;
+  r.grad = grad;
+  if (grad == nullptr) return;
+  const int64_t t = r.step + 1;
+  r.step = t;
+  const double lr = s.lr_device != nullptr ? static_cast<double>(*s.lr_device) : s.lr;
+  r.factor = factor;
+  r.decay = static_cast<float>(1.0 - lr * s.weight_decay);
+  r.step_size = static_cast<float>(lr / (1.0 - pow(s.beta1, static_cast<double>(t))));
+  r.inverse_root = static_cast<float>(1.0 / sqrt(1.0 - pow(s.beta2, static_cast<double>(t))));
+}
+
+struct UpdateScalars {
+  float beta1, rest1, beta2, rest2, eps;  // rest = 1 - beta
+  uint32_t seed_low, seed_high;
+};
+
+// The random bits of step t at positions whose upper 32 bits are `high`.
+__device__ __forceinline__ uint32_t random_key(const UpdateScalars& s, int64_t t, uint32_t high) {
+  return mix(s.seed_low ^ mix(s.seed_high + mix(static_cast<uint32_t>(t) + high * 0x9E3779B1u)));
+}
+
+template <typename P, typename G, int kBits, bool kWhole>
+__device__ __forceinline__ void adamw_update_chunk(const Record& r, int64_t begin, const UpdateScalars& s) {
+  constexpr bool kRandom = kBits == 8 || sizeof(P) == 2;
+  P* const param = static_cast<P*>(r.param);
+  const G* const grad = static_cast<const G*>(r.grad);
+  const int64_t count = r.count;
+  const int64_t padded = (count + kSpan - 1) / kSpan * kSpan;
+  const float factor = r.factor, decay = r.decay, step_size = r.step_size, inverse_root = r.inverse_root;
+  fvec<4> p[kVectors], g[kVectors], m[kVectors], v[kVectors];
+  uint32_t m_code[kVectors], v_code[kVectors], m_top[kVectors], v_top[kVectors];
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k) {
+    const int64_t at = begin + (k * kBlock + static_cast<int>(threadIdx.x)) * 4;
+    p[k] = load4<kWhole>(param, at, count);
+    g[k] = load4<kWhole>(grad, at, count);
+    if constexpr (kBits == 32) {
+      m[k] = load4<kWhole>(static_cast<const float*>(r.exp_avg), at, count);
+      v[k] = load4<kWhole>(static_cast<const float*>(r.exp_avg_sq), at, count);
+    } else {
+      const bool live = kWhole || at < padded;
+      m_code[k] = live ? static_cast<const uint32_t*>(r.exp_avg)[at / 4] : 0u;
+      v_code[k] = live ? static_cast<const uint32_t*>(r.exp_avg_sq)[at / 4] : 0u;
+      m_top[k] = live ? r.exp_avg_scale[at / kSpan] : kBinades<true>;
+      v_top[k] = live ? r.exp_avg_sq_scale[at / kSpan] : kBinades<false>;
+    }
+  }
+  const uint32_t high = static_cast<uint32_t>((r.position + begin) >> 32);
+  const uint32_t key = kRandom ? random_key(s, r.step, high) : 0u;
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k) {
+    const int64_t at = begin + (k * kBlock + static_cast<int>(threadIdx.x)) * 4;
+    float new_p[4], new_m[4], new_v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float old_m, old_v;
+      if constexpr (kBits == 32) {
+        old_m = m[k].v[i];
+        old_v = v[k].v[i];
+      } else {
+        old_m = decode<true>(m_code[k] >> (8 * i) & 0xFFu, m_top[k]);
+        old_v = decode<false>(v_code[k] >> (8 * i) & 0xFFu, v_top[k]);
+      }
+      const float scaled = g[k].v[i] * factor;
+      new_m[i] = old_m * s.beta1 + scaled * s.rest1;
+      new_v[i] = old_v * s.beta2 + (scaled * scaled) * s.rest2;
+      new_p[i] = p[k].v[i] * decay - (new_m[i] / (sqrtf(new_v[i]) * inverse_root + s.eps)) * step_size;
+    }
+    uint32_t bits[4];
+    if constexpr (kRandom) {
+      const uint64_t position = r.position + at;
+      const uint32_t own_high = static_cast<uint32_t>(position >> 32);
+      const uint32_t own_key = own_high == high ? key : random_key(s, r.step, own_high);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bits[i] = mix((static_cast<uint32_t>(position) + i) ^ own_key);
+    }
+    if constexpr (sizeof(P) == 2) {
+      P rounded[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t word = __float_as_uint(new_p[i]);
+        const uint32_t noise = mix(bits[i] + 0x9E3779B1u) & 0xFFFFu;
+        // infinities stay, NaN stays NaN (quiet)
+        const bool finite = (word & 0x7F800000u) != 0x7F800000u;
+        const uint32_t special = (word & 0x007FFFFFu) != 0u ? word | 0x00400000u : word;
+        rounded[i] = static_cast<P>((finite ? word + noise : special) >> 16);
+      }
+      store4<kWhole>(param, at, count, rounded);
+    } else {
+      store4<kWhole>(param, at, count, new_p);
+    }
+    if constexpr (kBits == 32) {
+      store4<kWhole>(static_cast<float*>(r.exp_avg), at, count, new_m);
+      store4<kWhole>(static_cast<float*>(r.exp_avg_sq), at, count, new_v);
+    } else {
+      uint32_t low[4], upper[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        low[i] = bits[i] & 0xFFFFu;
+        upper[i] = bits[i] >> 16;
+        if (!kWhole && at + i >= count) new_m[i] = new_v[i] = 0.0f;  // padding stays 0
+      }
+      uint32_t top_m, top_v;
+      const uint32_t packed_m = encode4<true>(new_m, low, top_m);
+      const uint32_t packed_v = encode4<false>(new_v, upper, top_v);
+      if (kWhole || at < padded) {
+        static_cast<uint32_t*>(r.exp_avg)[at / 4] = packed_m;
+        static_cast<uint32_t*>(r.exp_avg_sq)[at / 4] = packed_v;
+        if ((threadIdx.x & 7) == 0) {
+          r.exp_avg_scale[at / kSpan] = static_cast<uint8_t>(top_m);
+          r.exp_avg_sq_scale[at / kSpan] = static_cast<uint8_t>(top_v);
+        }
+      }
+    }
+  }
+}
+
+template <typename P, typename G, int kBits>
+__global__ __launch_bounds__(kBlock) void adamw_update_kernel(const Record* __restrict__ records,
+                                                              const Chunk* __restrict__ chunks, int64_t n_chunks,
+                                                              UpdateScalars s) {
+  const int64_t block = block_index();
+  if (block >= n_chunks) return;
+  const Chunk chunk = chunks[block];
+  const Record& r = records[chunk.tensor];
+  if (r.grad == nullptr) return;
+  const int64_t begin = static_cast<int64_t>(chunk.index) * kChunk;
+  if (r.count - begin >= kChunk) adamw_update_chunk<P, G, kBits, true>(r, begin, s);
+  else adamw_update_chunk<P, G, kBits, false>(r, begin, s);
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit moments as float32 values, and back
+// ---------------------------------------------------------------------------
+
+__global__ __launch_bounds__(kBlock) void adamw_values_kernel(PointerList list, Record* __restrict__ records,
+                                                              int first, int count, int which) {
+  const int i = blockIdx.x * kBlock + threadIdx.x;
+  if (i < count) records[first + i].values[which] = static_cast<float*>(const_cast<void*>(list.p[i]));
+}
+
+// kRead: codes to values.  Otherwise values to the nearest codes.
+template <bool kRead>
+__global__ __launch_bounds__(kBlock) void adamw_codes_kernel(const Record* __restrict__ records,
+                                                             const Chunk* __restrict__ chunks, int64_t n_chunks) {
+  const int64_t block = block_index();
+  if (block >= n_chunks) return;
+  const Chunk chunk = chunks[block];
+  const Record& r = records[chunk.tensor];
+  float* const m_values = r.values[0];
+  float* const v_values = r.values[1];
+  const int64_t count = r.count;
+  const int64_t padded = (count + kSpan - 1) / kSpan * kSpan;
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k) {
+    const int64_t at = static_cast<int64_t>(chunk.index) * kChunk + (k * kBlock + static_cast<int>(threadIdx.x)) * 4;
+    const bool live = at < padded;
+    const bool whole = at + 4 <= count;
+    if constexpr (kRead) {
+      if (!live) continue;
+      const uint32_t m_code = static_cast<const uint32_t*>(r.exp_avg)[at / 4];
+      const uint32_t v_code = static_cast<const uint32_t*>(r.exp_avg_sq)[at / 4];
+      const uint32_t m_top = r.exp_avg_scale[at / kSpan], v_top = r.exp_avg_sq_scale[at / kSpan];
+      float m[4], v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m[i] = decode<true>(m_code >> (8 * i) & 0xFFu, m_top);
+        v[i] = decode<false>(v_code >> (8 * i) & 0xFFu, v_top);
+      }
+      if (whole) {
+        store4<true>(m_values, at, count, m);
+        store4<true>(v_values, at, count, v);
+      } else {
+        store4<false>(m_values, at, count, m);
+        store4<false>(v_values, at, count, v);
+      }
+    } else {
+      // every lane takes part in the exponents of its 8 lanes
+      const fvec<4> m = whole ? load4<true>(m_values, at, count) : load4<false>(m_values, at, count);
+      const fvec<4> v = whole ? load4<true>(v_values, at, count) : load4<false>(v_values, at, count);
+      const uint32_t half[4] = {0x8000u, 0x8000u, 0x8000u, 0x8000u};
+      uint32_t top_m, top_v;
+      const uint32_t packed_m = encode4<true>(m.v, half, top_m);
+      const uint32_t packed_v = encode4<false>(v.v, half, top_v);
+      if (live) {
+        static_cast<uint32_t*>(r.exp_avg)[at / 4] = packed_m;
+        static_cast<uint32_t*>(r.exp_avg_sq)[at / 4] = packed_v;
+        if ((threadIdx.x & 7) == 0) {
+          r.exp_avg_scale[at / kSpan] = static_cast<uint8_t>(top_m);
+          r.exp_avg_sq_scale[at / kSpan] = static_cast<uint8_t>(top_v);
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// gradient norm
+// ---------------------------------------------------------------------------
+//
+// Each launch takes up to kNormTensors gradients by value.  Its workgroups take
+// equal runs of chunks; a thread sums squares in 64 bits (the card's float64
+// rate hides behind the stream), a workgroup leaves one partial, and a last
+// small launch adds all partials in their order.
+
+constexpr int kNormTensors = 180;
+constexpr int kNormBlocks = 2048;      // workgroups of one launch
+constexpr int kNormChunk = 8192;       // elements
+
+struct NormList {
+  const void* p[kNormTensors];
+  int64_t count[kNormTensors];         // elements * 2, and 1 for bfloat16
+  uint32_t first[kNormTensors + 1];    // chunks before each tensor
+};
+
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const T* __restrict__ p, int64_t begin, int64_t count) {
+  double sum = 0.0;
+  if (count - begin >= kNormChunk) {
+#pragma unroll
+    for (int k = 0; k < kNormChunk / (kBlock * 4); ++k) {
+      const fvec<4> g = load4<true>(p, begin + (k * kBlock + static_cast<int>(threadIdx.x)) * 4, count);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = __builtin_fma(static_cast<double>(g.v[i]), static_cast<double>(g.v[i]), sum);
+    }
+  } else {
+    for (int64_t at = begin + threadIdx.x; at < count; at += kBlock) {
+      const double g = to_float(p[at]);
+      sum = __builtin_fma(g, g, sum);
+    }
+  }
+  return sum;
+}
+
+__device__ __forceinline__ double block_sum(double value) {
+  __shared__ double waves[kBlock / 64];
+  value = group_sum<64>(value);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = value;
+  __syncthreads();
+  double total = waves[0];
+#pragma unroll
+  for (int w = 1; w < kBlock / 64; ++w) total += waves[w];
+  return total;
+}
+
+__global__ __launch_bounds__(kBlock) void grad_norm_kernel(NormList list, int tensors, uint32_t chunks,
+                                                           double* __restrict__ partial) {
+  const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * blockIdx.x / gridDim.x);
+  const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (blockIdx.x + 1) / gridDim.x);
+  int low = 0, high = tensors - 1;  // the tensor of chunk `begin`: the last that starts at or before it
+  while (low < high) {
+    const int middle = (low + high + 1) >> 1;
+    if (list.first[middle] <= begin) low = middle;
+    else high = middle - 1;
+  }
+  double sum = 0.0;
+  for (uint32_t chunk = begin; chunk < end; ++chunk) {
+    while (chunk >= list.first[low + 1]) ++low;
+    const int64_t at = static_cast<int64_t>(chunk - list.first[low]) * kNormChunk;
+    const int64_t count = list.count[low] >> 1;
+    if (list.count[low] & 1) sum += chunk_squares(static_cast<const uint16_t*>(list.p[low]), at, count);
+    else sum += chunk_squares(static_cast<const float*>(list.p[low]), at, count);
+  }
+  const double total = block_sum(sum);
+  if (threadIdx.x == 0) partial[blockIdx.x] = total;
+}
+
+__global__ __launch_bounds__(kBlock) void grad_norm_total_kernel(const double* __restrict__ partial, int64_t count,
+                                                                 double max_norm, float* __restrict__ norm,
+                                                                 float* __restrict__ factor) {
+  double sum = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += kBlock) sum += partial[i];
+  const double total = sqrt(block_sum(sum));
+  if (threadIdx.x != 0) return;
+  const float rounded = static_cast<float>(total);
+  *norm = rounded;
+  const double wanted = max_norm > 0.0 ? max_norm / (total + 1.0e-6) : 1.0;
+  *factor = fabsf(rounded) < INFINITY ? static_cast<float>(wanted < 1.0 ? wanted : 1.0) : NAN;
+}
+
+int64_t norm_chunks(int64_t count) { return (count + kNormChunk - 1) / kNormChunk; }
+
+// Workgroups of the launch over tensors [first, last), or -1 where a size is out of range.
+int64_t norm_blocks(const int64_t* counts, int64_t first, int64_t last, uint32_t* starts) {
+  int64_t chunks = 0;
+  for (int64_t i = first; i < last; ++i) {
+    if (starts != nullptr) starts[i - first] = static_cast<uint32_t>(chunks);
+    if (counts[i] < 0 || counts[i] > (int64_t(1) << 44)) return -1;
+    chunks += norm_chunks(counts[i]);
+  }
+  if (starts != nullptr) starts[last - first] = static_cast<uint32_t>(chunks);
+  if (chunks > 0x7FFFFFFF) return -1;
+  return chunks < kNormBlocks ? chunks : kNormBlocks;
+}
+
+int64_t tensor_chunks(int64_t count) { return (count + kChunk - 1) / kChunk; }
+
+size_t chunk_offset(int64_t n_tensors) { return round_up_256(static_cast<size_t>(n_tensors) * sizeof(Record)); }
+
+// Chunks of a plan, or -1 where a size is out of range.
+int64_t plan_chunks(const int64_t* counts, int64_t n_tensors, int64_t stride) {
+  if (n_tensors < 0 || n_tensors > 0x7FFFFFFF || (n_tensors > 0 && counts == nullptr)) return -1;
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < n_tensors; ++i) {
+    const int64_t count = counts[i * stride];
+    if (count < 0 || tensor_chunks(count) > 0x7FFFFFFF) return -1;
+    chunks += tensor_chunks(count);
+  }
+  return chunks;
+}
+
+constexpr int64_t kStructStride = sizeof(dpa4k_adamw_tensor) / sizeof(int64_t);
+static_assert(sizeof(dpa4k_adamw_tensor) == 56, "seven 8-byte fields");
+
+int check_plan(const char* what, const void* plan, int64_t n_tensors, int64_t n_chunks) {
+  if (n_tensors < 0 || n_chunks < 0) return fail(DPA4K_EINVAL, "%s: negative sizes", what);
+  if (n_tensors > 0x7FFFFFFF || !grid_fits(n_chunks, kBlock)) return fail(DPA4K_EINVAL, "%s: plan exceeds the launch limit", what);
+  if (n_tensors > 0 && plan == nullptr) return fail(DPA4K_EINVAL, "%s: null pointer", what);
+  return DPA4K_OK;
+}
+
+template <typename Launch>
+void each_list(const void* const* pointers, int64_t n_tensors, Launch launch) {
+  for (int64_t first = 0; first < n_tensors; first += kPointers) {
+    const int count = static_cast<int>(n_tensors - first < kPointers ? n_tensors - first : kPointers);
+    PointerList list;
+    std::memset(&list, 0, sizeof(list));
+    std::memcpy(list.p, pointers + first, count * sizeof(void*));
+    launch(list, static_cast<int>(first), count);
+  }
+}
+
+template <bool kRead>
+int move_states(const char* what, void* plan, int64_t n_tensors, int64_t n_chunks, const void* const* exp_avgs,
+                const void* const* exp_avg_sqs, hipStream_t stream) {
+  if (int s = check_plan(what, plan, n_tensors, n_chunks)) return s;
+  if (n_chunks == 0) return DPA4K_OK;
+  if (exp_avgs == nullptr || exp_avg_sqs == nullptr) return fail(DPA4K_EINVAL, "%s: null pointer", what);
+  Record* records = static_cast<Record*>(plan);
+  const Chunk* chunks = reinterpret_cast<const Chunk*>(static_cast<char*>(plan) + chunk_offset(n_tensors));
+  for (int which = 0; which < 2; ++which)
+    each_list(which == 0 ? exp_avgs : exp_avg_sqs, n_tensors, [&](const PointerList& list, int first, int count) {
+      adamw_values_kernel<<<blocks_for(count, kBlock), kBlock, 0, stream>>>(list, records, first, count, which);
+    });
+  adamw_codes_kernel<kRead><<<launch_grid(n_chunks, kBlock), kBlock, 0, stream>>>(records, chunks, n_chunks);
+  return launched("adamw_codes_kernel");
+}
+
+}  // namespace
+}  // namespace dpa4k
+
+using namespace dpa4k;
+
+extern "C" size_t dpa4k_grad_norm_workspace_size(const int64_t* counts, int64_t n_tensors) {
+  if (counts == nullptr || n_tensors <= 0) return 0;
+  int64_t blocks = 0;
+  for (int64_t first = 0; first < n_tensors; first += kNormTensors) {
+    const int64_t last = first + kNormTensors < n_tensors ? first + kNormTensors : n_tensors;
+    const int64_t b = norm_blocks(counts, first, last, nullptr);
+    if (b < 0) return 0;
+    blocks += b;
+  }
+  return round_up_256(static_cast<size_t>(blocks) * sizeof(double));
+}
+
+extern "C" int dpa4k_grad_norm(const void* const* grads, const int64_t* counts, const int32_t* types,
+                               int64_t n_tensors, double max_norm, float* norm, float* factor, void* workspace,
+                               size_t workspace_bytes, dpa4k_stream_t stream_handle) {
+  clear_error();
+  if (n_tensors < 0) return fail(DPA4K_EINVAL, "gradient norm: negative tensor count");
+  if (n_tensors > 0 && (grads == nullptr || counts == nullptr || types == nullptr))
+    return fail(DPA4K_EINVAL, "gradient norm: null pointer");
+  if (norm == nullptr || factor == nullptr) return fail(DPA4K_EINVAL, "gradient norm: null pointer");
+  if (!(max_norm < INFINITY)) return fail(DPA4K_EINVAL, "gradient norm: max_norm must be finite");
+  for (int64_t i = 0; i < n_tensors; ++i) {
+    if (types[i] != DPA4K_TYPE_F32 && types[i] != DPA4K_TYPE_BF16)
+      return fail(DPA4K_EINVAL, "gradient norm: gradient %lld has an unknown type", static_cast<long long>(i));
+    if (counts[i] < 0 || counts[i] > (int64_t(1) << 44) || (counts[i] > 0 && grads[i] == nullptr))
+      return fail(DPA4K_EINVAL, "gradient norm: gradient %lld has a bad size or pointer", static_cast<long long>(i));
+  }
+  const size_t needed = dpa4k_grad_norm_workspace_size(counts, n_tensors);
+  if (workspace_bytes < needed || (needed > 0 && workspace == nullptr))
+    return fail(DPA4K_EWORKSPACE, "gradient norm: workspace of %zu bytes is smaller than %zu", workspace_bytes, needed);
+  hipStream_t stream = as_stream(stream_handle);
+  double* partial = static_cast<double*>(workspace);
+  int64_t partials = 0;
+  for (int64_t first = 0; first < n_tensors; first += kNormTensors) {
+    const int64_t last = first + kNormTensors < n_tensors ? first + kNormTensors : n_tensors;
+    NormList list;
+    std::memset(&list, 0, sizeof(list));
+    const int64_t blocks = norm_blocks(counts, first, last, list.first);
+    if (blocks < 0) return fail(DPA4K_EINVAL, "gradient norm: too many elements");
+    for (int64_t i = first; i < last; ++i) {
+      list.p[i - first] = grads[i];
+      list.count[i - first] = counts[i] * 2 + (types[i] == DPA4K_TYPE_BF16 ? 1 : 0);
+    }
+    if (blocks == 0) continue;
+    const int tensors = static_cast<int>(last - first);
+    grad_norm_kernel<<<static_cast<unsigned int>(blocks), kBlock, 0, stream>>>(list, tensors, list.first[tensors],
+                                                                               partial + partials);
+    if (int s = launched("grad_norm_kernel")) return s;
+    partials += blocks;
+  }
+  grad_norm_total_kernel<<<1, kBlock, 0, stream>>>(partial, partials, max_norm, norm, factor);
+  return launched("grad_norm_total_kernel");
+}
+
+extern "C" size_t dpa4k_adamw_plan_size(const int64_t* counts, int64_t n_tensors) {
+  const int64_t chunks = plan_chunks(counts, n_tensors, 1);
+  if (chunks < 0) return 0;
+  return chunk_offset(n_tensors) + round_up_256(static_cast<size_t>(chunks) * sizeof(Chunk));
+}
+
+extern "C" int dpa4k_adamw_plan(const dpa4k_adamw_tensor* tensors, int64_t n_tensors, int state_bits,
+                                void* plan_host, size_t bytes, int64_t* n_chunks) {
+  clear_error();
+  if (state_bits != 32 && state_bits != 8) return fail(DPA4K_EINVAL, "AdamW plan: state_bits must be 32 or 8");
+  if (n_chunks == nullptr || (n_tensors > 0 && (tensors == nullptr || plan_host == nullptr)))
+    return fail(DPA4K_EINVAL, "AdamW plan: null pointer");
+  const int64_t chunks = plan_chunks(n_tensors > 0 ? &tensors[0].count : nullptr, n_tensors, kStructStride);
+  if (chunks < 0) return fail(DPA4K_EINVAL, "AdamW plan: a size is negative or too large");
+  const size_t needed = chunk_offset(n_tensors) + round_up_256(static_cast<size_t>(chunks) * sizeof(Chunk));
+  if (bytes < needed) return fail(DPA4K_EWORKSPACE, "AdamW plan: %zu bytes are fewer than %zu", bytes, needed);
+  *n_chunks = chunks;
+  if (n_tensors == 0) return DPA4K_OK;
+  std::memset(plan_host, 0, needed);
+  Record* records = static_cast<Record*>(plan_host);
+  Chunk* table = reinterpret_cast<Chunk*>(static_cast<char*>(plan_host) + chunk_offset(n_tensors));
+  uint64_t position = 0;
+  int64_t at = 0;
+  for (int64_t i = 0; i < n_tensors; ++i) {
+    const dpa4k_adamw_tensor& t = tensors[i];
+    if (t.step < 0) return fail(DPA4K_EINVAL, "AdamW plan: tensor %lld has a negative step", static_cast<long long>(i));
+    if (t.count > 0 && (t.param == nullptr || t.exp_avg == nullptr || t.exp_avg_sq == nullptr ||
+                        (state_bits == 8 && (t.exp_avg_scale == nullptr || t.exp_avg_sq_scale == nullptr))))
+      return fail(DPA4K_EINVAL, "AdamW plan: tensor %lld has a null pointer", static_cast<long long>(i));
+    Record& r = records[i];
+    r.param = t.param;
+    r.exp_avg = t.exp_avg;
+    r.exp_avg_sq = t.exp_avg_sq;
+    r.exp_avg_scale = t.exp_avg_scale;
+    r.exp_avg_sq_scale = t.exp_avg_sq_scale;
+    r.count = t.count;
+    r.position = position;
+    r.step = t.step;
+    position += static_cast<uint64_t>((t.count + kSpan - 1) / kSpan * kSpan);
+    for (int64_t c = 0; c < tensor_chunks(t.count); ++c) table[at++] = {static_cast<int32_t>(i), static_cast<int32_t>(c)};
+  }
+  return DPA4K_OK;
+}
+
+extern "C" int dpa4k_adamw_step(void* plan, int64_t n_tensors, int64_t n_chunks, int state_bits, int param_type,
+                                int grad_type, const void* const* grads, double lr, const float* lr_device,
+                                double beta1, double beta2, double eps, double weight_decay,
+                                const float* grad_factor, uint64_t seed, dpa4k_stream_t stream_handle) {
+  clear_error();
+  if (int s = check_plan("AdamW step", plan, n_tensors, n_chunks)) return s;
+  if (state_bits != 32 && state_bits != 8) return fail(DPA4K_EINVAL, "AdamW step: state_bits must be 32 or 8");
+  if ((param_type != DPA4K_TYPE_F32 && param_type != DPA4K_TYPE_BF16) ||
+      (grad_type != DPA4K_TYPE_F32 && grad_type != DPA4K_TYPE_BF16))
+    return fail(DPA4K_EINVAL, "AdamW step: unknown type");
+  if (!(lr >= 0.0 && lr < INFINITY) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) ||
+      !(static_cast<float>(eps) > 0.0f && eps < INFINITY) || !(weight_decay >= 0.0 && weight_decay < INFINITY))
+    return fail(DPA4K_EINVAL, "AdamW step: lr, betas, eps or weight_decay out of range");
+  if (n_tensors == 0) return DPA4K_OK;
+  if (grads == nullptr) return fail(DPA4K_EINVAL, "AdamW step: null pointer");
+  hipStream_t stream = as_stream(stream_handle);
+  Record* records = static_cast<Record*>(plan);
+  const Chunk* chunks = reinterpret_cast<const Chunk*>(static_cast<char*>(plan) + chunk_offset(n_tensors));
+  const StepScalars begin = {lr, beta1, beta2, weight_decay, lr_device, grad_factor};
+  each_list(grads, n_tensors, [&](const PointerList& list, int first, int count) {
+    adamw_begin_kernel<<<blocks_for(count, kBlock), kBlock, 0, stream>>>(list, records, first, count, begin);
+  });
+  if (int s = launched("adamw_begin_kernel")) return s;
+  if (n_chunks == 0) return DPA4K_OK;
+  const UpdateScalars update = {static_cast<float>(beta1), static_cast<float>(1.0 - beta1), static_cast<float>(beta2),
+                                static_cast<float>(1.0 - beta2), static_cast<float>(eps),
+                                static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32)};
+  const dim3 grid = launch_grid(n_chunks, kBlock);
+#define DPA4K_ADAMW(P, G)                                                                               \
+  (state_bits == 32 ? adamw_update_kernel<P, G, 32> : adamw_update_kernel<P, G, 8>)<<<grid, kBlock, 0, stream>>>( \
+      records, chunks, n_chunks, update)
+  if (param_type == DPA4K_TYPE_F32) {
+    if (grad_type == DPA4K_TYPE_F32) DPA4K_ADAMW(float, float);
+    else DPA4K_ADAMW(float, uint16_t);
+  } else {
+    if (grad_type == DPA4K_TYPE_F32) DPA4K_ADAMW(uint16_t, float);
+    else DPA4K_ADAMW(uint16_t, uint16_t);
+  }
+#undef DPA4K_ADAMW
+  return launched("adamw_update_kernel");
+}
+
+extern "C" int dpa4k_adamw_read_states(void* plan, int64_t n_tensors, int64_t n_chunks, float* const* exp_avgs,
+                                       float* const* exp_avg_sqs, dpa4k_stream_t stream) {
+  clear_error();
+  return move_states<true>("AdamW read states", plan, n_tensors, n_chunks,
+                           reinterpret_cast<const void* const*>(exp_avgs),
+                           reinterpret_cast<const void* const*>(exp_avg_sqs), as_stream(stream));
+}
+
+extern "C" int dpa4k_adamw_write_states(void* plan, int64_t n_tensors, int64_t n_chunks, const float* const* exp_avgs,
+                                        const float* const* exp_avg_sqs, dpa4k_stream_t stream) {
+  clear_error();
+  return move_states<false>("AdamW write states", plan, n_tensors, n_chunks,
+                            reinterpret_cast<const void* const*>(exp_avgs),
+                            reinterpret_cast<const void* const*>(exp_avg_sqs), as_stream(stream));
+}

@@ -17,7 +17,9 @@ inputs; ``segment_offsets``, ``group_by_key``, ``gie_group`` and the
 ``segment_softmax_plan`` builds the degree plan that
 ``segment_softmax_forward/backward(..., plan=...)`` accept;
 ``gie_rmsnorm_forward_csr`` is the fused GIE -> RMSNorm forward;
-``edge_stream_combine`` is the fused edge-stream elementwise chain.
+``edge_stream_combine`` is the fused edge-stream elementwise chain;
+``group_norm_forward/backward``, ``grad_norm`` and the ``adamw_*`` entry
+points are the operators of a training step.
 """
 from __future__ import annotations
 
@@ -847,3 +849,202 @@ __all__ = [
     "segment_sum_backward",
     "segment_sum_forward",
 ]
+
+
+# ---------------------------------------------------------------------------
+# group norm, channels last (no reference implementation)
+# ---------------------------------------------------------------------------
+
+ELEMENT_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
+GROUP_NORM_MAX_CHANNELS = 4096
+
+
+def _group_norm_sizes(x, groups, scale, bias, offsets):
+    """(samples, entries, inner, channels) of a call, its tensors checked."""
+    _check(isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in ELEMENT_TYPES and x.is_contiguous(),
+           "group norm input: expected a contiguous gfx950 float32, bfloat16 or float16 tensor")
+    _check(x.dim() >= 2, "group norm input must have at least two dimensions")
+    channels = int(x.shape[-1])
+    _check(1 <= channels <= GROUP_NORM_MAX_CHANNELS and groups >= 1 and channels % groups == 0,
+           f"group norm takes 1 to {GROUP_NORM_MAX_CHANNELS} channels in groups of equal size")
+    for what, tensor in (("scale", scale), ("bias", bias)):
+        if tensor is not None:
+            _f32(tensor, f"group norm {what}")
+            _check(tuple(tensor.shape) == (channels,), f"group norm {what} must have shape (channels,)")
+    entries = int(x.shape[0])
+    inner = 1
+    for size in x.shape[1:-1]:
+        inner *= int(size)
+    samples = entries if offsets is None else _offsets(offsets, "group norm offsets")
+    _same_device(x, scale, bias, offsets)
+    return samples, entries, inner, channels
+
+
+def group_norm_forward(x, groups, scale=None, bias=None, offsets=None, eps: float = 1.0e-5, silu: bool = False):
+    """``(y, mean, rstd)``; ``mean`` and ``rstd`` are ``(samples, groups)`` float32."""
+    groups = int(groups)
+    samples, entries, inner, channels = _group_norm_sizes(x, groups, scale, bias, offsets)
+    y = torch.empty_like(x)
+    statistics = torch.empty((2, samples, groups), dtype=torch.float32, device=x.device)
+    mean, rstd = statistics[0], statistics[1]
+    code = ELEMENT_TYPES[x.dtype]
+    nbytes = _LIB.dpa4k_group_norm_workspace_size(samples, entries, inner, channels, groups, code, 0)
+    workspace = _workspace(nbytes, x.device)
+    with _on(x.device) as stream:
+        status = _LIB.dpa4k_group_norm_forward(
+            _ptr(x), _ptr(scale), _ptr(bias), _ptr(offsets), _ptr(y), _ptr(mean), _ptr(rstd), samples, entries, inner,
+            channels, groups, float(eps), int(bool(silu)), code, workspace.data_ptr(), nbytes, stream)
+    _lib.check(status)
+    return y, mean, rstd
+
+
+def group_norm_backward(grad_output, x, groups, scale, bias, offsets, mean, rstd, silu: bool = False, *,
+                        want_x: bool = True, want_scale: bool = True, want_bias: bool = True):
+    """``(grad_x, grad_scale, grad_bias)``, None where not wanted."""
+    groups = int(groups)
+    samples, entries, inner, channels = _group_norm_sizes(x, groups, scale, bias, offsets)
+    _check(isinstance(grad_output, torch.Tensor) and grad_output.is_contiguous() and grad_output.dtype == x.dtype
+           and grad_output.shape == x.shape, "group norm grad_output must be like the input")
+    for tensor in (mean, rstd):
+        _f32(tensor, "group norm statistics")
+        _check(tuple(tensor.shape) == (samples, groups), "group norm statistics must have shape (samples, groups)")
+    _same_device(x, grad_output, mean, rstd)
+    grad_x = torch.empty_like(x) if want_x else None
+    grad_scale = torch.empty((channels,), dtype=torch.float32, device=x.device) if want_scale else None
+    grad_bias = torch.empty((channels,), dtype=torch.float32, device=x.device) if want_bias else None
+    code = ELEMENT_TYPES[x.dtype]
+    nbytes = _LIB.dpa4k_group_norm_workspace_size(samples, entries, inner, channels, groups, code, 1)
+    workspace = _workspace(nbytes, x.device)
+    with _on(x.device) as stream:
+        status = _LIB.dpa4k_group_norm_backward(
+            _ptr(grad_output), _ptr(x), _ptr(scale), _ptr(bias), _ptr(offsets), _ptr(mean), _ptr(rstd), _ptr(grad_x),
+            _ptr(grad_scale), _ptr(grad_bias), samples, entries, inner, channels, groups, int(bool(silu)), code,
+            workspace.data_ptr(), nbytes, stream)
+    _lib.check(status)
+    return grad_x, grad_scale, grad_bias
+
+
+# ---------------------------------------------------------------------------
+# optimiser step (no reference implementation)
+# ---------------------------------------------------------------------------
+
+def _addresses(tensors, n: int):
+    """A host array of the tensors' device addresses; None stands for NULL."""
+    return (ctypes.c_void_p * n)(*[None if t is None else t.data_ptr() for t in tensors])
+
+
+def grad_norm(grads, max_norm: float = 0.0):
+    """``(norm, factor)`` of contiguous float32 or bfloat16 tensors on one device (at least one)."""
+    n = len(grads)
+    _check(n >= 1, "gradient norm needs at least one gradient")
+    device = grads[0].device
+    types = [g.dtype for g in grads]
+    _check(all(t in (torch.float32, torch.bfloat16) for t in set(types)),
+           "gradient norm: expected float32 or bfloat16 tensors")
+    _check(all([g.is_contiguous() for g in grads]), "gradient norm: expected contiguous tensors")
+    _check(device.type == "cuda" and all([g.device == device for g in grads]),
+           "gradient norm: expected gfx950 tensors on one device")
+    counts = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
+    codes = (ctypes.c_int32 * n)(*[ELEMENT_TYPES[t] for t in types])
+    result = torch.empty((2,), dtype=torch.float32, device=device)
+    nbytes = _LIB.dpa4k_grad_norm_workspace_size(counts, n)
+    workspace = _workspace(nbytes, device)
+    with _on(device) as stream:
+        status = _LIB.dpa4k_grad_norm(_addresses(grads, n), counts, codes, n, float(max_norm), result.data_ptr(),
+                                      result.data_ptr() + 4, workspace.data_ptr(), nbytes, stream)
+    _lib.check(status)
+    return result[0], result[1]
+
+
+ADAMW_SPAN = 32   # elements that share a scale
+
+
+class AdamWPlan:
+    """The tensors of an AdamW step: parameters, moments and step counts, and their table on the device."""
+
+    def __init__(self, params, state_bits):
+        self.params = params
+        self.state_bits = state_bits
+        self.dtype = params[0].dtype
+        self.device = params[0].device
+        self.shapes = [p.shape for p in params]
+        self.addresses = [p.data_ptr() for p in params]
+        self.exp_avgs = self.exp_avg_sqs = None             # 32 bits: float32 tensors
+        self.codes = self.scales = None                     # 8 bits: (2, padded) and (2, padded / 32) bytes
+        self.words = None
+        self.n_chunks = 0
+
+    def steps(self) -> torch.Tensor:
+        """Steps taken per tensor: a copy of the device's counts, int64."""
+        n = len(self.params)
+        words = self.words[: n * _lib.ADAMW_RECORD_BYTES].view(torch.int64).view(n, -1)
+        return words[:, _lib.ADAMW_STEP_OFFSET // 8].clone()
+
+    def parts(self):
+        """Each tensor's 8-bit moments: views of its codes (2, padded) and scales (2, padded / 32)."""
+        at = 0
+        for p in self.params:
+            end = at + -(-p.numel() // ADAMW_SPAN)
+            yield self.codes[:, at * ADAMW_SPAN: end * ADAMW_SPAN], self.scales[:, at:end]
+            at = end
+
+
+def adamw_plan(params, exp_avgs, exp_avg_sqs, steps, state_bits: int) -> AdamWPlan:
+    """The plan of checked tensors; moments None start at 0, 8-bit ones at the nearest codes of those given."""
+    plan = AdamWPlan(list(params), int(state_bits))
+    n, device = len(plan.params), plan.device
+    counts = [p.numel() for p in plan.params]
+    table = (_lib.AdamwTensor * n)()
+    if state_bits == 32:
+        plan.exp_avgs, plan.exp_avg_sqs = (
+            [torch.zeros_like(p, dtype=torch.float32) for p in plan.params] if given is None else list(given)
+            for given in (exp_avgs, exp_avg_sqs))
+    else:
+        spans = [-(-count // ADAMW_SPAN) for count in counts]
+        total = sum(spans)
+        plan.codes = torch.zeros((2, total * ADAMW_SPAN), dtype=torch.uint8, device=device)
+        plan.scales = torch.full((2, total), 32, dtype=torch.uint8, device=device)
+    at = 0
+    for k, p in enumerate(plan.params):
+        entry = table[k]
+        entry.param, entry.count, entry.step = p.data_ptr(), counts[k], int(steps[k])
+        if state_bits == 32:
+            entry.exp_avg, entry.exp_avg_sq = plan.exp_avgs[k].data_ptr(), plan.exp_avg_sqs[k].data_ptr()
+        else:
+            entry.exp_avg, entry.exp_avg_sq = (plan.codes.data_ptr() + (which * total + at) * ADAMW_SPAN for which in (0, 1))
+            entry.exp_avg_scale, entry.exp_avg_sq_scale = (plan.scales.data_ptr() + which * total + at for which in (0, 1))
+            at += spans[k]
+    nbytes = _LIB.dpa4k_adamw_plan_size((ctypes.c_int64 * n)(*counts), n)
+    host = torch.zeros((nbytes,), dtype=torch.uint8)
+    chunks = ctypes.c_int64(0)
+    _lib.check(_LIB.dpa4k_adamw_plan(table, n, int(state_bits), host.data_ptr(), nbytes, ctypes.byref(chunks)))
+    plan.n_chunks = chunks.value
+    plan.words = host.to(device)
+    if state_bits == 8 and exp_avgs is not None:
+        _move_states(_LIB.dpa4k_adamw_write_states, plan, exp_avgs, exp_avg_sqs)
+    return plan
+
+
+def _move_states(entry_point, plan, exp_avgs, exp_avg_sqs) -> None:
+    n = len(plan.params)
+    with _on(plan.device) as stream:
+        status = entry_point(plan.words.data_ptr(), n, plan.n_chunks, _addresses(exp_avgs, n),
+                             _addresses(exp_avg_sqs, n), stream)
+    _lib.check(status)
+
+
+def adamw_read_states(plan, exp_avgs, exp_avg_sqs) -> None:
+    """The 8-bit moments of ``plan`` as values in the float32 tensors given."""
+    _move_states(_LIB.dpa4k_adamw_read_states, plan, exp_avgs, exp_avg_sqs)
+
+
+def adamw_step(plan, addresses, grad_dtype, lr: float, lr_tensor, beta1: float, beta2: float, eps: float,
+               weight_decay: float, grad_factor, seed: int) -> None:
+    """One step; ``addresses``: a gradient's device address per tensor, None or 0 where it has none."""
+    n = len(plan.params)
+    with _on(plan.device) as stream:
+        status = _LIB.dpa4k_adamw_step(
+            plan.words.data_ptr(), n, plan.n_chunks, plan.state_bits, ELEMENT_TYPES[plan.dtype],
+            ELEMENT_TYPES[grad_dtype], (ctypes.c_void_p * n)(*addresses), lr, _ptr(lr_tensor), beta1, beta2, eps,
+            weight_decay, _ptr(grad_factor), seed & 0xFFFFFFFFFFFFFFFF, stream)
+    _lib.check(status)

@@ -15,14 +15,20 @@ from pathlib import Path
 LIBRARY_PATH = Path(__file__).resolve().parent.parent / "libdpa4k.so"
 
 OK, EINVAL, EHIP, EWORKSPACE = 0, 1, 2, 3
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 _F32 = ctypes.c_float
 _INT = ctypes.c_int
+_F64 = ctypes.c_double
 
+# Element types (DPA4K_TYPE_*).
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+
+# Layout of an AdamW plan's records (DPA4K_ADAMW_*).
+ADAMW_RECORD_BYTES, ADAMW_STEP_OFFSET = 128, 56
 
 
 class EdgeOperand(ctypes.Structure):
@@ -32,6 +38,13 @@ class EdgeOperand(ctypes.Structure):
 
 
 _OPERANDS = ctypes.POINTER(EdgeOperand)
+
+
+class AdamwTensor(ctypes.Structure):
+    """``dpa4k_adamw_tensor``: one tensor of an AdamW plan."""
+
+    _fields_ = [("param", _P), ("exp_avg", _P), ("exp_avg_sq", _P), ("exp_avg_scale", _P),
+                ("exp_avg_sq_scale", _P), ("count", _I64), ("step", _I64)]
 
 # name -> (restype, argtypes); mirrors include/dpa4k.h one to one.
 PROTOTYPES: dict[str, tuple[object, list[object]]] = {
@@ -89,6 +102,17 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "dpa4k_edge_stream_combine": (
         _INT, [_OPERANDS, _OPERANDS, ctypes.POINTER(_F32), _INT, _INT, _OPERANDS, ctypes.POINTER(ctypes.c_int32), _P,
                _I64, _I64, _I64, _P]),
+    "dpa4k_group_norm_workspace_size": (_SZ, [_I64] * 5 + [_INT, _INT]),
+    "dpa4k_group_norm_forward": (_INT, [_P] * 7 + [_I64] * 5 + [_F32, _INT, _INT, _P, _SZ, _P]),
+    "dpa4k_group_norm_backward": (_INT, [_P] * 10 + [_I64] * 5 + [_INT, _INT, _P, _SZ, _P]),
+    "dpa4k_grad_norm_workspace_size": (_SZ, [_P, _I64]),
+    "dpa4k_grad_norm": (_INT, [_P, _P, _P, _I64, _F64, _P, _P, _P, _SZ, _P]),
+    "dpa4k_adamw_plan_size": (_SZ, [_P, _I64]),
+    "dpa4k_adamw_plan": (_INT, [_P, _I64, _INT, _P, _SZ, ctypes.POINTER(_I64)]),
+    "dpa4k_adamw_step": (
+        _INT, [_P, _I64, _I64, _INT, _INT, _INT, _P, _F64, _P, _F64, _F64, _F64, _F64, _P, ctypes.c_uint64, _P]),
+    "dpa4k_adamw_read_states": (_INT, [_P, _I64, _I64, _P, _P, _P]),
+    "dpa4k_adamw_write_states": (_INT, [_P, _I64, _I64, _P, _P, _P]),
     "dpa4k_stream_calibrate": (_INT, [_P, _I64, _P, _I64, _P]),
     "dpa4k_set_launch_row_limit": (_INT, [_I64]),
     "dpa4k_set_host_words": (_INT, [_I64]),

@@ -1,0 +1,358 @@
+"""The optimiser step over all tensors of a model: gradient norm, AdamW, moments in 32 or in 8 bits.
+
+The operators' backward passes give a model's gradients; these turn them into
+a step in a few launches, whatever the number of tensors, without waiting for
+the GPU:
+
+    norm, factor = grad_norm(grads, max_norm=1.0)
+    plan = adamw_plan(params, state_bits=8)                       # once
+    adamw_step(plan, grads, lr=1e-3, grad_factor=factor)
+
+or, as a ``torch.optim.Optimizer``, ``AdamW(params, lr=1e-3, max_norm=1.0)``.
+No counterpart in the reference; not part of ``kernels.__all__``.
+
+Moments in 8 bits take 2.06 bytes an element instead of 8.  Blocks of 32
+consecutive elements of a tensor share a power of two, and a code is a float
+with 3 mantissa bits in the 16 (first moment, with a sign) or 32 (second)
+binades below it.  They are rounded stochastically, as bfloat16 parameters are: a
+slow average moves by less than half a step at a time, which a nearest
+rounding would lose every time.
+"""
+from __future__ import annotations
+
+import math
+import numbers
+
+import torch
+
+from .native import _extension, require_dcu
+
+DTYPES = (torch.float32, torch.bfloat16)
+STATE_BITS = (32, 8)
+
+
+def _tensors(values, what: str, *, allow_none: bool = False) -> list:
+    if isinstance(values, torch.Tensor) or not hasattr(values, "__iter__"):
+        raise TypeError(f"{what} must be a sequence of tensors")
+    values = list(values)
+    for value in values:
+        if not isinstance(value, torch.Tensor) and not (allow_none and value is None):
+            raise TypeError(f"{what} must be a sequence of tensors")
+    return values
+
+
+def _real(value, what: str, low: float, high: float = math.inf, *, above: bool = False) -> float:
+    if isinstance(value, bool) or not isinstance(value, numbers.Real):
+        raise TypeError(f"{what} must be a real number")
+    value = float(value)
+    if not math.isfinite(value) or value < low or value >= high or (above and value == low):
+        raise ValueError(f"{what} is out of range: {value}")
+    return value
+
+
+def _scalar_tensor(value, what: str, device=None):
+    if value.dtype != torch.float32 or value.numel() != 1:
+        raise ValueError(f"{what} must be a float32 tensor of one element")
+    if device is not None and value.device != device:
+        raise ValueError(f"{what} must be on the parameters' device")
+    return value
+
+
+# ---------------------------------------------------------------------------
+# gradient norm
+# ---------------------------------------------------------------------------
+
+def grad_norm(grads, max_norm: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(norm, factor)``: the norm over all gradients, and what they are to be multiplied with so that it is at most ``max_norm``.
+
+    ``grads``: contiguous float32 or bfloat16 tensors on one device; None
+    entries count as 0.  Both results are float32 tensors without dimensions
+    on that device; nothing waits for the GPU.  The squares are summed in 64
+    bits in a fixed order.  ``factor`` is ``min(1, max_norm / (norm + 1e-6))``,
+    1 without ``max_norm``, and NaN where the norm is not finite:
+    ``adamw_step`` then takes no step.
+    """
+    grads = [g for g in _tensors(grads, "grad_norm gradients", allow_none=True) if g is not None]
+    if not grads:
+        raise ValueError("grad_norm needs at least one gradient")
+    limit = 0.0 if max_norm is None else _real(max_norm, "grad_norm max_norm", 0.0, above=True)
+    device = grads[0].device
+    for g in grads:
+        if g.dtype not in DTYPES:
+            raise TypeError("grad_norm requires float32 or bfloat16 gradients")
+        if not g.is_contiguous():
+            raise ValueError("grad_norm gradients must be contiguous")
+        if g.device != device:
+            raise ValueError("grad_norm gradients must share a device")
+    require_dcu(grads[0])
+    return _extension("grad_norm").grad_norm(grads, limit)
+
+
+# ---------------------------------------------------------------------------
+# AdamW
+# ---------------------------------------------------------------------------
+
+def _refuse_overlaps(tensors) -> None:
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("AdamW parameters and moments must not overlap")
+
+
+def _moments(values, params, what: str):
+    values = _tensors(values, what)
+    if len(values) != len(params):
+        raise ValueError(f"{what}: expected one tensor per parameter")
+    for value, p in zip(values, params):
+        if value.dtype != torch.float32:
+            raise TypeError(f"{what} must be float32")
+        if value.shape != p.shape or value.device != p.device or not value.is_contiguous():
+            raise ValueError(f"{what} must be contiguous, of the parameters' shapes and device")
+    return values
+
+
+def adamw_plan(params, exp_avgs=None, exp_avg_sqs=None, *, step=0, state_bits: int = 32):
+    """The tensors of ``adamw_step`` with their moments, listed once on the device.
+
+    ``params``: contiguous tensors of one dtype (float32 or bfloat16) and
+    device that do not overlap.  ``exp_avgs``, ``exp_avg_sqs``: float32
+    tensors of their shapes, both or neither; with ``state_bits`` 32 they are
+    the plan's moments, updated in place, with 8 the plan starts from their
+    nearest codes.  ``step``: steps taken so far, one number or one per
+    tensor.  Building a plan copies its table to the device and waits for it.
+    """
+    params = _tensors(params, "AdamW parameters")
+    if not params:
+        raise ValueError("AdamW needs at least one parameter")
+    if isinstance(state_bits, bool) or state_bits not in STATE_BITS:
+        raise ValueError(f"AdamW state_bits must be 32 or 8, got {state_bits!r}")
+    for p in params:
+        if p.dtype not in DTYPES:
+            raise TypeError("AdamW requires float32 or bfloat16 parameters")
+        if p.dtype != params[0].dtype or p.device != params[0].device:
+            raise ValueError("the parameters of a plan must share a dtype and a device")
+        if not p.is_contiguous():
+            raise ValueError("AdamW parameters must be contiguous")
+    if (exp_avgs is None) != (exp_avg_sqs is None):
+        raise ValueError("AdamW moments: give both or neither")
+    if exp_avgs is not None:
+        exp_avgs = _moments(exp_avgs, params, "AdamW exp_avgs")
+        exp_avg_sqs = _moments(exp_avg_sqs, params, "AdamW exp_avg_sqs")
+    _refuse_overlaps(params + (exp_avgs or []) + (exp_avg_sqs or []))
+    steps = [step] * len(params) if isinstance(step, numbers.Integral) else list(step)
+    if len(steps) != len(params):
+        raise ValueError("AdamW step: expected one number per parameter")
+    for value in steps:
+        if isinstance(value, bool) or not isinstance(value, numbers.Integral):
+            raise TypeError("AdamW step must be an integer")
+        if value < 0:
+            raise ValueError("AdamW step must not be negative")
+    require_dcu(params[0])
+    return _extension("adamw_plan").adamw_plan(params, exp_avgs, exp_avg_sqs, steps, state_bits)
+
+
+def adamw_step(plan, grads, *, lr, betas=(0.9, 0.999), eps: float = 1.0e-8, weight_decay: float = 1.0e-2,
+               grad_factor: torch.Tensor | None = None, seed: int = 0) -> None:
+    """One AdamW step over the tensors of ``plan``, in place.
+
+        g = grad * grad_factor
+        m = beta1 m + (1 - beta1) g,    v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+    every operation rounded to float32, so that a step equals the eager chain
+    bit for bit.  ``grads``: one tensor per parameter (contiguous, of its
+    shape; all float32 or all bfloat16) or None where it takes no step.
+    ``lr``: a number, or a float32 tensor of one element on the device (read
+    when the step runs, also in a captured graph).  ``grad_factor``: such a
+    tensor; a NaN leaves parameters, moments and step counts as they are.
+    ``seed``: of the stochastic roundings of bfloat16 parameters and 8-bit
+    moments, which also depend on the step.  Calls on one plan must not
+    overlap in time.
+    """
+    params = plan.params
+    if len(grads) != len(params):
+        raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients")
+    if [p.data_ptr() for p in params] != plan.addresses:
+        raise RuntimeError("adamw_step: a parameter's memory has moved since the plan was built")
+    try:
+        given = [g for g in grads if g is not None]
+        dtypes = {g.dtype for g in given}
+        addresses = [0 if g is None else g.data_ptr() for g in grads]
+        contiguous = all([g.is_contiguous() for g in given])
+        devices = {g.device for g in given}
+    except AttributeError as error:
+        raise TypeError("adamw_step gradients must be tensors or None") from error
+    if not given:
+        return
+    if len(dtypes) != 1 or not dtypes <= set(DTYPES):
+        raise TypeError("adamw_step requires gradients of one dtype, float32 or bfloat16")
+    if any([g is not None and g.shape != shape for g, shape in zip(grads, plan.shapes)]):
+        raise ValueError("adamw_step gradients must have their parameters' shapes")
+    if not contiguous:
+        raise ValueError("adamw_step gradients must be contiguous")
+    if devices != {plan.device}:
+        raise ValueError("adamw_step gradients must be on the parameters' device")
+    lr_tensor = None
+    if isinstance(lr, torch.Tensor):
+        lr_tensor, lr = _scalar_tensor(lr, "adamw_step lr", plan.device), 0.0
+    else:
+        lr = _real(lr, "adamw_step lr", 0.0)
+    if not isinstance(betas, (tuple, list)) or len(betas) != 2:
+        raise TypeError("adamw_step betas must be a pair")
+    beta1, beta2 = (_real(b, "adamw_step beta", 0.0, 1.0) for b in betas)
+    eps = _real(eps, "adamw_step eps", 1.0e-38)
+    weight_decay = _real(weight_decay, "adamw_step weight_decay", 0.0)
+    if grad_factor is not None:
+        if not isinstance(grad_factor, torch.Tensor):
+            raise TypeError("adamw_step grad_factor must be a tensor or None")
+        _scalar_tensor(grad_factor, "adamw_step grad_factor", plan.device)
+    if isinstance(seed, bool) or not isinstance(seed, numbers.Integral):
+        raise TypeError("adamw_step seed must be an integer")
+    native = _extension("adamw_step")
+    native.adamw_step(plan, addresses, dtypes.pop(), lr, lr_tensor, beta1, beta2, eps, weight_decay, grad_factor,
+                      int(seed))
+    # the kernels write behind autograd's back: saved tensors and caches of derived data see it by the counter
+    torch.autograd.graph.increment_version(params)
+
+
+def adamw_states(plan, exp_avgs=None, exp_avg_sqs=None) -> tuple[list, list]:
+    """The moments of ``plan`` as float32 tensors of the parameters' shapes: copies, or written into the tensors given."""
+    out = []
+    for values, what in ((exp_avgs, "AdamW exp_avgs"), (exp_avg_sqs, "AdamW exp_avg_sqs")):
+        out.append([torch.empty_like(p, dtype=torch.float32) for p in plan.params] if values is None
+                   else _moments(values, plan.params, what))
+    if plan.state_bits == 32:
+        for to, values in zip(out, (plan.exp_avgs, plan.exp_avg_sqs)):
+            torch._foreach_copy_(to, values)
+    else:
+        _extension("adamw_read_states").adamw_read_states(plan, *out)
+        for values in out:
+            torch.autograd.graph.increment_version(values)
+    return out[0], out[1]
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over all tensors at once, as a ``torch.optim.Optimizer``.
+
+    ``lr`` (a number, or a float32 tensor of one element on the device),
+    ``betas``, ``eps`` and ``weight_decay`` may differ between parameter
+    groups; ``max_norm`` clips the norm over all gradients of all groups (or,
+    where that norm is not finite, takes no step); ``state_bits`` is 32 or 8.
+    Parameters are contiguous float32 or bfloat16 tensors on one device.
+    After ``step`` the attribute ``norm`` is the gradients' norm before
+    clipping, a tensor on the device, or None without ``max_norm``.
+
+    The plans are built in the first step; later steps may be captured in a
+    HIP graph (with ``lr`` a tensor where a schedule changes it between
+    replays).  Checkpoints hold each parameter's step count and moments; 8-bit
+    moments are kept as their codes.
+    """
+
+    def __init__(self, params, lr=1.0e-3, betas=(0.9, 0.999), eps: float = 1.0e-8, weight_decay: float = 1.0e-2, *,
+                 max_norm: float | None = None, state_bits: int = 32, seed: int = 0):
+        if isinstance(state_bits, bool) or state_bits not in STATE_BITS:
+            raise ValueError(f"AdamW state_bits must be 32 or 8, got {state_bits!r}")
+        self.max_norm = None if max_norm is None else _real(max_norm, "AdamW max_norm", 0.0, above=True)
+        self.state_bits, self.seed, self.norm = state_bits, int(seed), None
+        self._plans: dict = {}     # (group, dtype): plan
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        if isinstance(group["lr"], torch.Tensor):
+            _scalar_tensor(group["lr"], "AdamW lr")
+        else:
+            _real(group["lr"], "AdamW lr", 0.0)
+        if not isinstance(group["betas"], (tuple, list)) or len(group["betas"]) != 2:
+            raise TypeError("AdamW betas must be a pair")
+        for beta in group["betas"]:
+            _real(beta, "AdamW beta", 0.0, 1.0)
+        _real(group["eps"], "AdamW eps", 1.0e-38)
+        _real(group["weight_decay"], "AdamW weight_decay", 0.0)
+        for p in group["params"]:
+            if p.dtype not in DTYPES:
+                raise TypeError("AdamW requires float32 or bfloat16 parameters")
+            if not p.is_contiguous():
+                raise ValueError("AdamW parameters must be contiguous")
+
+    def _plan(self, key, params):
+        plan = self._plans.get(key)
+        if plan is not None and len(plan.params) == len(params) and \
+                all([a is b for a, b in zip(plan.params, params)]) and [p.data_ptr() for p in params] == plan.addresses:
+            return plan
+        held = {} if plan is None else self._held(plan)
+        return self._build(key, params, held)
+
+    def _build(self, key, params, held):
+        """A plan of ``params`` that goes on from ``held``: {parameter: its part of a checkpoint}."""
+        known = {k: held[p] for k, p in enumerate(params) if p in held}
+        steps = [int(known[k]["step"]) if k in known else 0 for k in range(len(params))]
+        if self.state_bits == 32:
+            moments = [[known[k][name].to(device=p.device, dtype=torch.float32).reshape(p.shape).contiguous().clone()
+                        if k in known else torch.zeros_like(p, dtype=torch.float32).detach()
+                        for k, p in enumerate(params)] for name in ("exp_avg", "exp_avg_sq")]
+            plan = adamw_plan(params, *moments, step=steps)
+        else:
+            plan = adamw_plan(params, step=steps, state_bits=8)
+            for k, (codes, scales) in enumerate(plan.parts()):
+                if k in known:
+                    codes.copy_(known[k]["codes"])
+                    scales.copy_(known[k]["scales"])
+        self._plans[key] = plan
+        return plan
+
+    @staticmethod
+    def _held(plan) -> dict:
+        steps = plan.steps().tolist()
+        if plan.state_bits == 32:
+            return {p: {"step": t, "exp_avg": m, "exp_avg_sq": v}
+                    for p, t, m, v in zip(plan.params, steps, plan.exp_avgs, plan.exp_avg_sqs)}
+        return {p: {"step": t, "codes": codes, "scales": scales}
+                for p, t, (codes, scales) in zip(plan.params, steps, plan.parts())}
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step over the parameters that have a gradient; returns the closure's loss."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = []
+        for index, group in enumerate(self.param_groups):
+            for dtype in DTYPES:
+                params = [p for p in group["params"] if p.dtype == dtype]
+                grads = [p.grad for p in params]
+                if any([g is not None for g in grads]):
+                    work.append((group, self._plan((index, dtype), params), grads, index * 2 + (dtype == torch.bfloat16)))
+        self.norm = factor = None
+        if self.max_norm is not None and work:
+            self.norm, factor = grad_norm([g for _, _, grads, _ in work for g in grads if g is not None], self.max_norm)
+        for group, plan, grads, stream in work:
+            adamw_step(plan, grads, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                       weight_decay=group["weight_decay"], grad_factor=factor, seed=self.seed + stream * 0x9E3779B97F4A7C15)
+        return loss
+
+    def state_dict(self) -> dict:
+        result = super().state_dict()
+        numbers_of = {p: k for k, p in enumerate(p for group in self.param_groups for p in group["params"])}
+        result["state"] = {numbers_of[p]: {name: value.clone() if isinstance(value, torch.Tensor) else value
+                                           for name, value in part.items()}
+                           for plan in self._plans.values() for p, part in self._held(plan).items()}
+        result["state_bits"] = self.state_bits
+        return result
+
+    def load_state_dict(self, state_dict) -> None:
+        if state_dict.get("state_bits", self.state_bits) != self.state_bits:
+            raise ValueError(f"the checkpoint holds {state_dict['state_bits']}-bit moments, not {self.state_bits}-bit ones")
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        params = [p for group in self.param_groups for p in group["params"]]
+        held = {params[int(k)]: part for k, part in state_dict["state"].items()}
+        self._plans = {}
+        for index, group in enumerate(self.param_groups):
+            for dtype in DTYPES:
+                own = [p for p in group["params"] if p.dtype == dtype]
+                if any([p in held for p in own]):
+                    self._build((index, dtype), own, held)
+
+
+__all__ = ["AdamW", "grad_norm", "adamw_plan", "adamw_step", "adamw_states", "DTYPES", "STATE_BITS"]

@@ -61,7 +61,7 @@ const char* dpa4k_last_error(void);
 
 /* ABI version of this header (bumped on any signature change). */
 int dpa4k_abi_version(void);
-#define DPA4K_ABI_VERSION 10
+#define DPA4K_ABI_VERSION 11
 
 /* ------------------------------------------------------------------------
  * CSR construction
@@ -524,6 +524,119 @@ int dpa4k_rmsnorm_backward_noalloc(const float* grad, const float* x,
                                    float* grad_x, float* grad_scale,
                                    int64_t rows, int64_t width,
                                    dpa4k_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Group norm with an activation, channels last (no reference counterpart)
+ * ---------------------------------------------------------------------- */
+
+/* Element types of tensors that need not be float. */
+enum { DPA4K_TYPE_F32 = 0, DPA4K_TYPE_BF16 = 1, DPA4K_TYPE_F16 = 2 };
+
+/* x, y[entries, inner, C] of `type`.  Sample s owns the entries [offsets[s],
+ * offsets[s + 1]) (the CSR contract; clamped to [0, entries]), or with offsets
+ * NULL the entry s (samples == entries).  Over the rows of a sample and a group
+ * of C / groups neighbouring channels
+ *   h = (x - mean) / sqrt(var + eps),  z = h scale + bias,
+ *   y = z, or z sigmoid(z) if silu != 0
+ * with var the mean squared deviation; statistics in float32 or wider.
+ * scale, bias: float[C] or NULL; mean, rstd[samples, groups] are kept for the
+ * backward.  Rows of no sample get y = 0.  C <=
+ * DPA4K_GROUP_NORM_MAX_CHANNELS; eps finite and > 0.  Tensors may start at any
+ * element. */
+#define DPA4K_GROUP_NORM_MAX_CHANNELS 4096
+size_t dpa4k_group_norm_workspace_size(int64_t samples, int64_t entries,
+                                       int64_t inner, int64_t channels,
+                                       int64_t groups, int type, int backward);
+int dpa4k_group_norm_forward(const void* x, const float* scale,
+                             const float* bias, const int64_t* offsets, void* y,
+                             float* mean, float* rstd, int64_t samples,
+                             int64_t entries, int64_t inner, int64_t channels,
+                             int64_t groups, float eps, int silu, int type,
+                             void* workspace, size_t workspace_bytes,
+                             dpa4k_stream_t stream);
+
+/* dz = grad act'(z), u = dz scale:
+ *   grad_x = (u - mean(u) - h mean(u h)) / sqrt(var + eps)
+ *   grad_scale[c] = sum dz h,  grad_bias[c] = sum dz  over all rows
+ * grad, grad_x like x; any output may be NULL.  Rows of no sample get grad_x =
+ * 0 and count in no sum. */
+int dpa4k_group_norm_backward(const void* grad, const void* x,
+                              const float* scale, const float* bias,
+                              const int64_t* offsets, const float* mean,
+                              const float* rstd, void* grad_x,
+                              float* grad_scale, float* grad_bias,
+                              int64_t samples, int64_t entries, int64_t inner,
+                              int64_t channels, int64_t groups, int silu,
+                              int type, void* workspace,
+                              size_t workspace_bytes, dpa4k_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Optimiser step (no reference counterpart)
+ * ---------------------------------------------------------------------- */
+
+/* norm = sqrt(sum of g^2) over every gradient, summed in 64 bits in a fixed
+ * order; factor = min(1, max_norm / (norm + 1e-6)), 1 where max_norm <= 0, and
+ * NaN where the norm is not a finite float.  `grads`, `counts` and `types`
+ * (DPA4K_TYPE_F32 or _BF16) are host arrays of n_tensors entries, `grads` of
+ * device pointers at any element alignment; norm and factor are device floats.
+ * The workspace query reads counts on the host. */
+size_t dpa4k_grad_norm_workspace_size(const int64_t* counts, int64_t n_tensors);
+int dpa4k_grad_norm(const void* const* grads, const int64_t* counts,
+                    const int32_t* types, int64_t n_tensors, double max_norm,
+                    float* norm, float* factor, void* workspace,
+                    size_t workspace_bytes, dpa4k_stream_t stream);
+
+/* One tensor of an AdamW plan; device pointers.  With moments in 32 bits
+ * exp_avg and exp_avg_sq are float[count] and the scales NULL.  With moments in
+ * 8 bits they are codes, one byte per element of `count` rounded up to a
+ * multiple of 32 and 4-byte aligned, and the scales one byte per 32 elements
+ * (at least 16 and 32); codes of 0 stand for moments of 0. */
+typedef struct {
+  void* param;
+  void* exp_avg;
+  void* exp_avg_sq;
+  uint8_t* exp_avg_scale;
+  uint8_t* exp_avg_sq_scale;
+  int64_t count;
+  int64_t step; /* steps taken so far */
+} dpa4k_adamw_tensor;
+
+/* Writes the plan of `tensors` (a host array) to host memory; the caller copies
+ * it to the device (256-byte aligned) once.  *n_chunks (host) is handed to the
+ * calls below.  The plan holds each tensor's count of steps, a 64-bit word at
+ * byte DPA4K_ADAMW_STEP_OFFSET of its DPA4K_ADAMW_RECORD_BYTES.  No device call. */
+#define DPA4K_ADAMW_RECORD_BYTES 128
+#define DPA4K_ADAMW_STEP_OFFSET 56
+size_t dpa4k_adamw_plan_size(const int64_t* counts, int64_t n_tensors);
+int dpa4k_adamw_plan(const dpa4k_adamw_tensor* tensors, int64_t n_tensors,
+                     int state_bits, void* plan_host, size_t bytes,
+                     int64_t* n_chunks);
+
+/* One step over every tensor of a device plan, in place:
+ *   g' = g * factor,  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * every operation rounded to float32.  `grads`: host array of n_tensors device
+ * pointers; a NULL entry leaves its tensor, moments and step count as they are.
+ * lr_device (a device float, or NULL) replaces lr; grad_factor (a device float,
+ * or NULL for 1): a NaN takes no step at all.  bfloat16 parameters and 8-bit
+ * moments are rounded stochastically with bits drawn from (seed, t, position).
+ * Calls that share a plan, its tensors or its moments must not overlap. */
+int dpa4k_adamw_step(void* plan, int64_t n_tensors, int64_t n_chunks,
+                     int state_bits, int param_type, int grad_type,
+                     const void* const* grads, double lr,
+                     const float* lr_device, double beta1, double beta2,
+                     double eps, double weight_decay, const float* grad_factor,
+                     uint64_t seed, dpa4k_stream_t stream);
+
+/* The 8-bit moments of a plan as float32 values, and values rounded to the
+ * nearest codes.  Host arrays of n_tensors device pointers, float[count] each. */
+int dpa4k_adamw_read_states(void* plan, int64_t n_tensors, int64_t n_chunks,
+                            float* const* exp_avgs, float* const* exp_avg_sqs,
+                            dpa4k_stream_t stream);
+int dpa4k_adamw_write_states(void* plan, int64_t n_tensors, int64_t n_chunks,
+                             const float* const* exp_avgs,
+                             const float* const* exp_avg_sqs,
+                             dpa4k_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Stream calibration (measurement aid; no reference counterpart)
