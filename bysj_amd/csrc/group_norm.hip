@@ -9,16 +9,23 @@
 //   dz = dy act'(z),  dbias = sum dz,  dscale = sum dz h,  u = dz scale
 //   dx = rstd (u - mean(u) - h mean(u h))
 //
-// Samples are ragged (CSR offsets) or of equal length, from no row to all of
-// them, so the rows are cut into tiles of equal length whatever the samples: a
-// workgroup per tile, which walks the pieces of samples in it.  A piece leaves
-// its sums in slot (tile + sample), which is different for every piece since
-// one of the two grows from piece to piece; a sample's slots are consecutive.
+// Bound by its streams.  Two schedules:
 //
-// A tile is read as one run of vectors.  Vector q of a run holds the channels
-// (q V + j) mod C, so a stride of a multiple of lcm(C, V) elements keeps each
-// thread on the same V channels at any width C: no access is scalar but in the
-// ragged last vector of a piece.
+//  - direct: a workgroup of 64 to 1,024 threads per sample holds the sample in
+//    registers between its statistics and its output, one launch and one read.
+//  - tiles: samples too long for that (or of unknown length) are cut, whatever
+//    their lengths, by tiles of equal rows, a workgroup per tile that walks the
+//    pieces of samples in it.  A piece leaves its sums in slot (tile + sample),
+//    a number no other piece has, since from piece to piece one of the two
+//    grows; a sample's slots are consecutive.  A small launch merges them, a
+//    third writes the output, with the tiles in reverse order: what was read
+//    last is still in the memory-side cache.
+//
+// A sample, or a piece, is read as one run of 16-byte vectors.  Vector q of a
+// run holds the channels (q V + j) mod C, so with a stride of a multiple of
+// lcm(C, V) elements a thread stays on the same V channels at any width C, and
+// no access is scalar but in the ragged last vector of a run.  Where V divides
+// D (kUniform) a vector lies in one group and runs have no ragged vector.
 #include <cmath>
 
 #include "common.h"
@@ -26,16 +33,18 @@
 namespace dpa4k {
 namespace {
 
-constexpr int kBlock = 512;
+constexpr int kTileBlock = 256;
 constexpr int kMaxChannels = DPA4K_GROUP_NORM_MAX_CHANNELS;
-constexpr int64_t kTileBytes = 32768;   // least bytes of a tile
-constexpr int64_t kTiles = 1024;        // most tiles, where they are larger than that: 4 workgroups per CU
+constexpr int64_t kTileBytes = 16384;   // least bytes of a tile
+constexpr int64_t kTiles = 1024;        // most tiles where they are larger than that: 4 workgroups per CU
+constexpr int kLdsGroups = 1024;        // groups of a direct workgroup, whose statistics are kept in LDS
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Shape {
   int64_t samples, entries, inner;   // a sample owns entries, an entry `inner` rows
   int channels, groups;
   int64_t tile_rows, tiles;
+  int64_t long_rows;                 // samples of more rows than this take tiles
   const int64_t* offsets;            // null: sample s is entry s
 };
 
@@ -50,6 +59,8 @@ template <typename T>
 struct vector_of {
   typedef T type __attribute__((ext_vector_type(kVec<T>), aligned(sizeof(T))));
 };
+template <typename T>
+using Raw = typename vector_of<T>::type;
 
 template <typename T>
 struct Values {
@@ -57,12 +68,21 @@ struct Values {
 };
 
 template <typename T>
-__device__ __forceinline__ Values<T> load_whole(const T* __restrict__ p) {
-  const auto raw = *reinterpret_cast<const typename vector_of<T>::type*>(p);
+__device__ __forceinline__ Values<T> to_values(const Raw<T>& raw) {
   Values<T> out;
 #pragma unroll
   for (int j = 0; j < kVec<T>; ++j) out.v[j] = static_cast<float>(raw[j]);
   return out;
+}
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* __restrict__ p) {
+  return *reinterpret_cast<const Raw<T>*>(p);
+}
+
+template <typename T>
+__device__ __forceinline__ Values<T> load_whole(const T* __restrict__ p) {
+  return to_values<T>(load_raw(p));
 }
 
 // The first `live` elements, zeros behind them.
@@ -76,10 +96,10 @@ __device__ __forceinline__ Values<T> load_part(const T* __restrict__ p, int live
 
 template <typename T>
 __device__ __forceinline__ void store_whole(T* __restrict__ p, const Values<T>& value) {
-  typename vector_of<T>::type raw;
+  Raw<T> raw;
 #pragma unroll
   for (int j = 0; j < kVec<T>; ++j) raw[j] = static_cast<T>(value.v[j]);
-  *reinterpret_cast<typename vector_of<T>::type*>(p) = raw;
+  __builtin_nontemporal_store(raw, reinterpret_cast<Raw<T>*>(p));
 }
 
 template <typename T>
@@ -91,6 +111,16 @@ __device__ __forceinline__ void store_part(T* __restrict__ p, const Values<T>& v
 
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
+}
+
+__device__ __forceinline__ float activated(float z, bool silu) { return silu ? z * sigmoid(z) : z; }
+
+// grad act'(z) at z = h weight + shift.
+__device__ __forceinline__ float through_activation(float grad, float h, float weight, float shift, bool silu) {
+  if (!silu) return grad;
+  const float z = fmaf(h, weight, shift);
+  const float gate = sigmoid(z);
+  return grad * (gate * fmaf(z, 1.0f - gate, 1.0f));
 }
 
 // ---------------------------------------------------------------------------
@@ -108,11 +138,11 @@ struct Columns {
 int gcd_of(int a, int b) { return b == 0 ? a : gcd_of(b, a % b); }
 
 template <typename T>
-Columns columns_for(int channels) {
+Columns columns_for(int channels, int block) {
   Columns c;
   c.period_vectors = channels / gcd_of(channels, kVec<T>);
-  c.copies = c.period_vectors < kBlock ? kBlock / c.period_vectors : 1;
-  c.passes = (c.period_vectors + kBlock - 1) / kBlock;
+  c.copies = c.period_vectors < block ? block / c.period_vectors : 1;
+  c.passes = (c.period_vectors + block - 1) / block;
   return c;
 }
 
@@ -123,23 +153,57 @@ struct Share {
   int first, channel;
 };
 
-template <typename T>
+template <typename T, int BLOCK>
 __device__ __forceinline__ Share share_of(const Columns& columns, int pass, int channels) {
   Share s;
-  s.first = pass * kBlock + static_cast<int>(threadIdx.x);
-  s.live = s.first < (columns.copies > 1 ? columns.stride_vectors() : columns.period_vectors);
-  s.channel = static_cast<int>(static_cast<int64_t>(s.first) * kVec<T> % channels);
+  s.first = pass * BLOCK + static_cast<int>(threadIdx.x);
+  s.live = s.first < columns.stride_vectors();
+  s.channel = static_cast<int>(static_cast<uint32_t>(s.first) * kVec<T> % static_cast<uint32_t>(channels));
   return s;
 }
 
-__device__ __forceinline__ int channel_at(const Share& s, int j, int channels) {
-  int c = s.channel + j;
-  while (c >= channels) c -= channels;  // at most V / C times
-  return c;
+// Whether the ragged vector behind the `whole` ones is this thread's.
+__device__ __forceinline__ bool owns(const Share& share, int64_t whole, int stride) {
+  return share.live && whole >= share.first && (whole - share.first) % stride == 0;
+}
+
+// Scale, bias and group of a thread's channels.
+template <typename T, bool kUniform>
+struct Channels {
+  static constexpr int V = kVec<T>;
+  float weight[V], shift[V];
+  int group[kUniform ? 1 : V];
+  __device__ __forceinline__ Channels(const Share& share, const float* __restrict__ scale,
+                                      const float* __restrict__ bias, int channels, int width) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      int c = share.channel + j;
+      while (c >= channels) c -= channels;  // at most V / C times
+      if (!kUniform || j == 0) group[kUniform ? 0 : j] = c / width;
+      weight[j] = scale != nullptr ? scale[c] : 1.0f;
+      shift[j] = bias != nullptr ? bias[c] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ int group_of(int j) const { return group[kUniform ? 0 : j]; }
+};
+
+// A value per channel of a thread, one where its channels share a group.
+template <typename T, bool kUniform>
+struct PerGroup {
+  float v[kUniform ? 1 : kVec<T>];
+  __device__ __forceinline__ float at(int j) const { return v[kUniform ? 0 : j]; }
+};
+
+template <typename T, bool kUniform>
+__device__ __forceinline__ PerGroup<T, kUniform> per_group(const float* values, const Channels<T, kUniform>& channels) {
+  PerGroup<T, kUniform> out;
+#pragma unroll
+  for (int j = 0; j < (kUniform ? 1 : kVec<T>); ++j) out.v[j] = values[channels.group_of(j)];
+  return out;
 }
 
 // ---------------------------------------------------------------------------
-// samples in a tile
+// samples
 // ---------------------------------------------------------------------------
 
 __device__ __forceinline__ int64_t clamped_offset(const Shape& s, int64_t sample) {
@@ -148,537 +212,953 @@ __device__ __forceinline__ int64_t clamped_offset(const Shape& s, int64_t sample
   return o < 0 ? 0 : (o > s.entries ? s.entries : o);
 }
 
-// The last sample that starts at or before `entry`, -1 where none does.
+// The last sample that starts at or before `entry`, -1 where none does: 64
+// places of the offsets at a time.  Wave-uniform.
 __device__ __forceinline__ int64_t sample_at(const Shape& s, int64_t entry) {
   if (s.offsets == nullptr) return entry < s.samples ? entry : s.samples - 1;
-  int64_t low = -1, high = s.samples - 1;
-  while (low < high) {
-    const int64_t middle = low + ((high - low + 1) >> 1);
-    if (s.offsets[middle] <= entry) low = middle;
-    else high = middle - 1;
+  const int lane = threadIdx.x & 63;
+  int64_t base = 0, left = s.samples;
+  while (left > 0) {
+    const int64_t step = (left + 63) >> 6;
+    const int64_t at = lane * step;
+    const bool before = at < left && s.offsets[base + at] <= entry;
+    const int count = __popcll(__ballot(before));
+    if (count == 0) break;
+    const int64_t skip = (count - 1) * step + 1;
+    left = step - 1 < left - skip ? step - 1 : left - skip;
+    base += skip;
   }
-  return low;
+  return base - 1;
 }
 
-// Calls piece(sample, first row, last row) for every sample with rows in the
-// tile, in order; wave-uniform.
+// Calls piece(sample, first row, last row) for every long sample with rows in
+// the tile, in order; wave-uniform.  Short samples are passed over 64 at a time.
 template <typename Piece>
 __device__ __forceinline__ void each_piece(const Shape& s, int64_t tile, Piece piece) {
   const int64_t begin = tile * s.tile_rows;
   const int64_t rows = s.entries * s.inner;
   const int64_t end = begin + s.tile_rows < rows ? begin + s.tile_rows : rows;
-  int64_t sample = sample_at(s, begin / s.inner);
-  if (sample < 0) sample = 0;
-  for (; sample < s.samples; ++sample) {
-    const int64_t first = clamped_offset(s, sample) * s.inner;
-    if (first >= end) break;
-    const int64_t last = clamped_offset(s, sample + 1) * s.inner;
-    const int64_t a = uniform_i64(first > begin ? first : begin);
-    const int64_t b = uniform_i64(last < end ? last : end);
-    if (a < b) piece(uniform_i64(sample), a, b);
+  const int lane = threadIdx.x & 63;
+  int64_t base = s.samples <= 64 ? 0 : sample_at(s, begin / s.inner);
+  if (base < 0) base = 0;
+  for (;; base += 64) {
+    const int64_t sample = base + lane;
+    const bool in = sample < s.samples;
+    const int64_t first = in ? clamped_offset(s, sample) * s.inner : end;
+    const int64_t last = in ? clamped_offset(s, sample + 1) * s.inner : end;
+    const bool stop = first >= end;
+    const uint64_t stops = __ballot(stop);
+    uint64_t hits = __ballot(!stop && last > begin && last - first > s.long_rows);
+    if (stops != 0) hits &= (stops & (~stops + 1)) - 1;
+    while (hits != 0) {
+      const int b = __builtin_ctzll(hits);
+      hits &= hits - 1;
+      const int64_t f = uniform_lane_i64(first, b), l = uniform_lane_i64(last, b);
+      piece(uniform_i64(base + b), f > begin ? f : begin, l < end ? l : end);
+    }
+    if (stops != 0) return;
   }
 }
 
-// ---------------------------------------------------------------------------
-// sums of a workgroup by group of channels
-// ---------------------------------------------------------------------------
-
-// Lanes that add one group's `entries` terms, a power of two.
-__device__ __forceinline__ int lanes_for(int entries) {
-  int lanes = 1;
-  while (lanes < 64 && lanes < entries) lanes <<= 1;
-  return lanes;
+// Rows [begin, end) that belong to no sample (before the first offset, behind the last).
+template <typename T, int BLOCK>
+__device__ __forceinline__ void zero_outside(T* __restrict__ out, const Shape& s, int64_t begin, int64_t end) {
+  if (s.offsets == nullptr) return;
+  const int64_t first = s.samples > 0 ? clamped_offset(s, 0) * s.inner : end;
+  const int64_t last = s.samples > 0 ? clamped_offset(s, s.samples) * s.inner : end;
+  const int64_t head = (first < end ? first : end) * s.channels;
+  int64_t tail = last > begin ? last : begin;
+  if (tail < (first < end ? first : end)) tail = first < end ? first : end;
+  for (int64_t i = begin * s.channels + threadIdx.x; i < head; i += BLOCK) out[i] = static_cast<T>(0.0f);
+  for (int64_t i = tail * s.channels + threadIdx.x; i < end * s.channels; i += BLOCK) out[i] = static_cast<T>(0.0f);
 }
 
-__device__ __forceinline__ double lanes_sum(double value, int lanes) {
+// ---------------------------------------------------------------------------
+// a workgroup's terms by group of channels
+// ---------------------------------------------------------------------------
+//
+// The threads put their terms into LDS, one per vector (kUniform) or one per
+// element, as rows of W units per period row; group g owns the units [g dw,
+// (g + 1) dw) of each.  `lanes` lanes (a power of two) add a group's terms.
+struct Units {
+  int row, per_group, origin, held, first_row, terms, lanes;
+};
+
+template <int BLOCK, int V, bool kUniform>
+__device__ __forceinline__ Units units_of(const Columns& columns, int pass, int channels, int groups) {
+  Units u;
+  u.row = kUniform ? channels / V : channels;
+  u.per_group = u.row / groups;
+  constexpr int kPer = kUniform ? 1 : V;
+  u.origin = pass * BLOCK * kPer;
+  const int span = columns.stride_vectors() * kPer - u.origin;
+  u.held = span < BLOCK * kPer ? span : BLOCK * kPer;
+  u.first_row = u.origin / u.row;
+  const int last_row = (u.origin + u.held - 1) / u.row;
+  u.terms = u.per_group * (last_row - u.first_row + 1);
+  const int share = BLOCK / groups;  // threads per group, if each has some
+  u.lanes = 1;
+  while (u.lanes < 64 && u.lanes < u.terms && 2 * u.lanes <= share) u.lanes <<= 1;
+  return u;
+}
+
+// Calls term(place) for the terms lane, lane + lanes, ... of group g.
+template <typename Term>
+__device__ __forceinline__ void each_term(const Units& u, int g, int lane, Term term) {
+  const int rows = u.lanes / u.per_group, columns = u.lanes - rows * u.per_group;  // one step
+  int row = lane / u.per_group;
+  int column = lane - row * u.per_group;
+  for (int i = lane; i < u.terms; i += u.lanes) {
+    const int e = (u.first_row + row) * u.row + g * u.per_group + column - u.origin;
+    if (e >= 0 && e < u.held) term(e);
+    row += rows;
+    column += columns;
+    if (column >= u.per_group) {
+      column -= u.per_group;
+      ++row;
+    }
+  }
+}
+
+template <typename F>
+__device__ __forceinline__ F lanes_sum(F value, int lanes) {
   for (int mask = 1; mask < lanes; mask <<= 1) value += __shfl_xor(value, mask);
   return value;
 }
 
 // ---------------------------------------------------------------------------
-// forward: moments of each piece
+// moments
 // ---------------------------------------------------------------------------
 //
-// A thread merges batches of kBatch vectors into a running mean and sum of
-// squared deviations per channel: the batch's own mean is taken off first, so
-// neither a mean far from 0 nor a long sample costs digits.  The threads' pairs
-// meet in LDS and are merged per group in 64 bits.
-constexpr int kBatch = 4;
+// A thread merges batches into a running mean and sum of squared deviations:
+// the batch's own mean is taken off first, so neither a mean far from 0 nor a
+// long sum costs digits.  The threads' pairs meet in LDS and are merged per
+// group relative to the first of them, in float32; slots and what follows in 64 bits.
+template <typename T>
+constexpr int kBatch = 32 / kVec<T>;  // vectors in flight: 32 elements
 
-struct Moments {
-  double count, mean, squares;
-};
-
-__device__ __forceinline__ Moments merged(const Moments& a, const Moments& b) {
-  const double count = a.count + b.count;
-  if (count == 0.0) return a;
-  const double delta = b.mean - a.mean;
-  const double share = b.count / count;
-  return {count, a.mean + delta * share, a.squares + b.squares + delta * delta * a.count * share};
+// Vectors of a thread's share in [q, whole), at most K; where to load the k-th:
+// places past the run repeat its last vector, so that no load sits in a branch.
+template <int K>
+__device__ __forceinline__ int in_reach(int64_t q, int64_t whole, int stride) {
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) n += q + static_cast<int64_t>(k) * stride < whole ? 1 : 0;
+  return n;
+}
+__device__ __forceinline__ int64_t place_of(int64_t q, int k, int stride, int64_t whole) {
+  const int64_t at = q + static_cast<int64_t>(k) * stride;
+  return at < whole ? at : whole - 1;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kBlock) void group_norm_moments_kernel(const T* __restrict__ x, Shape s, Columns columns,
-                                                                    Moments* __restrict__ slots) {
-  constexpr int V = kVec<T>;
-  __shared__ float thread_mean[kBlock * V], thread_squares[kBlock * V];
-  __shared__ int thread_count[kBlock];
+template <typename T, bool kUniform>
+struct Running {
+  static constexpr int V = kVec<T>, N = kUniform ? 1 : V;
+  int count = 0, left = 0;  // vectors, and elements of a last part: element j has count + (j < left) terms
+  float mean[N], squares[N];
+  __device__ __forceinline__ Running() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) mean[i] = squares[i] = 0.0f;
+  }
+  // The first `n` of the vectors, n > 0.
+  template <int K, bool kAll>
+  __device__ __forceinline__ void add(const Raw<T> (&batch)[K], int n) {
+    count += kAll ? K : n;
+    const float share = 1.0f / static_cast<float>((kAll ? K : n) * (kUniform ? V : 1));
+    const float weight = static_cast<float>(kAll ? K : n) / static_cast<float>(count);
+    const float cross = static_cast<float>(count - (kAll ? K : n)) * weight * (kUniform ? V : 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < (kUniform ? V : 1); ++j) {
+          const float value = static_cast<float>(batch[k][kUniform ? j : i]);
+          sum += kAll || k < n ? value : 0.0f;
+        }
+      const float own = sum * share;
+      float spread = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < (kUniform ? V : 1); ++j) {
+          const float d = static_cast<float>(batch[k][kUniform ? j : i]) - own;
+          const float kept = kAll || k < n ? d : 0.0f;
+          spread = fmaf(kept, kept, spread);
+        }
+      const float delta = own - mean[i];
+      mean[i] = fmaf(delta, weight, mean[i]);
+      squares[i] += fmaf(delta * delta, cross, spread);
+    }
+  }
+  // The elements behind the last whole vector: one more for some channels.
+  __device__ __forceinline__ void add_part(const Values<T>& part, int live) {
+    left = live;
+    const float weight = 1.0f / static_cast<float>(count + 1);
+    const float cross = static_cast<float>(count) * weight;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < live) {
+        const float delta = part.v[i] - mean[i];
+        mean[i] = fmaf(delta, weight, mean[i]);
+        squares[i] = fmaf(delta * delta, cross, squares[i]);
+      }
+  }
+  __device__ __forceinline__ void add_run(const T* __restrict__ run, int64_t elements, const Share& share, int stride) {
+    if (!share.live) return;
+    const int64_t whole = elements / V;
+    int64_t q = share.first;
+    for (; q < whole; q += static_cast<int64_t>(kBatch<T>) * stride) {
+      Raw<T> batch[kBatch<T>];
+#pragma unroll
+      for (int k = 0; k < kBatch<T>; ++k) batch[k] = load_raw(run + place_of(q, k, stride, whole) * V);
+      const int n = in_reach<kBatch<T>>(q, whole, stride);
+      if (n == kBatch<T>) add<kBatch<T>, true>(batch, n);
+      else add<kBatch<T>, false>(batch, n);
+    }
+    if constexpr (!kUniform) {
+      const int part = static_cast<int>(elements - whole * V);
+      if (part > 0 && owns(share, whole, stride)) add_part(load_part(run + whole * V, part), part);
+    }
+  }
+};
+
+template <int BLOCK, int V, bool kUniform>
+struct MomentsLds {
+  float mean[BLOCK * (kUniform ? 1 : V)], squares[BLOCK * (kUniform ? 1 : V)];
+  int count[BLOCK];
+};
+
+// Calls emit(group, terms, mean, squares) in one lane for every group.
+template <int BLOCK, typename T, bool kUniform, typename Emit>
+__device__ __forceinline__ void merge_moments(const Running<T, kUniform>& mine, bool live,
+                                              MomentsLds<BLOCK, kVec<T>, kUniform>& lds, const Units& u, int groups,
+                                              Emit emit) {
+  constexpr int V = kVec<T>, N = kUniform ? 1 : V;
+  if (live) {
+    lds.count[threadIdx.x] = kUniform ? mine.count * V : mine.count * V + mine.left;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      lds.mean[threadIdx.x * N + i] = mine.mean[i];
+      lds.squares[threadIdx.x * N + i] = mine.squares[i];
+    }
+  }
+  __syncthreads();
+  const auto count_of = [&](int e) {
+    if (kUniform) return static_cast<float>(lds.count[e]);
+    const int packed = lds.count[e / V];
+    return static_cast<float>(packed / V + (e % V < packed % V ? 1 : 0));
+  };
+  const int lane = threadIdx.x & (u.lanes - 1);
+  const int per_round = BLOCK / u.lanes;
+  for (int g = static_cast<int>(threadIdx.x) / u.lanes; g < (groups + per_round - 1) / per_round * per_round; g += per_round) {
+    const bool in = g < groups;
+    const int start = u.first_row * u.row + (in ? g : 0) * u.per_group - u.origin;
+    const float pivot = lds.mean[start >= 0 && start < u.held ? start : 0];
+    float total = 0.0f, sum = 0.0f, spread = 0.0f;
+    if (in)
+      each_term(u, g, lane, [&](int e) {
+        const float n = count_of(e);
+        total += n;
+        if (n > 0.0f) sum = fmaf(n, lds.mean[e] - pivot, sum);
+      });
+    total = lanes_sum(total, u.lanes);
+    sum = lanes_sum(sum, u.lanes);
+    const float centre = total > 0.0f ? sum / total : 0.0f;
+    if (in)
+      each_term(u, g, lane, [&](int e) {
+        const float n = count_of(e);
+        const float delta = (lds.mean[e] - pivot) - centre;
+        if (n > 0.0f) spread += fmaf(n * delta, delta, lds.squares[e]);
+      });
+    spread = lanes_sum(spread, u.lanes);
+    if (lane == 0 && in) emit(g, total, pivot + centre, spread);
+  }
+}
+
+struct Slot {
+  float count, mean, squares;
+};
+
+__device__ __forceinline__ float inverse_root(double squares, double count, float eps) {
+  return static_cast<float>(1.0 / sqrt(squares / count + static_cast<double>(eps)));
+}
+
+// Merges `n` slots, `stride` apart, over `lanes` lanes: (count, mean, squares)
+// in every lane.  One sweep: deviations from the first slot's mean, in 64 bits.
+struct Merged {
+  double count, mean, squares;
+};
+__device__ __forceinline__ Merged merge_slots(const Slot* __restrict__ slots, int64_t n, int64_t stride, int lane, int lanes) {
+  constexpr int U = 8;  // loads in flight
+  const double pivot = n > 0 ? slots[0].mean : 0.0;
+  double total = 0.0, sum = 0.0, spread = 0.0;
+  for (int64_t i = lane; i < n; i += U * lanes) {
+    Slot s[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t at = i + k * lanes;
+      s[k] = slots[(at < n ? at : i) * stride];
+      if (at >= n) s[k].count = 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (!(s[k].count > 0.0f)) continue;
+      const double delta = s[k].mean - pivot, weighed = s[k].count * delta;
+      total += s[k].count;
+      sum += weighed;
+      spread += fma(weighed, delta, static_cast<double>(s[k].squares));
+    }
+  }
+  total = lanes_sum(total, lanes);
+  sum = lanes_sum(sum, lanes);
+  spread = lanes_sum(spread, lanes);
+  const double centre = total > 0.0 ? sum / total : 0.0;
+  const double squares = fma(-sum, centre, spread);
+  return {total, pivot + centre, squares < 0.0 ? 0.0 : squares};
+}
+
+// ---------------------------------------------------------------------------
+// tiles, forward
+// ---------------------------------------------------------------------------
+
+template <typename T, bool kUniform>
+__global__ __launch_bounds__(kTileBlock) void group_norm_moments_kernel(const T* __restrict__ x, Shape s, Columns columns,
+                                                                        Slot* __restrict__ slots) {
+  __shared__ MomentsLds<kTileBlock, kVec<T>, kUniform> lds;
   const int64_t tile = block_index();
   if (tile >= s.tiles) return;
-  const int C = s.channels, D = C / s.groups;
   each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
-    const T* run = x + a * C;
-    const int64_t elements = (b - a) * C;
-    const int64_t whole = elements / V;
-    Moments* out = slots + (tile + sample) * s.groups;
+    Slot* out = slots + (tile + sample) * columns.passes * s.groups;
     for (int pass = 0; pass < columns.passes; ++pass) {
-      const Share share = share_of<T>(columns, pass, C);
-      float mean[V], squares[V];
-      int count = 0;
-#pragma unroll
-      for (int j = 0; j < V; ++j) mean[j] = squares[j] = 0.0f;
-      const int64_t stride = columns.stride_vectors();
-      if (share.live) {
-        int64_t q = share.first;
-        for (; q + (kBatch - 1) * stride < whole; q += kBatch * stride) {
-          Values<T> batch[kBatch];
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k) batch[k] = load_whole(run + (q + k * stride) * V);
-          count += kBatch;
-          const float weight = static_cast<float>(kBatch) / static_cast<float>(count);
-          const float cross = static_cast<float>(count - kBatch) * weight;
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            float sum = batch[0].v[j];
-#pragma unroll
-            for (int k = 1; k < kBatch; ++k) sum += batch[k].v[j];
-            const float own = sum * (1.0f / kBatch);
-            float spread = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const float d = batch[k].v[j] - own;
-              spread = fmaf(d, d, spread);
-            }
-            const float delta = own - mean[j];
-            mean[j] = fmaf(delta, weight, mean[j]);
-            squares[j] = squares[j] + fmaf(delta * delta, cross, spread);
-          }
-        }
-        for (; q < whole; q += stride) {
-          const Values<T> value = load_whole(run + q * V);
-          ++count;
-          const float weight = 1.0f / static_cast<float>(count);
-          const float cross = static_cast<float>(count - 1) * weight;
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float delta = value.v[j] - mean[j];
-            mean[j] = fmaf(delta, weight, mean[j]);
-            squares[j] = fmaf(delta * delta, cross, squares[j]);
-          }
-        }
-        // the elements behind the last whole vector: one more for some channels
-        const int left = q == whole ? static_cast<int>(elements - whole * V) : 0;
-        if (left > 0) {
-          const Values<T> value = load_part(run + whole * V, left);
-          const float weight = 1.0f / static_cast<float>(count + 1);
-          const float cross = static_cast<float>(count) * weight;
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (j < left) {
-              const float delta = value.v[j] - mean[j];
-              mean[j] = fmaf(delta, weight, mean[j]);
-              squares[j] = fmaf(delta * delta, cross, squares[j]);
-            }
-        }
-        thread_count[threadIdx.x] = count * V + left;  // element j of a thread has count + (j < left) terms
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          thread_mean[threadIdx.x * V + j] = mean[j];
-          thread_squares[threadIdx.x * V + j] = squares[j];
-        }
-      }
-      __syncthreads();
-      // this pass holds the elements [origin, origin + held) of each period
-      const int origin = pass * kBlock * V;
-      const int span = columns.copies > 1 ? columns.stride_vectors() * V : columns.period_vectors * V;
-      const int held = span - origin < kBlock * V ? span - origin : kBlock * V;
-      const int first_row = origin / C, last_row = (origin + held - 1) / C;
-      const int terms = D * (last_row - first_row + 1);
-      const int lanes = lanes_for(terms);
-      const int lane = threadIdx.x & (lanes - 1);
-      for (int g = static_cast<int>(threadIdx.x) / lanes; g < (s.groups + kBlock / lanes - 1) / (kBlock / lanes) * (kBlock / lanes);
-           g += kBlock / lanes) {
-        double total = 0.0, sum = 0.0;
-        if (g < s.groups)
-          for (int i = lane; i < terms; i += lanes) {
-            const int e = (first_row + i / D) * C + g * D + i % D - origin;
-            if (e < 0 || e >= held) continue;
-            const int packed = thread_count[e / V];
-            const double n = packed / V + (e % V < packed % V ? 1 : 0);
-            total += n;
-            sum += n * thread_mean[e];
-          }
-        total = lanes_sum(total, lanes);
-        sum = lanes_sum(sum, lanes);
-        const double centre = total > 0.0 ? sum / total : 0.0;
-        double spread = 0.0;
-        if (g < s.groups)
-          for (int i = lane; i < terms; i += lanes) {
-            const int e = (first_row + i / D) * C + g * D + i % D - origin;
-            if (e < 0 || e >= held) continue;
-            const int packed = thread_count[e / V];
-            const double n = packed / V + (e % V < packed % V ? 1 : 0);
-            const double delta = thread_mean[e] - centre;
-            if (n > 0.0) spread += thread_squares[e] + n * delta * delta;
-          }
-        spread = lanes_sum(spread, lanes);
-        if (lane == 0 && g < s.groups) {
-          Moments mine = {total, centre, spread};
-          if (pass > 0) mine = merged(out[g], mine);
-          out[g] = mine;
-        }
-      }
+      const Share share = share_of<T, kTileBlock>(columns, pass, s.channels);
+      const Units u = units_of<kTileBlock, kVec<T>, kUniform>(columns, pass, s.channels, s.groups);
+      Running<T, kUniform> running;
+      running.add_run(x + a * s.channels, (b - a) * s.channels, share, columns.stride_vectors());
+      merge_moments<kTileBlock>(running, share.live, lds, u, s.groups, [&](int g, float count, float mean, float squares) {
+        out[pass * s.groups + g] = {count, mean, squares};
+      });
       __syncthreads();
     }
   });
 }
 
-// A wave per (sample, group): its slots in their order, in 64 bits.  A sample
-// without rows gets mean 0 and the rstd of variance 0; nothing reads them.
-__global__ __launch_bounds__(256) void group_norm_finish_kernel(const Moments* __restrict__ slots, Shape s, float eps,
-                                                                float* __restrict__ mean, float* __restrict__ rstd) {
-  const int64_t unit = block_index() * 4 + (threadIdx.x >> 6);
+// The slots of a sample's rows [first, last): where they start and how many.
+__device__ __forceinline__ int64_t slots_of(const Shape& s, int passes, int64_t sample, int64_t first, int64_t last,
+                                            int64_t& start) {
+  const int64_t tile = first / s.tile_rows;
+  start = (tile + sample) * passes;
+  return ((last - 1) / s.tile_rows - tile + 1) * passes;
+}
+
+// A wave per (sample, group) of the long samples.
+__global__ __launch_bounds__(256) void group_norm_finish_kernel(const Slot* __restrict__ slots, Shape s, int passes,
+                                                                float eps, float* __restrict__ mean,
+                                                                float* __restrict__ rstd) {
+  const int64_t unit = uniform_i64(block_index() * 4 + (threadIdx.x >> 6));
   if (unit >= s.samples * s.groups) return;
-  const int lane = threadIdx.x & 63;
   const int64_t sample = unit / s.groups;
   const int64_t first = clamped_offset(s, sample) * s.inner, last = clamped_offset(s, sample + 1) * s.inner;
-  Moments total = {0.0, 0.0, 0.0};
-  if (first < last) {
-    const int64_t begin = first / s.tile_rows, end = (last - 1) / s.tile_rows;
-    for (int64_t t = begin + lane; t <= end; t += 64) total = merged(total, slots[(t + sample) * s.groups + unit % s.groups]);
-  }
-#pragma unroll
-  for (int mask = 1; mask < 64; mask <<= 1) {
-    const Moments other = {__shfl_xor(total.count, mask), __shfl_xor(total.mean, mask), __shfl_xor(total.squares, mask)};
-    total = (lane & mask) == 0 ? merged(total, other) : merged(other, total);
-  }
+  const int lane = threadIdx.x & 63;
+  if (last - first <= s.long_rows) return;
+  int64_t start;
+  const int64_t n = slots_of(s, passes, sample, first, last, start);
+  const Merged m = merge_slots(slots + start * s.groups + unit % s.groups, n, s.groups, lane, 64);
   if (lane != 0) return;
-  mean[unit] = static_cast<float>(total.mean);
-  const double variance = total.count > 0.0 ? total.squares / total.count : 0.0;
-  rstd[unit] = static_cast<float>(1.0 / sqrt(variance + static_cast<double>(eps)));
+  mean[unit] = static_cast<float>(m.mean);
+  rstd[unit] = inverse_root(m.squares, m.count, eps);
 }
 
-// ---------------------------------------------------------------------------
-// forward: apply
-// ---------------------------------------------------------------------------
-
-// Rows of the tile that belong to no sample (before the first offset, behind the last).
-template <typename T>
-__device__ __forceinline__ void zero_outside(T* __restrict__ out, const Shape& s, int64_t tile) {
-  if (s.offsets == nullptr) return;
-  const int64_t begin = tile * s.tile_rows, rows = s.entries * s.inner;
-  const int64_t end = begin + s.tile_rows < rows ? begin + s.tile_rows : rows;
-  const int64_t first = s.samples > 0 ? clamped_offset(s, 0) * s.inner : rows;
-  const int64_t last = s.samples > 0 ? clamped_offset(s, s.samples) * s.inner : rows;
-  const int64_t head = (first < end ? first : end) * s.channels;
-  const int64_t tail = (last > begin ? last : begin) * s.channels;
-  for (int64_t i = begin * s.channels + threadIdx.x; i < head; i += kBlock) out[i] = static_cast<T>(0.0f);
-  for (int64_t i = tail + threadIdx.x; i < end * s.channels; i += kBlock) out[i] = static_cast<T>(0.0f);
-}
-
-template <typename T, bool kSilu>
-__global__ __launch_bounds__(kBlock) void group_norm_apply_kernel(const T* __restrict__ x, const float* __restrict__ scale,
-                                                                  const float* __restrict__ bias,
-                                                                  const float* __restrict__ mean,
-                                                                  const float* __restrict__ rstd, T* __restrict__ y,
-                                                                  Shape s, Columns columns) {
-  constexpr int V = kVec<T>;
-  const int64_t tile = block_index();
-  if (tile >= s.tiles) return;
-  const int C = s.channels, D = C / s.groups;
+// Merging a sample's slots again in every tile instead of in a launch of its
+// own was slower: 1,024 tiles on one sample of 100 MB took 60 us against 35 + 5.
+template <typename T, bool kUniform>
+__global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
+    const T* __restrict__ x, const float* __restrict__ scale, const float* __restrict__ bias, bool silu,
+    const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ y, Shape s, Columns columns) {
+  constexpr int V = kVec<T>, K = kBatch<T> / 2;
+  const int64_t block = block_index();
+  if (block >= s.tiles) return;
+  const int64_t tile = s.tiles - 1 - block;
+  const int C = s.channels, G = s.groups;
+  const int stride = columns.stride_vectors();
   for (int pass = 0; pass < columns.passes; ++pass) {
-    const Share share = share_of<T>(columns, pass, C);
-    if (!share.live) continue;
-    float weight[V], shift[V];
-    int group[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = channel_at(share, j, C);
-      group[j] = c / D;
-      weight[j] = scale != nullptr ? scale[c] : 1.0f;
-      shift[j] = bias != nullptr ? bias[c] : 0.0f;
-    }
+    const Share share = share_of<T, kTileBlock>(columns, pass, C);
+    const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
     each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
+      if (!share.live) return;
+      const int64_t elements = (b - a) * C;
+      const int64_t whole = elements / V;
       const T* run = x + a * C;
       T* out = y + a * C;
-      const int64_t elements = (b - a) * C;
-      const int64_t whole = elements / V;
-      float centre[V], inverse[V];
+      const PerGroup<T, kUniform> centre = per_group<T, kUniform>(mean + sample * G, channels);
+      const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(rstd + sample * G, channels);
+      float slope[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        centre[j] = mean[sample * s.groups + group[j]];
-        inverse[j] = rstd[sample * s.groups + group[j]];
-      }
+      for (int j = 0; j < V; ++j) slope[j] = inverse.at(j) * channels.weight[j];
       const auto normed = [&](Values<T> value) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float z = fmaf((value.v[j] - centre[j]) * inverse[j], weight[j], shift[j]);
-          value.v[j] = kSilu ? z * sigmoid(z) : z;
-        }
+        for (int j = 0; j < V; ++j)
+          value.v[j] = activated(fmaf(value.v[j] - centre.at(j), slope[j], channels.shift[j]), silu);
         return value;
       };
-      int64_t q = share.first;
-      for (; q < whole; q += columns.stride_vectors()) store_whole(out + q * V, normed(load_whole(run + q * V)));
-      const int left = static_cast<int>(elements - whole * V);
-      if (q == whole && left > 0) store_part(out + whole * V, normed(load_part(run + whole * V, left)), left);
+      for (int64_t q = share.first; q < whole; q += static_cast<int64_t>(K) * stride) {
+        Raw<T> raw[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) raw[k] = load_raw(run + place_of(q, k, stride, whole) * V);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (q + static_cast<int64_t>(k) * stride < whole)
+            store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
+      }
+      if constexpr (!kUniform) {
+        const int left = static_cast<int>(elements - whole * V);
+        if (left > 0 && owns(share, whole, stride))
+          store_part(out + whole * V, normed(load_part(run + whole * V, left)), left);
+      }
     });
   }
-  zero_outside(y, s, tile);
+  const int64_t begin = tile * s.tile_rows, rows = s.entries * s.inner;
+  zero_outside<T, kTileBlock>(y, s, begin, begin + s.tile_rows < rows ? begin + s.tile_rows : rows);
 }
 
 // ---------------------------------------------------------------------------
-// backward
+// direct, forward
+// ---------------------------------------------------------------------------
+//
+// TS threads hold 32 elements each of a sample.  A sample that is longer
+// (max_rows was too small) is streamed twice.  Blocks behind the samples write
+// the zeros of rows without a sample.
+template <typename T>
+constexpr int kHeld = 32 / kVec<T>;  // vectors
+
+// Statistics of one sample for the threads of a workgroup, by group.
+struct Statistics {
+  float mean[kLdsGroups], rstd[kLdsGroups];
+};
+
+template <typename T, bool kUniform, int TS>
+__global__ __launch_bounds__(TS) void group_norm_direct_kernel(
+    const T* __restrict__ x, const float* __restrict__ scale, const float* __restrict__ bias, float eps, bool silu,
+    float* __restrict__ mean, float* __restrict__ rstd, T* __restrict__ y, Shape s, Columns columns, int64_t zero_blocks) {
+  constexpr int V = kVec<T>;
+  __shared__ MomentsLds<TS, V, kUniform> lds;
+  __shared__ Statistics statistics;
+  const int C = s.channels, G = s.groups;
+  const int64_t sample = block_index();
+  if (sample >= s.samples) {
+    const int64_t part = sample - s.samples, rows = s.entries * s.inner;
+    if (part >= zero_blocks) return;
+    const int64_t each = (rows + zero_blocks - 1) / zero_blocks;
+    const int64_t begin = part * each < rows ? part * each : rows;
+    zero_outside<T, TS>(y, s, begin, begin + each < rows ? begin + each : rows);
+    return;
+  }
+  const int64_t first = clamped_offset(s, sample) * s.inner, last = clamped_offset(s, sample + 1) * s.inner;
+  if (first >= last || last - first > s.long_rows) return;
+  const int64_t elements = (last - first) * C;
+  const int64_t whole = elements / V;
+  const int left = kUniform ? 0 : static_cast<int>(elements - whole * V);
+  const T* run = x + first * C;
+  T* out = y + first * C;
+  const Share share = share_of<T, TS>(columns, 0, C);
+  const int stride = columns.stride_vectors();
+  const bool held = whole <= static_cast<int64_t>(stride) * kHeld<T>;
+  const bool tail = !kUniform && left > 0 && owns(share, whole, stride);
+  Running<T, kUniform> running;
+  Raw<T> raw[kHeld<T>];
+  int mine = 0;  // held vectors of this thread
+  if (held) {
+#pragma unroll
+    for (int k = 0; k < kHeld<T>; ++k)
+      if (static_cast<int64_t>(k) * stride < whole) {  // uniform: no thread has a vector k otherwise
+        const int64_t q = share.first + static_cast<int64_t>(k) * stride;
+        raw[k] = load_raw(run + (q < whole ? q : whole - 1) * V);
+        mine += share.live && q < whole ? 1 : 0;
+      }
+  }
+  const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+  if (held) {
+    if (mine > 0) running.template add<kHeld<T>, false>(raw, mine);
+    if (tail) running.add_part(load_part(run + whole * V, left), left);
+  } else {
+    running.add_run(run, elements, share, stride);
+  }
+  const Units u = units_of<TS, V, kUniform>(columns, 0, C, G);
+  merge_moments<TS>(running, share.live, lds, u, G, [&](int g, float count, float centre, float squares) {
+    statistics.mean[g] = centre;
+    statistics.rstd[g] = 1.0f / sqrtf(squares / count + eps);
+    mean[sample * G + g] = statistics.mean[g];
+    rstd[sample * G + g] = statistics.rstd[g];
+  });
+  __syncthreads();
+  if (!share.live) return;
+  const PerGroup<T, kUniform> centre = per_group<T, kUniform>(statistics.mean, channels);
+  const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(statistics.rstd, channels);
+  float slope[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) slope[j] = inverse.at(j) * channels.weight[j];
+  const auto normed = [&](Values<T> value) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) value.v[j] = activated(fmaf(value.v[j] - centre.at(j), slope[j], channels.shift[j]), silu);
+    return value;
+  };
+  if (held) {
+#pragma unroll
+    for (int k = 0; k < kHeld<T>; ++k)
+      if (k < mine) store_whole(out + (share.first + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
+  } else {
+    for (int64_t q = share.first; q < whole; q += stride) store_whole(out + q * V, normed(load_whole(run + q * V)));
+  }
+  if (tail) store_part(out + whole * V, normed(load_part(run + whole * V, left)), left);
+}
+
+// ---------------------------------------------------------------------------
+// backward: sums
 // ---------------------------------------------------------------------------
 
-// dz of one element, and h.
-template <bool kSilu>
-__device__ __forceinline__ float slope_times(float grad, float h, float weight, float shift) {
-  if constexpr (!kSilu) return grad;
-  const float z = fmaf(h, weight, shift);
-  const float gate = sigmoid(z);
-  return grad * (gate * fmaf(z, 1.0f - gate, 1.0f));
+// A thread's sums of dz and dz h per channel.
+template <typename T>
+struct Sums {
+  static constexpr int V = kVec<T>;
+  float z[V], zh[V];
+  __device__ __forceinline__ Sums() {
+#pragma unroll
+    for (int j = 0; j < V; ++j) z[j] = zh[j] = 0.0f;
+  }
+  template <bool kUniform>
+  __device__ __forceinline__ void add(const Values<T>& grad, const Values<T>& x, const Channels<T, kUniform>& channels,
+                                      const PerGroup<T, kUniform>& centre, const PerGroup<T, kUniform>& inverse, bool silu) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float h = (x.v[j] - centre.at(j)) * inverse.at(j);
+      const float dz = through_activation(grad.v[j], h, channels.weight[j], channels.shift[j], silu);
+      z[j] += dz;
+      zh[j] = fmaf(dz, h, zh[j]);
+    }
+  }
+  // The elements behind the last whole vector; the others add nothing.
+  __device__ __forceinline__ void add_part(const Values<T>& grad, const Values<T>& x, int live, const Channels<T, false>& channels,
+                                           const PerGroup<T, false>& centre, const PerGroup<T, false>& inverse, bool silu) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < live) {
+        const float h = (x.v[j] - centre.at(j)) * inverse.at(j);
+        const float dz = through_activation(grad.v[j], h, channels.weight[j], channels.shift[j], silu);
+        z[j] += dz;
+        zh[j] = fmaf(dz, h, zh[j]);
+      }
+  }
+  __device__ __forceinline__ void add(const Sums& other) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      z[j] += other.z[j];
+      zh[j] += other.zh[j];
+    }
+  }
+};
+
+// One term per unit in LDS, for two sums at once.
+template <int BLOCK, int V>
+struct SumsLds {
+  float a[BLOCK * V], b[BLOCK * V];
+};
+
+// Calls emit(group, sum u, sum u h) in one lane for every group.
+template <int BLOCK, typename T, bool kUniform, typename Emit>
+__device__ __forceinline__ void merge_sums(const Sums<T>& mine, const Channels<T, kUniform>& channels, bool live,
+                                           SumsLds<BLOCK, kVec<T>>& lds, const Units& u, int groups, Emit emit) {
+  constexpr int V = kVec<T>;
+  if (live) {
+    if constexpr (kUniform) {
+      float sum_u = 0.0f, sum_uh = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        sum_u = fmaf(mine.z[j], channels.weight[j], sum_u);
+        sum_uh = fmaf(mine.zh[j], channels.weight[j], sum_uh);
+      }
+      lds.a[threadIdx.x] = sum_u;
+      lds.b[threadIdx.x] = sum_uh;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        lds.a[threadIdx.x * V + j] = mine.z[j] * channels.weight[j];
+        lds.b[threadIdx.x * V + j] = mine.zh[j] * channels.weight[j];
+      }
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & (u.lanes - 1);
+  const int per_round = BLOCK / u.lanes;
+  for (int g = static_cast<int>(threadIdx.x) / u.lanes; g < (groups + per_round - 1) / per_round * per_round; g += per_round) {
+    float sum_u = 0.0f, sum_uh = 0.0f;
+    if (g < groups)
+      each_term(u, g, lane, [&](int e) {
+        sum_u += lds.a[e];
+        sum_uh += lds.b[e];
+      });
+    sum_u = lanes_sum(sum_u, u.lanes);
+    sum_uh = lanes_sum(sum_uh, u.lanes);
+    if (lane == 0 && g < groups) emit(g, sum_u, sum_uh);
+  }
 }
+
+// A workgroup's sums of dz and dz h per channel, over the threads that share
+// it; pass 0 writes `out`, later passes add to it (the same thread each time).
+template <int BLOCK, typename T>
+__device__ __forceinline__ void write_columns(const Sums<T>& mine, bool live, SumsLds<BLOCK, kVec<T>>& lds,
+                                              const Columns& columns, int pass, int channels, float2* __restrict__ out) {
+  constexpr int V = kVec<T>;
+  if (live)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      lds.a[threadIdx.x * V + j] = mine.z[j];
+      lds.b[threadIdx.x * V + j] = mine.zh[j];
+    }
+  __syncthreads();
+  const int origin = pass * BLOCK * V;
+  const int span = columns.stride_vectors() * V - origin;
+  const int held = span < BLOCK * V ? span : BLOCK * V;
+  for (int c = threadIdx.x; c < channels; c += BLOCK) {
+    float z = 0.0f, zh = 0.0f;
+    int e = c - origin % channels;
+    if (e < 0) e += channels;
+    for (; e < held; e += channels) {
+      z += lds.a[e];
+      zh += lds.b[e];
+    }
+    if (pass == 0) out[c] = {z, zh};
+    else out[c] = {out[c].x + z, out[c].y + zh};
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------
+// tiles, backward
+// ---------------------------------------------------------------------------
 
 // Per piece: sum u and sum u h of each group.  Per tile: sum dz and sum dz h of
-// each channel, over all its pieces (kept in registers across them; with more
-// than one pass, pass by pass).
-template <typename T, bool kSilu>
-__global__ __launch_bounds__(kBlock) void group_norm_sums_kernel(
+// each channel over all its pieces, kept in registers across them.
+template <typename T, bool kUniform>
+__global__ __launch_bounds__(kTileBlock) void group_norm_sums_kernel(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
-    const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd, Shape s,
-    Columns columns, double2* __restrict__ slots, float2* __restrict__ tile_sums) {
-  constexpr int V = kVec<T>;
-  __shared__ float thread_u[kBlock * V], thread_uh[kBlock * V];
+    const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd, bool silu, Shape s,
+    Columns columns, float2* __restrict__ slots, float2* __restrict__ column_sums) {
+  constexpr int V = kVec<T>, K = kBatch<T> / 2;
+  __shared__ SumsLds<kTileBlock, V> lds;
   const int64_t tile = block_index();
   if (tile >= s.tiles) return;
-  const int C = s.channels, D = C / s.groups;
+  const int C = s.channels, G = s.groups;
   for (int pass = 0; pass < columns.passes; ++pass) {
-    const Share share = share_of<T>(columns, pass, C);
-    const int origin = pass * kBlock * V;
-    const int span = columns.copies > 1 ? columns.stride_vectors() * V : columns.period_vectors * V;
-    const int held = span - origin < kBlock * V ? span - origin : kBlock * V;
-    float weight[V], shift[V], tile_z[V], tile_zh[V];
-    int group[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = channel_at(share, j, C);
-      group[j] = c / D;
-      weight[j] = scale != nullptr ? scale[c] : 1.0f;
-      shift[j] = bias != nullptr ? bias[c] : 0.0f;
-      tile_z[j] = tile_zh[j] = 0.0f;
-    }
+    const Share share = share_of<T, kTileBlock>(columns, pass, C);
+    const Units u = units_of<kTileBlock, V, kUniform>(columns, pass, C, G);
+    const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+    const int stride = columns.stride_vectors();
+    Sums<T> total;
     each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
       const int64_t elements = (b - a) * C;
       const int64_t whole = elements / V;
-      float sum_z[V], sum_zh[V], centre[V], inverse[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        sum_z[j] = sum_zh[j] = 0.0f;
-        centre[j] = mean[sample * s.groups + group[j]];
-        inverse[j] = rstd[sample * s.groups + group[j]];
-      }
-      const auto add = [&](const Values<T>& gv, const Values<T>& xv) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float h = (xv.v[j] - centre[j]) * inverse[j];
-          const float dz = slope_times<kSilu>(gv.v[j], h, weight[j], shift[j]);
-          sum_z[j] += dz;
-          sum_zh[j] = fmaf(dz, h, sum_zh[j]);
-        }
-      };
-      if (share.live) {
-        int64_t q = share.first;
-        for (; q < whole; q += columns.stride_vectors())
-          add(load_whole(grad + a * C + q * V), load_whole(x + a * C + q * V));
-        const int left = static_cast<int>(elements - whole * V);
-        if (q == whole && left > 0) {
-          // a gradient of 0 adds nothing, unless h is not finite
-          const Values<T> gv = load_part(grad + a * C + whole * V, left);
-          Values<T> xv = load_part(x + a * C + whole * V, left);
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (j >= left) xv.v[j] = centre[j];
-          add(gv, xv);
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          thread_u[threadIdx.x * V + j] = sum_z[j] * weight[j];
-          thread_uh[threadIdx.x * V + j] = sum_zh[j] * weight[j];
-          tile_z[j] += sum_z[j];
-          tile_zh[j] += sum_zh[j];
-        }
-      }
-      __syncthreads();
-      const int first_row = origin / C, last_row = (origin + held - 1) / C;
-      const int terms = D * (last_row - first_row + 1);
-      const int lanes = lanes_for(terms);
-      const int lane = threadIdx.x & (lanes - 1);
-      double2* out = slots + (tile + sample) * s.groups;
-      for (int g = static_cast<int>(threadIdx.x) / lanes; g < (s.groups + kBlock / lanes - 1) / (kBlock / lanes) * (kBlock / lanes);
-           g += kBlock / lanes) {
-        double u = 0.0, uh = 0.0;
-        if (g < s.groups)
-          for (int i = lane; i < terms; i += lanes) {
-            const int e = (first_row + i / D) * C + g * D + i % D - origin;
-            if (e < 0 || e >= held) continue;
-            u += thread_u[e];
-            uh += thread_uh[e];
-          }
-        u = lanes_sum(u, lanes);
-        uh = lanes_sum(uh, lanes);
-        if (lane == 0 && g < s.groups) {
-          if (pass > 0) {
-            u += out[g].x;
-            uh += out[g].y;
-          }
-          out[g] = {u, uh};
-        }
-      }
-      __syncthreads();
-    });
-    if (tile_sums == nullptr) continue;
-    if (share.live)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        thread_u[threadIdx.x * V + j] = tile_z[j];
-        thread_uh[threadIdx.x * V + j] = tile_zh[j];
-      }
-    __syncthreads();
-    for (int c = threadIdx.x; c < C; c += kBlock) {
-      float z = 0.0f, zh = 0.0f;
-      bool any = false;
-      for (int e = c - origin % C; e < held; e += C)
-        if (e >= 0) {
-          z += thread_u[e];
-          zh += thread_uh[e];
-          any = true;
-        }
-      float2* out = tile_sums + tile * C + c;
-      if (pass == 0) *out = {z, zh};
-      else if (any) *out = {out->x + z, out->y + zh};
-    }
-    __syncthreads();
-  }
-}
-
-// A wave per (sample, group): means of u and u h over its slots.
-__global__ __launch_bounds__(256) void group_norm_means_kernel(const double2* __restrict__ slots, Shape s,
-                                                               float2* __restrict__ means) {
-  const int64_t unit = block_index() * 4 + (threadIdx.x >> 6);
-  if (unit >= s.samples * s.groups) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t sample = unit / s.groups;
-  const int64_t first = clamped_offset(s, sample) * s.inner, last = clamped_offset(s, sample + 1) * s.inner;
-  double u = 0.0, uh = 0.0;
-  if (first < last) {
-    const int64_t begin = first / s.tile_rows, end = (last - 1) / s.tile_rows;
-    for (int64_t t = begin + lane; t <= end; t += 64) {
-      const double2 v = slots[(t + sample) * s.groups + unit % s.groups];
-      u += v.x;
-      uh += v.y;
-    }
-  }
-  u = group_sum<64>(u);
-  uh = group_sum<64>(uh);
-  const double count = static_cast<double>((last - first) * (s.channels / s.groups));
-  if (lane == 0 && first < last) means[unit] = {static_cast<float>(u / count), static_cast<float>(uh / count)};
-}
-
-template <typename T, bool kSilu>
-__global__ __launch_bounds__(kBlock) void group_norm_backward_kernel(
-    const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
-    const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd,
-    const float2* __restrict__ means, T* __restrict__ grad_x, Shape s, Columns columns) {
-  constexpr int V = kVec<T>;
-  const int64_t tile = block_index();
-  if (tile >= s.tiles) return;
-  const int C = s.channels, D = C / s.groups;
-  for (int pass = 0; pass < columns.passes; ++pass) {
-    const Share share = share_of<T>(columns, pass, C);
-    if (!share.live) continue;
-    float weight[V], shift[V];
-    int group[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = channel_at(share, j, C);
-      group[j] = c / D;
-      weight[j] = scale != nullptr ? scale[c] : 1.0f;
-      shift[j] = bias != nullptr ? bias[c] : 0.0f;
-    }
-    each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
-      const int64_t elements = (b - a) * C;
-      const int64_t whole = elements / V;
-      float centre[V], inverse[V], mean_u[V], mean_uh[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int64_t at = sample * s.groups + group[j];
-        centre[j] = mean[at];
-        inverse[j] = rstd[at];
-        mean_u[j] = means[at].x;
-        mean_uh[j] = means[at].y;
-      }
-      const auto gradient = [&](const Values<T>& gv, const Values<T>& xv) {
-        Values<T> out;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float h = (xv.v[j] - centre[j]) * inverse[j];
-          const float u = slope_times<kSilu>(gv.v[j], h, weight[j], shift[j]) * weight[j];
-          out.v[j] = inverse[j] * ((u - mean_u[j]) - h * mean_uh[j]);
-        }
-        return out;
-      };
       const T* run_g = grad + a * C;
       const T* run_x = x + a * C;
-      T* out = grad_x + a * C;
-      int64_t q = share.first;
-      for (; q < whole; q += columns.stride_vectors())
-        store_whole(out + q * V, gradient(load_whole(run_g + q * V), load_whole(run_x + q * V)));
-      const int left = static_cast<int>(elements - whole * V);
-      if (q == whole && left > 0)
-        store_part(out + whole * V, gradient(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left)), left);
+      Sums<T> sums;
+      if (share.live) {
+        const PerGroup<T, kUniform> centre = per_group<T, kUniform>(mean + sample * G, channels);
+        const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(rstd + sample * G, channels);
+        for (int64_t q = share.first; q < whole; q += static_cast<int64_t>(K) * stride) {
+          Raw<T> gv[K], xv[K];
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            const int64_t at = place_of(q, k, stride, whole) * V;
+            gv[k] = load_raw(run_g + at);
+            xv[k] = load_raw(run_x + at);
+          }
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if (q + static_cast<int64_t>(k) * stride < whole)
+              sums.add(to_values<T>(gv[k]), to_values<T>(xv[k]), channels, centre, inverse, silu);
+        }
+        if constexpr (!kUniform) {
+          const int left = static_cast<int>(elements - whole * V);
+          if (left > 0 && owns(share, whole, stride))
+            sums.add_part(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left), left, channels, centre,
+                          inverse, silu);
+        }
+      }
+      float2* out = slots + ((tile + sample) * columns.passes + pass) * G;
+      merge_sums<kTileBlock>(sums, channels, share.live, lds, u, G,
+                             [&](int g, float sum_u, float sum_uh) { out[g] = {sum_u, sum_uh}; });
+      total.add(sums);
+      __syncthreads();
     });
+    if (column_sums != nullptr)
+      write_columns<kTileBlock, T>(total, share.live, lds, columns, pass, C, column_sums + tile * C);
   }
-  zero_outside(grad_x, s, tile);
 }
 
-// dbias and dscale: a workgroup per 64 channels, its 16 waves on shares of the
-// tiles, in 64 bits, added in order.
-constexpr int kColumnWaves = 16;
-
-__global__ __launch_bounds__(kColumnWaves * 64) void group_norm_columns_kernel(const float2* __restrict__ tile_sums,
-                                                                               int64_t tiles, int channels,
-                                                                               float* __restrict__ grad_scale,
-                                                                               float* __restrict__ grad_bias) {
-  __shared__ double2 wave_sum[kColumnWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int channel = blockIdx.x * 64 + lane;
-  double z = 0.0, zh = 0.0;
-  if (channel < channels)
-    for (int64_t t = wave; t < tiles; t += kColumnWaves) {
-      const float2 v = tile_sums[t * channels + channel];
-      z += v.x;
-      zh += v.y;
-    }
-  wave_sum[wave][lane] = {z, zh};
-  __syncthreads();
-  if (wave != 0 || channel >= channels) return;
+__device__ __forceinline__ float2 merge_sum_slots(const float2* __restrict__ slots, int64_t n, int64_t stride, int lane,
+                                                  int lanes, double count) {
+  constexpr int U = 8;  // loads in flight
+  double sum_u = 0.0, sum_uh = 0.0;
+  for (int64_t i = lane; i < n; i += U * lanes) {
+    float2 v[U];
 #pragma unroll
-  for (int w = 1; w < kColumnWaves; ++w) {
-    z += wave_sum[w][lane].x;
-    zh += wave_sum[w][lane].y;
+    for (int k = 0; k < U; ++k) {
+      const int64_t at = i + k * lanes;
+      v[k] = slots[(at < n ? at : i) * stride];
+      if (at >= n) v[k] = {0.0f, 0.0f};
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      sum_u += v[k].x;
+      sum_uh += v[k].y;
+    }
+  }
+  sum_u = lanes_sum(sum_u, lanes);
+  sum_uh = lanes_sum(sum_uh, lanes);
+  return {static_cast<float>(sum_u / count), static_cast<float>(sum_uh / count)};
+}
+
+// A wave per (sample, group): means of u and u h.
+__global__ __launch_bounds__(256) void group_norm_means_kernel(const float2* __restrict__ slots, Shape s, int passes,
+                                                               float2* __restrict__ means) {
+  const int64_t unit = uniform_i64(block_index() * 4 + (threadIdx.x >> 6));
+  if (unit >= s.samples * s.groups) return;
+  const int64_t sample = unit / s.groups;
+  const int64_t first = clamped_offset(s, sample) * s.inner, last = clamped_offset(s, sample + 1) * s.inner;
+  if (last - first <= s.long_rows) return;
+  int64_t start;
+  const int64_t n = slots_of(s, passes, sample, first, last, start);
+  const int lane = threadIdx.x & 63;
+  const double count = static_cast<double>(last - first) * (s.channels / s.groups);
+  const float2 m = merge_sum_slots(slots + start * s.groups + unit % s.groups, n, s.groups, lane, 64, count);
+  if (lane == 0) means[unit] = m;
+}
+
+// dbias and dscale: a workgroup per 8 channels, whose 128 threads of each take
+// the rows of column sums in turn (8 loads in flight), in 64 bits; a wave's
+// rows are added by butterfly, the waves' in order.  64 channels a workgroup
+// took 16 us for 2,048 rows of 64 channels.
+constexpr int kColumnBlock = 1024;
+constexpr int kColumnChannels = 8;
+
+__global__ __launch_bounds__(kColumnBlock) void group_norm_columns_kernel(const float2* __restrict__ column_sums,
+                                                                          int64_t rows, int channels,
+                                                                          float* __restrict__ grad_scale,
+                                                                          float* __restrict__ grad_bias) {
+  constexpr int kRows = kColumnBlock / kColumnChannels, kWaves = kColumnBlock / 64, U = 8;
+  __shared__ double2 lds[kWaves][kColumnChannels];
+  const int of = threadIdx.x % kColumnChannels;
+  const int channel = blockIdx.x * kColumnChannels + of;
+  double z = 0.0, zh = 0.0;
+  if (channel < channels) {
+    const float2* at = column_sums + channel;
+    int64_t t = threadIdx.x / kColumnChannels;
+    for (; t + (U - 1) * kRows < rows; t += U * kRows) {
+      float2 v[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) v[i] = at[(t + i * kRows) * channels];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        z += v[i].x;
+        zh += v[i].y;
+      }
+    }
+    for (; t < rows; t += kRows) {
+      z += at[t * channels].x;
+      zh += at[t * channels].y;
+    }
+  }
+  z = across_sum<kColumnChannels>(z);
+  zh = across_sum<kColumnChannels>(zh);
+  if ((threadIdx.x & 63) < kColumnChannels) lds[threadIdx.x >> 6][of] = {z, zh};
+  __syncthreads();
+  if (threadIdx.x >= kColumnChannels || channel >= channels) return;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+    z += lds[w][of].x;
+    zh += lds[w][of].y;
   }
   if (grad_bias != nullptr) grad_bias[channel] = static_cast<float>(z);
   if (grad_scale != nullptr) grad_scale[channel] = static_cast<float>(zh);
+}
+
+// grad_x of one vector.
+template <typename T, bool kUniform>
+__device__ __forceinline__ Values<T> gradient_of(const Values<T>& grad, const Values<T>& x, const Channels<T, kUniform>& channels,
+                                                 const PerGroup<T, kUniform>& centre, const PerGroup<T, kUniform>& inverse,
+                                                 const PerGroup<T, kUniform>& mean_u, const PerGroup<T, kUniform>& mean_uh,
+                                                 bool silu) {
+  Values<T> out;
+#pragma unroll
+  for (int j = 0; j < kVec<T>; ++j) {
+    const float h = (x.v[j] - centre.at(j)) * inverse.at(j);
+    const float u = through_activation(grad.v[j], h, channels.weight[j], channels.shift[j], silu) * channels.weight[j];
+    out.v[j] = inverse.at(j) * ((u - mean_u.at(j)) - h * mean_uh.at(j));
+  }
+  return out;
+}
+
+template <typename T, bool kUniform>
+__global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
+    const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
+    const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd,
+    const float2* __restrict__ means, bool silu, T* __restrict__ grad_x, Shape s, Columns columns) {
+  constexpr int V = kVec<T>, K = kBatch<T> / 2;
+  const int64_t block = block_index();
+  if (block >= s.tiles) return;
+  const int64_t tile = s.tiles - 1 - block;
+  const int C = s.channels, G = s.groups;
+  const int stride = columns.stride_vectors();
+  for (int pass = 0; pass < columns.passes; ++pass) {
+    const Share share = share_of<T, kTileBlock>(columns, pass, C);
+    const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+    each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
+      if (!share.live) return;
+      const int64_t elements = (b - a) * C;
+      const int64_t whole = elements / V;
+      const T* run_g = grad + a * C;
+      const T* run_x = x + a * C;
+      T* out = grad_x + a * C;
+      const PerGroup<T, kUniform> centre = per_group<T, kUniform>(mean + sample * G, channels);
+      const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(rstd + sample * G, channels);
+      PerGroup<T, kUniform> mean_u, mean_uh;
+#pragma unroll
+      for (int j = 0; j < (kUniform ? 1 : V); ++j) {
+        const float2 m = means[sample * G + channels.group_of(j)];
+        mean_u.v[j] = m.x;
+        mean_uh.v[j] = m.y;
+      }
+      const auto gradient = [&](const Values<T>& gv, const Values<T>& xv) {
+        return gradient_of<T, kUniform>(gv, xv, channels, centre, inverse, mean_u, mean_uh, silu);
+      };
+      for (int64_t q = share.first; q < whole; q += static_cast<int64_t>(K) * stride) {
+        Raw<T> gv[K], xv[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int64_t at = place_of(q, k, stride, whole) * V;
+          gv[k] = load_raw(run_g + at);
+          xv[k] = load_raw(run_x + at);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (q + static_cast<int64_t>(k) * stride < whole)
+            store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, gradient(to_values<T>(gv[k]), to_values<T>(xv[k])));
+      }
+      if constexpr (!kUniform) {
+        const int left = static_cast<int>(elements - whole * V);
+        if (left > 0 && owns(share, whole, stride))
+          store_part(out + whole * V, gradient(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left)), left);
+      }
+    });
+  }
+  const int64_t begin = tile * s.tile_rows, rows = s.entries * s.inner;
+  zero_outside<T, kTileBlock>(grad_x, s, begin, begin + s.tile_rows < rows ? begin + s.tile_rows : rows);
+}
+
+// ---------------------------------------------------------------------------
+// direct, backward
+// ---------------------------------------------------------------------------
+//
+// TS threads hold 16 elements each of a sample's x and gradient (fewer
+// than the forward: both tensors, and the channel sums, stay in registers).  A
+// workgroup takes the samples b, b + workgroups, ... and keeps its sums per
+// channel across them, one row of column sums in the end.
+template <typename T>
+constexpr int kHeldBoth = 16 / kVec<T>;
+
+template <typename T, bool kUniform, int TS>
+__global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
+    const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
+    const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd, bool silu,
+    T* __restrict__ grad_x, Shape s, Columns columns, float2* __restrict__ column_sums, int64_t workers) {
+  constexpr int V = kVec<T>;
+  __shared__ SumsLds<TS, V> lds;
+  __shared__ Statistics means;
+  const int C = s.channels, G = s.groups;
+  const int64_t worker = blockIdx.x;
+  if (worker >= workers) {
+    const int64_t part = worker - workers, parts = gridDim.x - workers, rows = s.entries * s.inner;
+    const int64_t each = (rows + parts - 1) / parts;
+    const int64_t begin = part * each < rows ? part * each : rows;
+    zero_outside<T, TS>(grad_x, s, begin, begin + each < rows ? begin + each : rows);
+    return;
+  }
+  const Share share = share_of<T, TS>(columns, 0, C);
+  const Units u = units_of<TS, V, kUniform>(columns, 0, C, G);
+  const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+  const int stride = columns.stride_vectors();
+  Sums<T> total;
+  for (int64_t sample = worker; sample < s.samples; sample += workers) {
+    const int64_t first = clamped_offset(s, sample) * s.inner, last = clamped_offset(s, sample + 1) * s.inner;
+    if (first >= last || last - first > s.long_rows) continue;
+    const int64_t elements = (last - first) * C;
+    const int64_t whole = elements / V;
+    const int left = kUniform ? 0 : static_cast<int>(elements - whole * V);
+    const T* run_g = grad + first * C;
+    const T* run_x = x + first * C;
+    const bool held = whole <= static_cast<int64_t>(stride) * kHeldBoth<T>;
+    const bool tail = !kUniform && left > 0 && owns(share, whole, stride);
+    Raw<T> gv[kHeldBoth<T>], xv[kHeldBoth<T>];
+    int mine = 0;
+    if (held) {
+#pragma unroll
+      for (int k = 0; k < kHeldBoth<T>; ++k)
+        if (static_cast<int64_t>(k) * stride < whole) {
+          const int64_t q = share.first + static_cast<int64_t>(k) * stride;
+          const int64_t at = (q < whole ? q : whole - 1) * V;
+          gv[k] = load_raw(run_g + at);
+          xv[k] = load_raw(run_x + at);
+          mine += share.live && q < whole ? 1 : 0;
+        }
+    }
+    const PerGroup<T, kUniform> centre = per_group<T, kUniform>(mean + sample * G, channels);
+    const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(rstd + sample * G, channels);
+    Sums<T> sums;
+    if (held) {
+#pragma unroll
+      for (int k = 0; k < kHeldBoth<T>; ++k)
+        if (k < mine) sums.add(to_values<T>(gv[k]), to_values<T>(xv[k]), channels, centre, inverse, silu);
+    } else if (share.live) {
+      for (int64_t q = share.first; q < whole; q += stride)
+        sums.add(load_whole(run_g + q * V), load_whole(run_x + q * V), channels, centre, inverse, silu);
+    }
+    if constexpr (!kUniform)
+      if (tail)
+        sums.add_part(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left), left, channels, centre, inverse,
+                      silu);
+    total.add(sums);
+    if (grad_x == nullptr) continue;
+    const float share_of_one = 1.0f / (static_cast<float>(last - first) * static_cast<float>(C / G));
+    merge_sums<TS>(sums, channels, share.live, lds, u, G, [&](int g, float sum_u, float sum_uh) {
+      means.mean[g] = sum_u * share_of_one;
+      means.rstd[g] = sum_uh * share_of_one;
+    });
+    __syncthreads();
+    if (share.live) {
+      T* out = grad_x + first * C;
+      const PerGroup<T, kUniform> mean_u = per_group<T, kUniform>(means.mean, channels);
+      const PerGroup<T, kUniform> mean_uh = per_group<T, kUniform>(means.rstd, channels);
+      const auto gradient = [&](const Values<T>& g, const Values<T>& v) {
+        return gradient_of<T, kUniform>(g, v, channels, centre, inverse, mean_u, mean_uh, silu);
+      };
+      if (held) {
+#pragma unroll
+        for (int k = 0; k < kHeldBoth<T>; ++k)
+          if (k < mine)
+            store_whole(out + (share.first + static_cast<int64_t>(k) * stride) * V,
+                        gradient(to_values<T>(gv[k]), to_values<T>(xv[k])));
+      } else {
+        for (int64_t q = share.first; q < whole; q += stride)
+          store_whole(out + q * V, gradient(load_whole(run_g + q * V), load_whole(run_x + q * V)));
+      }
+      if (tail)
+        store_part(out + whole * V, gradient(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left)), left);
+    }
+    // the next sample's terms go to LDS behind this sample's sync: its means have been written from them by then
+  }
+  if (column_sums == nullptr) return;
+  __syncthreads();
+  write_columns<TS, T>(total, share.live, lds, columns, 0, C, column_sums + worker * C);
 }
 
 // ---------------------------------------------------------------------------
@@ -687,9 +1167,26 @@ __global__ __launch_bounds__(kColumnWaves * 64) void group_norm_columns_kernel(c
 
 int64_t type_bytes(int type) { return type == DPA4K_TYPE_F32 ? 4 : 2; }
 
-// Checks the sizes and cuts the rows into tiles.
-int shape_of(const char* what, int64_t samples, int64_t entries, int64_t inner, int64_t channels, int64_t groups,
-             int type, const int64_t* offsets, Shape& s) {
+// How a call is scheduled, from its sizes alone.
+struct Schedule {
+  Shape shape;
+  int threads;            // of a direct workgroup; 0: tiles alone
+  bool tiles;             // whether samples may be longer than a direct workgroup holds
+  int passes;             // of a tile
+  int64_t workers;        // direct workgroups of the backward
+  int64_t zero_blocks;    // direct workgroups for rows without a sample
+  int64_t column_rows;    // rows of column sums
+};
+
+constexpr int kDirectThreads[] = {64, 256, 512, 1024};
+constexpr int64_t kWorkers = 2048;
+
+// Checks the sizes, cuts the rows into tiles, and chooses the schedule.  A
+// direct workgroup holds 32 elements a thread, 16 in the backward.  The smallest that holds the
+// longest sample is taken; where the longest is not known, one that holds twice
+// the mean, and the rest goes to tiles.
+int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inner, int64_t channels, int64_t groups,
+                int type, const int64_t* offsets, int64_t max_entries, bool backward, Schedule& out) {
   if (samples < 0 || entries < 0 || inner < 0) return fail(DPA4K_EINVAL, "%s: negative sizes", what);
   if (channels <= 0 || channels > kMaxChannels)
     return fail(DPA4K_EINVAL, "%s: 1 to %d channels, got %lld", what, kMaxChannels, static_cast<long long>(channels));
@@ -701,84 +1198,180 @@ int shape_of(const char* what, int64_t samples, int64_t entries, int64_t inner, 
   if ((inner > 0 && entries > most / inner) || samples > most)
     return fail(DPA4K_EINVAL, "%s: the element count overflows 64 bits", what);
   const int64_t rows = entries * inner;
-  const int64_t least = kTileBytes / (channels * type_bytes(type));
+  const int64_t row_bytes = channels * type_bytes(type);
+  const int64_t least = kTileBytes / row_bytes;
   int64_t tile_rows = (rows + kTiles - 1) / kTiles;
   if (tile_rows < least) tile_rows = least;
   if (tile_rows < 1) tile_rows = 1;
-  s = {samples, entries, inner, static_cast<int>(channels), static_cast<int>(groups), tile_rows,
-       (rows + tile_rows - 1) / tile_rows, offsets};
-  if (!grid_fits(samples * groups / 4 + 1, 256)) return fail(DPA4K_EINVAL, "%s: the sample count exceeds the launch limit", what);
+  out = {};
+  out.shape = {samples, entries, inner, static_cast<int>(channels), static_cast<int>(groups), tile_rows,
+               (rows + tile_rows - 1) / tile_rows, 0, offsets};
+  if (!grid_fits(samples * groups / 4 + 1, 256) || !grid_fits(samples + 4096, 1024))
+    return fail(DPA4K_EINVAL, "%s: the sample count exceeds the launch limit", what);
+  const int vec = static_cast<int>(16 / type_bytes(type));
+  const int period = static_cast<int>(channels) / gcd_of(static_cast<int>(channels), vec);
+  out.passes = (period + kTileBlock - 1) / kTileBlock;
+  // rows of the longest sample, or what most samples are expected not to pass
+  const bool known = offsets == nullptr || max_entries >= 0;
+  int64_t wanted = offsets == nullptr ? inner : 0;
+  if (offsets != nullptr) {
+    if (known) wanted = (max_entries < entries ? max_entries : entries) * inner;
+    else wanted = samples > 0 ? 2 * (rows / samples) + 1 : 0;
+  }
+  const int64_t elements = wanted * channels;
+  if (groups <= kLdsGroups)
+    for (int threads : kDirectThreads) {
+      if (period > threads) continue;
+      const int64_t holds = static_cast<int64_t>(threads / period) * period * (backward ? 16 : 32);
+      if (elements > holds && (known || threads < 1024)) continue;
+      out.threads = threads;
+      out.shape.long_rows = holds / channels;
+      break;
+    }
+  if (out.threads != 0 && known) out.shape.long_rows = INT64_MAX;  // nothing is left to tiles: a longer sample is streamed
+  out.tiles = out.threads == 0 || !known;
+  out.workers = out.threads == 0 ? 0 : (samples < kWorkers ? samples : kWorkers);
+  const int64_t kilobytes64 = rows * row_bytes / 65536 + 1;
+  out.zero_blocks = offsets == nullptr || out.tiles ? 0 : (kilobytes64 < 256 ? kilobytes64 : 256);
+  out.column_rows = out.workers + (out.tiles ? out.shape.tiles : 0);
   return DPA4K_OK;
 }
 
 struct Workspace {
-  void* slots;        // Moments or double2 per (piece, group)
-  float2* means;      // per (sample, group), backward
-  float2* tile_sums;  // per (tile, channel), backward
+  Slot* slots;          // per (piece, pass, group), forward
+  float2* sum_slots;    // per (piece, pass, group), backward
+  float2* means;        // per (sample, group), backward
+  float2* column_sums;  // rows of channels, backward
 };
 
-bool carve(Carver& carver, const Shape& s, bool backward, Workspace& w) {
-  const size_t pieces = static_cast<size_t>(s.tiles + s.samples) * s.groups;
+template <typename Take>
+void each_array(const Schedule& c, bool backward, Take take) {
+  const size_t pieces = c.tiles ? static_cast<size_t>(c.shape.tiles + c.shape.samples) * c.passes * c.shape.groups : 0;
   if (!backward) {
-    w.slots = carver.take<Moments>(pieces);
-    return w.slots != nullptr;
+    take(&Workspace::slots, pieces);
+    return;
   }
-  w.slots = carver.take<double2>(pieces);
-  w.means = carver.take<float2>(static_cast<size_t>(s.samples) * s.groups);
-  w.tile_sums = carver.take<float2>(static_cast<size_t>(s.tiles) * s.channels);
-  return w.slots != nullptr && w.means != nullptr && w.tile_sums != nullptr;
+  take(&Workspace::sum_slots, pieces);
+  take(&Workspace::means, c.tiles ? static_cast<size_t>(c.shape.samples) * c.shape.groups : 0);
+  take(&Workspace::column_sums, static_cast<size_t>(c.column_rows) * c.shape.channels);
 }
 
-size_t workspace_bytes_of(const Shape& s, bool backward) {
-  const size_t pieces = static_cast<size_t>(s.tiles + s.samples) * s.groups;
-  if (!backward) return round_up_256(pieces * sizeof(Moments));
-  return round_up_256(pieces * sizeof(double2)) + round_up_256(static_cast<size_t>(s.samples) * s.groups * sizeof(float2)) +
-         round_up_256(static_cast<size_t>(s.tiles) * s.channels * sizeof(float2));
+size_t workspace_bytes_of(const Schedule& c, bool backward) {
+  size_t bytes = 0;
+  each_array(c, backward, [&](auto member, size_t count) {
+    Workspace w{};
+    bytes += round_up_256(count * sizeof(*(w.*member)));
+  });
+  return bytes;
+}
+
+bool carve(const Schedule& c, bool backward, void* workspace, size_t bytes, Workspace& w) {
+  if (workspace == nullptr) bytes = 0;
+  Carver carver{static_cast<char*>(workspace), bytes};
+  bool fits = true;
+  each_array(c, backward, [&](auto member, size_t count) {
+    using Element = std::remove_reference_t<decltype(*(w.*member))>;
+    w.*member = count > 0 ? carver.take<Element>(count) : nullptr;
+    fits = fits && (count == 0 || w.*member != nullptr);
+  });
+  return fits;
 }
 
 template <typename T>
-int forward(const void* x, const float* scale, const float* bias, void* y, float* mean, float* rstd, const Shape& s,
-            float eps, bool silu, const Workspace& w, hipStream_t stream) {
-  const Columns columns = columns_for<T>(s.channels);
-  Moments* slots = static_cast<Moments*>(w.slots);
-  const dim3 grid = launch_grid(s.tiles, kBlock);
-  group_norm_moments_kernel<T><<<grid, kBlock, 0, stream>>>(static_cast<const T*>(x), s, columns, slots);
+bool uniform_groups(const Shape& s) {
+  return s.channels / s.groups % kVec<T> == 0;
+}
+
+// Calls LAUNCH(TS) for the schedule's direct workgroup.
+#define DPA4K_DIRECT(threads, LAUNCH) \
+  if (threads == 64) LAUNCH(64);      \
+  else if (threads == 256) LAUNCH(256); \
+  else if (threads == 512) LAUNCH(512); \
+  else LAUNCH(1024);
+
+template <typename T, bool kUniform>
+int forward_as(const T* x, const float* scale, const float* bias, T* y, float* mean, float* rstd, const Schedule& c,
+               float eps, bool silu, const Workspace& w, hipStream_t stream) {
+  const Shape& s = c.shape;
+  if (c.threads != 0) {
+    const Columns columns = columns_for<T>(s.channels, c.threads);
+    const dim3 grid = launch_grid(s.samples + c.zero_blocks > 0 ? s.samples + c.zero_blocks : 1, c.threads);
+#define DPA4K_LAUNCH(TS)                                                                                              \
+  group_norm_direct_kernel<T, kUniform, TS><<<grid, TS, 0, stream>>>(x, scale, bias, eps, silu, mean, rstd, y, s, columns, \
+                                                                     c.zero_blocks)
+    DPA4K_DIRECT(c.threads, DPA4K_LAUNCH)
+#undef DPA4K_LAUNCH
+    if (int e = launched("group_norm_direct_kernel")) return e;
+  }
+  if (!c.tiles) return DPA4K_OK;
+  const Columns columns = columns_for<T>(s.channels, kTileBlock);
+  const dim3 grid = launch_grid(s.tiles, kTileBlock);
+  group_norm_moments_kernel<T, kUniform><<<grid, kTileBlock, 0, stream>>>(x, s, columns, w.slots);
   if (int e = launched("group_norm_moments_kernel")) return e;
   if (s.samples > 0) {
-    group_norm_finish_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(slots, s, eps, mean, rstd);
+    group_norm_finish_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(w.slots, s, columns.passes,
+                                                                                                  eps, mean, rstd);
     if (int e = launched("group_norm_finish_kernel")) return e;
   }
-  (silu ? group_norm_apply_kernel<T, true> : group_norm_apply_kernel<T, false>)<<<grid, kBlock, 0, stream>>>(
-      static_cast<const T*>(x), scale, bias, mean, rstd, static_cast<T*>(y), s, columns);
+  group_norm_apply_kernel<T, kUniform><<<grid, kTileBlock, 0, stream>>>(x, scale, bias, silu, mean, rstd, y, s, columns);
   return launched("group_norm_apply_kernel");
+}
+
+template <typename T, bool kUniform>
+int backward_as(const T* grad, const T* x, const float* scale, const float* bias, const float* mean, const float* rstd,
+                T* grad_x, float* grad_scale, float* grad_bias, const Schedule& c, bool silu, const Workspace& w,
+                hipStream_t stream) {
+  const Shape& s = c.shape;
+  const bool parameters = grad_scale != nullptr || grad_bias != nullptr;
+  float2* tile_columns = parameters ? w.column_sums : nullptr;
+  float2* direct_columns = parameters ? w.column_sums + (c.tiles ? s.tiles * s.channels : 0) : nullptr;
+  if (c.threads != 0 && (c.workers > 0 || (grad_x != nullptr && c.zero_blocks > 0))) {
+    const Columns columns = columns_for<T>(s.channels, c.threads);
+    const unsigned int grid = static_cast<unsigned int>(c.workers + (grad_x != nullptr ? c.zero_blocks : 0));
+#define DPA4K_LAUNCH(TS)                                                                                                  \
+  group_norm_direct_backward_kernel<T, kUniform, TS><<<grid, TS, 0, stream>>>(grad, x, scale, bias, mean, rstd, silu, grad_x, s, \
+                                                                              columns, direct_columns, c.workers)
+    DPA4K_DIRECT(c.threads, DPA4K_LAUNCH)
+#undef DPA4K_LAUNCH
+    if (int e = launched("group_norm_direct_backward_kernel")) return e;
+  }
+  if (c.tiles) {
+    const Columns columns = columns_for<T>(s.channels, kTileBlock);
+    const dim3 grid = launch_grid(s.tiles, kTileBlock);
+    group_norm_sums_kernel<T, kUniform><<<grid, kTileBlock, 0, stream>>>(grad, x, scale, bias, mean, rstd, silu, s, columns,
+                                                                        w.sum_slots, tile_columns);
+    if (int e = launched("group_norm_sums_kernel")) return e;
+    if (grad_x != nullptr) {
+      if (s.samples > 0) {
+        group_norm_means_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(w.sum_slots, s,
+                                                                                                     columns.passes, w.means);
+        if (int e = launched("group_norm_means_kernel")) return e;
+      }
+      group_norm_backward_kernel<T, kUniform><<<grid, kTileBlock, 0, stream>>>(grad, x, scale, bias, mean, rstd, w.means, silu,
+                                                                              grad_x, s, columns);
+      if (int e = launched("group_norm_backward_kernel")) return e;
+    }
+  }
+  if (!parameters) return DPA4K_OK;
+  group_norm_columns_kernel<<<blocks_for(s.channels, kColumnChannels), kColumnBlock, 0, stream>>>(w.column_sums, c.column_rows, s.channels,
+                                                                                    grad_scale, grad_bias);
+  return launched("group_norm_columns_kernel");
+}
+
+template <typename T>
+int forward(const void* x, const float* scale, const float* bias, void* y, float* mean, float* rstd, const Schedule& c,
+            float eps, bool silu, const Workspace& w, hipStream_t stream) {
+  return (uniform_groups<T>(c.shape) ? forward_as<T, true> : forward_as<T, false>)(
+      static_cast<const T*>(x), scale, bias, static_cast<T*>(y), mean, rstd, c, eps, silu, w, stream);
 }
 
 template <typename T>
 int backward(const void* grad, const void* x, const float* scale, const float* bias, const float* mean,
-             const float* rstd, void* grad_x, float* grad_scale, float* grad_bias, const Shape& s, bool silu,
+             const float* rstd, void* grad_x, float* grad_scale, float* grad_bias, const Schedule& c, bool silu,
              const Workspace& w, hipStream_t stream) {
-  const Columns columns = columns_for<T>(s.channels);
-  double2* slots = static_cast<double2*>(w.slots);
-  const bool parameters = grad_scale != nullptr || grad_bias != nullptr;
-  const dim3 grid = launch_grid(s.tiles, kBlock);
-  (silu ? group_norm_sums_kernel<T, true> : group_norm_sums_kernel<T, false>)<<<grid, kBlock, 0, stream>>>(
-      static_cast<const T*>(grad), static_cast<const T*>(x), scale, bias, mean, rstd, s, columns, slots,
-      parameters ? w.tile_sums : nullptr);
-  if (int e = launched("group_norm_sums_kernel")) return e;
-  if (grad_x != nullptr) {
-    if (s.samples > 0) {
-      group_norm_means_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(slots, s, w.means);
-      if (int e = launched("group_norm_means_kernel")) return e;
-    }
-    (silu ? group_norm_backward_kernel<T, true> : group_norm_backward_kernel<T, false>)<<<grid, kBlock, 0, stream>>>(
-        static_cast<const T*>(grad), static_cast<const T*>(x), scale, bias, mean, rstd, w.means, static_cast<T*>(grad_x), s,
-        columns);
-    if (int e = launched("group_norm_backward_kernel")) return e;
-  }
-  if (!parameters) return DPA4K_OK;
-  group_norm_columns_kernel<<<blocks_for(s.channels, 64), kColumnWaves * 64, 0, stream>>>(w.tile_sums, s.tiles, s.channels,
-                                                                                        grad_scale, grad_bias);
-  return launched("group_norm_columns_kernel");
+  return (uniform_groups<T>(c.shape) ? backward_as<T, true> : backward_as<T, false>)(
+      static_cast<const T*>(grad), static_cast<const T*>(x), scale, bias, mean, rstd, static_cast<T*>(grad_x), grad_scale,
+      grad_bias, c, silu, w, stream);
 }
 
 }  // namespace
@@ -787,45 +1380,48 @@ int backward(const void* grad, const void* x, const float* scale, const float* b
 using namespace dpa4k;
 
 extern "C" size_t dpa4k_group_norm_workspace_size(int64_t samples, int64_t entries, int64_t inner, int64_t channels,
-                                                  int64_t groups, int type, int backward) {
-  Shape s;
+                                                  int64_t groups, int ragged, int64_t max_entries, int type, int backward) {
+  Schedule c;
   static const int64_t some = 0;  // any offsets: the size does not depend on them
-  if (shape_of("group norm", samples, entries, inner, channels, groups, type, &some, s)) return 0;
-  return workspace_bytes_of(s, backward != 0);
+  if (schedule_of("group norm", samples, entries, inner, channels, groups, type, ragged != 0 ? &some : nullptr, max_entries,
+                  backward != 0, c))
+    return 0;
+  return workspace_bytes_of(c, backward != 0);
 }
 
 extern "C" int dpa4k_group_norm_forward(const void* x, const float* scale, const float* bias, const int64_t* offsets,
                                         void* y, float* mean, float* rstd, int64_t samples, int64_t entries,
-                                        int64_t inner, int64_t channels, int64_t groups, float eps, int silu, int type,
-                                        void* workspace, size_t workspace_bytes, dpa4k_stream_t stream_handle) {
+                                        int64_t inner, int64_t channels, int64_t groups, int64_t max_entries, float eps,
+                                        int silu, int type, void* workspace, size_t workspace_bytes,
+                                        dpa4k_stream_t stream_handle) {
   clear_error();
-  Shape s;
-  if (int e = shape_of("group norm", samples, entries, inner, channels, groups, type, offsets, s)) return e;
+  Schedule c;
+  if (int e = schedule_of("group norm", samples, entries, inner, channels, groups, type, offsets, max_entries, false, c)) return e;
   if (!(eps > 0.0f) || !(eps < INFINITY)) return fail(DPA4K_EINVAL, "group norm eps must be a finite positive number");
-  if (s.tiles == 0) return DPA4K_OK;
+  if (c.shape.tiles == 0) return DPA4K_OK;
   if (x == nullptr || y == nullptr || (samples > 0 && (mean == nullptr || rstd == nullptr)))
     return fail(DPA4K_EINVAL, "group norm: null pointer");
-  Carver carver{static_cast<char*>(workspace), workspace == nullptr ? 0 : workspace_bytes};
   Workspace w{};
-  if (!carve(carver, s, false, w))
+  if (!carve(c, false, workspace, workspace_bytes, w))
     return fail(DPA4K_EWORKSPACE, "group norm: workspace of %zu bytes is smaller than %zu", workspace_bytes,
-                workspace_bytes_of(s, false));
+                workspace_bytes_of(c, false));
   hipStream_t stream = as_stream(stream_handle);
-  if (type == DPA4K_TYPE_F32) return forward<float>(x, scale, bias, y, mean, rstd, s, eps, silu != 0, w, stream);
-  if (type == DPA4K_TYPE_BF16) return forward<__bf16>(x, scale, bias, y, mean, rstd, s, eps, silu != 0, w, stream);
-  return forward<_Float16>(x, scale, bias, y, mean, rstd, s, eps, silu != 0, w, stream);
+  if (type == DPA4K_TYPE_F32) return forward<float>(x, scale, bias, y, mean, rstd, c, eps, silu != 0, w, stream);
+  if (type == DPA4K_TYPE_BF16) return forward<__bf16>(x, scale, bias, y, mean, rstd, c, eps, silu != 0, w, stream);
+  return forward<_Float16>(x, scale, bias, y, mean, rstd, c, eps, silu != 0, w, stream);
 }
 
 extern "C" int dpa4k_group_norm_backward(const void* grad, const void* x, const float* scale, const float* bias,
                                          const int64_t* offsets, const float* mean, const float* rstd, void* grad_x,
                                          float* grad_scale, float* grad_bias, int64_t samples, int64_t entries,
-                                         int64_t inner, int64_t channels, int64_t groups, int silu, int type,
-                                         void* workspace, size_t workspace_bytes, dpa4k_stream_t stream_handle) {
+                                         int64_t inner, int64_t channels, int64_t groups, int64_t max_entries, int silu,
+                                         int type, void* workspace, size_t workspace_bytes, dpa4k_stream_t stream_handle) {
   clear_error();
-  Shape s;
-  if (int e = shape_of("group norm backward", samples, entries, inner, channels, groups, type, offsets, s)) return e;
+  Schedule c;
+  if (int e = schedule_of("group norm backward", samples, entries, inner, channels, groups, type, offsets, max_entries, true, c))
+    return e;
   hipStream_t stream = as_stream(stream_handle);
-  if (s.tiles == 0) {
+  if (c.shape.tiles == 0) {
     for (float* out : {grad_scale, grad_bias})
       if (out != nullptr)
         if (int e = zero_fill(out, channels * sizeof(float), stream)) return e;
@@ -834,14 +1430,13 @@ extern "C" int dpa4k_group_norm_backward(const void* grad, const void* x, const 
   if (grad == nullptr || x == nullptr || (samples > 0 && (mean == nullptr || rstd == nullptr)))
     return fail(DPA4K_EINVAL, "group norm backward: null pointer");
   if (grad_x == nullptr && grad_scale == nullptr && grad_bias == nullptr) return DPA4K_OK;
-  Carver carver{static_cast<char*>(workspace), workspace == nullptr ? 0 : workspace_bytes};
   Workspace w{};
-  if (!carve(carver, s, true, w))
+  if (!carve(c, true, workspace, workspace_bytes, w))
     return fail(DPA4K_EWORKSPACE, "group norm backward: workspace of %zu bytes is smaller than %zu", workspace_bytes,
-                workspace_bytes_of(s, true));
+                workspace_bytes_of(c, true));
   if (type == DPA4K_TYPE_F32)
-    return backward<float>(grad, x, scale, bias, mean, rstd, grad_x, grad_scale, grad_bias, s, silu != 0, w, stream);
+    return backward<float>(grad, x, scale, bias, mean, rstd, grad_x, grad_scale, grad_bias, c, silu != 0, w, stream);
   if (type == DPA4K_TYPE_BF16)
-    return backward<__bf16>(grad, x, scale, bias, mean, rstd, grad_x, grad_scale, grad_bias, s, silu != 0, w, stream);
-  return backward<_Float16>(grad, x, scale, bias, mean, rstd, grad_x, grad_scale, grad_bias, s, silu != 0, w, stream);
+    return backward<__bf16>(grad, x, scale, bias, mean, rstd, grad_x, grad_scale, grad_bias, c, silu != 0, w, stream);
+  return backward<_Float16>(grad, x, scale, bias, mean, rstd, grad_x, grad_scale, grad_bias, c, silu != 0, w, stream);
 }

@@ -880,7 +880,8 @@ def _group_norm_sizes(x, groups, scale, bias, offsets):
     return samples, entries, inner, channels
 
 
-def group_norm_forward(x, groups, scale=None, bias=None, offsets=None, eps: float = 1.0e-5, silu: bool = False):
+def group_norm_forward(x, groups, scale=None, bias=None, offsets=None, eps: float = 1.0e-5, silu: bool = False, *,
+                       max_rows=None):
     """``(y, mean, rstd)``; ``mean`` and ``rstd`` are ``(samples, groups)`` float32."""
     groups = int(groups)
     samples, entries, inner, channels = _group_norm_sizes(x, groups, scale, bias, offsets)
@@ -888,18 +889,19 @@ def group_norm_forward(x, groups, scale=None, bias=None, offsets=None, eps: floa
     statistics = torch.empty((2, samples, groups), dtype=torch.float32, device=x.device)
     mean, rstd = statistics[0], statistics[1]
     code = ELEMENT_TYPES[x.dtype]
-    nbytes = _LIB.dpa4k_group_norm_workspace_size(samples, entries, inner, channels, groups, code, 0)
+    most = -1 if max_rows is None else min(int(max_rows), entries)
+    nbytes = _LIB.dpa4k_group_norm_workspace_size(samples, entries, inner, channels, groups, offsets is not None, most, code, 0)
     workspace = _workspace(nbytes, x.device)
     with _on(x.device) as stream:
         status = _LIB.dpa4k_group_norm_forward(
             _ptr(x), _ptr(scale), _ptr(bias), _ptr(offsets), _ptr(y), _ptr(mean), _ptr(rstd), samples, entries, inner,
-            channels, groups, float(eps), int(bool(silu)), code, workspace.data_ptr(), nbytes, stream)
+            channels, groups, most, float(eps), int(bool(silu)), code, workspace.data_ptr(), nbytes, stream)
     _lib.check(status)
     return y, mean, rstd
 
 
 def group_norm_backward(grad_output, x, groups, scale, bias, offsets, mean, rstd, silu: bool = False, *,
-                        want_x: bool = True, want_scale: bool = True, want_bias: bool = True):
+                        want_x: bool = True, want_scale: bool = True, want_bias: bool = True, max_rows=None):
     """``(grad_x, grad_scale, grad_bias)``, None where not wanted."""
     groups = int(groups)
     samples, entries, inner, channels = _group_norm_sizes(x, groups, scale, bias, offsets)
@@ -913,12 +915,13 @@ def group_norm_backward(grad_output, x, groups, scale, bias, offsets, mean, rstd
     grad_scale = torch.empty((channels,), dtype=torch.float32, device=x.device) if want_scale else None
     grad_bias = torch.empty((channels,), dtype=torch.float32, device=x.device) if want_bias else None
     code = ELEMENT_TYPES[x.dtype]
-    nbytes = _LIB.dpa4k_group_norm_workspace_size(samples, entries, inner, channels, groups, code, 1)
+    most = -1 if max_rows is None else min(int(max_rows), entries)
+    nbytes = _LIB.dpa4k_group_norm_workspace_size(samples, entries, inner, channels, groups, offsets is not None, most, code, 1)
     workspace = _workspace(nbytes, x.device)
     with _on(x.device) as stream:
         status = _LIB.dpa4k_group_norm_backward(
             _ptr(grad_output), _ptr(x), _ptr(scale), _ptr(bias), _ptr(offsets), _ptr(mean), _ptr(rstd), _ptr(grad_x),
-            _ptr(grad_scale), _ptr(grad_bias), samples, entries, inner, channels, groups, int(bool(silu)), code,
+            _ptr(grad_scale), _ptr(grad_bias), samples, entries, inner, channels, groups, most, int(bool(silu)), code,
             workspace.data_ptr(), nbytes, stream)
     _lib.check(status)
     return grad_x, grad_scale, grad_bias

@@ -102,9 +102,9 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "dpa4k_edge_stream_combine": (
         _INT, [_OPERANDS, _OPERANDS, ctypes.POINTER(_F32), _INT, _INT, _OPERANDS, ctypes.POINTER(ctypes.c_int32), _P,
                _I64, _I64, _I64, _P]),
-    "dpa4k_group_norm_workspace_size": (_SZ, [_I64] * 5 + [_INT, _INT]),
-    "dpa4k_group_norm_forward": (_INT, [_P] * 7 + [_I64] * 5 + [_F32, _INT, _INT, _P, _SZ, _P]),
-    "dpa4k_group_norm_backward": (_INT, [_P] * 10 + [_I64] * 5 + [_INT, _INT, _P, _SZ, _P]),
+    "dpa4k_group_norm_workspace_size": (_SZ, [_I64] * 5 + [_INT, _I64, _INT, _INT]),
+    "dpa4k_group_norm_forward": (_INT, [_P] * 7 + [_I64] * 6 + [_F32, _INT, _INT, _P, _SZ, _P]),
+    "dpa4k_group_norm_backward": (_INT, [_P] * 10 + [_I64] * 6 + [_INT, _INT, _P, _SZ, _P]),
     "dpa4k_grad_norm_workspace_size": (_SZ, [_P, _I64]),
     "dpa4k_grad_norm": (_INT, [_P, _P, _P, _I64, _F64, _P, _P, _P, _SZ, _P]),
     "dpa4k_adamw_plan_size": (_SZ, [_P, _I64]),

@@ -85,7 +85,8 @@ class _GroupNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, offsets, groups, max_rows, eps, silu):
         native = _extension("group_norm_forward")
-        y, mean, rstd = native.group_norm_forward(x, groups, scale, bias, offsets, eps, silu)
+        y, mean, rstd = native.group_norm_forward(x, groups, scale, bias, offsets, eps, silu,
+                                                  max_rows=max_rows)
         ctx.save_for_backward(x, scale, bias, offsets, mean, rstd)
         ctx.arguments = groups, max_rows, silu
         return y
@@ -98,7 +99,7 @@ class _GroupNormFunction(torch.autograd.Function):
         want = ctx.needs_input_grad
         native = _extension("group_norm_backward")
         grads = native.group_norm_backward(grad_output.contiguous(), x, groups, scale, bias, offsets, mean, rstd, silu,
-                                           want_x=want[0], want_scale=want[1], want_bias=want[2])
+                                           want_x=want[0], want_scale=want[1], want_bias=want[2], max_rows=max_rows)
         return (*grads, None, None, None, None, None)
 
 

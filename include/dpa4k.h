@@ -542,18 +542,23 @@ enum { DPA4K_TYPE_F32 = 0, DPA4K_TYPE_BF16 = 1, DPA4K_TYPE_F16 = 2 };
  * scale, bias: float[C] or NULL; mean, rstd[samples, groups] are kept for the
  * backward.  Rows of no sample get y = 0.  C <=
  * DPA4K_GROUP_NORM_MAX_CHANNELS; eps finite and > 0.  Tensors may start at any
- * element. */
+ * element.  max_entries: entries of the longest sample, or -1 where the caller
+ * does not know; it selects the schedule only, and results are right (if
+ * slower) where it is too small.  The workspace query takes ragged = offsets !=
+ * NULL. */
 #define DPA4K_GROUP_NORM_MAX_CHANNELS 4096
 size_t dpa4k_group_norm_workspace_size(int64_t samples, int64_t entries,
                                        int64_t inner, int64_t channels,
-                                       int64_t groups, int type, int backward);
+                                       int64_t groups, int ragged,
+                                       int64_t max_entries, int type,
+                                       int backward);
 int dpa4k_group_norm_forward(const void* x, const float* scale,
                              const float* bias, const int64_t* offsets, void* y,
                              float* mean, float* rstd, int64_t samples,
                              int64_t entries, int64_t inner, int64_t channels,
-                             int64_t groups, float eps, int silu, int type,
-                             void* workspace, size_t workspace_bytes,
-                             dpa4k_stream_t stream);
+                             int64_t groups, int64_t max_entries, float eps,
+                             int silu, int type, void* workspace,
+                             size_t workspace_bytes, dpa4k_stream_t stream);
 
 /* dz = grad act'(z), u = dz scale:
  *   grad_x = (u - mean(u) - h mean(u h)) / sqrt(var + eps)
@@ -566,9 +571,10 @@ int dpa4k_group_norm_backward(const void* grad, const void* x,
                               const float* rstd, void* grad_x,
                               float* grad_scale, float* grad_bias,
                               int64_t samples, int64_t entries, int64_t inner,
-                              int64_t channels, int64_t groups, int silu,
-                              int type, void* workspace,
-                              size_t workspace_bytes, dpa4k_stream_t stream);
+                              int64_t channels, int64_t groups,
+                              int64_t max_entries, int silu, int type,
+                              void* workspace, size_t workspace_bytes,
+                              dpa4k_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Optimiser step (no reference counterpart)

@@ -179,7 +179,7 @@ def test_c_entry_points_refuse_bad_sizes_before_any_device_call():
     some = ctypes.c_void_p(256)  # never dereferenced
 
     def norm(*sizes, eps=eps, type_=f32, offsets=some, x=null):
-        return lib.dpa4k_group_norm_forward(x, null, null, offsets, null, null, null, *sizes, eps, 0, type_, null, 0, null)
+        return lib.dpa4k_group_norm_forward(x, null, null, offsets, null, null, null, *sizes, -1, eps, 0, type_, null, 0, null)
 
     cases = [
         (norm(1, -1, 1, 8, 2), "negative"),
@@ -198,14 +198,14 @@ def test_c_entry_points_refuse_bad_sizes_before_any_device_call():
     for call, (_, fragment) in zip((lambda: norm(1, 4, 1, 8, 3), lambda: norm(1, 4, 1, 8, 2)), ((0, "divide"), (0, "null"))):
         call()
         assert fragment in lib.dpa4k_last_error().decode()
-    backward = lib.dpa4k_group_norm_backward(null, null, null, null, some, null, null, null, null, null, 1, 4, 1, 8, 2, 0, f32,
+    backward = lib.dpa4k_group_norm_backward(null, null, null, null, some, null, null, null, null, null, 1, 4, 1, 8, 2, -1, 0, f32,
                                              null, 0, null)
     assert backward == _lib.EINVAL
-    status = lib.dpa4k_group_norm_forward(some, null, null, some, some, some, some, 1, 4, 1, 8, 2, eps, 0, f32, null, 0, null)
+    status = lib.dpa4k_group_norm_forward(some, null, null, some, some, some, some, 1, 4, 1, 8, 2, -1, eps, 0, f32, null, 0, null)
     assert status == _lib.EWORKSPACE
-    assert lib.dpa4k_group_norm_workspace_size(1, 4, 1, 8, 3, f32, 0) == 0
+    assert lib.dpa4k_group_norm_workspace_size(1, 4, 1, 8, 3, 1, -1, f32, 0) == 0
     for backward in (0, 1):
-        small, large = (lib.dpa4k_group_norm_workspace_size(10, rows, 1, 64, 8, f32, backward) for rows in (100, 10**7))
+        small, large = (lib.dpa4k_group_norm_workspace_size(10, rows, 1, 64, 8, 1, -1, f32, backward) for rows in (100, 10**7))
         assert 0 < small <= large and large % 256 == 0
 
     counts, types = (ctypes.c_int64 * 1)(4), (ctypes.c_int32 * 1)(0)
