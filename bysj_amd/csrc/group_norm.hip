@@ -576,7 +576,7 @@ template <typename T, bool kUniform>
 __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
     const T* __restrict__ x, const float* __restrict__ scale, const float* __restrict__ bias, bool silu,
     const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ y, Shape s, Columns columns) {
-  constexpr int V = kVec<T>, K = kBatch<T> / 2;
+  constexpr int V = kVec<T>, K = 4;
   const int64_t block = block_index();
   if (block >= s.tiles) return;
   const int64_t tile = s.tiles - 1 - block;
@@ -602,7 +602,15 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
           value.v[j] = activated(fmaf(value.v[j] - centre.at(j), slope[j], channels.shift[j]), silu);
         return value;
       };
-      for (int64_t q = share.first; q < whole; q += static_cast<int64_t>(K) * stride) {
+      int64_t q = share.first;
+      for (; q + static_cast<int64_t>(K - 1) * stride < whole; q += static_cast<int64_t>(K) * stride) {
+        Raw<T> raw[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) raw[k] = load_raw(run + (q + static_cast<int64_t>(k) * stride) * V);
+#pragma unroll
+        for (int k = 0; k < K; ++k) store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
+      }
+      if (q < whole) {
         Raw<T> raw[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) raw[k] = load_raw(run + place_of(q, k, stride, whole) * V);

@@ -43,8 +43,7 @@ namespace dpa4k {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kChunk = 4096;           // elements of a workgroup: 4 vectors of 4 per thread
-constexpr int kVectors = kChunk / (kBlock * 4);
+constexpr int kChunk = 4096;           // elements of a workgroup
 constexpr int kSpan = 32;              // elements that share a scale
 constexpr int kPointers = 440;         // gradients passed by value: kernel arguments below 4 KB
 
@@ -82,102 +81,170 @@ __host__ __device__ inline uint32_t mix(uint32_t x) {
 }
 
 // ---------------------------------------------------------------------------
-// four elements
+// vectors of E elements
 // ---------------------------------------------------------------------------
 
-// Vectors of any element alignment: one access each.
+// Up to 16 bytes at any element alignment: one access.
 template <typename T>
-struct vec4_of {
-  typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+constexpr int kWide = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
+template <typename T, int N>
+struct vector_of {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(uint16_t bf16) { return __uint_as_float(static_cast<uint32_t>(bf16) << 16); }
 
-// Elements [at, at + 4) of a stream of `count` as float32, zeros past its end.
-template <bool kWhole, typename T>
-__device__ __forceinline__ fvec<4> load4(const T* __restrict__ p, int64_t at, int64_t count) {
-  fvec<4> out;
+// Addresses read from a plan are addresses of global memory, which the compiler
+// cannot see: it would use flat accesses, which occupy the LDS path as well.
+template <typename T>
+using Global = __attribute__((address_space(1))) T;
+template <typename T>
+__device__ __forceinline__ Global<T>* global(T* p) {
+  return (Global<T>*)p;
+}
+
+template <int E>
+struct Floats {
+  float v[E];
+};
+
+// Elements [at, at + E) of a stream of `count` as float32, zeros past its end.
+template <bool kWhole, int E, typename T>
+__device__ __forceinline__ Floats<E> load(const T* __restrict__ p, int64_t at, int64_t count) {
+  constexpr int N = E < kWide<T> ? E : kWide<T>;
+  Floats<E> out;
   if (kWhole) {
-    const auto raw = *reinterpret_cast<const typename vec4_of<T>::type*>(p + at);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out.v[i] = to_float(raw[i]);
+    for (int part = 0; part < E / N; ++part) {
+      const typename vector_of<T, N>::type raw = *(const Global<typename vector_of<T, N>::type>*)(p + at + part * N);
+#pragma unroll
+      for (int i = 0; i < N; ++i) out.v[part * N + i] = to_float(raw[i]);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out.v[i] = at + i < count ? to_float(p[at + i]) : 0.0f;
+    for (int i = 0; i < E; ++i) out.v[i] = at + i < count ? to_float(global(p)[at + i]) : 0.0f;
   }
   return out;
 }
 
-template <bool kWhole, typename T>
-__device__ __forceinline__ void store4(T* __restrict__ p, int64_t at, int64_t count, const T (&value)[4]) {
+template <bool kWhole, int E, typename T>
+__device__ __forceinline__ void store(T* __restrict__ p, int64_t at, int64_t count, const T (&value)[E]) {
+  constexpr int N = E < kWide<T> ? E : kWide<T>;
   if (kWhole) {
-    typename vec4_of<T>::type raw;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = value[i];
-    *reinterpret_cast<typename vec4_of<T>::type*>(p + at) = raw;
+    for (int part = 0; part < E / N; ++part) {
+      typename vector_of<T, N>::type raw;
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = value[part * N + i];
+      *(Global<typename vector_of<T, N>::type>*)(p + at + part * N) = raw;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (at + i < count) p[at + i] = value[i];
+    for (int i = 0; i < E; ++i)
+      if (at + i < count) global(p)[at + i] = value[i];
   }
 }
 
 // ---------------------------------------------------------------------------
 // codes of 8 bits
 // ---------------------------------------------------------------------------
+//
+// A lane holds E of the 32 values that share a scale: 8 where the parameters are
+// bfloat16 (16 bytes), 4 where they are float32 (8 would leave every store half
+// a line: the values of 72M codes took 175 us that way, 123 us with 4).
 
-__device__ __forceinline__ uint32_t group8_max(uint32_t value) {
-  int x = static_cast<int>(value);
-  int y = xor_lane<1>(x);
-  x = x > y ? x : y;
-  y = xor_lane<2>(x);
-  x = x > y ? x : y;
-  y = xor_lane<4>(x);
-  return static_cast<uint32_t>(x > y ? x : y);
+// The largest `value` of the 32 / E lanes of a block.
+template <int E>
+__device__ __forceinline__ uint32_t block_max(uint32_t value) {
+  const auto with = [&](int other) { value = value > static_cast<uint32_t>(other) ? value : static_cast<uint32_t>(other); };
+  with(xor_lane<1>(static_cast<int>(value)));
+  with(xor_lane<2>(static_cast<int>(value)));
+  if constexpr (E == 4) with(xor_lane<4>(static_cast<int>(value)));
+  return value;
+}
+
+// A lane's E codes, four to a word.
+template <int E>
+struct Codes {
+  uint32_t word[E / 4];
+};
+template <int E>
+__device__ __forceinline__ Codes<E> load_codes(const void* p, int64_t at) {
+  Codes<E> out;
+  const Global<uint32_t>* words = global(static_cast<uint32_t*>(const_cast<void*>(p))) + at / 4;
+#pragma unroll
+  for (int i = 0; i < E / 4; ++i) out.word[i] = words[i];
+  return out;
+}
+template <int E>
+__device__ __forceinline__ void store_codes(void* p, int64_t at, const Codes<E>& codes) {
+  Global<uint32_t>* words = global(static_cast<uint32_t*>(p)) + at / 4;
+#pragma unroll
+  for (int i = 0; i < E / 4; ++i) words[i] = codes.word[i];
 }
 
 // A signed code has a sign bit and 16 binades, an unsigned one 32.
 template <bool kSigned>
 constexpr uint32_t kBinades = kSigned ? 16u : 32u;
 
-template <bool kSigned>
-__device__ __forceinline__ float decode(uint32_t code, uint32_t top) {
-  const uint32_t c = kSigned ? code & 0x7Fu : code;
-  uint32_t word = c == 0 ? 0u : (c + ((top - kBinades<kSigned> + 1u) << 3)) << 20;
-  if (kSigned) word |= (code & 0x80u) << 24;
-  return top == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(word);
+// The value of code `i` where the scale is not 255 (then the whole block stands
+// for NaN: poison_of).
+template <bool kSigned, int E>
+__device__ __forceinline__ float decode(const Codes<E>& codes, int i, uint32_t top) {
+  const uint32_t word = codes.word[i / 4];
+  const uint32_t c = __builtin_amdgcn_ubfe(word, 8 * (i & 3), kSigned ? 7 : 8);
+  const uint32_t magnitude = c == 0u ? 0u : (c + ((top - kBinades<kSigned> + 1u) << 3)) << 20;
+  if (!kSigned) return __uint_as_float(magnitude);
+  return __uint_as_float((word << (24 - 8 * (i & 3)) & 0x80000000u) | magnitude);
 }
 
-// The shared exponent of the 32 values held by 8 consecutive lanes, and this
-// lane's four codes.  A block with an infinity or NaN takes X = 255 and stands
-// for NaN.  `random16`: 16 bits a value, compared with the 20 bits cut off.
-template <bool kSigned>
-__device__ __forceinline__ uint32_t encode4(const float (&value)[4], const uint32_t (&random16)[4], uint32_t& top) {
-  uint32_t word[4], most = kBinades<kSigned>;
+__device__ __forceinline__ float poison_of(uint32_t top) { return top == 255u ? NAN : 0.0f; }
+
+// The shared exponent of a block, and this lane's codes.  A block with an
+// infinity or NaN takes X = 255 and stands for NaN.  `random`: 16 bits a value
+// (its lower or upper half), compared with the 20 bits cut off.
+template <bool kSigned, int E>
+__device__ __forceinline__ Codes<E> encode(const float (&value)[E], const uint32_t (&random)[E], uint32_t& top) {
+  const auto half_of = [&](int i) { return kSigned ? random[i] & 0xFFFFu : random[i] >> 16; };
+  uint32_t word[E], most = 0u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    word[i] = __float_as_uint(value[i]) & 0x7FFFFFFFu;
-    const uint32_t exponent = (word[i] + 0xFFFFFu) >> 23;
-    most = exponent > most ? exponent : most;
+  for (int i = 0; i < E; ++i) {
+    word[i] = kSigned ? __float_as_uint(value[i]) & 0x7FFFFFFFu : __float_as_uint(value[i]);
+    most = word[i] > most ? word[i] : most;
   }
-  most = group8_max(most);
+  most = (block_max<E>(most) + 0xFFFFFu) >> 23;
+  most = most > kBinades<kSigned> ? most : kBinades<kSigned>;
   top = most < 255u ? most : 255u;
   const uint32_t low = (top - kBinades<kSigned> + 1u) << 3;
-  const float least = __uint_as_float((low + 1u) << 20);
-  uint32_t packed = 0;
+  int code[E], least_code = 1;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    int code = static_cast<int>((word[i] + (random16[i] << 4)) >> 20) - static_cast<int>(low);
-    if (kSigned) {
-      // below the least code: up to it as often as the value's share of it
-      const float share = least * (static_cast<float>(random16[i]) * 1.52587890625e-5f);
-      if (code < 1) code = __uint_as_float(word[i]) > share ? 1 : 0;
-      code = (code & 0x7F) | static_cast<int>((__float_as_uint(value[i]) >> 24) & 0x80u);
-    } else if (code < 1) {
-      code = word[i] != 0u ? 1 : 0;
+  for (int i = 0; i < E; ++i) {
+    code[i] = static_cast<int>((word[i] + (half_of(i) << 4)) >> 20) - static_cast<int>(low);
+    least_code = code[i] < least_code ? code[i] : least_code;
+  }
+  // below the least code (few values are): a first moment goes up to it as often
+  // as it is its share of it, a second moment unless it is 0
+  if (least_code < 1) {
+    const float least = __uint_as_float((low + 1u) << 20);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (code[i] < 1) {
+        if (kSigned) code[i] = __uint_as_float(word[i]) > least * (static_cast<float>(half_of(i)) * 1.52587890625e-5f) ? 1 : 0;
+        else code[i] = word[i] != 0u ? 1 : 0;
+      }
+  }
+  Codes<E> packed;
+#pragma unroll
+  for (int w = 0; w < E / 4; ++w) {
+    packed.word[w] = 0u;
+#pragma unroll
+    for (int i = 4 * w; i < 4 * w + 4; ++i) {
+      uint32_t byte = static_cast<uint32_t>(code[i]);
+      if (kSigned) byte = (byte & 0x7Fu) | (__float_as_uint(value[i]) >> 24 & 0x80u);
+      else byte &= 0xFFu;
+      packed.word[w] |= byte << (8 * (i & 3));
     }
-    packed |= (static_cast<uint32_t>(code) & 0xFFu) << (8 * i);
   }
   return packed;
 }
@@ -222,96 +289,96 @@ __device__ __forceinline__ uint32_t random_key(const UpdateScalars& s, int64_t t
   return mix(s.seed_low ^ mix(s.seed_high + mix(static_cast<uint32_t>(t) + high * 0x9E3779B1u)));
 }
 
+// Elements of a lane's vector.
+template <typename P, int kBits>
+constexpr int kElements = kBits == 8 && sizeof(P) == 2 ? 8 : 4;
+
 template <typename P, typename G, int kBits, bool kWhole>
 __device__ __forceinline__ void adamw_update_chunk(const Record& r, int64_t begin, const UpdateScalars& s) {
   constexpr bool kRandom = kBits == 8 || sizeof(P) == 2;
+  constexpr int E = kElements<P, kBits>, K = kChunk / (kBlock * E);
   P* const param = static_cast<P*>(r.param);
   const G* const grad = static_cast<const G*>(r.grad);
   const int64_t count = r.count;
   const int64_t padded = (count + kSpan - 1) / kSpan * kSpan;
   const float factor = r.factor, decay = r.decay, step_size = r.step_size, inverse_root = r.inverse_root;
-  fvec<4> p[kVectors], g[kVectors], m[kVectors], v[kVectors];
-  uint32_t m_code[kVectors], v_code[kVectors], m_top[kVectors], v_top[kVectors];
+  Floats<E> p[K], g[K], m[K], v[K];
+  Codes<E> m_codes[K], v_codes[K];
+  uint32_t m_top[K], v_top[K];
 #pragma unroll
-  for (int k = 0; k < kVectors; ++k) {
-    const int64_t at = begin + (k * kBlock + static_cast<int>(threadIdx.x)) * 4;
-    p[k] = load4<kWhole>(param, at, count);
-    g[k] = load4<kWhole>(grad, at, count);
+  for (int k = 0; k < K; ++k) {
+    const int64_t at = begin + (k * kBlock + static_cast<int>(threadIdx.x)) * E;
+    p[k] = load<kWhole, E>(param, at, count);
+    g[k] = load<kWhole, E>(grad, at, count);
     if constexpr (kBits == 32) {
-      m[k] = load4<kWhole>(static_cast<const float*>(r.exp_avg), at, count);
-      v[k] = load4<kWhole>(static_cast<const float*>(r.exp_avg_sq), at, count);
+      m[k] = load<kWhole, E>(static_cast<const float*>(r.exp_avg), at, count);
+      v[k] = load<kWhole, E>(static_cast<const float*>(r.exp_avg_sq), at, count);
     } else {
       const bool live = kWhole || at < padded;
-      m_code[k] = live ? static_cast<const uint32_t*>(r.exp_avg)[at / 4] : 0u;
-      v_code[k] = live ? static_cast<const uint32_t*>(r.exp_avg_sq)[at / 4] : 0u;
-      m_top[k] = live ? r.exp_avg_scale[at / kSpan] : kBinades<true>;
-      v_top[k] = live ? r.exp_avg_sq_scale[at / kSpan] : kBinades<false>;
+      m_codes[k] = live ? load_codes<E>(r.exp_avg, at) : Codes<E>{};
+      v_codes[k] = live ? load_codes<E>(r.exp_avg_sq, at) : Codes<E>{};
+      m_top[k] = live ? global(r.exp_avg_scale)[at / kSpan] : kBinades<true>;
+      v_top[k] = live ? global(r.exp_avg_sq_scale)[at / kSpan] : kBinades<false>;
     }
   }
   const uint32_t high = static_cast<uint32_t>((r.position + begin) >> 32);
   const uint32_t key = kRandom ? random_key(s, r.step, high) : 0u;
 #pragma unroll
-  for (int k = 0; k < kVectors; ++k) {
-    const int64_t at = begin + (k * kBlock + static_cast<int>(threadIdx.x)) * 4;
-    float new_p[4], new_m[4], new_v[4];
+  for (int k = 0; k < K; ++k) {
+    const int64_t at = begin + (k * kBlock + static_cast<int>(threadIdx.x)) * E;
+    float new_p[E], new_m[E], new_v[E];
+    const float m_poison = kBits == 8 ? poison_of(m_top[k]) : 0.0f, v_poison = kBits == 8 ? poison_of(v_top[k]) : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float old_m, old_v;
-      if constexpr (kBits == 32) {
-        old_m = m[k].v[i];
-        old_v = v[k].v[i];
-      } else {
-        old_m = decode<true>(m_code[k] >> (8 * i) & 0xFFu, m_top[k]);
-        old_v = decode<false>(v_code[k] >> (8 * i) & 0xFFu, v_top[k]);
-      }
+    for (int i = 0; i < E; ++i) {
       const float scaled = g[k].v[i] * factor;
-      new_m[i] = old_m * s.beta1 + scaled * s.rest1;
-      new_v[i] = old_v * s.beta2 + (scaled * scaled) * s.rest2;
+      if constexpr (kBits == 32) {
+        new_m[i] = m[k].v[i] * s.beta1 + scaled * s.rest1;
+        new_v[i] = v[k].v[i] * s.beta2 + (scaled * scaled) * s.rest2;
+      } else {
+        new_m[i] = decode<true, E>(m_codes[k], i, m_top[k]) * (s.beta1 + m_poison) + scaled * s.rest1;
+        new_v[i] = decode<false, E>(v_codes[k], i, v_top[k]) * (s.beta2 + v_poison) + (scaled * scaled) * s.rest2;
+      }
       new_p[i] = p[k].v[i] * decay - (new_m[i] / (sqrtf(new_v[i]) * inverse_root + s.eps)) * step_size;
     }
-    uint32_t bits[4];
+    uint32_t bits[E];
     if constexpr (kRandom) {
       const uint64_t position = r.position + at;
       const uint32_t own_high = static_cast<uint32_t>(position >> 32);
       const uint32_t own_key = own_high == high ? key : random_key(s, r.step, own_high);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bits[i] = mix((static_cast<uint32_t>(position) + i) ^ own_key);
+      for (int i = 0; i < E; ++i) bits[i] = mix((static_cast<uint32_t>(position) + i) ^ own_key);
     }
     if constexpr (sizeof(P) == 2) {
-      P rounded[4];
+      P rounded[E];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < E; ++i) {
         const uint32_t word = __float_as_uint(new_p[i]);
         const uint32_t noise = mix(bits[i] + 0x9E3779B1u) & 0xFFFFu;
         // infinities stay, NaN stays NaN (quiet)
-        const bool finite = (word & 0x7F800000u) != 0x7F800000u;
-        const uint32_t special = (word & 0x007FFFFFu) != 0u ? word | 0x00400000u : word;
-        rounded[i] = static_cast<P>((finite ? word + noise : special) >> 16);
+        const uint32_t kept = __builtin_isnan(new_p[i]) ? word | 0x00400000u : word;
+        rounded[i] = static_cast<P>((__builtin_isfinite(new_p[i]) ? word + noise : kept) >> 16);
       }
-      store4<kWhole>(param, at, count, rounded);
+      store<kWhole, E>(param, at, count, rounded);
     } else {
-      store4<kWhole>(param, at, count, new_p);
+      store<kWhole, E>(param, at, count, new_p);
     }
     if constexpr (kBits == 32) {
-      store4<kWhole>(static_cast<float*>(r.exp_avg), at, count, new_m);
-      store4<kWhole>(static_cast<float*>(r.exp_avg_sq), at, count, new_v);
+      store<kWhole, E>(static_cast<float*>(r.exp_avg), at, count, new_m);
+      store<kWhole, E>(static_cast<float*>(r.exp_avg_sq), at, count, new_v);
     } else {
-      uint32_t low[4], upper[4];
+      if (!kWhole)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        low[i] = bits[i] & 0xFFFFu;
-        upper[i] = bits[i] >> 16;
-        if (!kWhole && at + i >= count) new_m[i] = new_v[i] = 0.0f;  // padding stays 0
-      }
+        for (int i = 0; i < E; ++i)
+          if (at + i >= count) new_m[i] = new_v[i] = 0.0f;  // padding stays 0
       uint32_t top_m, top_v;
-      const uint32_t packed_m = encode4<true>(new_m, low, top_m);
-      const uint32_t packed_v = encode4<false>(new_v, upper, top_v);
+      const Codes<E> packed_m = encode<true, E>(new_m, bits, top_m);
+      const Codes<E> packed_v = encode<false, E>(new_v, bits, top_v);
       if (kWhole || at < padded) {
-        static_cast<uint32_t*>(r.exp_avg)[at / 4] = packed_m;
-        static_cast<uint32_t*>(r.exp_avg_sq)[at / 4] = packed_v;
-        if ((threadIdx.x & 7) == 0) {
-          r.exp_avg_scale[at / kSpan] = static_cast<uint8_t>(top_m);
-          r.exp_avg_sq_scale[at / kSpan] = static_cast<uint8_t>(top_v);
+        store_codes<E>(r.exp_avg, at, packed_m);
+        store_codes<E>(r.exp_avg_sq, at, packed_v);
+        if ((threadIdx.x & (kSpan / E - 1)) == 0) {
+          global(r.exp_avg_scale)[at / kSpan] = static_cast<uint8_t>(top_m);
+          global(r.exp_avg_sq_scale)[at / kSpan] = static_cast<uint8_t>(top_v);
         }
       }
     }
@@ -342,6 +409,48 @@ __global__ __launch_bounds__(kBlock) void adamw_values_kernel(PointerList list, 
   if (i < count) records[first + i].values[which] = static_cast<float*>(const_cast<void*>(list.p[i]));
 }
 
+template <bool kRead, bool kWhole>
+__device__ __forceinline__ void adamw_codes_chunk(const Record& r, int64_t begin) {
+  constexpr int E = 4;
+  const int64_t count = r.count;
+  const int64_t padded = (count + kSpan - 1) / kSpan * kSpan;
+#pragma unroll
+  for (int k = 0; k < kChunk / (kBlock * E); ++k) {
+    const int64_t at = begin + (k * kBlock + static_cast<int>(threadIdx.x)) * E;
+    const bool live = kWhole || at < padded;
+    if constexpr (kRead) {
+      if (!live) continue;
+      const Codes<E> m_codes = load_codes<E>(r.exp_avg, at), v_codes = load_codes<E>(r.exp_avg_sq, at);
+      const uint32_t m_top = global(r.exp_avg_scale)[at / kSpan], v_top = global(r.exp_avg_sq_scale)[at / kSpan];
+      float m[E], v[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        m[i] = m_top == 255u ? NAN : decode<true, E>(m_codes, i, m_top);
+        v[i] = v_top == 255u ? NAN : decode<false, E>(v_codes, i, v_top);
+      }
+      store<kWhole, E>(r.values[0], at, count, m);
+      store<kWhole, E>(r.values[1], at, count, v);
+    } else {
+      // every lane takes part in the exponent of its block
+      const Floats<E> m = load<kWhole, E>(r.values[0], at, count);
+      const Floats<E> v = load<kWhole, E>(r.values[1], at, count);
+      uint32_t half[E], top_m, top_v;
+#pragma unroll
+      for (int i = 0; i < E; ++i) half[i] = 0x80008000u;
+      const Codes<E> packed_m = encode<true, E>(m.v, half, top_m);
+      const Codes<E> packed_v = encode<false, E>(v.v, half, top_v);
+      if (live) {
+        store_codes<E>(r.exp_avg, at, packed_m);
+        store_codes<E>(r.exp_avg_sq, at, packed_v);
+        if ((threadIdx.x & (kSpan / E - 1)) == 0) {
+          global(r.exp_avg_scale)[at / kSpan] = static_cast<uint8_t>(top_m);
+          global(r.exp_avg_sq_scale)[at / kSpan] = static_cast<uint8_t>(top_v);
+        }
+      }
+    }
+  }
+}
+
 // kRead: codes to values.  Otherwise values to the nearest codes.
 template <bool kRead>
 __global__ __launch_bounds__(kBlock) void adamw_codes_kernel(const Record* __restrict__ records,
@@ -350,51 +459,9 @@ __global__ __launch_bounds__(kBlock) void adamw_codes_kernel(const Record* __res
   if (block >= n_chunks) return;
   const Chunk chunk = chunks[block];
   const Record& r = records[chunk.tensor];
-  float* const m_values = r.values[0];
-  float* const v_values = r.values[1];
-  const int64_t count = r.count;
-  const int64_t padded = (count + kSpan - 1) / kSpan * kSpan;
-#pragma unroll
-  for (int k = 0; k < kVectors; ++k) {
-    const int64_t at = static_cast<int64_t>(chunk.index) * kChunk + (k * kBlock + static_cast<int>(threadIdx.x)) * 4;
-    const bool live = at < padded;
-    const bool whole = at + 4 <= count;
-    if constexpr (kRead) {
-      if (!live) continue;
-      const uint32_t m_code = static_cast<const uint32_t*>(r.exp_avg)[at / 4];
-      const uint32_t v_code = static_cast<const uint32_t*>(r.exp_avg_sq)[at / 4];
-      const uint32_t m_top = r.exp_avg_scale[at / kSpan], v_top = r.exp_avg_sq_scale[at / kSpan];
-      float m[4], v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m[i] = decode<true>(m_code >> (8 * i) & 0xFFu, m_top);
-        v[i] = decode<false>(v_code >> (8 * i) & 0xFFu, v_top);
-      }
-      if (whole) {
-        store4<true>(m_values, at, count, m);
-        store4<true>(v_values, at, count, v);
-      } else {
-        store4<false>(m_values, at, count, m);
-        store4<false>(v_values, at, count, v);
-      }
-    } else {
-      // every lane takes part in the exponents of its 8 lanes
-      const fvec<4> m = whole ? load4<true>(m_values, at, count) : load4<false>(m_values, at, count);
-      const fvec<4> v = whole ? load4<true>(v_values, at, count) : load4<false>(v_values, at, count);
-      const uint32_t half[4] = {0x8000u, 0x8000u, 0x8000u, 0x8000u};
-      uint32_t top_m, top_v;
-      const uint32_t packed_m = encode4<true>(m.v, half, top_m);
-      const uint32_t packed_v = encode4<false>(v.v, half, top_v);
-      if (live) {
-        static_cast<uint32_t*>(r.exp_avg)[at / 4] = packed_m;
-        static_cast<uint32_t*>(r.exp_avg_sq)[at / 4] = packed_v;
-        if ((threadIdx.x & 7) == 0) {
-          r.exp_avg_scale[at / kSpan] = static_cast<uint8_t>(top_m);
-          r.exp_avg_sq_scale[at / kSpan] = static_cast<uint8_t>(top_v);
-        }
-      }
-    }
-  }
+  const int64_t begin = static_cast<int64_t>(chunk.index) * kChunk;
+  if (r.count - begin >= kChunk) adamw_codes_chunk<kRead, true>(r, begin);
+  else adamw_codes_chunk<kRead, false>(r, begin);
 }
 
 // ---------------------------------------------------------------------------
@@ -408,7 +475,7 @@ __global__ __launch_bounds__(kBlock) void adamw_codes_kernel(const Record* __res
 
 constexpr int kNormTensors = 180;
 constexpr int kNormBlocks = 2048;      // workgroups of one launch
-constexpr int kNormChunk = 8192;       // elements
+constexpr int kNormChunk = 2048;       // elements
 
 struct NormList {
   const void* p[kNormTensors];
@@ -416,23 +483,37 @@ struct NormList {
   uint32_t first[kNormTensors + 1];    // chunks before each tensor
 };
 
+// The squares of elements [begin, end), over the threads of a workgroup.
 template <typename T>
-__device__ __forceinline__ double chunk_squares(const T* __restrict__ p, int64_t begin, int64_t count) {
-  double sum = 0.0;
-  if (count - begin >= kNormChunk) {
+__device__ __forceinline__ double run_squares(const T* __restrict__ p, int64_t begin, int64_t end) {
+  constexpr int E = kWide<T>, U = 32 / E;  // 32 elements of a thread in flight
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  int64_t at = begin;
+  for (; at + U * kBlock * E <= end; at += U * kBlock * E) {
+    Floats<E> g[U];
 #pragma unroll
-    for (int k = 0; k < kNormChunk / (kBlock * 4); ++k) {
-      const fvec<4> g = load4<true>(p, begin + (k * kBlock + static_cast<int>(threadIdx.x)) * 4, count);
+    for (int k = 0; k < U; ++k) g[k] = load<true, E>(p, at + (k * kBlock + static_cast<int>(threadIdx.x)) * E, end);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum = __builtin_fma(static_cast<double>(g.v[i]), static_cast<double>(g.v[i]), sum);
-    }
-  } else {
-    for (int64_t at = begin + threadIdx.x; at < count; at += kBlock) {
-      const double g = to_float(p[at]);
-      sum = __builtin_fma(g, g, sum);
-    }
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        sum[i & 3] = __builtin_fma(static_cast<double>(g[k].v[i]), static_cast<double>(g[k].v[i]), sum[i & 3]);
   }
-  return sum;
+  // what is left, 8 elements of a thread in flight: places past the end repeat
+  // the last one and count as 0, so that no load sits in a branch (one element a
+  // thread at a time took as long as the whole of a large tensor)
+  for (; at < end; at += 8 * kBlock) {
+    float g[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t place = at + k * kBlock + static_cast<int>(threadIdx.x);
+      g[k] = to_float(global(p)[place < end ? place : end - 1]);
+      if (place >= end) g[k] = 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k & 3] = __builtin_fma(static_cast<double>(g[k]), static_cast<double>(g[k]), sum[k & 3]);
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 __device__ __forceinline__ double block_sum(double value) {
@@ -457,12 +538,14 @@ __global__ __launch_bounds__(kBlock) void grad_norm_kernel(NormList list, int te
     else high = middle - 1;
   }
   double sum = 0.0;
-  for (uint32_t chunk = begin; chunk < end; ++chunk) {
-    while (chunk >= list.first[low + 1]) ++low;
-    const int64_t at = static_cast<int64_t>(chunk - list.first[low]) * kNormChunk;
+  for (uint32_t chunk = begin; chunk < end; ++low) {  // the run's part of one tensor at a time
+    const uint32_t first = list.first[low], next = list.first[low + 1];
+    const uint32_t last = next < end ? next : end;
     const int64_t count = list.count[low] >> 1;
-    if (list.count[low] & 1) sum += chunk_squares(static_cast<const uint16_t*>(list.p[low]), at, count);
-    else sum += chunk_squares(static_cast<const float*>(list.p[low]), at, count);
+    const int64_t from = static_cast<int64_t>(chunk - first) * kNormChunk, to = static_cast<int64_t>(last - first) * kNormChunk;
+    if (list.count[low] & 1) sum += run_squares(static_cast<const uint16_t*>(list.p[low]), from, to < count ? to : count);
+    else sum += run_squares(static_cast<const float*>(list.p[low]), from, to < count ? to : count);
+    chunk = last > chunk ? last : chunk;
   }
   const double total = block_sum(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = total;

@@ -24,7 +24,9 @@ points are the operators of a training step.
 from __future__ import annotations
 
 import ctypes
+import operator
 import weakref
+from array import array
 
 import torch
 
@@ -863,66 +865,68 @@ def _group_norm_sizes(x, groups, scale, bias, offsets):
     """(samples, entries, inner, channels) of a call, its tensors checked."""
     _check(isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in ELEMENT_TYPES and x.is_contiguous(),
            "group norm input: expected a contiguous gfx950 float32, bfloat16 or float16 tensor")
-    _check(x.dim() >= 2, "group norm input must have at least two dimensions")
-    channels = int(x.shape[-1])
+    shape = x.shape
+    _check(len(shape) >= 2, "group norm input must have at least two dimensions")
+    entries, channels = shape[0], shape[-1]
     _check(1 <= channels <= GROUP_NORM_MAX_CHANNELS and groups >= 1 and channels % groups == 0,
            f"group norm takes 1 to {GROUP_NORM_MAX_CHANNELS} channels in groups of equal size")
     for what, tensor in (("scale", scale), ("bias", bias)):
         if tensor is not None:
-            _f32(tensor, f"group norm {what}")
-            _check(tuple(tensor.shape) == (channels,), f"group norm {what} must have shape (channels,)")
-    entries = int(x.shape[0])
-    inner = 1
-    for size in x.shape[1:-1]:
-        inner *= int(size)
+            _f32(tensor, what)
+            _check(tensor.shape == (channels,), f"group norm {what} must have shape (channels,)")
     samples = entries if offsets is None else _offsets(offsets, "group norm offsets")
     _same_device(x, scale, bias, offsets)
+    inner = 1
+    for size in shape[1:-1]:
+        inner *= size
     return samples, entries, inner, channels
 
 
 def group_norm_forward(x, groups, scale=None, bias=None, offsets=None, eps: float = 1.0e-5, silu: bool = False, *,
                        max_rows=None):
-    """``(y, mean, rstd)``; ``mean`` and ``rstd`` are ``(samples, groups)`` float32."""
+    """``(y, statistics)``; ``statistics`` is ``(2, samples, groups)`` float32: means and 1 / sqrt(var + eps)."""
     groups = int(groups)
     samples, entries, inner, channels = _group_norm_sizes(x, groups, scale, bias, offsets)
+    device = x.device
     y = torch.empty_like(x)
-    statistics = torch.empty((2, samples, groups), dtype=torch.float32, device=x.device)
-    mean, rstd = statistics[0], statistics[1]
+    statistics = torch.empty((2, samples, groups), dtype=torch.float32, device=device)
     code = ELEMENT_TYPES[x.dtype]
     most = -1 if max_rows is None else min(int(max_rows), entries)
     nbytes = _LIB.dpa4k_group_norm_workspace_size(samples, entries, inner, channels, groups, offsets is not None, most, code, 0)
-    workspace = _workspace(nbytes, x.device)
-    with _on(x.device) as stream:
+    workspace = _workspace(nbytes, device) if nbytes else None
+    mean = statistics.data_ptr()
+    with _on(device) as stream:
         status = _LIB.dpa4k_group_norm_forward(
-            _ptr(x), _ptr(scale), _ptr(bias), _ptr(offsets), _ptr(y), _ptr(mean), _ptr(rstd), samples, entries, inner,
-            channels, groups, most, float(eps), int(bool(silu)), code, workspace.data_ptr(), nbytes, stream)
+            _ptr(x), _ptr(scale), _ptr(bias), _ptr(offsets), _ptr(y), mean, mean + 4 * samples * groups, samples, entries,
+            inner, channels, groups, most, float(eps), bool(silu), code, _ptr(workspace), nbytes, stream)
     _lib.check(status)
-    return y, mean, rstd
+    return y, statistics
 
 
-def group_norm_backward(grad_output, x, groups, scale, bias, offsets, mean, rstd, silu: bool = False, *,
+def group_norm_backward(grad_output, x, groups, scale, bias, offsets, statistics, silu: bool = False, *,
                         want_x: bool = True, want_scale: bool = True, want_bias: bool = True, max_rows=None):
     """``(grad_x, grad_scale, grad_bias)``, None where not wanted."""
     groups = int(groups)
     samples, entries, inner, channels = _group_norm_sizes(x, groups, scale, bias, offsets)
     _check(isinstance(grad_output, torch.Tensor) and grad_output.is_contiguous() and grad_output.dtype == x.dtype
            and grad_output.shape == x.shape, "group norm grad_output must be like the input")
-    for tensor in (mean, rstd):
-        _f32(tensor, "group norm statistics")
-        _check(tuple(tensor.shape) == (samples, groups), "group norm statistics must have shape (samples, groups)")
-    _same_device(x, grad_output, mean, rstd)
+    _f32(statistics, "group norm statistics")
+    _check(statistics.shape == (2, samples, groups), "group norm statistics must have shape (2, samples, groups)")
+    _same_device(x, grad_output, statistics)
+    device = x.device
     grad_x = torch.empty_like(x) if want_x else None
-    grad_scale = torch.empty((channels,), dtype=torch.float32, device=x.device) if want_scale else None
-    grad_bias = torch.empty((channels,), dtype=torch.float32, device=x.device) if want_bias else None
+    grad_scale = torch.empty((channels,), dtype=torch.float32, device=device) if want_scale else None
+    grad_bias = torch.empty((channels,), dtype=torch.float32, device=device) if want_bias else None
     code = ELEMENT_TYPES[x.dtype]
     most = -1 if max_rows is None else min(int(max_rows), entries)
     nbytes = _LIB.dpa4k_group_norm_workspace_size(samples, entries, inner, channels, groups, offsets is not None, most, code, 1)
-    workspace = _workspace(nbytes, x.device)
-    with _on(x.device) as stream:
+    workspace = _workspace(nbytes, device) if nbytes else None
+    mean = statistics.data_ptr()
+    with _on(device) as stream:
         status = _LIB.dpa4k_group_norm_backward(
-            _ptr(grad_output), _ptr(x), _ptr(scale), _ptr(bias), _ptr(offsets), _ptr(mean), _ptr(rstd), _ptr(grad_x),
-            _ptr(grad_scale), _ptr(grad_bias), samples, entries, inner, channels, groups, most, int(bool(silu)), code,
-            workspace.data_ptr(), nbytes, stream)
+            _ptr(grad_output), _ptr(x), _ptr(scale), _ptr(bias), _ptr(offsets), mean, mean + 4 * samples * groups,
+            _ptr(grad_x), _ptr(grad_scale), _ptr(grad_bias), samples, entries, inner, channels, groups, most, bool(silu),
+            code, _ptr(workspace), nbytes, stream)
     _lib.check(status)
     return grad_x, grad_scale, grad_bias
 
@@ -931,33 +935,39 @@ def group_norm_backward(grad_output, x, groups, scale, bias, offsets, mean, rstd
 # optimiser step (no reference implementation)
 # ---------------------------------------------------------------------------
 
-def _addresses(tensors, n: int):
-    """A host array of the tensors' device addresses; None stands for NULL."""
-    return (ctypes.c_void_p * n)(*[None if t is None else t.data_ptr() for t in tensors])
+def _addresses(tensors):
+    """The tensors' device addresses as a host array; None stands for 0."""
+    try:
+        return array("Q", map(torch.Tensor.data_ptr, tensors))
+    except TypeError:
+        return array("Q", [0 if t is None else t.data_ptr() for t in tensors])
 
 
 def grad_norm(grads, max_norm: float = 0.0):
     """``(norm, factor)`` of contiguous float32 or bfloat16 tensors on one device (at least one)."""
     n = len(grads)
     _check(n >= 1, "gradient norm needs at least one gradient")
+    dtypes = list(map(_DTYPE_OF, grads))
+    kinds = set(dtypes)
+    _check(kinds <= {torch.float32, torch.bfloat16}, "gradient norm: expected float32 or bfloat16 tensors")
+    _check(all(map(torch.Tensor.is_contiguous, grads)), "gradient norm: expected contiguous tensors")
+    devices = set(map(torch.Tensor.get_device, grads))
+    _check(len(devices) == 1 and -1 not in devices, "gradient norm: expected gfx950 tensors on one device")
     device = grads[0].device
-    types = [g.dtype for g in grads]
-    _check(all(t in (torch.float32, torch.bfloat16) for t in set(types)),
-           "gradient norm: expected float32 or bfloat16 tensors")
-    _check(all([g.is_contiguous() for g in grads]), "gradient norm: expected contiguous tensors")
-    _check(device.type == "cuda" and all([g.device == device for g in grads]),
-           "gradient norm: expected gfx950 tensors on one device")
-    counts = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
-    codes = (ctypes.c_int32 * n)(*[ELEMENT_TYPES[t] for t in types])
+    addresses, counts = _addresses(grads), array("q", map(torch.Tensor.numel, grads))
+    codes = array("i", [ELEMENT_TYPES[grads[0].dtype]]) * n if len(kinds) == 1 else array("i", map(ELEMENT_TYPES.get, dtypes))
     result = torch.empty((2,), dtype=torch.float32, device=device)
-    nbytes = _LIB.dpa4k_grad_norm_workspace_size(counts, n)
+    at = result.data_ptr()
+    nbytes = _LIB.dpa4k_grad_norm_workspace_size(counts.buffer_info()[0], n)
     workspace = _workspace(nbytes, device)
     with _on(device) as stream:
-        status = _LIB.dpa4k_grad_norm(_addresses(grads, n), counts, codes, n, float(max_norm), result.data_ptr(),
-                                      result.data_ptr() + 4, workspace.data_ptr(), nbytes, stream)
+        status = _LIB.dpa4k_grad_norm(addresses.buffer_info()[0], counts.buffer_info()[0], codes.buffer_info()[0], n,
+                                      float(max_norm), at, at + 4, workspace.data_ptr(), nbytes, stream)
     _lib.check(status)
-    return result[0], result[1]
+    return result.unbind()
 
+
+_DTYPE_OF = operator.attrgetter("dtype")
 
 ADAMW_SPAN = 32   # elements that share a scale
 
@@ -967,11 +977,12 @@ class AdamWPlan:
 
     def __init__(self, params, state_bits):
         self.params = params
+        self.count = len(params)
         self.state_bits = state_bits
         self.dtype = params[0].dtype
         self.device = params[0].device
         self.shapes = [p.shape for p in params]
-        self.addresses = [p.data_ptr() for p in params]
+        self.addresses = _addresses(params)
         self.exp_avgs = self.exp_avg_sqs = None             # 32 bits: float32 tensors
         self.codes = self.scales = None                     # 8 bits: (2, padded) and (2, padded / 32) bytes
         self.words = None
@@ -1029,10 +1040,10 @@ def adamw_plan(params, exp_avgs, exp_avg_sqs, steps, state_bits: int) -> AdamWPl
 
 
 def _move_states(entry_point, plan, exp_avgs, exp_avg_sqs) -> None:
-    n = len(plan.params)
+    first, second = _addresses(exp_avgs), _addresses(exp_avg_sqs)
     with _on(plan.device) as stream:
-        status = entry_point(plan.words.data_ptr(), n, plan.n_chunks, _addresses(exp_avgs, n),
-                             _addresses(exp_avg_sqs, n), stream)
+        status = entry_point(plan.words.data_ptr(), len(plan.params), plan.n_chunks, first.buffer_info()[0],
+                             second.buffer_info()[0], stream)
     _lib.check(status)
 
 
@@ -1041,13 +1052,14 @@ def adamw_read_states(plan, exp_avgs, exp_avg_sqs) -> None:
     _move_states(_LIB.dpa4k_adamw_read_states, plan, exp_avgs, exp_avg_sqs)
 
 
-def adamw_step(plan, addresses, grad_dtype, lr: float, lr_tensor, beta1: float, beta2: float, eps: float,
+def adamw_step(plan, grads, grad_dtype, lr: float, lr_tensor, beta1: float, beta2: float, eps: float,
                weight_decay: float, grad_factor, seed: int) -> None:
-    """One step; ``addresses``: a gradient's device address per tensor, None or 0 where it has none."""
-    n = len(plan.params)
+    """One step; ``grads``: checked gradients of one dtype, None where a tensor takes no step."""
+    n = plan.count
+    addresses = _addresses(grads)
     with _on(plan.device) as stream:
         status = _LIB.dpa4k_adamw_step(
             plan.words.data_ptr(), n, plan.n_chunks, plan.state_bits, ELEMENT_TYPES[plan.dtype],
-            ELEMENT_TYPES[grad_dtype], (ctypes.c_void_p * n)(*addresses), lr, _ptr(lr_tensor), beta1, beta2, eps,
+            ELEMENT_TYPES[grad_dtype], addresses.buffer_info()[0], lr, _ptr(lr_tensor), beta1, beta2, eps,
             weight_decay, _ptr(grad_factor), seed & 0xFFFFFFFFFFFFFFFF, stream)
     _lib.check(status)

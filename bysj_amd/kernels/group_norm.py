@@ -85,20 +85,19 @@ class _GroupNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, offsets, groups, max_rows, eps, silu):
         native = _extension("group_norm_forward")
-        y, mean, rstd = native.group_norm_forward(x, groups, scale, bias, offsets, eps, silu,
-                                                  max_rows=max_rows)
-        ctx.save_for_backward(x, scale, bias, offsets, mean, rstd)
+        y, statistics = native.group_norm_forward(x, groups, scale, bias, offsets, eps, silu, max_rows=max_rows)
+        ctx.save_for_backward(x, scale, bias, offsets, statistics)
         ctx.arguments = groups, max_rows, silu
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        x, scale, bias, offsets, mean, rstd = ctx.saved_tensors
+        x, scale, bias, offsets, statistics = ctx.saved_tensors
         groups, max_rows, silu = ctx.arguments
         want = ctx.needs_input_grad
         native = _extension("group_norm_backward")
-        grads = native.group_norm_backward(grad_output.contiguous(), x, groups, scale, bias, offsets, mean, rstd, silu,
+        grads = native.group_norm_backward(grad_output.contiguous(), x, groups, scale, bias, offsets, statistics, silu,
                                            want_x=want[0], want_scale=want[1], want_bias=want[2], max_rows=max_rows)
         return (*grads, None, None, None, None, None)
 

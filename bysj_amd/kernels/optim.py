@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import math
 import numbers
+import operator
 
 import torch
 
@@ -30,13 +31,17 @@ from .native import _extension, require_dcu
 DTYPES = (torch.float32, torch.bfloat16)
 STATE_BITS = (32, 8)
 
+# A model has hundreds of tensors and a step a few kernels of some microseconds,
+# so lists are checked attribute by attribute at the speed of map().
+_DTYPE_OF, _SHAPE_OF, _DEVICE_OF = (operator.attrgetter(name) for name in ("dtype", "shape", "device"))
+
 
 def _tensors(values, what: str, *, allow_none: bool = False) -> list:
     if isinstance(values, torch.Tensor) or not hasattr(values, "__iter__"):
         raise TypeError(f"{what} must be a sequence of tensors")
     values = list(values)
-    for value in values:
-        if not isinstance(value, torch.Tensor) and not (allow_none and value is None):
+    for kind in set(map(type, values)):
+        if not issubclass(kind, torch.Tensor) and not (allow_none and kind is type(None)):
             raise TypeError(f"{what} must be a sequence of tensors")
     return values
 
@@ -72,18 +77,18 @@ def grad_norm(grads, max_norm: float | None = None) -> tuple[torch.Tensor, torch
     1 without ``max_norm``, and NaN where the norm is not finite:
     ``adamw_step`` then takes no step.
     """
-    grads = [g for g in _tensors(grads, "grad_norm gradients", allow_none=True) if g is not None]
+    grads = _tensors(grads, "grad_norm gradients", allow_none=True)
+    if type(None) in set(map(type, grads)):
+        grads = [g for g in grads if g is not None]
     if not grads:
         raise ValueError("grad_norm needs at least one gradient")
     limit = 0.0 if max_norm is None else _real(max_norm, "grad_norm max_norm", 0.0, above=True)
-    device = grads[0].device
-    for g in grads:
-        if g.dtype not in DTYPES:
-            raise TypeError("grad_norm requires float32 or bfloat16 gradients")
-        if not g.is_contiguous():
-            raise ValueError("grad_norm gradients must be contiguous")
-        if g.device != device:
-            raise ValueError("grad_norm gradients must share a device")
+    if not set(map(_DTYPE_OF, grads)) <= set(DTYPES):
+        raise TypeError("grad_norm requires float32 or bfloat16 gradients")
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        raise ValueError("grad_norm gradients must be contiguous")
+    if len(set(map(_DEVICE_OF, grads))) > 1:
+        raise ValueError("grad_norm gradients must share a device")
     require_dcu(grads[0])
     return _extension("grad_norm").grad_norm(grads, limit)
 
@@ -102,11 +107,11 @@ def _moments(values, params, what: str):
     values = _tensors(values, what)
     if len(values) != len(params):
         raise ValueError(f"{what}: expected one tensor per parameter")
-    for value, p in zip(values, params):
-        if value.dtype != torch.float32:
-            raise TypeError(f"{what} must be float32")
-        if value.shape != p.shape or value.device != p.device or not value.is_contiguous():
-            raise ValueError(f"{what} must be contiguous, of the parameters' shapes and device")
+    if values and set(map(_DTYPE_OF, values)) != {torch.float32}:
+        raise TypeError(f"{what} must be float32")
+    if list(map(_SHAPE_OF, values)) != list(map(_SHAPE_OF, params)) or not all(map(torch.Tensor.is_contiguous, values)) \
+            or set(map(_DEVICE_OF, values)) != set(map(_DEVICE_OF, params)):
+        raise ValueError(f"{what} must be contiguous, of the parameters' shapes and device")
     return values
 
 
@@ -169,27 +174,24 @@ def adamw_step(plan, grads, *, lr, betas=(0.9, 0.999), eps: float = 1.0e-8, weig
     overlap in time.
     """
     params = plan.params
+    grads = _tensors(grads, "adamw_step gradients", allow_none=True)
     if len(grads) != len(params):
         raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients")
-    if [p.data_ptr() for p in params] != plan.addresses:
+    if list(map(torch.Tensor.data_ptr, params)) != list(plan.addresses):
         raise RuntimeError("adamw_step: a parameter's memory has moved since the plan was built")
-    try:
-        given = [g for g in grads if g is not None]
-        dtypes = {g.dtype for g in given}
-        addresses = [0 if g is None else g.data_ptr() for g in grads]
-        contiguous = all([g.is_contiguous() for g in given])
-        devices = {g.device for g in given}
-    except AttributeError as error:
-        raise TypeError("adamw_step gradients must be tensors or None") from error
-    if not given:
-        return
+    given, shapes = grads, plan.shapes
+    if type(None) in set(map(type, grads)):
+        given, shapes = [g for g in grads if g is not None], [s for g, s in zip(grads, shapes) if g is not None]
+        if not given:
+            return
+    dtypes = set(map(_DTYPE_OF, given))
     if len(dtypes) != 1 or not dtypes <= set(DTYPES):
         raise TypeError("adamw_step requires gradients of one dtype, float32 or bfloat16")
-    if any([g is not None and g.shape != shape for g, shape in zip(grads, plan.shapes)]):
+    if list(map(_SHAPE_OF, given)) != shapes:
         raise ValueError("adamw_step gradients must have their parameters' shapes")
-    if not contiguous:
+    if not all(map(torch.Tensor.is_contiguous, given)):
         raise ValueError("adamw_step gradients must be contiguous")
-    if devices != {plan.device}:
+    if set(map(_DEVICE_OF, given)) != {plan.device}:
         raise ValueError("adamw_step gradients must be on the parameters' device")
     lr_tensor = None
     if isinstance(lr, torch.Tensor):
@@ -208,7 +210,7 @@ def adamw_step(plan, grads, *, lr, betas=(0.9, 0.999), eps: float = 1.0e-8, weig
     if isinstance(seed, bool) or not isinstance(seed, numbers.Integral):
         raise TypeError("adamw_step seed must be an integer")
     native = _extension("adamw_step")
-    native.adamw_step(plan, addresses, dtypes.pop(), lr, lr_tensor, beta1, beta2, eps, weight_decay, grad_factor,
+    native.adamw_step(plan, grads, dtypes.pop(), lr, lr_tensor, beta1, beta2, eps, weight_decay, grad_factor,
                       int(seed))
     # the kernels write behind autograd's back: saved tensors and caches of derived data see it by the counter
     torch.autograd.graph.increment_version(params)
@@ -278,7 +280,7 @@ class AdamW(torch.optim.Optimizer):
     def _plan(self, key, params):
         plan = self._plans.get(key)
         if plan is not None and len(plan.params) == len(params) and \
-                all([a is b for a, b in zip(plan.params, params)]) and [p.data_ptr() for p in params] == plan.addresses:
+                all(map(operator.is_, plan.params, params)) and list(map(torch.Tensor.data_ptr, params)) == list(plan.addresses):
             return plan
         held = {} if plan is None else self._held(plan)
         return self._build(key, params, held)

@@ -595,7 +595,7 @@ int dpa4k_grad_norm(const void* const* grads, const int64_t* counts,
 /* One tensor of an AdamW plan; device pointers.  With moments in 32 bits
  * exp_avg and exp_avg_sq are float[count] and the scales NULL.  With moments in
  * 8 bits they are codes, one byte per element of `count` rounded up to a
- * multiple of 32 and 4-byte aligned, and the scales one byte per 32 elements
+ * multiple of 32 and 8-byte aligned, and the scales one byte per 32 elements
  * (at least 16 and 32); codes of 0 stand for moments of 0. */
 typedef struct {
   void* param;

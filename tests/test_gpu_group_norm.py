@@ -164,8 +164,8 @@ def test_tensors_that_start_anywhere(dtype, offset):
     views[0].copy_(x)
     views[1].copy_(grad)
     offsets = _on(_offsets(lengths))
-    y, mean, rstd = _C.group_norm_forward(views[0], 3, _on(scale), _on(bias), offsets, 1e-5, True)
-    grads = _C.group_norm_backward(views[1], views[0], 3, _on(scale), _on(bias), offsets, mean, rstd, True)
+    y, statistics = _C.group_norm_forward(views[0], 3, _on(scale), _on(bias), offsets, 1e-5, True)
+    grads = _C.group_norm_backward(views[1], views[0], 3, _on(scale), _on(bias), offsets, statistics, True)
     assert_close_scaled(y, group_norm_reference(x, 3, scale, bias, _offsets(lengths), 1e-5, "silu"), rtol=_rtol(dtype))
     wanted = group_norm_backward_reference(grad, x, 3, scale, bias, _offsets(lengths), 1e-5, "silu")
     for actual, expected in zip(grads, wanted):
@@ -176,11 +176,11 @@ def test_gradients_wanted_one_by_one_equal_those_wanted_together():
     lengths = [100, 7, 4000]
     x, grad, scale, bias = (t.to(DEV) for t in _inputs((sum(lengths), 24), torch.float32))
     offsets = _on(_offsets(lengths))
-    _, mean, rstd = _C.group_norm_forward(x, 4, scale, bias, offsets, 1e-5, True)
-    every = _C.group_norm_backward(grad, x, 4, scale, bias, offsets, mean, rstd, True)
+    _, statistics = _C.group_norm_forward(x, 4, scale, bias, offsets, 1e-5, True)
+    every = _C.group_norm_backward(grad, x, 4, scale, bias, offsets, statistics, True)
     for k, name in enumerate(("want_x", "want_scale", "want_bias")):
         wants = {n: n == name for n in ("want_x", "want_scale", "want_bias")}
-        alone = _C.group_norm_backward(grad, x, 4, scale, bias, offsets, mean, rstd, True, **wants)
+        alone = _C.group_norm_backward(grad, x, 4, scale, bias, offsets, statistics, True, **wants)
         assert [a is None for a in alone] == [i != k for i in range(3)]
         assert_bitwise(alone[k], every[k], name)
 
@@ -234,8 +234,8 @@ def test_captured_graphs_replay_the_eager_results():
         cases.append((x, grad, scale, bias))
 
     def both(x, grad, scale, bias):
-        y, mean, rstd = _C.group_norm_forward(x, 4, scale, bias, offsets, 1e-5, True)
-        return (y, *_C.group_norm_backward(grad, x, 4, scale, bias, offsets, mean, rstd, True))
+        y, statistics = _C.group_norm_forward(x, 4, scale, bias, offsets, 1e-5, True)
+        return (y, *_C.group_norm_backward(grad, x, 4, scale, bias, offsets, statistics, True))
 
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
