@@ -188,15 +188,32 @@ __device__ __forceinline__ void store_codes(void* p, int64_t at, const Codes<E>&
 template <bool kSigned>
 constexpr uint32_t kBinades = kSigned ? 16u : 32u;
 
-// The value of code `i` where the scale is not 255 (then the whole block stands
-// for NaN: poison_of).
+// What a condition of few lanes guards is skipped by the whole wave where no
+// lane has it.
+__device__ __forceinline__ bool any_lane(bool condition) { return __builtin_expect(__ballot(condition) != 0, 0); }
+
+// The values of a lane's codes, where the scale is not 255 (then the whole block
+// stands for NaN: poison_of).
 template <bool kSigned, int E>
-__device__ __forceinline__ float decode(const Codes<E>& codes, int i, uint32_t top) {
-  const uint32_t word = codes.word[i / 4];
-  const uint32_t c = __builtin_amdgcn_ubfe(word, 8 * (i & 3), kSigned ? 7 : 8);
-  const uint32_t magnitude = c == 0u ? 0u : (c + ((top - kBinades<kSigned> + 1u) << 3)) << 20;
-  if (!kSigned) return __uint_as_float(magnitude);
-  return __uint_as_float((word << (24 - 8 * (i & 3)) & 0x80000000u) | magnitude);
+__device__ __forceinline__ void decode(const Codes<E>& codes, uint32_t top, float (&value)[E]) {
+  const uint32_t low = top - kBinades<kSigned> + 1u;
+  uint32_t zeros = 0u;  // a bit for each code of 0 (and perhaps for a 1 above one)
+#pragma unroll
+  for (int w = 0; w < E / 4; ++w) {
+    const uint32_t word = kSigned ? codes.word[w] & 0x7F7F7F7Fu : codes.word[w];
+    zeros |= (word - 0x01010101u) & ~word & 0x80808080u;
+  }
+  uint32_t magnitude[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    magnitude[i] = (__builtin_amdgcn_ubfe(codes.word[i / 4], 8 * (i & 3), kSigned ? 7 : 8) + (low << 3)) << 20;
+  if (any_lane(zeros != 0u))
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (__builtin_amdgcn_ubfe(codes.word[i / 4], 8 * (i & 3), kSigned ? 7 : 8) == 0u) magnitude[i] = 0u;
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    value[i] = __uint_as_float(kSigned ? (codes.word[i / 4] << (24 - 8 * (i & 3)) & 0x80000000u) | magnitude[i] : magnitude[i]);
 }
 
 __device__ __forceinline__ float poison_of(uint32_t top) { return top == 255u ? NAN : 0.0f; }
@@ -225,7 +242,7 @@ __device__ __forceinline__ Codes<E> encode(const float (&value)[E], const uint32
   }
   // below the least code (few values are): a first moment goes up to it as often
   // as it is its share of it, a second moment unless it is 0
-  if (least_code < 1) {
+  if (any_lane(least_code < 1)) {
     const float least = __uint_as_float((low + 1u) << 20);
 #pragma unroll
     for (int i = 0; i < E; ++i)
@@ -327,17 +344,16 @@ __device__ __forceinline__ void adamw_update_chunk(const Record& r, int64_t begi
   for (int k = 0; k < K; ++k) {
     const int64_t at = begin + (k * kBlock + static_cast<int>(threadIdx.x)) * E;
     float new_p[E], new_m[E], new_v[E];
+    if constexpr (kBits == 8) {
+      decode<true, E>(m_codes[k], m_top[k], m[k].v);
+      decode<false, E>(v_codes[k], v_top[k], v[k].v);
+    }
     const float m_poison = kBits == 8 ? poison_of(m_top[k]) : 0.0f, v_poison = kBits == 8 ? poison_of(v_top[k]) : 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const float scaled = g[k].v[i] * factor;
-      if constexpr (kBits == 32) {
-        new_m[i] = m[k].v[i] * s.beta1 + scaled * s.rest1;
-        new_v[i] = v[k].v[i] * s.beta2 + (scaled * scaled) * s.rest2;
-      } else {
-        new_m[i] = decode<true, E>(m_codes[k], i, m_top[k]) * (s.beta1 + m_poison) + scaled * s.rest1;
-        new_v[i] = decode<false, E>(v_codes[k], i, v_top[k]) * (s.beta2 + v_poison) + (scaled * scaled) * s.rest2;
-      }
+      new_m[i] = m[k].v[i] * (kBits == 8 ? s.beta1 + m_poison : s.beta1) + scaled * s.rest1;
+      new_v[i] = v[k].v[i] * (kBits == 8 ? s.beta2 + v_poison : s.beta2) + (scaled * scaled) * s.rest2;
       new_p[i] = p[k].v[i] * decay - (new_m[i] / (sqrtf(new_v[i]) * inverse_root + s.eps)) * step_size;
     }
     uint32_t bits[E];
@@ -349,15 +365,21 @@ __device__ __forceinline__ void adamw_update_chunk(const Record& r, int64_t begi
       for (int i = 0; i < E; ++i) bits[i] = mix((static_cast<uint32_t>(position) + i) ^ own_key);
     }
     if constexpr (sizeof(P) == 2) {
-      P rounded[E];
+      uint32_t word[E], most = 0u;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const uint32_t word = __float_as_uint(new_p[i]);
-        const uint32_t noise = mix(bits[i] + 0x9E3779B1u) & 0xFFFFu;
-        // infinities stay, NaN stays NaN (quiet)
-        const uint32_t kept = __builtin_isnan(new_p[i]) ? word | 0x00400000u : word;
-        rounded[i] = static_cast<P>((__builtin_isfinite(new_p[i]) ? word + noise : kept) >> 16);
+        word[i] = __float_as_uint(new_p[i]) + (mix(bits[i] + 0x9E3779B1u) & 0xFFFFu);
+        const uint32_t magnitude = __float_as_uint(new_p[i]) & 0x7FFFFFFFu;
+        most = magnitude > most ? magnitude : most;
       }
+      if (any_lane(most >= 0x7F800000u))  // infinities stay, NaN stays NaN (quiet)
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (!__builtin_isfinite(new_p[i]))
+            word[i] = __builtin_isnan(new_p[i]) ? __float_as_uint(new_p[i]) | 0x00400000u : __float_as_uint(new_p[i]);
+      P rounded[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) rounded[i] = static_cast<P>(word[i] >> 16);
       store<kWhole, E>(param, at, count, rounded);
     } else {
       store<kWhole, E>(param, at, count, new_p);
@@ -423,10 +445,12 @@ __device__ __forceinline__ void adamw_codes_chunk(const Record& r, int64_t begin
       const Codes<E> m_codes = load_codes<E>(r.exp_avg, at), v_codes = load_codes<E>(r.exp_avg_sq, at);
       const uint32_t m_top = global(r.exp_avg_scale)[at / kSpan], v_top = global(r.exp_avg_sq_scale)[at / kSpan];
       float m[E], v[E];
+      decode<true, E>(m_codes, m_top, m);
+      decode<false, E>(v_codes, v_top, v);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        m[i] = m_top == 255u ? NAN : decode<true, E>(m_codes, i, m_top);
-        v[i] = v_top == 255u ? NAN : decode<false, E>(v_codes, i, v_top);
+        m[i] = m_top == 255u ? NAN : m[i];
+        v[i] = v_top == 255u ? NAN : v[i];
       }
       store<kWhole, E>(r.values[0], at, count, m);
       store<kWhole, E>(r.values[1], at, count, v);
