@@ -1067,12 +1067,12 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
 // direct, backward
 // ---------------------------------------------------------------------------
 //
-// TS threads hold 16 elements each of a sample's x and gradient (fewer
-// than the forward: both tensors, and the channel sums, stay in registers).  A
-// workgroup takes the samples b, b + workgroups, ... and keeps its sums per
-// channel across them, one row of column sums in the end.
-template <typename T>
-constexpr int kHeldBoth = 16 / kVec<T>;
+// TS threads hold 32 elements each of a sample's x and gradient, up to 512
+// threads (1,024 would leave 128 registers each, half of them held).  With 16
+// elements a thread samples of 60 rows of 64 took 512 threads, of which a CU
+// holds two workgroups: 51 us for 3,000 of them, 42 us with 32.  A workgroup
+// takes the samples b, b + workgroups, ... and keeps its sums per channel
+// across them, one row of column sums in the end.
 
 template <typename T, bool kUniform, int TS>
 __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
@@ -1104,13 +1104,13 @@ __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
     const int left = kUniform ? 0 : static_cast<int>(elements - whole * V);
     const T* run_g = grad + first * C;
     const T* run_x = x + first * C;
-    const bool held = whole <= static_cast<int64_t>(stride) * kHeldBoth<T>;
+    const bool held = whole <= static_cast<int64_t>(stride) * kHeld<T>;
     const bool tail = !kUniform && left > 0 && owns(share, whole, stride);
-    Raw<T> gv[kHeldBoth<T>], xv[kHeldBoth<T>];
+    Raw<T> gv[kHeld<T>], xv[kHeld<T>];
     int mine = 0;
     if (held) {
 #pragma unroll
-      for (int k = 0; k < kHeldBoth<T>; ++k)
+      for (int k = 0; k < kHeld<T>; ++k)
         if (static_cast<int64_t>(k) * stride < whole) {
           const int64_t q = share.first + static_cast<int64_t>(k) * stride;
           const int64_t at = (q < whole ? q : whole - 1) * V;
@@ -1124,7 +1124,7 @@ __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
     Sums<T> sums;
     if (held) {
 #pragma unroll
-      for (int k = 0; k < kHeldBoth<T>; ++k)
+      for (int k = 0; k < kHeld<T>; ++k)
         if (k < mine) sums.add(to_values<T>(gv[k]), to_values<T>(xv[k]), channels, centre, inverse, silu);
     } else if (share.live) {
       for (int64_t q = share.first; q < whole; q += stride)
@@ -1151,7 +1151,7 @@ __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
       };
       if (held) {
 #pragma unroll
-        for (int k = 0; k < kHeldBoth<T>; ++k)
+        for (int k = 0; k < kHeld<T>; ++k)
           if (k < mine)
             store_whole(out + (share.first + static_cast<int64_t>(k) * stride) * V,
                         gradient(to_values<T>(gv[k]), to_values<T>(xv[k])));
@@ -1187,10 +1187,13 @@ struct Schedule {
 };
 
 constexpr int kDirectThreads[] = {64, 256, 512, 1024};
-constexpr int64_t kWorkers = 2048;
+// Backward workgroups of a direct launch: as many as are resident at three waves
+// a SIMD (3,000 samples of 60 rows of 64: 39 us with 768 workgroups of 256
+// threads, 41 with 2,048, 47 with 1,024, whose last third finds the CUs full).
+constexpr int64_t workers_for(int threads) { return threads == 64 ? 3072 : (threads == 256 ? 768 : 512); }
 
 // Checks the sizes, cuts the rows into tiles, and chooses the schedule.  A
-// direct workgroup holds 32 elements a thread, 16 in the backward.  The smallest that holds the
+// direct workgroup holds 32 elements a thread.  The smallest that holds the
 // longest sample is taken; where the longest is not known, one that holds twice
 // the mean, and the rest goes to tiles.
 int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inner, int64_t channels, int64_t groups,
@@ -1229,16 +1232,16 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
   const int64_t elements = wanted * channels;
   if (groups <= kLdsGroups)
     for (int threads : kDirectThreads) {
-      if (period > threads) continue;
-      const int64_t holds = static_cast<int64_t>(threads / period) * period * (backward ? 16 : 32);
-      if (elements > holds && (known || threads < 1024)) continue;
+      if (period > threads || (backward && threads > 512)) continue;
+      const int64_t holds = static_cast<int64_t>(threads / period) * period * 32;
+      if (elements > holds && (known || threads < (backward ? 512 : 1024))) continue;
       out.threads = threads;
       out.shape.long_rows = holds / channels;
       break;
     }
   if (out.threads != 0 && known) out.shape.long_rows = INT64_MAX;  // nothing is left to tiles: a longer sample is streamed
   out.tiles = out.threads == 0 || !known;
-  out.workers = out.threads == 0 ? 0 : (samples < kWorkers ? samples : kWorkers);
+  out.workers = out.threads == 0 ? 0 : (samples < workers_for(out.threads) ? samples : workers_for(out.threads));
   const int64_t kilobytes64 = rows * row_bytes / 65536 + 1;
   out.zero_blocks = offsets == nullptr || out.tiles ? 0 : (kilobytes64 < 256 ? kilobytes64 : 256);
   out.column_rows = out.workers + (out.tiles ? out.shape.tiles : 0);
@@ -1291,11 +1294,10 @@ bool uniform_groups(const Shape& s) {
 }
 
 // Calls LAUNCH(TS) for the schedule's direct workgroup.
-#define DPA4K_DIRECT(threads, LAUNCH) \
-  if (threads == 64) LAUNCH(64);      \
+#define DPA4K_DIRECT(threads, LAUNCH)   \
+  if (threads == 64) LAUNCH(64);        \
   else if (threads == 256) LAUNCH(256); \
-  else if (threads == 512) LAUNCH(512); \
-  else LAUNCH(1024);
+  else LAUNCH(512);
 
 template <typename T, bool kUniform>
 int forward_as(const T* x, const float* scale, const float* bias, T* y, float* mean, float* rstd, const Schedule& c,
@@ -1307,7 +1309,8 @@ int forward_as(const T* x, const float* scale, const float* bias, T* y, float* m
 #define DPA4K_LAUNCH(TS)                                                                                              \
   group_norm_direct_kernel<T, kUniform, TS><<<grid, TS, 0, stream>>>(x, scale, bias, eps, silu, mean, rstd, y, s, columns, \
                                                                      c.zero_blocks)
-    DPA4K_DIRECT(c.threads, DPA4K_LAUNCH)
+    if (c.threads == 1024) DPA4K_LAUNCH(1024);
+    else DPA4K_DIRECT(c.threads, DPA4K_LAUNCH)
 #undef DPA4K_LAUNCH
     if (int e = launched("group_norm_direct_kernel")) return e;
   }

@@ -944,18 +944,13 @@ def _addresses(tensors):
 
 
 def grad_norm(grads, max_norm: float = 0.0):
-    """``(norm, factor)`` of contiguous float32 or bfloat16 tensors on one device (at least one)."""
+    """``(norm, factor)`` of checked gradients: contiguous float32 or bfloat16 tensors on one GPU, at least one."""
     n = len(grads)
-    _check(n >= 1, "gradient norm needs at least one gradient")
-    dtypes = list(map(_DTYPE_OF, grads))
-    kinds = set(dtypes)
-    _check(kinds <= {torch.float32, torch.bfloat16}, "gradient norm: expected float32 or bfloat16 tensors")
-    _check(all(map(torch.Tensor.is_contiguous, grads)), "gradient norm: expected contiguous tensors")
-    devices = set(map(torch.Tensor.get_device, grads))
-    _check(len(devices) == 1 and -1 not in devices, "gradient norm: expected gfx950 tensors on one device")
     device = grads[0].device
+    _check(device.type == "cuda", "gradient norm: expected gfx950 tensors")
+    dtypes = list(map(_DTYPE_OF, grads))
     addresses, counts = _addresses(grads), array("q", map(torch.Tensor.numel, grads))
-    codes = array("i", [ELEMENT_TYPES[grads[0].dtype]]) * n if len(kinds) == 1 else array("i", map(ELEMENT_TYPES.get, dtypes))
+    codes = array("i", map(ELEMENT_TYPES.__getitem__, dtypes))
     result = torch.empty((2,), dtype=torch.float32, device=device)
     at = result.data_ptr()
     nbytes = _LIB.dpa4k_grad_norm_workspace_size(counts.buffer_info()[0], n)
@@ -982,7 +977,7 @@ class AdamWPlan:
         self.dtype = params[0].dtype
         self.device = params[0].device
         self.shapes = [p.shape for p in params]
-        self.addresses = _addresses(params)
+        self.addresses = list(_addresses(params))
         self.exp_avgs = self.exp_avg_sqs = None             # 32 bits: float32 tensors
         self.codes = self.scales = None                     # 8 bits: (2, padded) and (2, padded / 32) bytes
         self.words = None

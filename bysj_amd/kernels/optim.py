@@ -36,6 +36,12 @@ STATE_BITS = (32, 8)
 _DTYPE_OF, _SHAPE_OF, _DEVICE_OF = (operator.attrgetter(name) for name in ("dtype", "shape", "device"))
 
 
+def _all_on(tensors, device) -> bool:
+    if device.type == "cuda":  # an index says it all, at half the cost of a device
+        return set(map(torch.Tensor.get_device, tensors)) == {device.index}
+    return set(map(_DEVICE_OF, tensors)) == {device}
+
+
 def _tensors(values, what: str, *, allow_none: bool = False) -> list:
     if isinstance(values, torch.Tensor) or not hasattr(values, "__iter__"):
         raise TypeError(f"{what} must be a sequence of tensors")
@@ -87,7 +93,7 @@ def grad_norm(grads, max_norm: float | None = None) -> tuple[torch.Tensor, torch
         raise TypeError("grad_norm requires float32 or bfloat16 gradients")
     if not all(map(torch.Tensor.is_contiguous, grads)):
         raise ValueError("grad_norm gradients must be contiguous")
-    if len(set(map(_DEVICE_OF, grads))) > 1:
+    if not _all_on(grads, grads[0].device):
         raise ValueError("grad_norm gradients must share a device")
     require_dcu(grads[0])
     return _extension("grad_norm").grad_norm(grads, limit)
@@ -103,14 +109,14 @@ def _refuse_overlaps(tensors) -> None:
         raise ValueError("AdamW parameters and moments must not overlap")
 
 
-def _moments(values, params, what: str):
+def _moments(values, shapes, device, what: str):
     values = _tensors(values, what)
-    if len(values) != len(params):
+    if len(values) != len(shapes):
         raise ValueError(f"{what}: expected one tensor per parameter")
-    if values and set(map(_DTYPE_OF, values)) != {torch.float32}:
+    if set(map(_DTYPE_OF, values)) != {torch.float32}:
         raise TypeError(f"{what} must be float32")
-    if list(map(_SHAPE_OF, values)) != list(map(_SHAPE_OF, params)) or not all(map(torch.Tensor.is_contiguous, values)) \
-            or set(map(_DEVICE_OF, values)) != set(map(_DEVICE_OF, params)):
+    if list(map(_SHAPE_OF, values)) != shapes or not all(map(torch.Tensor.is_contiguous, values)) \
+            or not _all_on(values, device):
         raise ValueError(f"{what} must be contiguous, of the parameters' shapes and device")
     return values
 
@@ -140,8 +146,9 @@ def adamw_plan(params, exp_avgs=None, exp_avg_sqs=None, *, step=0, state_bits: i
     if (exp_avgs is None) != (exp_avg_sqs is None):
         raise ValueError("AdamW moments: give both or neither")
     if exp_avgs is not None:
-        exp_avgs = _moments(exp_avgs, params, "AdamW exp_avgs")
-        exp_avg_sqs = _moments(exp_avg_sqs, params, "AdamW exp_avg_sqs")
+        shapes = list(map(_SHAPE_OF, params))
+        exp_avgs = _moments(exp_avgs, shapes, params[0].device, "AdamW exp_avgs")
+        exp_avg_sqs = _moments(exp_avg_sqs, shapes, params[0].device, "AdamW exp_avg_sqs")
     _refuse_overlaps(params + (exp_avgs or []) + (exp_avg_sqs or []))
     steps = [step] * len(params) if isinstance(step, numbers.Integral) else list(step)
     if len(steps) != len(params):
@@ -177,7 +184,7 @@ def adamw_step(plan, grads, *, lr, betas=(0.9, 0.999), eps: float = 1.0e-8, weig
     grads = _tensors(grads, "adamw_step gradients", allow_none=True)
     if len(grads) != len(params):
         raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients")
-    if list(map(torch.Tensor.data_ptr, params)) != list(plan.addresses):
+    if list(map(torch.Tensor.data_ptr, params)) != plan.addresses:
         raise RuntimeError("adamw_step: a parameter's memory has moved since the plan was built")
     given, shapes = grads, plan.shapes
     if type(None) in set(map(type, grads)):
@@ -191,7 +198,7 @@ def adamw_step(plan, grads, *, lr, betas=(0.9, 0.999), eps: float = 1.0e-8, weig
         raise ValueError("adamw_step gradients must have their parameters' shapes")
     if not all(map(torch.Tensor.is_contiguous, given)):
         raise ValueError("adamw_step gradients must be contiguous")
-    if set(map(_DEVICE_OF, given)) != {plan.device}:
+    if not _all_on(given, plan.device):
         raise ValueError("adamw_step gradients must be on the parameters' device")
     lr_tensor = None
     if isinstance(lr, torch.Tensor):
@@ -221,7 +228,7 @@ def adamw_states(plan, exp_avgs=None, exp_avg_sqs=None) -> tuple[list, list]:
     out = []
     for values, what in ((exp_avgs, "AdamW exp_avgs"), (exp_avg_sqs, "AdamW exp_avg_sqs")):
         out.append([torch.empty_like(p, dtype=torch.float32) for p in plan.params] if values is None
-                   else _moments(values, plan.params, what))
+                   else _moments(values, plan.shapes, plan.device, what))
     if plan.state_bits == 32:
         for to, values in zip(out, (plan.exp_avgs, plan.exp_avg_sqs)):
             torch._foreach_copy_(to, values)
@@ -280,7 +287,7 @@ class AdamW(torch.optim.Optimizer):
     def _plan(self, key, params):
         plan = self._plans.get(key)
         if plan is not None and len(plan.params) == len(params) and \
-                all(map(operator.is_, plan.params, params)) and list(map(torch.Tensor.data_ptr, params)) == list(plan.addresses):
+                all(map(operator.is_, plan.params, params)) and list(map(torch.Tensor.data_ptr, params)) == plan.addresses:
             return plan
         held = {} if plan is None else self._held(plan)
         return self._build(key, params, held)
