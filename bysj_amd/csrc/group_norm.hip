@@ -24,8 +24,10 @@
 // A sample, or a piece, is read as one run of 16-byte vectors.  Vector q of a
 // run holds the channels (q V + j) mod C, so with a stride of a multiple of
 // lcm(C, V) elements a thread stays on the same V channels at any width C, and
-// no access is scalar but in the ragged last vector of a run.  Where V divides
-// D (kUniform) a vector lies in one group and runs have no ragged vector.
+// no access is scalar but in the ragged last vector of a run.  A thread's
+// channels make N parts, each of one group: N = 1 where V divides D (runs then
+// have no ragged vector), N = 2 where D >= V (a vector crosses one border of
+// groups at most, after its first `split` channels), else N = V.
 #include <cmath>
 
 #include "common.h"
@@ -167,38 +169,48 @@ __device__ __forceinline__ bool owns(const Share& share, int64_t whole, int stri
   return share.live && whole >= share.first && (whole - share.first) % stride == 0;
 }
 
-// Scale, bias and group of a thread's channels.
-template <typename T, bool kUniform>
+// Scale and bias of a thread's channels, and the groups of its parts.
+template <typename T, int N>
 struct Channels {
   static constexpr int V = kVec<T>;
   float weight[V], shift[V];
-  int group[kUniform ? 1 : V];
+  int group[N], split;
   __device__ __forceinline__ Channels(const Share& share, const float* __restrict__ scale,
                                       const float* __restrict__ bias, int channels, int width) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       int c = share.channel + j;
       while (c >= channels) c -= channels;  // at most V / C times
-      if (!kUniform || j == 0) group[kUniform ? 0 : j] = c / width;
+      if (N == V || j == 0) group[N == V ? j : 0] = c / width;
       weight[j] = scale != nullptr ? scale[c] : 1.0f;
       shift[j] = bias != nullptr ? bias[c] : 0.0f;
     }
+    split = V;
+    if constexpr (N == 2) {
+      const int next = (group[0] + 1) * width;
+      split = next - share.channel < V ? next - share.channel : V;
+      group[1] = next < channels ? group[0] + 1 : 0;
+    }
   }
-  __device__ __forceinline__ int group_of(int j) const { return group[kUniform ? 0 : j]; }
+  __device__ __forceinline__ int part_of(int j) const { return N == 1 ? 0 : (N == 2 ? (j < split ? 0 : 1) : j); }
 };
 
 // A value per channel of a thread, one where its channels share a group.
-template <typename T, bool kUniform>
+template <typename T, int N>
 struct PerGroup {
-  float v[kUniform ? 1 : kVec<T>];
-  __device__ __forceinline__ float at(int j) const { return v[kUniform ? 0 : j]; }
+  float v[N == 1 ? 1 : kVec<T>];
+  __device__ __forceinline__ float at(int j) const { return v[N == 1 ? 0 : j]; }
 };
 
-template <typename T, bool kUniform>
-__device__ __forceinline__ PerGroup<T, kUniform> per_group(const float* values, const Channels<T, kUniform>& channels) {
-  PerGroup<T, kUniform> out;
+template <typename T, int N>
+__device__ __forceinline__ PerGroup<T, N> per_group(const float* values, const Channels<T, N>& channels) {
+  float of_part[N];
 #pragma unroll
-  for (int j = 0; j < (kUniform ? 1 : kVec<T>); ++j) out.v[j] = values[channels.group_of(j)];
+  for (int i = 0; i < N; ++i) of_part[i] = values[channels.group[i]];
+  PerGroup<T, N> out;
+#pragma unroll
+  for (int j = 0; j < (N == 1 ? 1 : kVec<T>); ++j)
+    out.v[j] = N == 2 ? (j < channels.split ? of_part[0] : of_part[N - 1]) : of_part[N == 1 ? 0 : j];
   return out;
 }
 
@@ -277,25 +289,27 @@ __device__ __forceinline__ void zero_outside(T* __restrict__ out, const Shape& s
 // a workgroup's terms by group of channels
 // ---------------------------------------------------------------------------
 //
-// The threads put their terms into LDS, one per vector (kUniform) or one per
-// element, as rows of W units per period row; group g owns the units [g dw,
-// (g + 1) dw) of each.  `lanes` lanes (a power of two) add a group's terms.
+// The threads put their terms into LDS, N each.  In every row of a period group
+// g owns D elements, which lie in the vectors of `per_row` threads at most; with
+// N = 2 it is the second part of a thread whose vector it starts inside of, and
+// the first of the others.  `lanes` lanes (a power of two) add a group's terms.
 struct Units {
-  int row, per_group, origin, held, first_row, terms, lanes;
+  int channels, width, pass_first, held;  // held: threads with a vector in this pass
+  int first_row, per_row, terms, lanes;
 };
 
-template <int BLOCK, int V, bool kUniform>
+template <int BLOCK, int V, int N>
 __device__ __forceinline__ Units units_of(const Columns& columns, int pass, int channels, int groups) {
   Units u;
-  u.row = kUniform ? channels / V : channels;
-  u.per_group = u.row / groups;
-  constexpr int kPer = kUniform ? 1 : V;
-  u.origin = pass * BLOCK * kPer;
-  const int span = columns.stride_vectors() * kPer - u.origin;
-  u.held = span < BLOCK * kPer ? span : BLOCK * kPer;
-  u.first_row = u.origin / u.row;
-  const int last_row = (u.origin + u.held - 1) / u.row;
-  u.terms = u.per_group * (last_row - u.first_row + 1);
+  u.channels = channels;
+  u.width = channels / groups;
+  u.pass_first = pass * BLOCK;
+  const int span = columns.stride_vectors() - u.pass_first;
+  u.held = span < BLOCK ? span : BLOCK;
+  u.first_row = u.pass_first * V / channels;
+  const int rows = ((u.pass_first + u.held) * V - 1) / channels - u.first_row + 1;
+  u.per_row = N == 1 ? u.width / V : (N == 2 ? (u.width + V - 2) / V + 1 : u.width);
+  u.terms = u.per_row * rows;
   const int share = BLOCK / groups;  // threads per group, if each has some
   u.lanes = 1;
   while (u.lanes < 64 && u.lanes < u.terms && 2 * u.lanes <= share) u.lanes <<= 1;
@@ -303,18 +317,26 @@ __device__ __forceinline__ Units units_of(const Columns& columns, int pass, int 
 }
 
 // Calls term(place) for the terms lane, lane + lanes, ... of group g.
-template <typename Term>
+template <int V, int N, typename Term>
 __device__ __forceinline__ void each_term(const Units& u, int g, int lane, Term term) {
-  const int rows = u.lanes / u.per_group, columns = u.lanes - rows * u.per_group;  // one step
-  int row = lane / u.per_group;
-  int column = lane - row * u.per_group;
+  const int rows = u.lanes / u.per_row, columns = u.lanes - rows * u.per_row;  // one step
+  int row = lane / u.per_row;
+  int column = lane - row * u.per_row;
   for (int i = lane; i < u.terms; i += u.lanes) {
-    const int e = (u.first_row + row) * u.row + g * u.per_group + column - u.origin;
-    if (e >= 0 && e < u.held) term(e);
+    const int start = (u.first_row + row) * u.channels + g * u.width;  // the group's first element in the period
+    if constexpr (N == V && V != 1) {
+      const int e = start + column - u.pass_first * V;
+      if (e >= 0 && e < u.held * V) term(e);
+    } else {
+      const int vector = start / V + column;
+      const int thread = vector - u.pass_first;
+      if (thread >= 0 && thread < u.held && vector * V < start + u.width)
+        term(N == 1 ? thread : thread * 2 + (column == 0 && start % V != 0 ? 1 : 0));
+    }
     row += rows;
     column += columns;
-    if (column >= u.per_group) {
-      column -= u.per_group;
+    if (column >= u.per_row) {
+      column -= u.per_row;
       ++row;
     }
   }
@@ -330,10 +352,11 @@ __device__ __forceinline__ F lanes_sum(F value, int lanes) {
 // moments
 // ---------------------------------------------------------------------------
 //
-// A thread merges batches into a running mean and sum of squared deviations:
-// the batch's own mean is taken off first, so neither a mean far from 0 nor a
-// long sum costs digits.  The threads' pairs meet in LDS and are merged per
-// group relative to the first of them, in float32; slots and what follows in 64 bits.
+// A thread merges batches into a running mean and sum of squared deviations.  A
+// batch is taken relative to the mean so far (the first one to its first value)
+// and then to its own mean, so neither a mean far from 0 nor a long sum costs
+// digits, and a constant sample has its exact mean.  The threads' pairs meet in
+// LDS and are merged pair by pair per group; slots and what follows in 64 bits.
 template <typename T>
 constexpr int kBatch = 32 / kVec<T>;  // vectors in flight: 32 elements
 
@@ -351,61 +374,88 @@ __device__ __forceinline__ int64_t place_of(int64_t q, int k, int stride, int64_
   return at < whole ? at : whole - 1;
 }
 
-template <typename T, bool kUniform>
+template <typename T, int N>
 struct Running {
-  static constexpr int V = kVec<T>, N = kUniform ? 1 : V;
-  int count = 0, left = 0;  // vectors, and elements of a last part: element j has count + (j < left) terms
-  float mean[N], squares[N];
+  static constexpr int V = kVec<T>;
+  float count[N], mean[N], squares[N];  // of each part
   __device__ __forceinline__ Running() {
 #pragma unroll
-    for (int i = 0; i < N; ++i) mean[i] = squares[i] = 0.0f;
+    for (int i = 0; i < N; ++i) count[i] = mean[i] = squares[i] = 0.0f;
+  }
+  // n terms of part i with the mean origin + delta, where `origin` is the mean so
+  // far (or near the terms where there is none yet).
+  __device__ __forceinline__ void merge(int i, float n, float origin, float delta, float spread) {
+    const float total = count[i] + n;
+    const float weight = n * __builtin_amdgcn_rcpf(total);
+    mean[i] = fmaf(delta, weight, origin);
+    squares[i] += fmaf(delta * delta, count[i] * weight, spread);
+    count[i] = total;
   }
   // The first `n` of the vectors, n > 0.
   template <int K, bool kAll>
-  __device__ __forceinline__ void add(const Raw<T> (&batch)[K], int n) {
-    count += kAll ? K : n;
-    const float share = 1.0f / static_cast<float>((kAll ? K : n) * (kUniform ? V : 1));
-    const float weight = static_cast<float>(kAll ? K : n) / static_cast<float>(count);
-    const float cross = static_cast<float>(count - (kAll ? K : n)) * weight * (kUniform ? V : 1);
+  __device__ __forceinline__ void add(const Raw<T> (&batch)[K], int n, int split) {
+    const float vectors = static_cast<float>(kAll ? K : n);
+    float origin[N], delta[N], spread[N], terms[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < (kUniform ? V : 1); ++j) {
-          const float value = static_cast<float>(batch[k][kUniform ? j : i]);
-          sum += kAll || k < n ? value : 0.0f;
-        }
-      const float own = sum * share;
-      float spread = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < (kUniform ? V : 1); ++j) {
-          const float d = static_cast<float>(batch[k][kUniform ? j : i]) - own;
-          const float kept = kAll || k < n ? d : 0.0f;
-          spread = fmaf(kept, kept, spread);
-        }
-      const float delta = own - mean[i];
-      mean[i] = fmaf(delta, weight, mean[i]);
-      squares[i] += fmaf(delta * delta, cross, spread);
+      delta[i] = spread[i] = 0.0f;
+      terms[i] = vectors * (N == 1 ? V : (N == 2 ? (i == 0 ? split : V - split) : 1));
+      origin[i] = count[i] > 0.0f ? mean[i] : static_cast<float>(batch[0][N == 2 && i == 1 ? V - 1 : (N == V ? i : 0)]);
     }
-  }
-  // The elements behind the last whole vector: one more for some channels.
-  __device__ __forceinline__ void add_part(const Values<T>& part, int live) {
-    left = live;
-    const float weight = 1.0f / static_cast<float>(count + 1);
-    const float cross = static_cast<float>(count) * weight;
+    const auto part = [&](const float(&of)[N], int j) { return N == 2 ? (j < split ? of[0] : of[N - 1]) : of[N == 1 ? 0 : j]; };
+    const auto add_to = [&](float(&to)[N], int j, float value) {
+      if constexpr (N == 2) {
+        to[0] += j < split ? value : 0.0f;
+        to[1] += j < split ? 0.0f : value;
+      } else {
+        to[N == 1 ? 0 : j] += value;
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float column = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float d = static_cast<float>(batch[k][j]) - part(origin, j);
+        column += kAll || k < n ? d : 0.0f;
+      }
+      add_to(delta, j, column);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) delta[i] *= __builtin_amdgcn_rcpf(N == 2 && i == 1 && split == V ? 1.0f : terms[i]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float column = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float d = (static_cast<float>(batch[k][j]) - part(origin, j)) - part(delta, j);
+        const float kept = kAll || k < n ? d : 0.0f;
+        column = fmaf(kept, kept, column);
+      }
+      add_to(spread, j, column);
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (i < live) {
-        const float delta = part.v[i] - mean[i];
-        mean[i] = fmaf(delta, weight, mean[i]);
-        squares[i] = fmaf(delta * delta, cross, squares[i]);
+      if (N != 2 || i == 0 || split < V) merge(i, terms[i], origin[i], delta[i], spread[i]);
+  }
+  // The elements behind the last whole vector, one at a time.
+  __device__ __forceinline__ void add_part(const Values<T>& part, int live, int split) {
+    const auto one = [&](int i, float value) {
+      const float origin = count[i] > 0.0f ? mean[i] : value;
+      merge(i, 1.0f, origin, value - origin, 0.0f);
+    };
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < live) {
+        if constexpr (N == 2) {
+          if (j < split) one(0, part.v[j]);
+          else one(1, part.v[j]);
+        } else {
+          one(N == 1 ? 0 : j, part.v[j]);
+        }
       }
   }
-  __device__ __forceinline__ void add_run(const T* __restrict__ run, int64_t elements, const Share& share, int stride) {
+  __device__ __forceinline__ void add_run(const T* __restrict__ run, int64_t elements, const Share& share, int stride, int split) {
     if (!share.live) return;
     const int64_t whole = elements / V;
     int64_t q = share.first;
@@ -414,66 +464,61 @@ struct Running {
 #pragma unroll
       for (int k = 0; k < kBatch<T>; ++k) batch[k] = load_raw(run + place_of(q, k, stride, whole) * V);
       const int n = in_reach<kBatch<T>>(q, whole, stride);
-      if (n == kBatch<T>) add<kBatch<T>, true>(batch, n);
-      else add<kBatch<T>, false>(batch, n);
+      if (n == kBatch<T>) add<kBatch<T>, true>(batch, n, split);
+      else add<kBatch<T>, false>(batch, n, split);
     }
-    if constexpr (!kUniform) {
+    if constexpr (N != 1) {
       const int part = static_cast<int>(elements - whole * V);
-      if (part > 0 && owns(share, whole, stride)) add_part(load_part(run + whole * V, part), part);
+      if (part > 0 && owns(share, whole, stride)) add_part(load_part(run + whole * V, part), part, split);
     }
   }
 };
 
-template <int BLOCK, int V, bool kUniform>
+// The first `split` of a thread's channels belong to its first group (N = 2).
+template <typename T, int N>
+__device__ __forceinline__ int split_of(const Share& share, int width) {
+  if (N != 2) return kVec<T>;
+  const int left = width - share.channel % width;
+  return left < kVec<T> ? left : kVec<T>;
+}
+
+template <int BLOCK, int N>
 struct MomentsLds {
-  float mean[BLOCK * (kUniform ? 1 : V)], squares[BLOCK * (kUniform ? 1 : V)];
-  int count[BLOCK];
+  float count[BLOCK * N], mean[BLOCK * N], squares[BLOCK * N];
 };
 
 // Calls emit(group, terms, mean, squares) in one lane for every group.
-template <int BLOCK, typename T, bool kUniform, typename Emit>
-__device__ __forceinline__ void merge_moments(const Running<T, kUniform>& mine, bool live,
-                                              MomentsLds<BLOCK, kVec<T>, kUniform>& lds, const Units& u, int groups,
-                                              Emit emit) {
-  constexpr int V = kVec<T>, N = kUniform ? 1 : V;
+template <int BLOCK, typename T, int N, typename Emit>
+__device__ __forceinline__ void merge_moments(const Running<T, N>& mine, bool live, MomentsLds<BLOCK, N>& lds, const Units& u,
+                                              int groups, Emit emit) {
   if (live) {
-    lds.count[threadIdx.x] = kUniform ? mine.count * V : mine.count * V + mine.left;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+      lds.count[threadIdx.x * N + i] = mine.count[i];
       lds.mean[threadIdx.x * N + i] = mine.mean[i];
       lds.squares[threadIdx.x * N + i] = mine.squares[i];
     }
   }
   __syncthreads();
-  const auto count_of = [&](int e) {
-    if (kUniform) return static_cast<float>(lds.count[e]);
-    const int packed = lds.count[e / V];
-    return static_cast<float>(packed / V + (e % V < packed % V ? 1 : 0));
-  };
   const int lane = threadIdx.x & (u.lanes - 1);
   const int per_round = BLOCK / u.lanes;
   for (int g = static_cast<int>(threadIdx.x) / u.lanes; g < (groups + per_round - 1) / per_round * per_round; g += per_round) {
-    const bool in = g < groups;
-    const int start = u.first_row * u.row + (in ? g : 0) * u.per_group - u.origin;
-    const float pivot = lds.mean[start >= 0 && start < u.held ? start : 0];
-    float total = 0.0f, sum = 0.0f, spread = 0.0f;
-    if (in)
-      each_term(u, g, lane, [&](int e) {
-        const float n = count_of(e);
-        total += n;
-        if (n > 0.0f) sum = fmaf(n, lds.mean[e] - pivot, sum);
-      });
-    total = lanes_sum(total, u.lanes);
-    sum = lanes_sum(sum, u.lanes);
-    const float centre = total > 0.0f ? sum / total : 0.0f;
-    if (in)
-      each_term(u, g, lane, [&](int e) {
-        const float n = count_of(e);
-        const float delta = (lds.mean[e] - pivot) - centre;
-        if (n > 0.0f) spread += fmaf(n * delta, delta, lds.squares[e]);
-      });
-    spread = lanes_sum(spread, u.lanes);
-    if (lane == 0 && in) emit(g, total, pivot + centre, spread);
+    float total = 0.0f, mean = 0.0f, squares = 0.0f;
+    const auto join = [&](float n, float other, float spread) {
+      if (!(n > 0.0f)) return;
+      const float origin = total > 0.0f ? mean : other;
+      const float delta = other - origin, sum = total + n;
+      const float weight = n * __builtin_amdgcn_rcpf(sum);
+      mean = fmaf(delta, weight, origin);
+      squares += fmaf(delta * delta, total * weight, spread);
+      total = sum;
+    };
+    if (g < groups) each_term<kVec<T>, N>(u, g, lane, [&](int e) { join(lds.count[e], lds.mean[e], lds.squares[e]); });
+    for (int mask = 1; mask < u.lanes; mask <<= 1) {
+      const float n = __shfl_xor(total, mask), other = __shfl_xor(mean, mask), spread = __shfl_xor(squares, mask);
+      join(n, other, spread);
+    }
+    if (lane == 0 && g < groups) emit(g, total, mean, squares);
   }
 }
 
@@ -523,19 +568,20 @@ __device__ __forceinline__ Merged merge_slots(const Slot* __restrict__ slots, in
 // tiles, forward
 // ---------------------------------------------------------------------------
 
-template <typename T, bool kUniform>
+template <typename T, int N>
 __global__ __launch_bounds__(kTileBlock) void group_norm_moments_kernel(const T* __restrict__ x, Shape s, Columns columns,
                                                                         Slot* __restrict__ slots) {
-  __shared__ MomentsLds<kTileBlock, kVec<T>, kUniform> lds;
+  __shared__ MomentsLds<kTileBlock, N> lds;
   const int64_t tile = block_index();
   if (tile >= s.tiles) return;
   each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
     Slot* out = slots + (tile + sample) * columns.passes * s.groups;
     for (int pass = 0; pass < columns.passes; ++pass) {
       const Share share = share_of<T, kTileBlock>(columns, pass, s.channels);
-      const Units u = units_of<kTileBlock, kVec<T>, kUniform>(columns, pass, s.channels, s.groups);
-      Running<T, kUniform> running;
-      running.add_run(x + a * s.channels, (b - a) * s.channels, share, columns.stride_vectors());
+      const Units u = units_of<kTileBlock, kVec<T>, N>(columns, pass, s.channels, s.groups);
+      Running<T, N> running;
+      running.add_run(x + a * s.channels, (b - a) * s.channels, share, columns.stride_vectors(),
+                      split_of<T, N>(share, s.channels / s.groups));
       merge_moments<kTileBlock>(running, share.live, lds, u, s.groups, [&](int g, float count, float mean, float squares) {
         out[pass * s.groups + g] = {count, mean, squares};
       });
@@ -572,7 +618,7 @@ __global__ __launch_bounds__(256) void group_norm_finish_kernel(const Slot* __re
 
 // Merging a sample's slots again in every tile instead of in a launch of its
 // own was slower: 1,024 tiles on one sample of 100 MB took 60 us against 35 + 5.
-template <typename T, bool kUniform>
+template <typename T, int N>
 __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
     const T* __restrict__ x, const float* __restrict__ scale, const float* __restrict__ bias, bool silu,
     const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ y, Shape s, Columns columns) {
@@ -584,15 +630,15 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
   const int stride = columns.stride_vectors();
   for (int pass = 0; pass < columns.passes; ++pass) {
     const Share share = share_of<T, kTileBlock>(columns, pass, C);
-    const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+    const Channels<T, N> channels(share, scale, bias, C, C / G);
     each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
       if (!share.live) return;
       const int64_t elements = (b - a) * C;
       const int64_t whole = elements / V;
       const T* run = x + a * C;
       T* out = y + a * C;
-      const PerGroup<T, kUniform> centre = per_group<T, kUniform>(mean + sample * G, channels);
-      const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(rstd + sample * G, channels);
+      const PerGroup<T, N> centre = per_group<T, N>(mean + sample * G, channels);
+      const PerGroup<T, N> inverse = per_group<T, N>(rstd + sample * G, channels);
       float slope[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) slope[j] = inverse.at(j) * channels.weight[j];
@@ -619,7 +665,7 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
           if (q + static_cast<int64_t>(k) * stride < whole)
             store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
       }
-      if constexpr (!kUniform) {
+      if constexpr (N != 1) {
         const int left = static_cast<int>(elements - whole * V);
         if (left > 0 && owns(share, whole, stride))
           store_part(out + whole * V, normed(load_part(run + whole * V, left)), left);
@@ -645,12 +691,12 @@ struct Statistics {
   float mean[kLdsGroups], rstd[kLdsGroups];
 };
 
-template <typename T, bool kUniform, int TS>
+template <typename T, int N, int TS>
 __global__ __launch_bounds__(TS) void group_norm_direct_kernel(
     const T* __restrict__ x, const float* __restrict__ scale, const float* __restrict__ bias, float eps, bool silu,
     float* __restrict__ mean, float* __restrict__ rstd, T* __restrict__ y, Shape s, Columns columns, int64_t zero_blocks) {
   constexpr int V = kVec<T>;
-  __shared__ MomentsLds<TS, V, kUniform> lds;
+  __shared__ MomentsLds<TS, N> lds;
   __shared__ Statistics statistics;
   const int C = s.channels, G = s.groups;
   const int64_t sample = block_index();
@@ -666,14 +712,14 @@ __global__ __launch_bounds__(TS) void group_norm_direct_kernel(
   if (first >= last || last - first > s.long_rows) return;
   const int64_t elements = (last - first) * C;
   const int64_t whole = elements / V;
-  const int left = kUniform ? 0 : static_cast<int>(elements - whole * V);
+  const int left = N == 1 ? 0 : static_cast<int>(elements - whole * V);
   const T* run = x + first * C;
   T* out = y + first * C;
   const Share share = share_of<T, TS>(columns, 0, C);
   const int stride = columns.stride_vectors();
   const bool held = whole <= static_cast<int64_t>(stride) * kHeld<T>;
-  const bool tail = !kUniform && left > 0 && owns(share, whole, stride);
-  Running<T, kUniform> running;
+  const bool tail = N != 1 && left > 0 && owns(share, whole, stride);
+  Running<T, N> running;
   Raw<T> raw[kHeld<T>];
   int mine = 0;  // held vectors of this thread
   if (held) {
@@ -685,14 +731,14 @@ __global__ __launch_bounds__(TS) void group_norm_direct_kernel(
         mine += share.live && q < whole ? 1 : 0;
       }
   }
-  const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+  const Channels<T, N> channels(share, scale, bias, C, C / G);
   if (held) {
-    if (mine > 0) running.template add<kHeld<T>, false>(raw, mine);
-    if (tail) running.add_part(load_part(run + whole * V, left), left);
+    if (mine > 0) running.template add<kHeld<T>, false>(raw, mine, channels.split);
+    if (tail) running.add_part(load_part(run + whole * V, left), left, channels.split);
   } else {
-    running.add_run(run, elements, share, stride);
+    running.add_run(run, elements, share, stride, channels.split);
   }
-  const Units u = units_of<TS, V, kUniform>(columns, 0, C, G);
+  const Units u = units_of<TS, V, N>(columns, 0, C, G);
   merge_moments<TS>(running, share.live, lds, u, G, [&](int g, float count, float centre, float squares) {
     statistics.mean[g] = centre;
     statistics.rstd[g] = 1.0f / sqrtf(squares / count + eps);
@@ -701,8 +747,8 @@ __global__ __launch_bounds__(TS) void group_norm_direct_kernel(
   });
   __syncthreads();
   if (!share.live) return;
-  const PerGroup<T, kUniform> centre = per_group<T, kUniform>(statistics.mean, channels);
-  const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(statistics.rstd, channels);
+  const PerGroup<T, N> centre = per_group<T, N>(statistics.mean, channels);
+  const PerGroup<T, N> inverse = per_group<T, N>(statistics.rstd, channels);
   float slope[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) slope[j] = inverse.at(j) * channels.weight[j];
@@ -734,9 +780,9 @@ struct Sums {
 #pragma unroll
     for (int j = 0; j < V; ++j) z[j] = zh[j] = 0.0f;
   }
-  template <bool kUniform>
-  __device__ __forceinline__ void add(const Values<T>& grad, const Values<T>& x, const Channels<T, kUniform>& channels,
-                                      const PerGroup<T, kUniform>& centre, const PerGroup<T, kUniform>& inverse, bool silu) {
+  template <int N>
+  __device__ __forceinline__ void add(const Values<T>& grad, const Values<T>& x, const Channels<T, N>& channels,
+                                      const PerGroup<T, N>& centre, const PerGroup<T, N>& inverse, bool silu) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float h = (x.v[j] - centre.at(j)) * inverse.at(j);
@@ -746,8 +792,9 @@ struct Sums {
     }
   }
   // The elements behind the last whole vector; the others add nothing.
-  __device__ __forceinline__ void add_part(const Values<T>& grad, const Values<T>& x, int live, const Channels<T, false>& channels,
-                                           const PerGroup<T, false>& centre, const PerGroup<T, false>& inverse, bool silu) {
+  template <int N>
+  __device__ __forceinline__ void add_part(const Values<T>& grad, const Values<T>& x, int live, const Channels<T, N>& channels,
+                                           const PerGroup<T, N>& centre, const PerGroup<T, N>& inverse, bool silu) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if (j < live) {
@@ -773,26 +820,31 @@ struct SumsLds {
 };
 
 // Calls emit(group, sum u, sum u h) in one lane for every group.
-template <int BLOCK, typename T, bool kUniform, typename Emit>
-__device__ __forceinline__ void merge_sums(const Sums<T>& mine, const Channels<T, kUniform>& channels, bool live,
+template <int BLOCK, typename T, int N, typename Emit>
+__device__ __forceinline__ void merge_sums(const Sums<T>& mine, const Channels<T, N>& channels, bool live,
                                            SumsLds<BLOCK, kVec<T>>& lds, const Units& u, int groups, Emit emit) {
   constexpr int V = kVec<T>;
   if (live) {
-    if constexpr (kUniform) {
-      float sum_u = 0.0f, sum_uh = 0.0f;
+    float sum_u[N], sum_uh[N];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        sum_u = fmaf(mine.z[j], channels.weight[j], sum_u);
-        sum_uh = fmaf(mine.zh[j], channels.weight[j], sum_uh);
-      }
-      lds.a[threadIdx.x] = sum_u;
-      lds.b[threadIdx.x] = sum_uh;
-    } else {
+    for (int i = 0; i < N; ++i) sum_u[i] = sum_uh[i] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        lds.a[threadIdx.x * V + j] = mine.z[j] * channels.weight[j];
-        lds.b[threadIdx.x * V + j] = mine.zh[j] * channels.weight[j];
+    for (int j = 0; j < V; ++j) {
+      const float a = mine.z[j] * channels.weight[j], b = mine.zh[j] * channels.weight[j];
+      if constexpr (N == 2) {
+        sum_u[0] += j < channels.split ? a : 0.0f;
+        sum_uh[0] += j < channels.split ? b : 0.0f;
+        sum_u[1] += j < channels.split ? 0.0f : a;
+        sum_uh[1] += j < channels.split ? 0.0f : b;
+      } else {
+        sum_u[N == 1 ? 0 : j] += a;
+        sum_uh[N == 1 ? 0 : j] += b;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      lds.a[threadIdx.x * N + i] = sum_u[i];
+      lds.b[threadIdx.x * N + i] = sum_uh[i];
     }
   }
   __syncthreads();
@@ -801,7 +853,7 @@ __device__ __forceinline__ void merge_sums(const Sums<T>& mine, const Channels<T
   for (int g = static_cast<int>(threadIdx.x) / u.lanes; g < (groups + per_round - 1) / per_round * per_round; g += per_round) {
     float sum_u = 0.0f, sum_uh = 0.0f;
     if (g < groups)
-      each_term(u, g, lane, [&](int e) {
+      each_term<V, N>(u, g, lane, [&](int e) {
         sum_u += lds.a[e];
         sum_uh += lds.b[e];
       });
@@ -847,7 +899,7 @@ __device__ __forceinline__ void write_columns(const Sums<T>& mine, bool live, Su
 
 // Per piece: sum u and sum u h of each group.  Per tile: sum dz and sum dz h of
 // each channel over all its pieces, kept in registers across them.
-template <typename T, bool kUniform>
+template <typename T, int N>
 __global__ __launch_bounds__(kTileBlock) void group_norm_sums_kernel(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
     const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd, bool silu, Shape s,
@@ -859,8 +911,8 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_sums_kernel(
   const int C = s.channels, G = s.groups;
   for (int pass = 0; pass < columns.passes; ++pass) {
     const Share share = share_of<T, kTileBlock>(columns, pass, C);
-    const Units u = units_of<kTileBlock, V, kUniform>(columns, pass, C, G);
-    const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+    const Units u = units_of<kTileBlock, V, N>(columns, pass, C, G);
+    const Channels<T, N> channels(share, scale, bias, C, C / G);
     const int stride = columns.stride_vectors();
     Sums<T> total;
     each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
@@ -870,8 +922,8 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_sums_kernel(
       const T* run_x = x + a * C;
       Sums<T> sums;
       if (share.live) {
-        const PerGroup<T, kUniform> centre = per_group<T, kUniform>(mean + sample * G, channels);
-        const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(rstd + sample * G, channels);
+        const PerGroup<T, N> centre = per_group<T, N>(mean + sample * G, channels);
+        const PerGroup<T, N> inverse = per_group<T, N>(rstd + sample * G, channels);
         for (int64_t q = share.first; q < whole; q += static_cast<int64_t>(K) * stride) {
           Raw<T> gv[K], xv[K];
 #pragma unroll
@@ -885,7 +937,7 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_sums_kernel(
             if (q + static_cast<int64_t>(k) * stride < whole)
               sums.add(to_values<T>(gv[k]), to_values<T>(xv[k]), channels, centre, inverse, silu);
         }
-        if constexpr (!kUniform) {
+        if constexpr (N != 1) {
           const int left = static_cast<int>(elements - whole * V);
           if (left > 0 && owns(share, whole, stride))
             sums.add_part(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left), left, channels, centre,
@@ -926,9 +978,9 @@ __device__ __forceinline__ float2 merge_sum_slots(const float2* __restrict__ slo
   return {static_cast<float>(sum_u / count), static_cast<float>(sum_uh / count)};
 }
 
-// A wave per (sample, group): means of u and u h.
+// A wave per (sample, group): means of u, then of u h, of each sample's groups.
 __global__ __launch_bounds__(256) void group_norm_means_kernel(const float2* __restrict__ slots, Shape s, int passes,
-                                                               float2* __restrict__ means) {
+                                                               float* __restrict__ means) {
   const int64_t unit = uniform_i64(block_index() * 4 + (threadIdx.x >> 6));
   if (unit >= s.samples * s.groups) return;
   const int64_t sample = unit / s.groups;
@@ -939,7 +991,9 @@ __global__ __launch_bounds__(256) void group_norm_means_kernel(const float2* __r
   const int lane = threadIdx.x & 63;
   const double count = static_cast<double>(last - first) * (s.channels / s.groups);
   const float2 m = merge_sum_slots(slots + start * s.groups + unit % s.groups, n, s.groups, lane, 64, count);
-  if (lane == 0) means[unit] = m;
+  if (lane != 0) return;
+  means[unit + sample * s.groups] = m.x;
+  means[unit + (sample + 1) * s.groups] = m.y;
 }
 
 // dbias and dscale: a workgroup per 8 channels, whose 128 threads of each take
@@ -991,10 +1045,10 @@ __global__ __launch_bounds__(kColumnBlock) void group_norm_columns_kernel(const 
 }
 
 // grad_x of one vector.
-template <typename T, bool kUniform>
-__device__ __forceinline__ Values<T> gradient_of(const Values<T>& grad, const Values<T>& x, const Channels<T, kUniform>& channels,
-                                                 const PerGroup<T, kUniform>& centre, const PerGroup<T, kUniform>& inverse,
-                                                 const PerGroup<T, kUniform>& mean_u, const PerGroup<T, kUniform>& mean_uh,
+template <typename T, int N>
+__device__ __forceinline__ Values<T> gradient_of(const Values<T>& grad, const Values<T>& x, const Channels<T, N>& channels,
+                                                 const PerGroup<T, N>& centre, const PerGroup<T, N>& inverse,
+                                                 const PerGroup<T, N>& mean_u, const PerGroup<T, N>& mean_uh,
                                                  bool silu) {
   Values<T> out;
 #pragma unroll
@@ -1006,11 +1060,11 @@ __device__ __forceinline__ Values<T> gradient_of(const Values<T>& grad, const Va
   return out;
 }
 
-template <typename T, bool kUniform>
+template <typename T, int N>
 __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
     const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd,
-    const float2* __restrict__ means, bool silu, T* __restrict__ grad_x, Shape s, Columns columns) {
+    const float* __restrict__ means, bool silu, T* __restrict__ grad_x, Shape s, Columns columns) {
   constexpr int V = kVec<T>, K = kBatch<T> / 2;
   const int64_t block = block_index();
   if (block >= s.tiles) return;
@@ -1019,7 +1073,7 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
   const int stride = columns.stride_vectors();
   for (int pass = 0; pass < columns.passes; ++pass) {
     const Share share = share_of<T, kTileBlock>(columns, pass, C);
-    const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+    const Channels<T, N> channels(share, scale, bias, C, C / G);
     each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
       if (!share.live) return;
       const int64_t elements = (b - a) * C;
@@ -1027,17 +1081,12 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
       const T* run_g = grad + a * C;
       const T* run_x = x + a * C;
       T* out = grad_x + a * C;
-      const PerGroup<T, kUniform> centre = per_group<T, kUniform>(mean + sample * G, channels);
-      const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(rstd + sample * G, channels);
-      PerGroup<T, kUniform> mean_u, mean_uh;
-#pragma unroll
-      for (int j = 0; j < (kUniform ? 1 : V); ++j) {
-        const float2 m = means[sample * G + channels.group_of(j)];
-        mean_u.v[j] = m.x;
-        mean_uh.v[j] = m.y;
-      }
+      const PerGroup<T, N> centre = per_group<T, N>(mean + sample * G, channels);
+      const PerGroup<T, N> inverse = per_group<T, N>(rstd + sample * G, channels);
+      const PerGroup<T, N> mean_u = per_group<T, N>(means + sample * 2 * G, channels);
+      const PerGroup<T, N> mean_uh = per_group<T, N>(means + (sample * 2 + 1) * G, channels);
       const auto gradient = [&](const Values<T>& gv, const Values<T>& xv) {
-        return gradient_of<T, kUniform>(gv, xv, channels, centre, inverse, mean_u, mean_uh, silu);
+        return gradient_of<T, N>(gv, xv, channels, centre, inverse, mean_u, mean_uh, silu);
       };
       for (int64_t q = share.first; q < whole; q += static_cast<int64_t>(K) * stride) {
         Raw<T> gv[K], xv[K];
@@ -1052,7 +1101,7 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
           if (q + static_cast<int64_t>(k) * stride < whole)
             store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, gradient(to_values<T>(gv[k]), to_values<T>(xv[k])));
       }
-      if constexpr (!kUniform) {
+      if constexpr (N != 1) {
         const int left = static_cast<int>(elements - whole * V);
         if (left > 0 && owns(share, whole, stride))
           store_part(out + whole * V, gradient(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left)), left);
@@ -1074,7 +1123,7 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
 // takes the samples b, b + workgroups, ... and keeps its sums per channel
 // across them, one row of column sums in the end.
 
-template <typename T, bool kUniform, int TS>
+template <typename T, int N, int TS>
 __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
     const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd, bool silu,
@@ -1092,8 +1141,8 @@ __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
     return;
   }
   const Share share = share_of<T, TS>(columns, 0, C);
-  const Units u = units_of<TS, V, kUniform>(columns, 0, C, G);
-  const Channels<T, kUniform> channels(share, scale, bias, C, C / G);
+  const Units u = units_of<TS, V, N>(columns, 0, C, G);
+  const Channels<T, N> channels(share, scale, bias, C, C / G);
   const int stride = columns.stride_vectors();
   Sums<T> total;
   for (int64_t sample = worker; sample < s.samples; sample += workers) {
@@ -1101,11 +1150,11 @@ __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
     if (first >= last || last - first > s.long_rows) continue;
     const int64_t elements = (last - first) * C;
     const int64_t whole = elements / V;
-    const int left = kUniform ? 0 : static_cast<int>(elements - whole * V);
+    const int left = N == 1 ? 0 : static_cast<int>(elements - whole * V);
     const T* run_g = grad + first * C;
     const T* run_x = x + first * C;
     const bool held = whole <= static_cast<int64_t>(stride) * kHeld<T>;
-    const bool tail = !kUniform && left > 0 && owns(share, whole, stride);
+    const bool tail = N != 1 && left > 0 && owns(share, whole, stride);
     Raw<T> gv[kHeld<T>], xv[kHeld<T>];
     int mine = 0;
     if (held) {
@@ -1119,8 +1168,8 @@ __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
           mine += share.live && q < whole ? 1 : 0;
         }
     }
-    const PerGroup<T, kUniform> centre = per_group<T, kUniform>(mean + sample * G, channels);
-    const PerGroup<T, kUniform> inverse = per_group<T, kUniform>(rstd + sample * G, channels);
+    const PerGroup<T, N> centre = per_group<T, N>(mean + sample * G, channels);
+    const PerGroup<T, N> inverse = per_group<T, N>(rstd + sample * G, channels);
     Sums<T> sums;
     if (held) {
 #pragma unroll
@@ -1130,7 +1179,7 @@ __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
       for (int64_t q = share.first; q < whole; q += stride)
         sums.add(load_whole(run_g + q * V), load_whole(run_x + q * V), channels, centre, inverse, silu);
     }
-    if constexpr (!kUniform)
+    if constexpr (N != 1)
       if (tail)
         sums.add_part(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left), left, channels, centre, inverse,
                       silu);
@@ -1144,10 +1193,10 @@ __global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
     __syncthreads();
     if (share.live) {
       T* out = grad_x + first * C;
-      const PerGroup<T, kUniform> mean_u = per_group<T, kUniform>(means.mean, channels);
-      const PerGroup<T, kUniform> mean_uh = per_group<T, kUniform>(means.rstd, channels);
+      const PerGroup<T, N> mean_u = per_group<T, N>(means.mean, channels);
+      const PerGroup<T, N> mean_uh = per_group<T, N>(means.rstd, channels);
       const auto gradient = [&](const Values<T>& g, const Values<T>& v) {
-        return gradient_of<T, kUniform>(g, v, channels, centre, inverse, mean_u, mean_uh, silu);
+        return gradient_of<T, N>(g, v, channels, centre, inverse, mean_u, mean_uh, silu);
       };
       if (held) {
 #pragma unroll
@@ -1251,7 +1300,7 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
 struct Workspace {
   Slot* slots;          // per (piece, pass, group), forward
   float2* sum_slots;    // per (piece, pass, group), backward
-  float2* means;        // per (sample, group), backward
+  float* means;         // per (sample, sum, group), backward
   float2* column_sums;  // rows of channels, backward
 };
 
@@ -1263,7 +1312,7 @@ void each_array(const Schedule& c, bool backward, Take take) {
     return;
   }
   take(&Workspace::sum_slots, pieces);
-  take(&Workspace::means, c.tiles ? static_cast<size_t>(c.shape.samples) * c.shape.groups : 0);
+  take(&Workspace::means, c.tiles ? static_cast<size_t>(c.shape.samples) * 2 * c.shape.groups : 0);
   take(&Workspace::column_sums, static_cast<size_t>(c.column_rows) * c.shape.channels);
 }
 
@@ -1288,18 +1337,13 @@ bool carve(const Schedule& c, bool backward, void* workspace, size_t bytes, Work
   return fits;
 }
 
-template <typename T>
-bool uniform_groups(const Shape& s) {
-  return s.channels / s.groups % kVec<T> == 0;
-}
-
 // Calls LAUNCH(TS) for the schedule's direct workgroup.
 #define DPA4K_DIRECT(threads, LAUNCH)   \
   if (threads == 64) LAUNCH(64);        \
   else if (threads == 256) LAUNCH(256); \
   else LAUNCH(512);
 
-template <typename T, bool kUniform>
+template <typename T, int N>
 int forward_as(const T* x, const float* scale, const float* bias, T* y, float* mean, float* rstd, const Schedule& c,
                float eps, bool silu, const Workspace& w, hipStream_t stream) {
   const Shape& s = c.shape;
@@ -1307,7 +1351,7 @@ int forward_as(const T* x, const float* scale, const float* bias, T* y, float* m
     const Columns columns = columns_for<T>(s.channels, c.threads);
     const dim3 grid = launch_grid(s.samples + c.zero_blocks > 0 ? s.samples + c.zero_blocks : 1, c.threads);
 #define DPA4K_LAUNCH(TS)                                                                                              \
-  group_norm_direct_kernel<T, kUniform, TS><<<grid, TS, 0, stream>>>(x, scale, bias, eps, silu, mean, rstd, y, s, columns, \
+  group_norm_direct_kernel<T, N, TS><<<grid, TS, 0, stream>>>(x, scale, bias, eps, silu, mean, rstd, y, s, columns, \
                                                                      c.zero_blocks)
     if (c.threads == 1024) DPA4K_LAUNCH(1024);
     else DPA4K_DIRECT(c.threads, DPA4K_LAUNCH)
@@ -1317,18 +1361,18 @@ int forward_as(const T* x, const float* scale, const float* bias, T* y, float* m
   if (!c.tiles) return DPA4K_OK;
   const Columns columns = columns_for<T>(s.channels, kTileBlock);
   const dim3 grid = launch_grid(s.tiles, kTileBlock);
-  group_norm_moments_kernel<T, kUniform><<<grid, kTileBlock, 0, stream>>>(x, s, columns, w.slots);
+  group_norm_moments_kernel<T, N><<<grid, kTileBlock, 0, stream>>>(x, s, columns, w.slots);
   if (int e = launched("group_norm_moments_kernel")) return e;
   if (s.samples > 0) {
     group_norm_finish_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(w.slots, s, columns.passes,
                                                                                                   eps, mean, rstd);
     if (int e = launched("group_norm_finish_kernel")) return e;
   }
-  group_norm_apply_kernel<T, kUniform><<<grid, kTileBlock, 0, stream>>>(x, scale, bias, silu, mean, rstd, y, s, columns);
+  group_norm_apply_kernel<T, N><<<grid, kTileBlock, 0, stream>>>(x, scale, bias, silu, mean, rstd, y, s, columns);
   return launched("group_norm_apply_kernel");
 }
 
-template <typename T, bool kUniform>
+template <typename T, int N>
 int backward_as(const T* grad, const T* x, const float* scale, const float* bias, const float* mean, const float* rstd,
                 T* grad_x, float* grad_scale, float* grad_bias, const Schedule& c, bool silu, const Workspace& w,
                 hipStream_t stream) {
@@ -1340,7 +1384,7 @@ int backward_as(const T* grad, const T* x, const float* scale, const float* bias
     const Columns columns = columns_for<T>(s.channels, c.threads);
     const unsigned int grid = static_cast<unsigned int>(c.workers + (grad_x != nullptr ? c.zero_blocks : 0));
 #define DPA4K_LAUNCH(TS)                                                                                                  \
-  group_norm_direct_backward_kernel<T, kUniform, TS><<<grid, TS, 0, stream>>>(grad, x, scale, bias, mean, rstd, silu, grad_x, s, \
+  group_norm_direct_backward_kernel<T, N, TS><<<grid, TS, 0, stream>>>(grad, x, scale, bias, mean, rstd, silu, grad_x, s, \
                                                                               columns, direct_columns, c.workers)
     DPA4K_DIRECT(c.threads, DPA4K_LAUNCH)
 #undef DPA4K_LAUNCH
@@ -1349,7 +1393,7 @@ int backward_as(const T* grad, const T* x, const float* scale, const float* bias
   if (c.tiles) {
     const Columns columns = columns_for<T>(s.channels, kTileBlock);
     const dim3 grid = launch_grid(s.tiles, kTileBlock);
-    group_norm_sums_kernel<T, kUniform><<<grid, kTileBlock, 0, stream>>>(grad, x, scale, bias, mean, rstd, silu, s, columns,
+    group_norm_sums_kernel<T, N><<<grid, kTileBlock, 0, stream>>>(grad, x, scale, bias, mean, rstd, silu, s, columns,
                                                                         w.sum_slots, tile_columns);
     if (int e = launched("group_norm_sums_kernel")) return e;
     if (grad_x != nullptr) {
@@ -1358,7 +1402,7 @@ int backward_as(const T* grad, const T* x, const float* scale, const float* bias
                                                                                                      columns.passes, w.means);
         if (int e = launched("group_norm_means_kernel")) return e;
       }
-      group_norm_backward_kernel<T, kUniform><<<grid, kTileBlock, 0, stream>>>(grad, x, scale, bias, mean, rstd, w.means, silu,
+      group_norm_backward_kernel<T, N><<<grid, kTileBlock, 0, stream>>>(grad, x, scale, bias, mean, rstd, w.means, silu,
                                                                               grad_x, s, columns);
       if (int e = launched("group_norm_backward_kernel")) return e;
     }
@@ -1369,10 +1413,18 @@ int backward_as(const T* grad, const T* x, const float* scale, const float* bias
   return launched("group_norm_columns_kernel");
 }
 
+// The parts of a vector: see the top.
+template <typename T>
+int parts_of(const Shape& s) {
+  const int width = s.channels / s.groups;
+  return width % kVec<T> == 0 ? 1 : (width >= kVec<T> ? 2 : kVec<T>);
+}
+
 template <typename T>
 int forward(const void* x, const float* scale, const float* bias, void* y, float* mean, float* rstd, const Schedule& c,
             float eps, bool silu, const Workspace& w, hipStream_t stream) {
-  return (uniform_groups<T>(c.shape) ? forward_as<T, true> : forward_as<T, false>)(
+  const int parts = parts_of<T>(c.shape);
+  return (parts == 1 ? forward_as<T, 1> : (parts == 2 ? forward_as<T, 2> : forward_as<T, kVec<T>>))(
       static_cast<const T*>(x), scale, bias, static_cast<T*>(y), mean, rstd, c, eps, silu, w, stream);
 }
 
@@ -1380,7 +1432,8 @@ template <typename T>
 int backward(const void* grad, const void* x, const float* scale, const float* bias, const float* mean,
              const float* rstd, void* grad_x, float* grad_scale, float* grad_bias, const Schedule& c, bool silu,
              const Workspace& w, hipStream_t stream) {
-  return (uniform_groups<T>(c.shape) ? backward_as<T, true> : backward_as<T, false>)(
+  const int parts = parts_of<T>(c.shape);
+  return (parts == 1 ? backward_as<T, 1> : (parts == 2 ? backward_as<T, 2> : backward_as<T, kVec<T>>))(
       static_cast<const T*>(grad), static_cast<const T*>(x), scale, bias, mean, rstd, static_cast<T*>(grad_x), grad_scale,
       grad_bias, c, silu, w, stream);
 }

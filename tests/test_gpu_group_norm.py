@@ -138,9 +138,11 @@ def test_malformed_offsets_stay_in_bounds():
 
 def test_constant_and_nonfinite_samples():
     """A constant sample gives the bias; a NaN or infinity stays in its own sample and group."""
-    x = torch.full((30, 8), 3.25)
-    y = group_norm(x.to(DEV), 2, None, torch.arange(8.0, device=DEV), offsets=torch.tensor([0, 30], device=DEV))
-    assert_bitwise(y, torch.arange(8.0).expand(30, 8), "constant")
+    for rows, channels, groups, value in ((30, 8, 2, 3.25), (77, 15, 3, 0.1), (5000, 30, 2, -1.7e5), (40000, 7, 7, 1e-3)):
+        x = torch.full((rows, channels), value)
+        bias = torch.arange(float(channels), device=DEV)
+        y = group_norm(x.to(DEV), groups, None, bias, offsets=torch.tensor([0, rows], device=DEV))
+        assert_bitwise(y, bias.cpu().expand(rows, channels), "constant")
     x = torch.randn(30, 8)
     clean = group_norm(x.to(DEV), 2, offsets=torch.tensor([0, 10, 20, 30], device=DEV))
     x[12, 5] = float("nan")
