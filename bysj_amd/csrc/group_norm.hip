@@ -1119,12 +1119,15 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
 // TS threads hold 32 elements each of a sample's x and gradient, up to 512
 // threads (1,024 would leave 128 registers each, half of them held).  With 16
 // elements a thread samples of 60 rows of 64 took 512 threads, of which a CU
-// holds two workgroups: 51 us for 3,000 of them, 42 us with 32.  A workgroup
-// takes the samples b, b + workgroups, ... and keeps its sums per channel
+// holds two workgroups: 51 us for 3,000 of them, 42 us with 32.  512 threads are
+// held to 128 registers, so that a CU holds two of them (some spill: 16M
+// elements in samples of 16,000 took 58 us with one, 50 us with two; 53 and 38
+// us in bfloat16); fewer threads are slower that way (47 and 54 us in samples of
+// 1,024).  A workgroup takes the samples b, b + workgroups, ... and keeps its sums per channel
 // across them, one row of column sums in the end.
 
 template <typename T, int N, int TS>
-__global__ __launch_bounds__(TS) void group_norm_direct_backward_kernel(
+__global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backward_kernel(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
     const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd, bool silu,
     T* __restrict__ grad_x, Shape s, Columns columns, float2* __restrict__ column_sums, int64_t workers) {
