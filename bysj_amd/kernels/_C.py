@@ -904,15 +904,24 @@ def group_norm_forward(x, groups, scale=None, bias=None, offsets=None, eps: floa
 
 
 def group_norm_backward(grad_output, x, groups, scale, bias, offsets, statistics, silu: bool = False, *,
-                        want_x: bool = True, want_scale: bool = True, want_bias: bool = True, max_rows=None):
-    """``(grad_x, grad_scale, grad_bias)``, None where not wanted."""
+                        want_x: bool = True, want_scale: bool = True, want_bias: bool = True, max_rows=None,
+                        sizes=None):
+    """``(grad_x, grad_scale, grad_bias)``, None where not wanted.
+
+    ``sizes``: what ``_group_norm_sizes`` said of the forward's arguments, where
+    the caller has kept them and the statistics (the autograd function, whose
+    backward is mostly host time for small samples).
+    """
     groups = int(groups)
-    samples, entries, inner, channels = _group_norm_sizes(x, groups, scale, bias, offsets)
     _check(isinstance(grad_output, torch.Tensor) and grad_output.is_contiguous() and grad_output.dtype == x.dtype
-           and grad_output.shape == x.shape, "group norm grad_output must be like the input")
-    _f32(statistics, "group norm statistics")
-    _check(statistics.shape == (2, samples, groups), "group norm statistics must have shape (2, samples, groups)")
-    _same_device(x, grad_output, statistics)
+           and grad_output.shape == x.shape and grad_output.device == x.device,
+           "group norm grad_output must be like the input")
+    if sizes is None:
+        sizes = _group_norm_sizes(x, groups, scale, bias, offsets)
+        _f32(statistics, "group norm statistics")
+        _check(statistics.shape == (2, sizes[0], groups), "group norm statistics must have shape (2, samples, groups)")
+        _same_device(x, statistics)
+    samples, entries, inner, channels = sizes
     device = x.device
     grad_x = torch.empty_like(x) if want_x else None
     grad_scale = torch.empty((channels,), dtype=torch.float32, device=device) if want_scale else None
@@ -1006,7 +1015,8 @@ def adamw_plan(params, exp_avgs, exp_avg_sqs, steps, state_bits: int) -> AdamWPl
     table = (_lib.AdamwTensor * n)()
     if state_bits == 32:
         plan.exp_avgs, plan.exp_avg_sqs = (
-            [torch.zeros_like(p, dtype=torch.float32) for p in plan.params] if given is None else list(given)
+            [torch.zeros_like(p, dtype=torch.float32).detach() for p in plan.params] if given is None
+            else [m.detach() for m in given]  # the plan's own hold on this memory, whatever becomes of the tensors given
             for given in (exp_avgs, exp_avg_sqs))
     else:
         spans = [-(-count // ADAMW_SPAN) for count in counts]

@@ -87,18 +87,21 @@ class _GroupNormFunction(torch.autograd.Function):
         native = _extension("group_norm_forward")
         y, statistics = native.group_norm_forward(x, groups, scale, bias, offsets, eps, silu, max_rows=max_rows)
         ctx.save_for_backward(x, scale, bias, offsets, statistics)
-        ctx.arguments = groups, max_rows, silu
+        entries, inner = x.shape[0], math.prod(x.shape[1:-1])
+        samples = entries if offsets is None else offsets.numel() - 1
+        ctx.arguments = groups, max_rows, silu, (samples, entries, inner, x.shape[-1])
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
         x, scale, bias, offsets, statistics = ctx.saved_tensors
-        groups, max_rows, silu = ctx.arguments
+        groups, max_rows, silu, sizes = ctx.arguments
         want = ctx.needs_input_grad
         native = _extension("group_norm_backward")
         grads = native.group_norm_backward(grad_output.contiguous(), x, groups, scale, bias, offsets, statistics, silu,
-                                           want_x=want[0], want_scale=want[1], want_bias=want[2], max_rows=max_rows)
+                                           want_x=want[0], want_scale=want[1], want_bias=want[2], max_rows=max_rows,
+                                           sizes=sizes)
         return (*grads, None, None, None, None, None)
 
 

@@ -331,7 +331,10 @@ class AdamW(torch.optim.Optimizer):
             for dtype in DTYPES:
                 params = [p for p in group["params"] if p.dtype == dtype]
                 grads = [p.grad for p in params]
-                if any([g is not None for g in grads]):
+                given = [g for g in grads if g is not None]
+                if not all(map(torch.Tensor.is_contiguous, given)):
+                    grads = [None if g is None else g.contiguous() for g in grads]
+                if given:
                     work.append((group, self._plan((index, dtype), params), grads, index * 2 + (dtype == torch.bfloat16)))
         self.norm = factor = None
         if self.max_norm is not None and work:
@@ -340,6 +343,9 @@ class AdamW(torch.optim.Optimizer):
             adamw_step(plan, grads, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                        weight_decay=group["weight_decay"], grad_factor=factor, seed=self.seed + stream * 0x9E3779B97F4A7C15)
         return loss
+
+    def __getstate__(self):
+        raise TypeError("the moments live in plans on the device: save state_dict() instead")
 
     def state_dict(self) -> dict:
         result = super().state_dict()
@@ -351,8 +357,9 @@ class AdamW(torch.optim.Optimizer):
         return result
 
     def load_state_dict(self, state_dict) -> None:
-        if state_dict.get("state_bits", self.state_bits) != self.state_bits:
-            raise ValueError(f"the checkpoint holds {state_dict['state_bits']}-bit moments, not {self.state_bits}-bit ones")
+        bits = state_dict.get("state_bits", 32)  # torch's own AdamW does not say
+        if bits != self.state_bits:
+            raise ValueError(f"the checkpoint holds {bits}-bit moments, not {self.state_bits}-bit ones")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         params = [p for group in self.param_groups for p in group["params"]]
         held = {params[int(k)]: part for k, part in state_dict["state"].items()}

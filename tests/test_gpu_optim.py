@@ -386,6 +386,48 @@ def test_parameters_that_move_keep_their_moments(bits):
         assert_bitwise(a, b, "moved")
 
 
+def test_a_checkpoint_of_torch_is_taken_over():
+    params, grads, _, _ = _model([64, 33])
+    twin = [p.clone().requires_grad_(True) for p in params]
+    theirs = torch.optim.AdamW(twin, lr=0.01)
+    for p, g in zip(twin, grads):
+        p.grad = g
+    theirs.step()
+    mine = [p.detach().clone().requires_grad_(True) for p in twin]
+    optimiser = optim.AdamW(mine, lr=0.01)
+    optimiser.load_state_dict(theirs.state_dict())
+    for p, g in zip(mine, grads):
+        p.grad = g
+    optimiser.step()
+    theirs.step()
+    for a, b in zip(mine, twin):
+        # both in float32: a step of at most 0.01 and its quotient of about ten roundings on each side
+        assert_close_scaled(a.detach(), b.detach(), rtol=2e-7, scale=2e-7, what="taken over")
+
+
+def test_gradients_of_any_layout_and_moments_that_are_replaced():
+    p = torch.randn(8, 16, generator=torch.Generator().manual_seed(0)).to(DEV).requires_grad_(True)
+    twin = p.detach().clone().requires_grad_(True)
+    g = torch.randn(16, 8, device=DEV)
+    pair = [optim.AdamW([t], max_norm=0.5) for t in (p, twin)]
+    p.grad, twin.grad = g.t(), g.t().contiguous()
+    for o in pair:
+        o.step()
+    assert_bitwise(p.detach(), twin.detach(), "transposed gradient")
+    m, v = torch.zeros(100, device=DEV), torch.zeros(100, device=DEV)
+    w = [torch.zeros(100, device=DEV)]
+    plan = optim.adamw_plan(w, [m], [v])
+    m.data = torch.full((100,), 7.0, device=DEV)
+    optim.adamw_step(plan, [torch.ones(100, device=DEV)], **HYPER)
+    assert (m == 7.0).all() and (plan.exp_avgs[0] > 0).all()  # the plan keeps the memory that it was given
+
+
+def test_an_optimiser_is_saved_by_its_state():
+    optimiser = optim.AdamW([torch.zeros(3, device=DEV, requires_grad=True)])
+    with pytest.raises(TypeError, match="state_dict"):
+        copy.deepcopy(optimiser)
+
+
 def test_scheduler_and_copies():
     params, grads, _, _ = _model([64])
     p = params[0].requires_grad_(True)
