@@ -565,6 +565,53 @@ __device__ __forceinline__ Merged merge_slots(const Slot* __restrict__ slots, in
 }
 
 // ---------------------------------------------------------------------------
+// loops over a thread's vectors of a run
+// ---------------------------------------------------------------------------
+
+// out = value(x) for the vectors q, q + stride, ... below `whole`, K loads in flight.
+template <typename T, int K, typename Value>
+__device__ __forceinline__ void map_run(const T* __restrict__ run, T* __restrict__ out, int64_t q, int64_t whole, int stride,
+                                        Value value) {
+  constexpr int V = kVec<T>;
+  for (; q + static_cast<int64_t>(K - 1) * stride < whole; q += static_cast<int64_t>(K) * stride) {
+    Raw<T> raw[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) raw[k] = load_raw(run + (q + static_cast<int64_t>(k) * stride) * V);
+#pragma unroll
+    for (int k = 0; k < K; ++k) store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, value(to_values<T>(raw[k])));
+  }
+  if (q < whole) {
+    Raw<T> raw[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) raw[k] = load_raw(run + place_of(q, k, stride, whole) * V);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (q + static_cast<int64_t>(k) * stride < whole)
+        store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, value(to_values<T>(raw[k])));
+  }
+}
+
+// visit(place, a, b) for the same vectors of two runs.
+template <typename T, int K, typename Visit>
+__device__ __forceinline__ void each_pair(const T* __restrict__ run_a, const T* __restrict__ run_b, int64_t q, int64_t whole,
+                                          int stride, Visit visit) {
+  constexpr int V = kVec<T>;
+  for (; q < whole; q += static_cast<int64_t>(K) * stride) {
+    Raw<T> a[K], b[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t at = place_of(q, k, stride, whole) * V;
+      a[k] = load_raw(run_a + at);
+      b[k] = load_raw(run_b + at);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (q + static_cast<int64_t>(k) * stride < whole)
+        visit((q + static_cast<int64_t>(k) * stride) * V, to_values<T>(a[k]), to_values<T>(b[k]));
+  }
+}
+
+// ---------------------------------------------------------------------------
 // tiles, forward
 // ---------------------------------------------------------------------------
 
@@ -648,23 +695,7 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
           value.v[j] = activated(fmaf(value.v[j] - centre.at(j), slope[j], channels.shift[j]), silu);
         return value;
       };
-      int64_t q = share.first;
-      for (; q + static_cast<int64_t>(K - 1) * stride < whole; q += static_cast<int64_t>(K) * stride) {
-        Raw<T> raw[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) raw[k] = load_raw(run + (q + static_cast<int64_t>(k) * stride) * V);
-#pragma unroll
-        for (int k = 0; k < K; ++k) store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
-      }
-      if (q < whole) {
-        Raw<T> raw[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) raw[k] = load_raw(run + place_of(q, k, stride, whole) * V);
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (q + static_cast<int64_t>(k) * stride < whole)
-            store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
-      }
+      map_run<T, K>(run, out, share.first, whole, stride, normed);
       if constexpr (N != 1) {
         const int left = static_cast<int>(elements - whole * V);
         if (left > 0 && owns(share, whole, stride))
@@ -762,7 +793,7 @@ __global__ __launch_bounds__(TS) void group_norm_direct_kernel(
     for (int k = 0; k < kHeld<T>; ++k)
       if (k < mine) store_whole(out + (share.first + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
   } else {
-    for (int64_t q = share.first; q < whole; q += stride) store_whole(out + q * V, normed(load_whole(run + q * V)));
+    map_run<T, 4>(run, out, share.first, whole, stride, normed);
   }
   if (tail) store_part(out + whole * V, normed(load_part(run + whole * V, left)), left);
 }
@@ -924,19 +955,9 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_sums_kernel(
       if (share.live) {
         const PerGroup<T, N> centre = per_group<T, N>(mean + sample * G, channels);
         const PerGroup<T, N> inverse = per_group<T, N>(rstd + sample * G, channels);
-        for (int64_t q = share.first; q < whole; q += static_cast<int64_t>(K) * stride) {
-          Raw<T> gv[K], xv[K];
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            const int64_t at = place_of(q, k, stride, whole) * V;
-            gv[k] = load_raw(run_g + at);
-            xv[k] = load_raw(run_x + at);
-          }
-#pragma unroll
-          for (int k = 0; k < K; ++k)
-            if (q + static_cast<int64_t>(k) * stride < whole)
-              sums.add(to_values<T>(gv[k]), to_values<T>(xv[k]), channels, centre, inverse, silu);
-        }
+        each_pair<T, K>(run_g, run_x, share.first, whole, stride, [&](int64_t, const Values<T>& gv, const Values<T>& xv) {
+          sums.add(gv, xv, channels, centre, inverse, silu);
+        });
         if constexpr (N != 1) {
           const int left = static_cast<int>(elements - whole * V);
           if (left > 0 && owns(share, whole, stride))
@@ -1088,19 +1109,9 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
       const auto gradient = [&](const Values<T>& gv, const Values<T>& xv) {
         return gradient_of<T, N>(gv, xv, channels, centre, inverse, mean_u, mean_uh, silu);
       };
-      for (int64_t q = share.first; q < whole; q += static_cast<int64_t>(K) * stride) {
-        Raw<T> gv[K], xv[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int64_t at = place_of(q, k, stride, whole) * V;
-          gv[k] = load_raw(run_g + at);
-          xv[k] = load_raw(run_x + at);
-        }
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (q + static_cast<int64_t>(k) * stride < whole)
-            store_whole(out + (q + static_cast<int64_t>(k) * stride) * V, gradient(to_values<T>(gv[k]), to_values<T>(xv[k])));
-      }
+      each_pair<T, K>(run_g, run_x, share.first, whole, stride, [&](int64_t at, const Values<T>& gv, const Values<T>& xv) {
+        store_whole(out + at, gradient(gv, xv));
+      });
       if constexpr (N != 1) {
         const int left = static_cast<int>(elements - whole * V);
         if (left > 0 && owns(share, whole, stride))
@@ -1179,8 +1190,10 @@ __global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backw
       for (int k = 0; k < kHeld<T>; ++k)
         if (k < mine) sums.add(to_values<T>(gv[k]), to_values<T>(xv[k]), channels, centre, inverse, silu);
     } else if (share.live) {
-      for (int64_t q = share.first; q < whole; q += stride)
-        sums.add(load_whole(run_g + q * V), load_whole(run_x + q * V), channels, centre, inverse, silu);
+      each_pair<T, kBatch<T> / 2>(run_g, run_x, share.first, whole, stride,
+                                  [&](int64_t, const Values<T>& g, const Values<T>& v) {
+                                    sums.add(g, v, channels, centre, inverse, silu);
+                                  });
     }
     if constexpr (N != 1)
       if (tail)
@@ -1208,8 +1221,8 @@ __global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backw
             store_whole(out + (share.first + static_cast<int64_t>(k) * stride) * V,
                         gradient(to_values<T>(gv[k]), to_values<T>(xv[k])));
       } else {
-        for (int64_t q = share.first; q < whole; q += stride)
-          store_whole(out + q * V, gradient(load_whole(run_g + q * V), load_whole(run_x + q * V)));
+        each_pair<T, kBatch<T> / 2>(run_g, run_x, share.first, whole, stride,
+                                    [&](int64_t at, const Values<T>& g, const Values<T>& v) { store_whole(out + at, gradient(g, v)); });
       }
       if (tail)
         store_part(out + whole * V, gradient(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left)), left);
@@ -1245,9 +1258,19 @@ constexpr int kDirectThreads[] = {64, 256, 512, 1024};
 constexpr int64_t workers_for(int threads) { return threads == 64 ? 3072 : (threads == 256 ? 768 : 512); }
 
 // Checks the sizes, cuts the rows into tiles, and chooses the schedule.  A
-// direct workgroup holds 32 elements a thread.  The smallest that holds the
-// longest sample is taken; where the longest is not known, one that holds twice
-// the mean, and the rest goes to tiles.
+// direct workgroup holds 32 elements a thread.  Samples of one length take the
+// smallest that holds one.  Ragged samples take the smallest that holds the
+// longest where all of them are resident at once, and else one that holds a
+// quarter more than the mean: a larger one would idle on most samples (4,096
+// samples cut anywhere in 200,000 rows of 64 floats, forward: 99 us with room for
+// the longest, 393 rows, 30 with room for 61; 50,000 samples: 176 and 56 us).  A
+// sample that is longer is streamed, up to kStreamed times what is held (samples
+// of 49 rows of 90 in the mean: 65 us up to 4 times, 43 up to 16).  Longer ones
+// take tiles, and all do where no workgroup holds the mean, or in the backward
+// one of 512 threads, two to a CU, would (1,000 samples: 86 us, tiles 70).
+constexpr int64_t kResidentThreads = 262144;  // 16 waves on each CU
+constexpr int64_t kStreamed = 16;
+
 int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inner, int64_t channels, int64_t groups,
                 int type, const int64_t* offsets, int64_t max_entries, bool backward, Schedule& out) {
   if (samples < 0 || entries < 0 || inner < 0) return fail(DPA4K_EINVAL, "%s: negative sizes", what);
@@ -1274,25 +1297,30 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
   const int vec = static_cast<int>(16 / type_bytes(type));
   const int period = static_cast<int>(channels) / gcd_of(static_cast<int>(channels), vec);
   out.passes = (period + kTileBlock - 1) / kTileBlock;
-  // rows of the longest sample, or what most samples are expected not to pass
-  const bool known = offsets == nullptr || max_entries >= 0;
-  int64_t wanted = offsets == nullptr ? inner : 0;
-  if (offsets != nullptr) {
-    if (known) wanted = (max_entries < entries ? max_entries : entries) * inner;
-    else wanted = samples > 0 ? 2 * (rows / samples) + 1 : 0;
-  }
-  const int64_t elements = wanted * channels;
-  if (groups <= kLdsGroups)
-    for (int threads : kDirectThreads) {
-      if (period > threads || (backward && threads > 512)) continue;
-      const int64_t holds = static_cast<int64_t>(threads / period) * period * 32;
-      if (elements > holds && (known || threads < (backward ? 512 : 1024))) continue;
-      out.threads = threads;
-      out.shape.long_rows = holds / channels;
-      break;
+  // the smallest direct workgroup that holds `sample_rows`, 0 where none does
+  const auto holds = [&](int threads) { return static_cast<int64_t>(threads / period) * period * 32 / channels; };
+  const auto threads_for = [&](int64_t sample_rows) {
+    if (groups <= kLdsGroups)
+      for (int threads : kDirectThreads)
+        if (period <= threads && !(backward && threads > 512) && sample_rows <= holds(threads)) return threads;
+    return 0;
+  };
+  if (offsets == nullptr) {
+    out.threads = threads_for(inner);
+    out.shape.long_rows = out.threads != 0 ? INT64_MAX : 0;
+    out.tiles = out.threads == 0;
+  } else {
+    const int64_t longest = max_entries < 0 ? INT64_MAX : (max_entries < entries ? max_entries : entries) * inner;
+    const int for_longest = threads_for(longest);
+    out.threads = for_longest;
+    if (for_longest == 0 || samples * for_longest > kResidentThreads) {
+      out.threads = threads_for(samples > 0 ? rows / samples * 5 / 4 + 1 : 1);
+      if (backward && out.threads == 512) out.threads = 0;
     }
-  if (out.threads != 0 && known) out.shape.long_rows = INT64_MAX;  // nothing is left to tiles: a longer sample is streamed
-  out.tiles = out.threads == 0 || !known;
+    const int64_t limit = kStreamed * holds(out.threads);
+    out.tiles = out.threads == 0 || longest > limit;
+    out.shape.long_rows = out.threads == 0 ? 0 : (out.tiles ? limit : INT64_MAX);  // with no tiles any sample is streamed
+  }
   out.workers = out.threads == 0 ? 0 : (samples < workers_for(out.threads) ? samples : workers_for(out.threads));
   const int64_t kilobytes64 = rows * row_bytes / 65536 + 1;
   out.zero_blocks = offsets == nullptr || out.tiles ? 0 : (kilobytes64 < 256 ? kilobytes64 : 256);
