@@ -12,14 +12,17 @@
 // Bound by its streams.  Two schedules:
 //
 //  - direct: a workgroup of 64 to 1,024 threads per sample holds the sample in
-//    registers between its statistics and its output, one launch and one read.
+//    registers between its statistics and its output, one launch and one read
+//    (16M float32 elements in samples of 8,000, forward: 23 us, 5.8 TB/s;
+//    backward 45 us, 4.5 TB/s).  Somewhat longer samples are read twice by it.
 //  - tiles: samples too long for that (or of unknown length) are cut, whatever
 //    their lengths, by tiles of equal rows, a workgroup per tile that walks the
 //    pieces of samples in it.  A piece leaves its sums in slot (tile + sample),
 //    a number no other piece has, since from piece to piece one of the two
 //    grows; a sample's slots are consecutive.  A small launch merges them, a
 //    third writes the output, with the tiles in reverse order: what was read
-//    last is still in the memory-side cache.
+//    last is still in the memory-side cache (one sample of 100 MB: forward 22 +
+//    7 + 35 us, backward 34 + 5 + 46 + 4 us).
 //
 // A sample, or a piece, is read as one run of 16-byte vectors.  Vector q of a
 // run holds the channels (q V + j) mod C, so with a stride of a multiple of
@@ -1130,12 +1133,15 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
 // TS threads hold 32 elements each of a sample's x and gradient, up to 512
 // threads (1,024 would leave 128 registers each, half of them held).  With 16
 // elements a thread samples of 60 rows of 64 took 512 threads, of which a CU
-// holds two workgroups: 51 us for 3,000 of them, 42 us with 32.  512 threads are
-// held to 128 registers, so that a CU holds two of them (some spill: 16M
-// elements in samples of 16,000 took 58 us with one, 50 us with two; 53 and 38
-// us in bfloat16); fewer threads are slower that way (47 and 54 us in samples of
-// 1,024).  A workgroup takes the samples b, b + workgroups, ... and keeps its sums per channel
-// across them, one row of column sums in the end.
+// holds two workgroups: 51 us for 3,000 of them (139 MB), 37 us with 32.  512
+// threads are held to 128 registers, so that a CU holds two of them (some spill:
+// 16M elements in samples of 16,000 took 58 us with one, 50 us with two; 53 and
+// 38 us in bfloat16); fewer threads are slower that way (47 and 54 us in samples
+// of 1,024).  A workgroup takes the samples b, b + workgroups, ... and keeps its
+// sums per channel across them, one row of column sums in the end.  A longer
+// sample is streamed, two vectors of each tensor at once: four would take the
+// registers of the third wave of a SIMD from every sample (37 -> 51 us above).
+constexpr int kStreamedAtOnce = 2;
 
 template <typename T, int N, int TS>
 __global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backward_kernel(
@@ -1190,7 +1196,7 @@ __global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backw
       for (int k = 0; k < kHeld<T>; ++k)
         if (k < mine) sums.add(to_values<T>(gv[k]), to_values<T>(xv[k]), channels, centre, inverse, silu);
     } else if (share.live) {
-      each_pair<T, kBatch<T> / 2>(run_g, run_x, share.first, whole, stride,
+      each_pair<T, kStreamedAtOnce>(run_g, run_x, share.first, whole, stride,
                                   [&](int64_t, const Values<T>& g, const Values<T>& v) {
                                     sums.add(g, v, channels, centre, inverse, silu);
                                   });
@@ -1221,7 +1227,7 @@ __global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backw
             store_whole(out + (share.first + static_cast<int64_t>(k) * stride) * V,
                         gradient(to_values<T>(gv[k]), to_values<T>(xv[k])));
       } else {
-        each_pair<T, kBatch<T> / 2>(run_g, run_x, share.first, whole, stride,
+        each_pair<T, kStreamedAtOnce>(run_g, run_x, share.first, whole, stride,
                                     [&](int64_t at, const Values<T>& g, const Values<T>& v) { store_whole(out + at, gradient(g, v)); });
       }
       if (tail)
