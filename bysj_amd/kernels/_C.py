@@ -883,10 +883,15 @@ def _group_norm_sizes(x, groups, scale, bias, offsets):
 
 
 def group_norm_forward(x, groups, scale=None, bias=None, offsets=None, eps: float = 1.0e-5, silu: bool = False, *,
-                       max_rows=None):
-    """``(y, statistics)``; ``statistics`` is ``(2, samples, groups)`` float32: means and 1 / sqrt(var + eps)."""
+                       max_rows=None, sizes=None):
+    """``(y, statistics)``; ``statistics`` is ``(2, samples, groups)`` float32: means and 1 / sqrt(var + eps).
+
+    ``sizes``: what ``_group_norm_sizes`` says, where the caller has checked the
+    arguments itself (``kernels.group_norm``: a call on small samples is mostly
+    host time).
+    """
     groups = int(groups)
-    samples, entries, inner, channels = _group_norm_sizes(x, groups, scale, bias, offsets)
+    samples, entries, inner, channels = sizes or _group_norm_sizes(x, groups, scale, bias, offsets)
     device = x.device
     y = torch.empty_like(x)
     statistics = torch.empty((2, samples, groups), dtype=torch.float32, device=device)
@@ -908,9 +913,7 @@ def group_norm_backward(grad_output, x, groups, scale, bias, offsets, statistics
                         sizes=None):
     """``(grad_x, grad_scale, grad_bias)``, None where not wanted.
 
-    ``sizes``: what ``_group_norm_sizes`` said of the forward's arguments, where
-    the caller has kept them and the statistics (the autograd function, whose
-    backward is mostly host time for small samples).
+    ``sizes``: as in the forward, where the caller has kept its arguments and statistics.
     """
     groups = int(groups)
     _check(isinstance(grad_output, torch.Tensor) and grad_output.is_contiguous() and grad_output.dtype == x.dtype

@@ -85,11 +85,12 @@ class _GroupNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, offsets, groups, max_rows, eps, silu):
         native = _extension("group_norm_forward")
-        y, statistics = native.group_norm_forward(x, groups, scale, bias, offsets, eps, silu, max_rows=max_rows)
+        shape = x.shape
+        samples = shape[0] if offsets is None else offsets.numel() - 1
+        sizes = samples, shape[0], math.prod(shape[1:-1]), shape[-1]
+        y, statistics = native.group_norm_forward(x, groups, scale, bias, offsets, eps, silu, max_rows=max_rows, sizes=sizes)
         ctx.save_for_backward(x, scale, bias, offsets, statistics)
-        entries, inner = x.shape[0], math.prod(x.shape[1:-1])
-        samples = entries if offsets is None else offsets.numel() - 1
-        ctx.arguments = groups, max_rows, silu, (samples, entries, inner, x.shape[-1])
+        ctx.arguments = groups, max_rows, silu, sizes
         return y
 
     @staticmethod
