@@ -1258,10 +1258,11 @@ struct Schedule {
 };
 
 constexpr int kDirectThreads[] = {64, 256, 512, 1024};
-// Backward workgroups of a direct launch: as many as are resident at three waves
-// a SIMD (3,000 samples of 60 rows of 64: 39 us with 768 workgroups of 256
-// threads, 41 with 2,048, 47 with 1,024, whose last third finds the CUs full).
-constexpr int64_t workers_for(int threads) { return threads == 64 ? 3072 : (threads == 256 ? 768 : 512); }
+// Backward workgroups of a direct launch: as many as are resident on 256 CUs at
+// three waves a SIMD, and two of 512 threads to a CU (3,000 samples of 60 rows of
+// 64: 39 us with 768 workgroups of 256 threads, 41 with 2,048, 47 with 1,024,
+// whose last third finds the CUs full).
+constexpr int64_t workers_for(int threads) { return 256 * (threads > 256 ? 2 : 12 / (threads / 64)); }
 
 // Checks the sizes, cuts the rows into tiles, and chooses the schedule.  A
 // direct workgroup holds 32 elements a thread.  Samples of one length take the
