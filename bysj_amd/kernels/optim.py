@@ -266,6 +266,7 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group) -> None:
+        self._refuse_variants([{**self.defaults, **param_group}])
         super().add_param_group(param_group)
         group = self.param_groups[-1]
         if isinstance(group["lr"], torch.Tensor):
@@ -283,6 +284,15 @@ class AdamW(torch.optim.Optimizer):
                 raise TypeError("AdamW requires float32 or bfloat16 parameters")
             if not p.is_contiguous():
                 raise ValueError("AdamW parameters must be contiguous")
+
+    @staticmethod
+    def _refuse_variants(groups) -> None:
+        """Options of torch's optimisers that change the step, as their checkpoints and parameter groups hold them."""
+        for group in groups:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("AdamW has neither amsgrad nor maximize")
+            if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
+                raise ValueError("AdamW's weight decay is decoupled from the gradient")
 
     def _plan(self, key, params):
         plan = self._plans.get(key)
@@ -360,6 +370,7 @@ class AdamW(torch.optim.Optimizer):
         bits = state_dict.get("state_bits", 32)  # torch's own AdamW does not say
         if bits != self.state_bits:
             raise ValueError(f"the checkpoint holds {bits}-bit moments, not {self.state_bits}-bit ones")
+        self._refuse_variants(state_dict["param_groups"])
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         params = [p for group in self.param_groups for p in group["params"]]
         held = {params[int(k)]: part for k, part in state_dict["state"].items()}

@@ -171,6 +171,23 @@ def test_optimiser_refusals(error, params, kwargs):
         optim.AdamW(params, **kwargs)
 
 
+@pytest.mark.parametrize("theirs,options", [
+    (torch.optim.AdamW, {"amsgrad": True}),
+    (torch.optim.AdamW, {"maximize": True}),
+    (torch.optim.Adam, {"weight_decay": 0.1}),  # added to the gradient there
+])
+def test_optimiser_refuses_options_that_it_does_not_have(theirs, options):
+    p = torch.nn.Parameter(torch.zeros(3))
+    mine = optim.AdamW([p], lr=0.5)
+    with pytest.raises(ValueError):
+        mine.load_state_dict(theirs([p], **options).state_dict())
+    assert mine.param_groups[0]["lr"] == 0.5
+    with pytest.raises(ValueError):
+        optim.AdamW([dict(theirs([p], **options).param_groups[0])])
+    mine.load_state_dict(theirs([p], lr=0.25, weight_decay=0.0).state_dict())
+    assert mine.param_groups[0]["lr"] == 0.25
+
+
 @BUILT
 def test_c_entry_points_refuse_bad_sizes_before_any_device_call():
     lib = _lib.load()
