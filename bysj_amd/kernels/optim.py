@@ -260,6 +260,8 @@ class AdamW(torch.optim.Optimizer):
                  max_norm: float | None = None, state_bits: int = 32, seed: int = 0):
         if isinstance(state_bits, bool) or state_bits not in STATE_BITS:
             raise ValueError(f"AdamW state_bits must be 32 or 8, got {state_bits!r}")
+        if isinstance(seed, bool) or not isinstance(seed, numbers.Integral):
+            raise TypeError("AdamW seed must be an integer")
         self.max_norm = None if max_norm is None else _real(max_norm, "AdamW max_norm", 0.0, above=True)
         self.state_bits, self.seed, self.norm = state_bits, int(seed), None
         self._plans: dict = {}     # (group, dtype): plan

@@ -188,6 +188,12 @@ def test_optimiser_refuses_options_that_it_does_not_have(theirs, options):
     assert mine.param_groups[0]["lr"] == 0.25
 
 
+@pytest.mark.parametrize("seed", [1.5, True, "1", None])
+def test_optimiser_refuses_seeds_that_are_not_integers(seed):
+    with pytest.raises(TypeError):
+        optim.AdamW(P, seed=seed)
+
+
 @BUILT
 def test_c_entry_points_refuse_bad_sizes_before_any_device_call():
     lib = _lib.load()
