@@ -296,13 +296,24 @@ class AdamW(torch.optim.Optimizer):
             if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
                 raise ValueError("AdamW's weight decay is decoupled from the gradient")
 
-    def _plan(self, key, params):
-        plan = self._plans.get(key)
-        if plan is not None and len(plan.params) == len(params) and \
-                all(map(operator.is_, plan.params, params)) and list(map(torch.Tensor.data_ptr, params)) == plan.addresses:
-            return plan
-        held = {} if plan is None else self._held(plan)
-        return self._build(key, params, held)
+    def _current(self) -> list:
+        """``[(group index, dtype), parameters]`` as they are now."""
+        return [((index, dtype), [p for p in group["params"] if p.dtype == dtype])
+                for index, group in enumerate(self.param_groups) for dtype in DTYPES]
+
+    def _follow(self, current) -> None:
+        """Rebuilds the plans if a parameter has moved, come or gone, or changed its dtype since they were built."""
+        for key, params in current:
+            plan = self._plans.get(key)
+            if plan is not None and not (len(plan.params) == len(params) and all(map(operator.is_, plan.params, params))
+                                         and list(map(torch.Tensor.data_ptr, params)) == plan.addresses):
+                return self._rebuild({p: part for plan in self._plans.values() for p, part in self._held(plan).items()})
+
+    def _rebuild(self, held) -> None:
+        self._plans = {}
+        for key, params in self._current():
+            if any([p in held for p in params]):
+                self._build(key, params, held)
 
     def _build(self, key, params, held):
         """A plan of ``params`` that goes on from ``held``: {parameter: its part of a checkpoint}."""
@@ -338,16 +349,17 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = []
-        for index, group in enumerate(self.param_groups):
-            for dtype in DTYPES:
-                params = [p for p in group["params"] if p.dtype == dtype]
-                grads = [p.grad for p in params]
-                given = [g for g in grads if g is not None]
-                if not all(map(torch.Tensor.is_contiguous, given)):
-                    grads = [None if g is None else g.contiguous() for g in grads]
-                if given:
-                    work.append((group, self._plan((index, dtype), params), grads, index * 2 + (dtype == torch.bfloat16)))
+        current, work = self._current(), []
+        self._follow(current)
+        for key, params in current:
+            grads = [p.grad for p in params]
+            given = [g for g in grads if g is not None]
+            if not all(map(torch.Tensor.is_contiguous, given)):
+                grads = [None if g is None else g.contiguous() for g in grads]
+            if given:
+                plan = self._plans.get(key) or self._build(key, params, {})
+                index, dtype = key
+                work.append((self.param_groups[index], plan, grads, index * 2 + (dtype == torch.bfloat16)))
         self.norm = factor = None
         if self.max_norm is not None and work:
             self.norm, factor = grad_norm([g for _, _, grads, _ in work for g in grads if g is not None], self.max_norm)
@@ -376,12 +388,7 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         params = [p for group in self.param_groups for p in group["params"]]
         held = {params[int(k)]: part for k, part in state_dict["state"].items()}
-        self._plans = {}
-        for index, group in enumerate(self.param_groups):
-            for dtype in DTYPES:
-                own = [p for p in group["params"] if p.dtype == dtype]
-                if any([p in held for p in own]):
-                    self._build((index, dtype), own, held)
+        self._rebuild(held)
 
 
 __all__ = ["AdamW", "grad_norm", "adamw_plan", "adamw_step", "adamw_states", "DTYPES", "STATE_BITS"]

@@ -386,6 +386,37 @@ def test_parameters_that_move_keep_their_moments(bits):
         assert_bitwise(a, b, "moved")
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("changed", [slice(0, 1), slice(0, 2)])
+def test_parameters_of_another_dtype_keep_their_moments(bits, changed):
+    params, grads, _, _ = _model([100, 40])
+    for p, g in zip(params, grads):
+        p.requires_grad_(True)
+        p.grad = g
+    optimiser = optim.AdamW(params, state_bits=bits)
+    optimiser.step()
+    before = optimiser.state_dict()["state"]
+    for p in params[changed]:
+        p.grad = None
+        p.data = p.data.to(torch.bfloat16)
+    optimiser.step()  # nothing for those that changed: their moments are as they were
+    after = optimiser.state_dict()["state"]
+    assert sorted(after) == [0, 1]
+    assert not [key for key, plan in optimiser._plans.items() if not plan.params or plan.params[0].dtype != key[1]]
+    for k, p in enumerate(params):
+        kept = p.dtype == torch.bfloat16
+        assert after[k]["step"] == before[k]["step"] + (0 if kept else 1)
+        if kept:
+            for name in before[k]:
+                if name != "step":
+                    assert_bitwise(after[k][name], before[k][name], name)
+    for p, g in zip(params, grads):
+        p.grad = g.to(p.dtype)
+    optimiser.step()
+    assert [part["step"] for _, part in sorted(optimiser.state_dict()["state"].items())] == \
+        [2 if p.dtype == torch.bfloat16 else 3 for p in params]
+
+
 def test_a_checkpoint_of_torch_is_taken_over():
     params, grads, _, _ = _model([64, 33])
     twin = [p.clone().requires_grad_(True) for p in params]
