@@ -714,9 +714,9 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
 // direct, forward
 // ---------------------------------------------------------------------------
 //
-// TS threads hold 32 elements each of a sample.  A sample that is longer
-// (max_rows was too small) is streamed twice.  Blocks behind the samples write
-// the zeros of rows without a sample.
+// TS threads hold 32 elements each of a sample.  A longer sample (the workgroup
+// is chosen for the mean, or max_rows was too small) is streamed twice.  Blocks
+// behind the samples write the zeros of rows without a sample.
 template <typename T>
 constexpr int kHeld = 32 / kVec<T>;  // vectors
 

@@ -78,8 +78,8 @@ def grad_norm(grads, max_norm: float | None = None) -> tuple[torch.Tensor, torch
 
     ``grads``: contiguous float32 or bfloat16 tensors on one device; None
     entries count as 0.  Both results are float32 tensors without dimensions
-    on that device; nothing waits for the GPU.  The squares are summed in 64
-    bits in a fixed order.  ``factor`` is ``min(1, max_norm / (norm + 1e-6))``,
+    on that device, without a gradient of their own; nothing waits for the GPU.
+    The squares are summed in 64 bits in a fixed order.  ``factor`` is ``min(1, max_norm / (norm + 1e-6))``,
     1 without ``max_norm``, and NaN where the norm is not finite:
     ``adamw_step`` then takes no step.
     """
@@ -224,7 +224,10 @@ def adamw_step(plan, grads, *, lr, betas=(0.9, 0.999), eps: float = 1.0e-8, weig
 
 
 def adamw_states(plan, exp_avgs=None, exp_avg_sqs=None) -> tuple[list, list]:
-    """The moments of ``plan`` as float32 tensors of the parameters' shapes: copies, or written into the tensors given."""
+    """The moments of ``plan`` as float32 tensors of the parameters' shapes: copies, or written into the tensors given.
+
+    Tensors given must not overlap each other.
+    """
     out = []
     for values, what in ((exp_avgs, "AdamW exp_avgs"), (exp_avg_sqs, "AdamW exp_avg_sqs")):
         out.append([torch.empty_like(p, dtype=torch.float32) for p in plan.params] if values is None
