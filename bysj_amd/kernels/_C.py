@@ -955,14 +955,19 @@ def _addresses(tensors):
         return array("Q", [0 if t is None else t.data_ptr() for t in tensors])
 
 
-def grad_norm(grads, max_norm: float = 0.0):
-    """``(norm, factor)`` of checked gradients: contiguous float32 or bfloat16 tensors on one GPU, at least one."""
+def grad_norm(grads, max_norm: float = 0.0, dtypes=None):
+    """``(norm, factor)`` of checked gradients: contiguous float32 or bfloat16 tensors on one GPU, at least one.
+
+    ``dtypes``: theirs, where the caller has listed them.
+    """
     n = len(grads)
     device = grads[0].device
     _check(device.type == "cuda", "gradient norm: expected gfx950 tensors")
-    dtypes = list(map(_DTYPE_OF, grads))
+    dtypes = list(map(_DTYPE_OF, grads)) if dtypes is None else dtypes
     addresses, counts = _addresses(grads), array("q", map(torch.Tensor.numel, grads))
-    codes = array("i", map(ELEMENT_TYPES.__getitem__, dtypes))
+    kinds = set(dtypes)
+    codes = array("i", [ELEMENT_TYPES[kinds.pop()]]) * n if len(kinds) == 1 else \
+        array("i", map(ELEMENT_TYPES.__getitem__, dtypes))
     result = torch.empty((2,), dtype=torch.float32, device=device)
     at = result.data_ptr()
     nbytes = _LIB.dpa4k_grad_norm_workspace_size(counts.buffer_info()[0], n)

@@ -89,14 +89,15 @@ def grad_norm(grads, max_norm: float | None = None) -> tuple[torch.Tensor, torch
     if not grads:
         raise ValueError("grad_norm needs at least one gradient")
     limit = 0.0 if max_norm is None else _real(max_norm, "grad_norm max_norm", 0.0, above=True)
-    if not set(map(_DTYPE_OF, grads)) <= set(DTYPES):
+    dtypes = list(map(_DTYPE_OF, grads))
+    if not set(dtypes) <= set(DTYPES):
         raise TypeError("grad_norm requires float32 or bfloat16 gradients")
     if not all(map(torch.Tensor.is_contiguous, grads)):
         raise ValueError("grad_norm gradients must be contiguous")
     if not _all_on(grads, grads[0].device):
         raise ValueError("grad_norm gradients must share a device")
     require_dcu(grads[0])
-    return _extension("grad_norm").grad_norm(grads, limit)
+    return _extension("grad_norm").grad_norm(grads, limit, dtypes)
 
 
 # ---------------------------------------------------------------------------
