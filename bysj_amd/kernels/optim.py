@@ -301,9 +301,16 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW's weight decay is decoupled from the gradient")
 
     def _current(self) -> list:
-        """``[(group index, dtype), parameters]`` as they are now."""
-        return [((index, dtype), [p for p in group["params"] if p.dtype == dtype])
-                for index, group in enumerate(self.param_groups) for dtype in DTYPES]
+        """``[(group index, dtype), parameters]`` as they are now: every parameter, or a refusal."""
+        current = []
+        for index, group in enumerate(self.param_groups):
+            params = group["params"]
+            kinds = set(map(_DTYPE_OF, params))
+            if not kinds <= set(DTYPES):
+                raise TypeError("AdamW requires float32 or bfloat16 parameters")
+            current += [((index, dtype), params if kinds == {dtype} else [p for p in params if p.dtype == dtype])
+                        for dtype in DTYPES]
+        return current
 
     def _follow(self, current) -> None:
         """Rebuilds the plans if a parameter has moved, come or gone, or changed its dtype since they were built."""

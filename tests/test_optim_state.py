@@ -1,0 +1,107 @@
+"""What ``kernels.optim.AdamW`` does with its state when something is refused, on the CPU.
+
+A stand-in takes the place of the GPU entry points: plans are the real ones (they are
+host work), a step is the oracle's chain.  Each test ends with the state as it should be,
+bit for bit, after the refusal.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from bysj_amd.kernels import _lib, optim
+from oracle import optim as ref
+
+pytestmark = pytest.mark.skipif(not _lib.LIBRARY_PATH.exists(), reason="libdpa4k.so is not built")
+
+
+class _Native:
+    """The entry points of ``kernels._C`` on CPU tensors."""
+
+    def __init__(self):
+        from bysj_amd.kernels import _C
+
+        self.adamw_plan = _C.adamw_plan
+
+    @staticmethod
+    def grad_norm(grads, limit, dtypes):
+        norm = torch.sqrt(sum(g.double().square().sum() for g in grads))
+        return norm.float(), (limit / (norm + 1e-6)).clamp(max=1.0).float()
+
+    @staticmethod
+    def adamw_step(plan, grads, grad_dtype, lr, lr_tensor, beta1, beta2, eps, weight_decay, factor, seed):
+        n = len(plan.params)
+        steps = plan.words[: n * _lib.ADAMW_RECORD_BYTES].view(torch.int64).view(n, -1)[:, _lib.ADAMW_STEP_OFFSET // 8]
+        for k, (p, g, part) in enumerate(zip(plan.params, grads, plan.parts() if plan.state_bits == 8 else [None] * n)):
+            if g is None:
+                continue
+            steps[k] += 1
+            if plan.state_bits == 8:    # anything that differs from step to step
+                part[0].fill_(int(steps[k]))
+                part[1].fill_(100 + int(steps[k]))
+                continue
+            m, v = plan.exp_avgs[k], plan.exp_avg_sqs[k]
+            new = ref.adamw_chain(p.detach().view(-1), g.view(-1), m.view(-1), v.view(-1), int(steps[k]),
+                                  lr=float(lr if lr_tensor is None else lr_tensor), betas=(beta1, beta2), eps=eps,
+                                  weight_decay=weight_decay, factor=1.0 if factor is None else float(factor), seed=seed)
+            for to, value in zip((p, m, v), new):
+                to.detach().view(-1).copy_(value)
+
+
+@pytest.fixture(autouse=True)
+def native(monkeypatch):
+    stand_in = _Native()
+    monkeypatch.setattr(optim, "_extension", lambda name: stand_in)
+    monkeypatch.setattr(optim, "require_dcu", lambda *tensors: None)
+    return stand_in
+
+
+def _trained(bits=32, **more):
+    """An optimiser of two groups after two steps, and its parameters with gradients."""
+    generator = torch.Generator().manual_seed(0)
+    params = [torch.randn(2, 3, generator=generator).requires_grad_(True), torch.randn(40, generator=generator).requires_grad_(True)]
+    optimiser = optim.AdamW([{"params": params[:1]}, {"params": params[1:], "lr": 1e-2}], state_bits=bits, **more)
+    for p in params:
+        p.grad = torch.randn(p.shape, generator=generator)
+    optimiser.step()
+    optimiser.step()
+    return optimiser, params
+
+
+def _same(a, b):
+    assert type(a) is type(b) or (isinstance(a, (int, float)) and isinstance(b, (int, float)))
+    if isinstance(a, torch.Tensor):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    elif isinstance(a, dict):
+        assert a.keys() == b.keys()
+        for key in a:
+            _same(a[key], b[key])
+    elif isinstance(a, (list, tuple)):
+        assert len(a) == len(b)
+        for x, y in zip(a, b):
+            _same(x, y)
+    else:
+        assert a == b
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("which", [[0], [0, 1]])
+def test_a_step_refuses_parameters_of_a_dtype_it_does_not_have(dtype, which, bits):
+    """After ``model.half()`` or ``model.double()``: no parameter is left out silently, no moment is lost."""
+    optimiser, params = _trained(bits, max_norm=1.0)
+    before, held = optimiser.state_dict(), [(p.data, p.grad) for p in params]
+    for k in which:
+        p = params[k]
+        p.grad, p.data = None, p.data.to(dtype)
+        p.grad = held[k][1].to(dtype)
+    values = [p.detach().clone() for p in params]
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        optimiser.step()
+    _same([p.detach() for p in params], values)
+    for p, (data, grad) in zip(params, held):
+        p.grad, p.data = None, data
+        p.grad = grad
+    _same(optimiser.state_dict(), before)
+    optimiser.step()
+    assert [optimiser.state_dict()["state"][k]["step"] for k in (0, 1)] == [3, 3]
