@@ -272,9 +272,17 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group) -> None:
+        """As torch's; a group that is refused is not kept."""
         self._refuse_variants([{**self.defaults, **param_group}])
         super().add_param_group(param_group)
-        group = self.param_groups[-1]
+        try:
+            self._check_group(self.param_groups[-1])
+        except BaseException:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_group(group) -> None:
         if isinstance(group["lr"], torch.Tensor):
             _scalar_tensor(group["lr"], "AdamW lr")
         else:

@@ -105,3 +105,19 @@ def test_a_step_refuses_parameters_of_a_dtype_it_does_not_have(dtype, which, bit
     _same(optimiser.state_dict(), before)
     optimiser.step()
     assert [optimiser.state_dict()["state"][k]["step"] for k in (0, 1)] == [3, 3]
+
+
+@pytest.mark.parametrize("error,group", [
+    (TypeError, {"params": [torch.zeros(3, dtype=torch.float16)]}),
+    (ValueError, {"params": [torch.zeros(4)[::2]]}),
+    (ValueError, {"params": [torch.zeros(3)], "lr": -1.0}),
+    (TypeError, {"params": [torch.zeros(3)], "betas": 0.9}),
+])
+def test_a_refused_group_is_not_kept(error, group):
+    optimiser, params = _trained()
+    before = optimiser.state_dict()
+    with pytest.raises(error):
+        optimiser.add_param_group(group)
+    assert [g["params"] for g in optimiser.param_groups] == [params[:1], params[1:]]
+    _same(optimiser.state_dict(), before)
+    optimiser.step()
