@@ -329,12 +329,10 @@ class AdamW(torch.optim.Optimizer):
                 return self._rebuild({p: part for plan in self._plans.values() for p, part in self._held(plan).items()})
 
     def _rebuild(self, held) -> None:
-        self._plans = {}
-        for key, params in self._current():
-            if any([p in held for p in params]):
-                self._build(key, params, held)
+        """New plans that go on from ``held``; the old ones stay until every new one stands."""
+        self._plans = {key: self._build(params, held) for key, params in self._current() if any([p in held for p in params])}
 
-    def _build(self, key, params, held):
+    def _build(self, params, held):
         """A plan of ``params`` that goes on from ``held``: {parameter: its part of a checkpoint}."""
         known = {k: held[p] for k, p in enumerate(params) if p in held}
         steps = [int(known[k]["step"]) if k in known else 0 for k in range(len(params))]
@@ -342,14 +340,12 @@ class AdamW(torch.optim.Optimizer):
             moments = [[known[k][name].to(device=p.device, dtype=torch.float32).reshape(p.shape).contiguous().clone()
                         if k in known else torch.zeros_like(p, dtype=torch.float32).detach()
                         for k, p in enumerate(params)] for name in ("exp_avg", "exp_avg_sq")]
-            plan = adamw_plan(params, *moments, step=steps)
-        else:
-            plan = adamw_plan(params, step=steps, state_bits=8)
-            for k, (codes, scales) in enumerate(plan.parts()):
-                if k in known:
-                    codes.copy_(known[k]["codes"])
-                    scales.copy_(known[k]["scales"])
-        self._plans[key] = plan
+            return adamw_plan(params, *moments, step=steps)
+        plan = adamw_plan(params, step=steps, state_bits=8)
+        for k, (codes, scales) in enumerate(plan.parts()):
+            if k in known:
+                codes.copy_(known[k]["codes"])
+                scales.copy_(known[k]["scales"])
         return plan
 
     @staticmethod
@@ -376,7 +372,9 @@ class AdamW(torch.optim.Optimizer):
             if not all(map(torch.Tensor.is_contiguous, given)):
                 grads = [None if g is None else g.contiguous() for g in grads]
             if given:
-                plan = self._plans.get(key) or self._build(key, params, {})
+                plan = self._plans.get(key)
+                if plan is None:
+                    plan = self._plans[key] = self._build(params, {})
                 index, dtype = key
                 work.append((self.param_groups[index], plan, grads, index * 2 + (dtype == torch.bfloat16)))
         self.norm = factor = None

@@ -121,3 +121,17 @@ def test_a_refused_group_is_not_kept(error, group):
     assert [g["params"] for g in optimiser.param_groups] == [params[:1], params[1:]]
     _same(optimiser.state_dict(), before)
     optimiser.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_that_cannot_list_its_parameters_keeps_the_moments(bits):
+    """A parameter's memory becomes strided: the step raises; with the layout put right training goes on where it was."""
+    optimiser, params = _trained(bits)
+    before = optimiser.state_dict()
+    params[1].data = torch.randn(80)[::2]
+    with pytest.raises(ValueError, match="contiguous"):
+        optimiser.step()
+    _same(optimiser.state_dict(), before)
+    params[1].data = params[1].data.contiguous()
+    optimiser.step()
+    assert [optimiser.state_dict()["state"][k]["step"] for k in (0, 1)] == [3, 3]
