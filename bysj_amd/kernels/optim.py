@@ -282,7 +282,9 @@ class AdamW(torch.optim.Optimizer):
             raise
 
     @staticmethod
-    def _check_group(group) -> None:
+    def _check_options(group) -> None:
+        if not {"lr", "betas", "eps", "weight_decay"} <= group.keys():
+            raise ValueError("an AdamW parameter group has lr, betas, eps and weight_decay")
         if isinstance(group["lr"], torch.Tensor):
             _scalar_tensor(group["lr"], "AdamW lr")
         else:
@@ -293,6 +295,10 @@ class AdamW(torch.optim.Optimizer):
             _real(beta, "AdamW beta", 0.0, 1.0)
         _real(group["eps"], "AdamW eps", 1.0e-38)
         _real(group["weight_decay"], "AdamW weight_decay", 0.0)
+
+    @classmethod
+    def _check_group(cls, group) -> None:
+        cls._check_options(group)
         for p in group["params"]:
             if p.dtype not in DTYPES:
                 raise TypeError("AdamW requires float32 or bfloat16 parameters")
@@ -326,11 +332,12 @@ class AdamW(torch.optim.Optimizer):
             plan = self._plans.get(key)
             if plan is not None and not (len(plan.params) == len(params) and all(map(operator.is_, plan.params, params))
                                          and list(map(torch.Tensor.data_ptr, params)) == plan.addresses):
-                return self._rebuild({p: part for plan in self._plans.values() for p, part in self._held(plan).items()})
+                self._plans = self._rebuilt({p: part for plan in self._plans.values() for p, part in self._held(plan).items()})
+                return
 
-    def _rebuild(self, held) -> None:
-        """New plans that go on from ``held``; the old ones stay until every new one stands."""
-        self._plans = {key: self._build(params, held) for key, params in self._current() if any([p in held for p in params])}
+    def _rebuilt(self, held) -> dict:
+        """New plans that go on from ``held``; the old ones stay until the caller replaces them."""
+        return {key: self._build(params, held) for key, params in self._current() if any([p in held for p in params])}
 
     def _build(self, params, held):
         """A plan of ``params`` that goes on from ``held``: {parameter: its part of a checkpoint}."""
@@ -397,15 +404,46 @@ class AdamW(torch.optim.Optimizer):
         result["state_bits"] = self.state_bits
         return result
 
+    def _check_part(self, p, part) -> None:
+        """One parameter's part of a checkpoint."""
+        if self.state_bits == 32:
+            wanted = {"exp_avg": p.shape, "exp_avg_sq": p.shape}
+        else:
+            spans = -(-p.numel() // 32)
+            wanted = {"codes": (2, spans * 32), "scales": (2, spans)}
+        if not isinstance(part, dict) or not {"step", *wanted} <= part.keys():
+            raise ValueError(f"the checkpoint's moments must have step, {' and '.join(wanted)}")
+        if float(part["step"]) != int(part["step"]) or part["step"] < 0:
+            raise ValueError(f"the checkpoint has a bad step count: {part['step']!r}")
+        for name, shape in wanted.items():
+            value = part[name]
+            if not isinstance(value, torch.Tensor) or value.shape != shape:
+                raise ValueError(f"the checkpoint's {name} must be a tensor of shape {tuple(shape)}")
+            if value.dtype != torch.uint8 if self.state_bits == 8 else not value.is_floating_point():
+                raise TypeError(f"the checkpoint's {name} has the wrong type: {value.dtype}")
+
     def load_state_dict(self, state_dict) -> None:
+        """Takes a checkpoint over; one that is refused leaves the optimiser as it was."""
         bits = state_dict.get("state_bits", 32)  # torch's own AdamW does not say
         if bits != self.state_bits:
             raise ValueError(f"the checkpoint holds {bits}-bit moments, not {self.state_bits}-bit ones")
-        self._refuse_variants(state_dict["param_groups"])
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        params = [p for group in self.param_groups for p in group["params"]]
-        held = {params[int(k)]: part for k, part in state_dict["state"].items()}
-        self._rebuild(held)
+        groups = state_dict["param_groups"]
+        if [len(group["params"]) for group in groups] != [len(group["params"]) for group in self.param_groups]:
+            raise ValueError("the checkpoint's parameter groups are of other sizes")
+        for group in groups:
+            self._check_options(group)
+        self._refuse_variants(groups)
+        saved = (k for group in groups for k in group["params"])
+        params = dict(zip(saved, (p for group in self.param_groups for p in group["params"])))
+        held = {}
+        for k, part in state_dict["state"].items():
+            if int(k) not in params:
+                raise ValueError(f"the checkpoint has moments of a parameter {k!r} that is in no group")
+            self._check_part(params[int(k)], part)
+            held[params[int(k)]] = part
+        plans = self._rebuilt(held)
+        super().load_state_dict({"state": {}, "param_groups": groups})
+        self._plans = plans
 
 
 __all__ = ["AdamW", "grad_norm", "adamw_plan", "adamw_step", "adamw_states", "DTYPES", "STATE_BITS"]

@@ -135,3 +135,63 @@ def test_a_step_that_cannot_list_its_parameters_keeps_the_moments(bits):
     params[1].data = params[1].data.contiguous()
     optimiser.step()
     assert [optimiser.state_dict()["state"][k]["step"] for k in (0, 1)] == [3, 3]
+
+
+def _without(part, name):
+    return {key: value for key, value in part.items() if key != name}
+
+
+@pytest.mark.parametrize("error,bits,change", [
+    (ValueError, 32, lambda d: d["state"][1].update(exp_avg=torch.zeros(39))),
+    (ValueError, 32, lambda d: d["state"][0].update(exp_avg=torch.zeros(3, 2))),    # as many elements
+    (ValueError, 32, lambda d: d["state"][0].update(exp_avg_sq=torch.zeros(()))),
+    (ValueError, 32, lambda d: d["state"].update({1: _without(d["state"][1], "exp_avg_sq")})),
+    (ValueError, 32, lambda d: d["state"].update({1: _without(d["state"][1], "step")})),
+    (ValueError, 32, lambda d: d["state"][1].update(step=-1)),
+    (ValueError, 32, lambda d: d["state"][1].update(step=2.5)),
+    (TypeError, 32, lambda d: d["state"][1].update(exp_avg=torch.zeros(40, dtype=torch.int32))),
+    (ValueError, 32, lambda d: d["state"].update({2: d["state"][1]})),
+    (ValueError, 8, lambda d: d["state"][1].update(codes=torch.zeros(2, 32, dtype=torch.uint8))),
+    (ValueError, 8, lambda d: d["state"][1].update(codes=torch.zeros(1, dtype=torch.uint8))),    # would be broadcast
+    (ValueError, 8, lambda d: d["state"][1].update(scales=torch.zeros(2, 1, dtype=torch.uint8))),
+    (TypeError, 8, lambda d: d["state"][1].update(codes=torch.zeros(2, 64))),
+    (ValueError, 32, lambda d: d.update(state_bits=8)),
+    (ValueError, 32, lambda d: d["param_groups"][1].update(lr=-1.0)),
+    (TypeError, 32, lambda d: d["param_groups"][1].update(betas=0.9)),
+    (ValueError, 32, lambda d: d["param_groups"][1].pop("eps")),
+    (ValueError, 32, lambda d: d["param_groups"][1].update(amsgrad=True)),
+    (ValueError, 32, lambda d: d["param_groups"].pop()),
+    (ValueError, 32, lambda d: d["param_groups"][1]["params"].append(2)),
+])
+def test_a_refused_checkpoint_changes_nothing(error, bits, change):
+    optimiser, params = _trained(bits)
+    twin, others = _trained(bits)
+    before, checkpoint = optimiser.state_dict(), optimiser.state_dict()
+    checkpoint["param_groups"][0]["lr"] = 0.5
+    change(checkpoint)
+    with pytest.raises(error):
+        optimiser.load_state_dict(checkpoint)
+    _same(optimiser.state_dict(), before)
+    optimiser.step()
+    twin.step()
+    _same([p.detach() for p in params], [p.detach() for p in others])
+    _same(optimiser.state_dict(), twin.state_dict())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_checkpoint_that_cannot_be_listed_changes_nothing(bits, native, monkeypatch):
+    """No memory for the new plans."""
+    optimiser, _ = _trained(bits)
+    before, checkpoint = optimiser.state_dict(), optimiser.state_dict()
+    checkpoint["param_groups"][0]["lr"] = 0.5
+
+    def refuse(*args):
+        raise RuntimeError("out of memory")
+
+    with monkeypatch.context() as patched:
+        patched.setattr(native, "adamw_plan", refuse)
+        with pytest.raises(RuntimeError, match="memory"):
+            optimiser.load_state_dict(checkpoint)
+    _same(optimiser.state_dict(), before)
+    optimiser.load_state_dict(checkpoint)
+    _same(optimiser.state_dict(), checkpoint)
