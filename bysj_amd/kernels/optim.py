@@ -257,7 +257,9 @@ class AdamW(torch.optim.Optimizer):
     The plans are built in the first step; later steps may be captured in a
     HIP graph (with ``lr`` a tensor where a schedule changes it between
     replays).  Checkpoints hold each parameter's step count and moments; 8-bit
-    moments are kept as their codes.
+    moments are kept as their codes.  They come from ``state_dict``, and its
+    hooks see them: ``state`` itself stays empty, for the moments live in the
+    plans.
     """
 
     def __init__(self, params, lr=1.0e-3, betas=(0.9, 0.999), eps: float = 1.0e-8, weight_decay: float = 1.0e-2, *,
@@ -396,13 +398,19 @@ class AdamW(torch.optim.Optimizer):
         raise TypeError("the moments live in plans on the device: save state_dict() instead")
 
     def state_dict(self) -> dict:
-        result = super().state_dict()
-        numbers_of = {p: k for k, p in enumerate(p for group in self.param_groups for p in group["params"])}
-        result["state"] = {numbers_of[p]: {name: value.clone() if isinstance(value, torch.Tensor) else value
-                                           for name, value in part.items()}
-                           for plan in self._plans.values() for p, part in self._held(plan).items()}
-        result["state_bits"] = self.state_bits
-        return result
+        """Groups, and each parameter's step count and moments; hooks see all of it."""
+        def fill(_, result):
+            numbers_of = {p: k for k, p in enumerate(p for group in self.param_groups for p in group["params"])}
+            result["state"] = {numbers_of[p]: {name: value.clone() if isinstance(value, torch.Tensor) else value
+                                               for name, value in part.items()}
+                               for plan in self._plans.values() for p, part in self._held(plan).items()}
+            result["state_bits"] = self.state_bits
+
+        hook = self.register_state_dict_post_hook(fill, prepend=True)
+        try:
+            return super().state_dict()
+        finally:
+            hook.remove()
 
     def _check_part(self, p, part) -> None:
         """One parameter's part of a checkpoint."""
@@ -422,8 +430,8 @@ class AdamW(torch.optim.Optimizer):
             if value.dtype != torch.uint8 if self.state_bits == 8 else not value.is_floating_point():
                 raise TypeError(f"the checkpoint's {name} has the wrong type: {value.dtype}")
 
-    def load_state_dict(self, state_dict) -> None:
-        """Takes a checkpoint over; one that is refused leaves the optimiser as it was."""
+    def _plans_of(self, state_dict) -> dict:
+        """The plans of a checkpoint, all of which is checked."""
         bits = state_dict.get("state_bits", 32)  # torch's own AdamW does not say
         if bits != self.state_bits:
             raise ValueError(f"the checkpoint holds {bits}-bit moments, not {self.state_bits}-bit ones")
@@ -441,9 +449,25 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"the checkpoint has moments of a parameter {k!r} that is in no group")
             self._check_part(params[int(k)], part)
             held[params[int(k)]] = part
-        plans = self._rebuilt(held)
-        super().load_state_dict({"state": {}, "param_groups": groups})
-        self._plans = plans
+        return self._rebuilt(held)
+
+    def load_state_dict(self, state_dict) -> None:
+        """Takes a checkpoint over; one that is refused leaves the optimiser as it was."""
+        plans = {}
+
+        def build(_, given):  # behind the hooks that may change the checkpoint, before anything is replaced
+            plans.update(self._plans_of(given))
+            return {**given, "state": {}}
+
+        def replace(_):  # before the hooks that look at the result
+            self._plans = plans
+
+        hooks = [self.register_load_state_dict_pre_hook(build), self.register_load_state_dict_post_hook(replace, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
 
 __all__ = ["AdamW", "grad_norm", "adamw_plan", "adamw_step", "adamw_states", "DTYPES", "STATE_BITS"]

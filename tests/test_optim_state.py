@@ -195,3 +195,38 @@ def test_a_checkpoint_that_cannot_be_listed_changes_nothing(bits, native, monkey
     _same(optimiser.state_dict(), before)
     optimiser.load_state_dict(checkpoint)
     _same(optimiser.state_dict(), checkpoint)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_hooks_see_the_whole_checkpoint(bits):
+    optimiser, _ = _trained(bits)
+    saved, given, loaded = [], [], []
+    optimiser.register_state_dict_post_hook(lambda o, d: saved.append({**d}))
+    checkpoint = optimiser.state_dict()
+    assert saved[0].keys() == checkpoint.keys()
+    _same(saved[0], checkpoint)
+    assert sorted(checkpoint["state"]) == [0, 1]
+
+    def longer(o, d):
+        given.append(d["state"].keys())
+        return {**d, "state": {k: {**part, "step": part["step"] + 5} for k, part in d["state"].items()}}
+
+    optimiser.register_load_state_dict_pre_hook(longer)
+    optimiser.register_load_state_dict_post_hook(lambda o: loaded.append(o.state_dict()))
+    for turn in (1, 2):
+        optimiser.load_state_dict(checkpoint)
+        assert given == [{0, 1}] * turn
+        assert [loaded[-1]["state"][k]["step"] for k in (0, 1)] == [7, 7]
+    for name, value in checkpoint["state"][1].items():
+        if name != "step":
+            assert torch.equal(loaded[-1]["state"][1][name], value)
+
+
+def test_hooks_of_a_refused_checkpoint_do_not_pile_up():
+    optimiser, _ = _trained()
+    checkpoint = optimiser.state_dict()
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            optimiser.load_state_dict({**checkpoint, "state_bits": 8})
+    optimiser.load_state_dict(checkpoint)
+    _same(optimiser.state_dict(), checkpoint)
