@@ -330,10 +330,11 @@ class AdamW(torch.optim.Optimizer):
 
     def _follow(self, current) -> None:
         """Rebuilds the plans if a parameter has moved, come or gone, or changed its dtype since they were built."""
-        for key, params in current:
-            plan = self._plans.get(key)
-            if plan is not None and not (len(plan.params) == len(params) and all(map(operator.is_, plan.params, params))
-                                         and list(map(torch.Tensor.data_ptr, params)) == plan.addresses):
+        now = dict(current)
+        for key, plan in self._plans.items():
+            params = now.get(key, ())
+            if not (len(plan.params) == len(params) and all(map(operator.is_, plan.params, params))
+                    and list(map(torch.Tensor.data_ptr, params)) == plan.addresses):
                 self._plans = self._rebuilt({p: part for plan in self._plans.values() for p, part in self._held(plan).items()})
                 return
 
@@ -403,7 +404,7 @@ class AdamW(torch.optim.Optimizer):
             numbers_of = {p: k for k, p in enumerate(p for group in self.param_groups for p in group["params"])}
             result["state"] = {numbers_of[p]: {name: value.clone() if isinstance(value, torch.Tensor) else value
                                                for name, value in part.items()}
-                               for plan in self._plans.values() for p, part in self._held(plan).items()}
+                               for plan in self._plans.values() for p, part in self._held(plan).items() if p in numbers_of}
             result["state_bits"] = self.state_bits
 
         hook = self.register_state_dict_post_hook(fill, prepend=True)

@@ -230,3 +230,20 @@ def test_hooks_of_a_refused_checkpoint_do_not_pile_up():
             optimiser.load_state_dict({**checkpoint, "state_bits": 8})
     optimiser.load_state_dict(checkpoint)
     _same(optimiser.state_dict(), checkpoint)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_taken_out_of_a_group_leave_the_checkpoint(bits):
+    """Before the next step too, and with the whole last group."""
+    optimiser, params = _trained(bits)
+    before = optimiser.state_dict()["state"]
+    group = optimiser.param_groups.pop()
+    assert sorted(optimiser.state_dict()["state"]) == [0]
+    _same(optimiser.state_dict()["state"][0], before[0])
+    optimiser.step()
+    assert sorted(optimiser.state_dict()["state"]) == [0] and len(optimiser._plans) == 1
+    optimiser.add_param_group(group)    # begins from zero: its moments went with it
+    optimiser.step()
+    assert [optimiser.state_dict()["state"][k]["step"] for k in (0, 1)] == [4, 1]
+    del optimiser.param_groups[1]["params"][0]
+    assert sorted(optimiser.state_dict()["state"]) == [0]
