@@ -335,7 +335,11 @@ class AdamW(torch.optim.Optimizer):
             params = now.get(key, ())
             if not (len(plan.params) == len(params) and all(map(operator.is_, plan.params, params))
                     and list(map(torch.Tensor.data_ptr, params)) == plan.addresses):
-                self._plans = self._rebuilt({p: part for plan in self._plans.values() for p, part in self._held(plan).items()})
+                plans = self._plans.values()
+                shapes = {p: shape for plan in plans for p, shape in zip(plan.params, plan.shapes)}
+                if any([p.shape != shapes.get(p, p.shape) for _, params in current for p in params]):
+                    raise ValueError("a parameter has another shape than its moments")
+                self._plans = self._rebuilt({p: part for plan in plans for p, part in self._held(plan).items()})
                 return
 
     def _rebuilt(self, held) -> dict:
@@ -347,7 +351,7 @@ class AdamW(torch.optim.Optimizer):
         known = {k: held[p] for k, p in enumerate(params) if p in held}
         steps = [int(known[k]["step"]) if k in known else 0 for k in range(len(params))]
         if self.state_bits == 32:
-            moments = [[known[k][name].to(device=p.device, dtype=torch.float32).reshape(p.shape).contiguous().clone()
+            moments = [[known[k][name].to(device=p.device, dtype=torch.float32).contiguous().clone()
                         if k in known else torch.zeros_like(p, dtype=torch.float32).detach()
                         for k, p in enumerate(params)] for name in ("exp_avg", "exp_avg_sq")]
             return adamw_plan(params, *moments, step=steps)

@@ -247,3 +247,20 @@ def test_parameters_taken_out_of_a_group_leave_the_checkpoint(bits):
     assert [optimiser.state_dict()["state"][k]["step"] for k in (0, 1)] == [4, 1]
     del optimiser.param_groups[1]["params"][0]
     assert sorted(optimiser.state_dict()["state"]) == [0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_of_another_shape_is_refused(bits):
+    """As many elements in another order: moments taken over by their place would belong to other elements."""
+    optimiser, params = _trained(bits)
+    before, p = optimiser.state_dict(), params[0]
+    data, grad = p.data, p.grad
+    p.grad, p.data = None, p.data.t().contiguous()
+    p.grad = grad.t().contiguous()
+    with pytest.raises(ValueError, match="shape"):
+        optimiser.step()
+    _same(optimiser.state_dict(), before)
+    p.grad, p.data = None, data.clone()
+    p.grad = grad
+    optimiser.step()
+    assert optimiser.state_dict()["state"][0]["step"] == 3
