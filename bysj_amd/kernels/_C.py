@@ -995,6 +995,9 @@ class AdamWPlan:
         self.device = params[0].device
         self.shapes = [p.shape for p in params]
         self.addresses = list(_addresses(params))
+        # the plan's own hold on the parameters' memory: while the table lists an address, nothing else can get it,
+        # so a parameter found there still has this memory
+        self.memory = [p.detach() for p in params]
         self.exp_avgs = self.exp_avg_sqs = None             # 32 bits: float32 tensors
         self.codes = self.scales = None                     # 8 bits: (2, padded) and (2, padded / 32) bytes
         self.words = None

@@ -264,3 +264,17 @@ def test_a_parameter_of_another_shape_is_refused(bits):
     p.grad = grad
     optimiser.step()
     assert optimiser.state_dict()["state"][0]["step"] == 3
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_memory_that_a_plan_lists_is_not_given_to_others(bits):
+    """A parameter lets go of its memory: nothing else may get that address while a plan would write to it."""
+    p = torch.zeros(1000)
+    plan, address = optim.adamw_plan([p], state_bits=bits), p.data_ptr()
+    p.data = torch.empty(0)
+    others = [torch.zeros(size) for size in [1000] * 40 + [900, 500, 100]]
+    assert address not in [t.data_ptr() for t in others]
+    p.data = others[0]
+    with pytest.raises(RuntimeError, match="moved"):
+        optim.adamw_step(plan, [torch.ones(1000)], lr=1.0)
+    assert not any(t.any() for t in others)
