@@ -302,6 +302,8 @@ class AdamW(torch.optim.Optimizer):
     def _check_group(cls, group) -> None:
         cls._check_options(group)
         for p in group["params"]:
+            if isinstance(group["lr"], torch.Tensor) and group["lr"].device != p.device and p.device.type != "cpu":
+                raise ValueError("AdamW lr must be on the parameters' device")
             if p.dtype not in DTYPES:
                 raise TypeError("AdamW requires float32 or bfloat16 parameters")
             if not p.is_contiguous():
@@ -462,7 +464,10 @@ class AdamW(torch.optim.Optimizer):
 
         def build(_, given):  # behind the hooks that may change the checkpoint, before anything is replaced
             plans.update(self._plans_of(given))
-            return {**given, "state": {}}
+            groups = [{**saved, "lr": saved["lr"].to(group["params"][0].device)}
+                      if isinstance(saved["lr"], torch.Tensor) and group["params"] else saved
+                      for saved, group in zip(given["param_groups"], self.param_groups)]
+            return {**given, "state": {}, "param_groups": groups}
 
         def replace(_):  # before the hooks that look at the result
             self._plans = plans

@@ -278,3 +278,17 @@ def test_memory_that_a_plan_lists_is_not_given_to_others(bits):
     with pytest.raises(RuntimeError, match="moved"):
         optim.adamw_step(plan, [torch.ones(1000)], lr=1.0)
     assert not any(t.any() for t in others)
+
+
+def test_a_learning_rate_tensor_is_on_the_parameters_device():
+    """Refused by the constructor, not by the first step; a checkpoint that was loaded to the CPU follows the parameters."""
+    there = torch.zeros(3, device="meta")
+    with pytest.raises(ValueError, match="device"):
+        optim.AdamW([there], lr=torch.tensor(0.1))
+    optimiser = optim.AdamW([there], lr=torch.tensor(0.1, device="meta"))
+    checkpoint = optimiser.state_dict()
+    checkpoint["param_groups"][0]["lr"] = torch.tensor(0.2)
+    optimiser.load_state_dict(checkpoint)
+    assert optimiser.param_groups[0]["lr"].device == there.device
+    assert checkpoint["param_groups"][0]["lr"].device.type == "cpu"
+    optim.AdamW([torch.zeros(3)], lr=torch.tensor(0.1, device="meta"))    # parameters that are still to be moved
