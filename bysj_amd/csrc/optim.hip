@@ -606,6 +606,20 @@ int64_t norm_blocks(const int64_t* counts, int64_t first, int64_t last, uint32_t
   return chunks < kNormBlocks ? chunks : kNormBlocks;
 }
 
+// Partials of all launches, or -1 where a size is out of range.
+int64_t norm_partials(const int64_t* counts, int64_t n_tensors) {
+  int64_t partials = 0;
+  for (int64_t first = 0; first < n_tensors; first += kNormTensors) {
+    const int64_t last = first + kNormTensors < n_tensors ? first + kNormTensors : n_tensors;
+    const int64_t blocks = norm_blocks(counts, first, last, nullptr);
+    if (blocks < 0) return -1;
+    partials += blocks;
+  }
+  return partials;
+}
+
+size_t partial_bytes(int64_t partials) { return round_up_256(static_cast<size_t>(partials) * sizeof(double)); }
+
 int64_t tensor_chunks(int64_t count) { return (count + kChunk - 1) / kChunk; }
 
 size_t chunk_offset(int64_t n_tensors) { return round_up_256(static_cast<size_t>(n_tensors) * sizeof(Record)); }
@@ -666,14 +680,8 @@ using namespace dpa4k;
 
 extern "C" size_t dpa4k_grad_norm_workspace_size(const int64_t* counts, int64_t n_tensors) {
   if (counts == nullptr || n_tensors <= 0) return 0;
-  int64_t blocks = 0;
-  for (int64_t first = 0; first < n_tensors; first += kNormTensors) {
-    const int64_t last = first + kNormTensors < n_tensors ? first + kNormTensors : n_tensors;
-    const int64_t b = norm_blocks(counts, first, last, nullptr);
-    if (b < 0) return 0;
-    blocks += b;
-  }
-  return round_up_256(static_cast<size_t>(blocks) * sizeof(double));
+  const int64_t partials = norm_partials(counts, n_tensors);
+  return partials < 0 ? 0 : partial_bytes(partials);
 }
 
 extern "C" int dpa4k_grad_norm(const void* const* grads, const int64_t* counts, const int32_t* types,
@@ -691,7 +699,9 @@ extern "C" int dpa4k_grad_norm(const void* const* grads, const int64_t* counts, 
     if (counts[i] < 0 || counts[i] > (int64_t(1) << 44) || (counts[i] > 0 && grads[i] == nullptr))
       return fail(DPA4K_EINVAL, "gradient norm: gradient %lld has a bad size or pointer", static_cast<long long>(i));
   }
-  const size_t needed = dpa4k_grad_norm_workspace_size(counts, n_tensors);
+  const int64_t all = norm_partials(counts, n_tensors);
+  if (all < 0) return fail(DPA4K_EINVAL, "gradient norm: too many elements");
+  const size_t needed = partial_bytes(all);
   if (workspace_bytes < needed || (needed > 0 && workspace == nullptr))
     return fail(DPA4K_EWORKSPACE, "gradient norm: workspace of %zu bytes is smaller than %zu", workspace_bytes, needed);
   hipStream_t stream = as_stream(stream_handle);
@@ -702,7 +712,6 @@ extern "C" int dpa4k_grad_norm(const void* const* grads, const int64_t* counts, 
     NormList list;
     std::memset(&list, 0, sizeof(list));
     const int64_t blocks = norm_blocks(counts, first, last, list.first);
-    if (blocks < 0) return fail(DPA4K_EINVAL, "gradient norm: too many elements");
     for (int64_t i = first; i < last; ++i) {
       list.p[i - first] = grads[i];
       list.count[i - first] = counts[i] * 2 + (types[i] == DPA4K_TYPE_BF16 ? 1 : 0);
