@@ -222,8 +222,10 @@ __device__ __forceinline__ void decode(const Codes<E>& codes, uint32_t top, floa
 __device__ __forceinline__ float poison_of(uint32_t top) { return top == 255u ? NAN : 0.0f; }
 
 // The shared exponent of a block, and this lane's codes.  A block with an
-// infinity or NaN takes X = 255 and stands for NaN.  `random`: 16 bits a value
-// (its lower or upper half), compared with the 20 bits cut off.
+// infinity, a NaN of either sign, a value above 1.875 2^127 (which three mantissa
+// bits round up to infinity) or a second moment below 0 takes X = 255 and stands
+// for NaN.  A second moment of -0 has to be given as 0.  `random`: 16 bits a
+// value (its lower or upper half), compared with the 20 bits cut off.
 template <bool kSigned, int E>
 __device__ __forceinline__ Codes<E> encode(const float (&value)[E], const uint32_t (&random)[E], uint32_t& top) {
   const auto half_of = [&](int i) { return kSigned ? random[i] & 0xFFFFu : random[i] >> 16; };
@@ -233,7 +235,8 @@ __device__ __forceinline__ Codes<E> encode(const float (&value)[E], const uint32
     word[i] = kSigned ? __float_as_uint(value[i]) & 0x7FFFFFFFu : __float_as_uint(value[i]);
     most = word[i] > most ? word[i] : most;
   }
-  most = (block_max<E>(most) + 0xFFFFFu) >> 23;
+  most = block_max<E>(most);
+  most = ((most < 0x7F800000u ? most : 0x7F800000u) + 0xFFFFFu) >> 23;
   most = most > kBinades<kSigned> ? most : kBinades<kSigned>;
   top = most < 255u ? most : 255u;
   const uint32_t low = (top - kBinades<kSigned> + 1u) << 3;
@@ -460,7 +463,9 @@ __device__ __forceinline__ void adamw_codes_chunk(const Record& r, int64_t begin
     } else {
       // every lane takes part in the exponent of its block
       const Floats<E> m = load<kWhole, E>(r.values[0], at, count);
-      const Floats<E> v = load<kWhole, E>(r.values[1], at, count);
+      Floats<E> v = load<kWhole, E>(r.values[1], at, count);
+#pragma unroll
+      for (int i = 0; i < E; ++i) v.v[i] += 0.0f;  // -0 becomes 0
       uint32_t half[E], top_m, top_v;
 #pragma unroll
       for (int i = 0; i < E; ++i) half[i] = 0x80008000u;
