@@ -10,6 +10,7 @@ import importlib
 import sys
 
 import torch
+from torch.autograd import forward_ad
 
 SUPPORTED_ARCHITECTURES = frozenset({"gfx950"})
 _NATIVE_MODULE = __name__.rsplit(".", 1)[0] + "._C"
@@ -125,7 +126,13 @@ def apply_function(function, *args):
     no tensor argument requires a gradient, ``apply`` would record nothing:
     calling the forward directly gives the same tensors without the autograd
     bookkeeping, which is most of the Python layer's cost per eager call.
+    A forward-mode tangent goes to ``apply`` too, which refuses it: the
+    forward alone would lose it.
     """
     if torch.is_grad_enabled() and any(isinstance(a, torch.Tensor) and a.requires_grad for a in args):
+        return function.apply(*args)
+    # tangents exist within a dual level alone (without the level's number, look at every tensor)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            isinstance(a, torch.Tensor) and forward_ad.unpack_dual(a).tangent is not None for a in args):
         return function.apply(*args)
     return function.forward(_Untracked(len(args)), *args)
