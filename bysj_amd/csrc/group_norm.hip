@@ -32,6 +32,7 @@
 // have no ragged vector), N = 2 where D >= V (a vector crosses one border of
 // groups at most, after its first `split` channels), else N = V.
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 
@@ -43,13 +44,15 @@ constexpr int kMaxChannels = DPA4K_GROUP_NORM_MAX_CHANNELS;
 constexpr int64_t kTileBytes = 16384;   // least bytes of a tile
 constexpr int64_t kTiles = 1024;        // most tiles where they are larger than that: 4 workgroups per CU
 constexpr int kLdsGroups = 1024;        // groups of a direct workgroup, whose statistics are kept in LDS
+constexpr int64_t kStreamed = 16;       // times what it holds: the longest sample that a direct workgroup is meant for
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Shape {
   int64_t samples, entries, inner;   // a sample owns entries, an entry `inner` rows
   int channels, groups;
   int64_t tile_rows, tiles;
-  int64_t long_rows;                 // samples of more rows than this take tiles
+  int64_t long_rows;                 // samples of more rows than this take tiles (or a launch of their own)
+  int64_t streamed_rows;             // the most rows that a direct workgroup is meant for
   const int64_t* offsets;            // null: sample s is entry s
 };
 
@@ -116,6 +119,16 @@ __device__ __forceinline__ void store_part(T* __restrict__ p, const Values<T>& v
 
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
+}
+
+// `condition`, which is the same everywhere, as a value of each lane.  The compiler
+// (of ROCm 7.2) keeps a branch's uniform condition as a mask of the lanes that are
+// active in a loop, and may use that mask again behind the loop, where lanes that
+// had left it are active: there the branch went the other way.
+__device__ __forceinline__ bool per_lane(bool condition) {
+  int value = condition ? 1 : 0;
+  asm volatile("" : "+v"(value));
+  return value != 0;
 }
 
 __device__ __forceinline__ float activated(float z, bool silu) { return silu ? z * sigmoid(z) : z; }
@@ -458,10 +471,8 @@ struct Running {
         }
       }
   }
-  __device__ __forceinline__ void add_run(const T* __restrict__ run, int64_t elements, const Share& share, int stride, int split) {
-    if (!share.live) return;
-    const int64_t whole = elements / V;
-    int64_t q = share.first;
+  // The vectors q, q + stride, ... below `whole`.
+  __device__ __forceinline__ void add_vectors(const T* __restrict__ run, int64_t q, int64_t whole, int stride, int split) {
     for (; q < whole; q += static_cast<int64_t>(kBatch<T>) * stride) {
       Raw<T> batch[kBatch<T>];
 #pragma unroll
@@ -470,6 +481,11 @@ struct Running {
       if (n == kBatch<T>) add<kBatch<T>, true>(batch, n, split);
       else add<kBatch<T>, false>(batch, n, split);
     }
+  }
+  __device__ __forceinline__ void add_run(const T* __restrict__ run, int64_t elements, const Share& share, int stride, int split) {
+    if (!share.live) return;
+    const int64_t whole = elements / V;
+    add_vectors(run, share.first, whole, stride, split);
     if constexpr (N != 1) {
       const int part = static_cast<int>(elements - whole * V);
       if (part > 0 && owns(share, whole, stride)) add_part(load_part(run + whole * V, part), part, split);
@@ -489,6 +505,47 @@ template <int BLOCK, int N>
 struct MomentsLds {
   float count[BLOCK * N], mean[BLOCK * N], squares[BLOCK * N];
 };
+
+// A run far longer than its workgroup is meant for, in pieces: the parts of each
+// are merged in 64 bits, in LDS that only their thread uses.  In 32 bits alone a
+// long run of values of one size lost digits (all roundings go the same way).
+// The caller's threads meet before they use the LDS for something else.
+template <int BLOCK, int N>
+struct MomentsFold {
+  double mean[BLOCK * N], squares[BLOCK * N];
+};
+template <typename T, int N, int BLOCK>
+__device__ __forceinline__ void add_pieces(Running<T, N>& running, MomentsFold<BLOCK, N>& fold, const T* __restrict__ run,
+                                           const Share& share, int64_t whole, int64_t piece, int stride, int split) {
+  double vectors = 0.0;  // merged so far
+  for (int64_t begin = 0;; begin += piece) {
+    const int64_t end = begin + piece < whole ? begin + piece : whole, q = share.first + begin;
+    running.add_vectors(run, q, end, stride, split);
+    const double more = q < end ? static_cast<double>((end - q + stride - 1) / stride) : 0.0;
+    const double weight = more > 0.0 ? more / (vectors + more) : 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      double& mean = fold.mean[threadIdx.x * N + i];
+      double& squares = fold.squares[threadIdx.x * N + i];
+      if (begin == 0) mean = running.mean[i], squares = running.squares[i];
+      else if (running.count[i] > 0.0f) {
+        const double delta = running.mean[i] - mean;
+        squares += running.squares[i] + delta * delta * (running.count[i] * (1.0 - weight));
+        mean += delta * weight;
+      }
+    }
+    vectors += more;
+    if (end == whole) break;
+    running = Running<T, N>();
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    constexpr int V = kVec<T>;
+    running.count[i] = static_cast<float>(vectors * (N == 1 ? V : (N == 2 ? (i == 0 ? split : V - split) : 1)));
+    running.mean[i] = static_cast<float>(fold.mean[threadIdx.x * N + i]);
+    running.squares[i] = static_cast<float>(fold.squares[threadIdx.x * N + i]);
+  }
+}
 
 // Calls emit(group, terms, mean, squares) in one lane for every group.
 template <int BLOCK, typename T, int N, typename Emit>
@@ -715,14 +772,24 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
 // ---------------------------------------------------------------------------
 //
 // TS threads hold 32 elements each of a sample.  A longer sample (the workgroup
-// is chosen for the mean, or max_rows was too small) is streamed twice.  Blocks
-// behind the samples write the zeros of rows without a sample.
+// is chosen for the mean) is streamed twice, and one that is longer than that
+// allows for (max_rows was too small) piece by piece.  Blocks behind the samples
+// write the zeros of rows without a sample.
 template <typename T>
 constexpr int kHeld = 32 / kVec<T>;  // vectors
 
-// Statistics of one sample for the threads of a workgroup, by group.
+// Vectors of a piece: no more than the longest sample that should come.
+template <typename T>
+__device__ __forceinline__ int64_t piece_of(int stride) {
+  return kStreamed * kHeld<T> * static_cast<int64_t>(stride);
+}
+
+// Statistics of one sample for the threads of a workgroup, by group.  A period of
+// at most TS vectors has at most TS groups of V channels or more.
+template <int TS, int V, int N>
 struct Statistics {
-  float mean[kLdsGroups], rstd[kLdsGroups];
+  static constexpr int kGroups = N != V ? TS : (TS * V < kLdsGroups ? TS * V : kLdsGroups);
+  float mean[kGroups], rstd[kGroups];
 };
 
 template <typename T, int N, int TS>
@@ -730,8 +797,11 @@ __global__ __launch_bounds__(TS) void group_norm_direct_kernel(
     const T* __restrict__ x, const float* __restrict__ scale, const float* __restrict__ bias, float eps, bool silu,
     float* __restrict__ mean, float* __restrict__ rstd, T* __restrict__ y, Shape s, Columns columns, int64_t zero_blocks) {
   constexpr int V = kVec<T>;
-  __shared__ MomentsLds<TS, N> lds;
-  __shared__ Statistics statistics;
+  __shared__ union {
+    MomentsLds<TS, N> lds;
+    MomentsFold<TS, N> fold;
+  } shared;
+  __shared__ Statistics<TS, V, N> statistics;
   const int C = s.channels, G = s.groups;
   const int64_t sample = block_index();
   if (sample >= s.samples) {
@@ -751,54 +821,64 @@ __global__ __launch_bounds__(TS) void group_norm_direct_kernel(
   T* out = y + first * C;
   const Share share = share_of<T, TS>(columns, 0, C);
   const int stride = columns.stride_vectors();
-  const bool held = whole <= static_cast<int64_t>(stride) * kHeld<T>;
-  const bool tail = N != 1 && left > 0 && owns(share, whole, stride);
-  Running<T, N> running;
-  Raw<T> raw[kHeld<T>];
-  int mine = 0;  // held vectors of this thread
-  if (held) {
+  const auto normalise = [&](auto is_long) {
+    constexpr bool kLong = decltype(is_long)::value;
+    const bool active = kLong ? per_lane(silu) : silu;
+    const bool held = !kLong && whole <= static_cast<int64_t>(stride) * kHeld<T>;
+    const bool tail = N != 1 && left > 0 && owns(share, whole, stride);
+    Running<T, N> running;
+    Raw<T> raw[kHeld<T>];
+    int mine = 0;  // held vectors of this thread
+    if (held) {
 #pragma unroll
-    for (int k = 0; k < kHeld<T>; ++k)
-      if (static_cast<int64_t>(k) * stride < whole) {  // uniform: no thread has a vector k otherwise
-        const int64_t q = share.first + static_cast<int64_t>(k) * stride;
-        raw[k] = load_raw(run + (q < whole ? q : whole - 1) * V);
-        mine += share.live && q < whole ? 1 : 0;
-      }
-  }
-  const Channels<T, N> channels(share, scale, bias, C, C / G);
-  if (held) {
-    if (mine > 0) running.template add<kHeld<T>, false>(raw, mine, channels.split);
+      for (int k = 0; k < kHeld<T>; ++k)
+        if (static_cast<int64_t>(k) * stride < whole) {  // uniform: no thread has a vector k otherwise
+          const int64_t q = share.first + static_cast<int64_t>(k) * stride;
+          raw[k] = load_raw(run + (q < whole ? q : whole - 1) * V);
+          mine += share.live && q < whole ? 1 : 0;
+        }
+    }
+    if constexpr (kLong) {
+      if (share.live) add_pieces(running, shared.fold, run, share, whole, piece_of<T>(stride), stride, split_of<T, N>(share, C / G));
+      __syncthreads();
+    }
+    const Channels<T, N> channels(share, scale, bias, C, C / G);
+    if (held) {
+      if (mine > 0) running.template add<kHeld<T>, false>(raw, mine, channels.split);
+    } else if (!kLong && share.live) {
+      running.add_vectors(run, share.first, whole, stride, channels.split);
+    }
     if (tail) running.add_part(load_part(run + whole * V, left), left, channels.split);
-  } else {
-    running.add_run(run, elements, share, stride, channels.split);
-  }
-  const Units u = units_of<TS, V, N>(columns, 0, C, G);
-  merge_moments<TS>(running, share.live, lds, u, G, [&](int g, float count, float centre, float squares) {
-    statistics.mean[g] = centre;
-    statistics.rstd[g] = 1.0f / sqrtf(squares / count + eps);
-    mean[sample * G + g] = statistics.mean[g];
-    rstd[sample * G + g] = statistics.rstd[g];
-  });
-  __syncthreads();
-  if (!share.live) return;
-  const PerGroup<T, N> centre = per_group<T, N>(statistics.mean, channels);
-  const PerGroup<T, N> inverse = per_group<T, N>(statistics.rstd, channels);
-  float slope[V];
+    const Units u = units_of<TS, V, N>(columns, 0, C, G);
+    merge_moments<TS>(running, share.live, shared.lds, u, G, [&](int g, float count, float centre, float squares) {
+      statistics.mean[g] = centre;
+      statistics.rstd[g] = 1.0f / sqrtf(squares / count + eps);
+      mean[sample * G + g] = statistics.mean[g];
+      rstd[sample * G + g] = statistics.rstd[g];
+    });
+    __syncthreads();
+    if (!share.live) return;
+    const PerGroup<T, N> centre = per_group<T, N>(statistics.mean, channels);
+    const PerGroup<T, N> inverse = per_group<T, N>(statistics.rstd, channels);
+    float slope[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) slope[j] = inverse.at(j) * channels.weight[j];
-  const auto normed = [&](Values<T> value) {
+    for (int j = 0; j < V; ++j) slope[j] = inverse.at(j) * channels.weight[j];
+    const auto normed = [&](Values<T> value) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) value.v[j] = activated(fmaf(value.v[j] - centre.at(j), slope[j], channels.shift[j]), silu);
-    return value;
+      for (int j = 0; j < V; ++j) value.v[j] = activated(fmaf(value.v[j] - centre.at(j), slope[j], channels.shift[j]), active);
+      return value;
+    };
+    if (held) {
+#pragma unroll
+      for (int k = 0; k < kHeld<T>; ++k)
+        if (k < mine) store_whole(out + (share.first + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
+    } else {
+      map_run<T, 4>(run, out, share.first, whole, stride, normed);
+    }
+    if (tail) store_part(out + whole * V, normed(load_part(run + whole * V, left)), left);
   };
-  if (held) {
-#pragma unroll
-    for (int k = 0; k < kHeld<T>; ++k)
-      if (k < mine) store_whole(out + (share.first + static_cast<int64_t>(k) * stride) * V, normed(to_values<T>(raw[k])));
-  } else {
-    map_run<T, 4>(run, out, share.first, whole, stride, normed);
-  }
-  if (tail) store_part(out + whole * V, normed(load_part(run + whole * V, left)), left);
+  if (last - first > s.streamed_rows) normalise(std::true_type());
+  else normalise(std::false_type());
 }
 
 // ---------------------------------------------------------------------------
@@ -851,6 +931,30 @@ struct Sums {
 template <int BLOCK, int V>
 struct SumsLds {
   float a[BLOCK * V], b[BLOCK * V];
+};
+
+// A thread's sums over the pieces of a long run: see MomentsFold.  Beside SumsLds,
+// not in its place: in a union with it the 512-thread kernels reloaded spilled
+// registers four times as often (bfloat16).
+template <int BLOCK, int V>
+struct SumsFold {
+  double z[BLOCK * V], zh[BLOCK * V];
+  template <typename T>
+  __device__ __forceinline__ void add(const Sums<T>& sums, bool first) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      z[threadIdx.x * V + j] = sums.z[j] + (first ? 0.0 : z[threadIdx.x * V + j]);
+      zh[threadIdx.x * V + j] = sums.zh[j] + (first ? 0.0 : zh[threadIdx.x * V + j]);
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void get(Sums<T>& sums) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      sums.z[j] = static_cast<float>(z[threadIdx.x * V + j]);
+      sums.zh[j] = static_cast<float>(zh[threadIdx.x * V + j]);
+    }
+  }
 };
 
 // Calls emit(group, sum u, sum u h) in one lane for every group.
@@ -1143,14 +1247,79 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
 // registers of the third wave of a SIMD from every sample (37 -> 51 us above).
 constexpr int kStreamedAtOnce = 2;
 
+// The samples of more than `rows` rows, in pieces: see MomentsFold.  They are left
+// for a walk of their own, so that the sums in 64 bits take no registers from the
+// others, and what it derives from its arguments it derives again.
 template <typename T, int N, int TS>
-__global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backward_kernel(
+__device__ __forceinline__ void long_samples(const T* __restrict__ grad, const T* __restrict__ x,
+                                             const float* __restrict__ scale, const float* __restrict__ bias,
+                                             const float* __restrict__ mean, const float* __restrict__ rstd, bool silu,
+                                             T* __restrict__ grad_x, const Shape& s, Columns columns, int64_t workers,
+                                             int64_t rows, Sums<T>& total, SumsLds<TS, kVec<T>>& lds,
+                                             SumsFold<TS, kVec<T>>& fold, Statistics<TS, kVec<T>, N>& means) {
+  constexpr int V = kVec<T>;
+  int C = s.channels, G = s.groups;
+  asm volatile("" : "+s"(columns.period_vectors), "+s"(columns.copies), "+s"(C), "+s"(G));
+  const bool active = per_lane(silu);
+  const Share share = share_of<T, TS>(columns, 0, C);
+  const Units u = units_of<TS, V, N>(columns, 0, C, G);
+  const Channels<T, N> channels(share, scale, bias, C, C / G);
+  const int stride = columns.stride_vectors();
+  const int64_t piece = piece_of<T>(stride);
+  for (int64_t sample = blockIdx.x; sample < s.samples; sample += workers) {
+    const int64_t first = clamped_offset(s, sample) * s.inner, last = clamped_offset(s, sample + 1) * s.inner;
+    if (first >= last || last - first <= rows) continue;
+    const int64_t elements = (last - first) * C;
+    const int64_t whole = elements / V;
+    const int left = N == 1 ? 0 : static_cast<int>(elements - whole * V);
+    const T* run_g = grad + first * C;
+    const T* run_x = x + first * C;
+    const bool tail = N != 1 && left > 0 && owns(share, whole, stride);
+    const PerGroup<T, N> centre = per_group<T, N>(mean + sample * G, channels);
+    const PerGroup<T, N> inverse = per_group<T, N>(rstd + sample * G, channels);
+    Sums<T> sums;
+    if (share.live) {
+      for (int64_t begin = 0; begin < whole; begin += piece) {
+        sums = Sums<T>();
+        each_pair<T, 1>(run_g, run_x, share.first + begin, begin + piece < whole ? begin + piece : whole, stride,
+                        [&](int64_t, const Values<T>& g, const Values<T>& v) {
+                          sums.add(g, v, channels, centre, inverse, active);
+                        });
+        fold.add(sums, begin == 0);
+      }
+      fold.get(sums);
+    }
+    if (tail)
+      sums.add_part(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left), left, channels, centre, inverse, active);
+    total.add(sums);
+    if (grad_x == nullptr) continue;
+    const float share_of_one = 1.0f / (static_cast<float>(last - first) * static_cast<float>(C / G));
+    merge_sums<TS>(sums, channels, share.live, lds, u, G, [&](int g, float sum_u, float sum_uh) {
+      means.mean[g] = sum_u * share_of_one;
+      means.rstd[g] = sum_uh * share_of_one;
+    });
+    __syncthreads();
+    if (!share.live) continue;
+    T* out = grad_x + first * C;
+    const PerGroup<T, N> mean_u = per_group<T, N>(means.mean, channels);
+    const PerGroup<T, N> mean_uh = per_group<T, N>(means.rstd, channels);
+    const auto gradient = [&](const Values<T>& g, const Values<T>& v) {
+      return gradient_of<T, N>(g, v, channels, centre, inverse, mean_u, mean_uh, active);
+    };
+    each_pair<T, 1>(run_g, run_x, share.first, whole, stride,
+                    [&](int64_t at, const Values<T>& g, const Values<T>& v) { store_whole(out + at, gradient(g, v)); });
+    if (tail) store_part(out + whole * V, gradient(load_part(run_g + whole * V, left), load_part(run_x + whole * V, left)), left);
+  }
+}
+
+template <typename T, int N, int TS>
+__global__ __launch_bounds__(TS, TS == 512 ? 4 : (N == kVec<T> ? 2 : 3)) void group_norm_direct_backward_kernel(
     const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
     const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd, bool silu,
     T* __restrict__ grad_x, Shape s, Columns columns, float2* __restrict__ column_sums, int64_t workers) {
   constexpr int V = kVec<T>;
   __shared__ SumsLds<TS, V> lds;
-  __shared__ Statistics means;
+  __shared__ Statistics<TS, V, N> means;
   const int C = s.channels, G = s.groups;
   const int64_t worker = blockIdx.x;
   if (worker >= workers) {
@@ -1165,9 +1334,14 @@ __global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backw
   const Channels<T, N> channels(share, scale, bias, C, C / G);
   const int stride = columns.stride_vectors();
   Sums<T> total;
+  bool any_long = false;
   for (int64_t sample = worker; sample < s.samples; sample += workers) {
     const int64_t first = clamped_offset(s, sample) * s.inner, last = clamped_offset(s, sample + 1) * s.inner;
     if (first >= last || last - first > s.long_rows) continue;
+    if (TS != 512 && last - first > s.streamed_rows) {
+      any_long = true;
+      continue;
+    }
     const int64_t elements = (last - first) * C;
     const int64_t whole = elements / V;
     const int left = N == 1 ? 0 : static_cast<int>(elements - whole * V);
@@ -1235,9 +1409,35 @@ __global__ __launch_bounds__(TS, TS == 512 ? 4 : 1) void group_norm_direct_backw
     }
     // the next sample's terms go to LDS behind this sample's sync: its means have been written from them by then
   }
+  if constexpr (TS != 512) {
+    __shared__ SumsFold<TS, V> fold;
+    if (any_long)
+      long_samples<T, N, TS>(grad, x, scale, bias, mean, rstd, silu, grad_x, s, columns, workers, s.streamed_rows, total, lds,
+                             fold, means);
+  }
   if (column_sums == nullptr) return;
   __syncthreads();
   write_columns<TS, T>(total, share.live, lds, columns, 0, C, column_sums + worker * C);
+}
+
+// The long walk of workgroups of 512 threads, which are short of registers: with
+// both walks in one kernel 16M elements in samples of 16,000 took 88 us, with the
+// first alone 69.
+template <typename T, int N>
+__global__ __launch_bounds__(512, 2) void group_norm_long_backward_kernel(
+    const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ scale,
+    const float* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd, bool silu,
+    T* __restrict__ grad_x, Shape s, Columns columns, float2* __restrict__ column_sums, int64_t workers) {
+  constexpr int V = kVec<T>;
+  __shared__ SumsLds<512, V> lds;
+  __shared__ SumsFold<512, V> fold;
+  __shared__ Statistics<512, V, N> means;
+  Sums<T> total;
+  long_samples<T, N, 512>(grad, x, scale, bias, mean, rstd, silu, grad_x, s, columns, workers, s.long_rows, total, lds, fold, means);
+  if (column_sums == nullptr) return;
+  __syncthreads();
+  write_columns<512, T>(total, share_of<T, 512>(columns, 0, s.channels).live, lds, columns, 0, s.channels,
+                        column_sums + blockIdx.x * static_cast<int64_t>(s.channels));
 }
 
 // ---------------------------------------------------------------------------
@@ -1254,6 +1454,7 @@ struct Schedule {
   int passes;             // of a tile
   int64_t workers;        // direct workgroups of the backward
   int64_t zero_blocks;    // direct workgroups for rows without a sample
+  bool long_launch;       // whether samples of more than long_rows rows take a direct launch of their own, in the backward
   int64_t column_rows;    // rows of column sums
 };
 
@@ -1276,7 +1477,6 @@ constexpr int64_t workers_for(int threads) { return 256 * (threads > 256 ? 2 : 1
 // take tiles, and all do where no workgroup holds the mean, or in the backward
 // one of 512 threads, two to a CU, would (1,000 samples: 86 us, tiles 70).
 constexpr int64_t kResidentThreads = 262144;  // 16 waves on each CU
-constexpr int64_t kStreamed = 16;
 
 int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inner, int64_t channels, int64_t groups,
                 int type, const int64_t* offsets, int64_t max_entries, bool backward, Schedule& out) {
@@ -1298,7 +1498,7 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
   if (tile_rows < 1) tile_rows = 1;
   out = {};
   out.shape = {samples, entries, inner, static_cast<int>(channels), static_cast<int>(groups), tile_rows,
-               (rows + tile_rows - 1) / tile_rows, 0, offsets};
+               (rows + tile_rows - 1) / tile_rows, 0, 0, offsets};
   if (!grid_fits(samples * groups / 4 + 1, 256) || !grid_fits(samples + 4096, 1024))
     return fail(DPA4K_EINVAL, "%s: the sample count exceeds the launch limit", what);
   const int vec = static_cast<int>(16 / type_bytes(type));
@@ -1331,7 +1531,12 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
   out.workers = out.threads == 0 ? 0 : (samples < workers_for(out.threads) ? samples : workers_for(out.threads));
   const int64_t kilobytes64 = rows * row_bytes / 65536 + 1;
   out.zero_blocks = offsets == nullptr || out.tiles ? 0 : (kilobytes64 < 256 ? kilobytes64 : 256);
-  out.column_rows = out.workers + (out.tiles ? out.shape.tiles : 0);
+  out.shape.streamed_rows = kStreamed * holds(out.threads);
+  if (backward && out.threads == 512 && offsets != nullptr && !out.tiles && rows > out.shape.streamed_rows) {
+    out.long_launch = true;
+    out.shape.long_rows = out.shape.streamed_rows;
+  }
+  out.column_rows = out.workers * (out.long_launch ? 2 : 1) + (out.tiles ? out.shape.tiles : 0);
   return DPA4K_OK;
 }
 
@@ -1427,6 +1632,12 @@ int backward_as(const T* grad, const T* x, const float* scale, const float* bias
     DPA4K_DIRECT(c.threads, DPA4K_LAUNCH)
 #undef DPA4K_LAUNCH
     if (int e = launched("group_norm_direct_backward_kernel")) return e;
+    if (c.long_launch && c.workers > 0) {
+      group_norm_long_backward_kernel<T, N><<<static_cast<unsigned int>(c.workers), 512, 0, stream>>>(
+          grad, x, scale, bias, mean, rstd, silu, grad_x, s, columns,
+          parameters ? direct_columns + c.workers * s.channels : nullptr, c.workers);
+      if (int e = launched("group_norm_long_backward_kernel")) return e;
+    }
   }
   if (c.tiles) {
     const Columns columns = columns_for<T>(s.channels, kTileBlock);

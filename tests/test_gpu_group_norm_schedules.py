@@ -10,9 +10,12 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_group_norm import _check, _inputs, _offsets
+from bysj_amd.kernels.group_norm import group_norm
+from parity import announce, assert_close_scaled
+from test_gpu_group_norm import _check, _inputs, _offsets, _rtol
 
 pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
 
 LAYOUTS = [(64, 8), (90, 6), (12, 4)]
 ELEMENTS = [1000, 5000, 12000, 30000, 200000]    # of a sample: 64, 256, 512 and 1,024 threads, tiles
@@ -59,3 +62,97 @@ def test_longer_samples_among_many(dtype, channels, groups, mean, threads, activ
     lengths[5], lengths[77] = 6 * rows, 0
     x, grad, scale, bias = _inputs((sum(lengths), channels), dtype, seed=mean)
     _check(x, grad, groups, scale, bias, _offsets(lengths), activation, max_rows=6 * rows, what=f"about {mean} elements")
+
+
+@pytest.mark.parametrize("activation", [None, "silu"])
+@pytest.mark.parametrize("said", [500, 5000, 12000, 30000])
+@pytest.mark.parametrize("channels,groups", LAYOUTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_samples_longer_than_said_among_others(dtype, channels, groups, said, activation):
+    """Samples of the length that was said, of up to 16 times that, and of more, in turn."""
+    rows = said // channels
+    lengths = [rows, 20 * rows + 1, 0, 3 * rows, 1, 33 * rows - 1, rows // 2, rows, 17 * rows]
+    x, grad, scale, bias = _inputs((sum(lengths), channels), dtype, seed=said)
+    _check(x, grad, groups, scale, bias, _offsets(lengths), activation, max_rows=rows, what=f"said {said} elements")
+
+
+# ---------------------------------------------------------------------------
+# long sums
+# ---------------------------------------------------------------------------
+#
+# Terms that are all alike do not average their roundings out: a running sum of n
+# of them in 32 bits is off by up to n 2^-25 of it.  The rule of 1e-5 leaves room
+# for about 300 in sequence.
+
+def _even_gradients(x, groups, scale, bias, offsets, value, activation, max_rows):
+    """(y, grad_x, grad_scale, grad_bias) for a gradient of ``value`` everywhere, the definition's in 64 bits on the GPU, and
+    what the roundings of h leave of grad_scale."""
+    leaves = [t.requires_grad_(True) for t in (x, scale, bias)]
+    y = group_norm(x, groups, scale, bias, offsets=offsets, max_rows=max_rows, activation=activation)
+    grad = torch.full_like(y, value)
+    actual = torch.autograd.grad(y, leaves, grad)
+    with torch.no_grad():
+        rows = x.double().reshape(-1, groups, x.shape[-1] // groups)
+        centred = rows - rows.mean((0, 2), keepdim=True)
+        inverse = 1.0 / torch.sqrt(centred.square().mean((0, 2), keepdim=True) + 1e-5)
+        hat = (centred * inverse).reshape(-1, x.shape[-1])
+        z = hat * scale.double() + bias.double()
+        gate = torch.sigmoid(z)
+        dz = grad.double().reshape(hat.shape) * (gate * (1.0 + z * (1.0 - gate)) if activation else 1.0)
+        wanted_y = (z * gate if activation else z).view(x.shape)
+        u = (dz * scale.double()).view(rows.shape)
+        h = hat.view(rows.shape)
+        grad_x = inverse * (u - u.mean((0, 2), keepdim=True) - h * (u * h).mean((0, 2), keepdim=True))
+        wanted = grad_x.view(x.shape), (dz * hat).sum(0), dz.sum(0)
+        # grad_scale adds dz h over all rows, and its terms may cancel.  A row's h is off by 2^-24 (|mean| rstd + 2 |h|) at
+        # most (the stored mean's rounding, the difference's, rstd's), whatever the sum does with its own roundings.
+        far = (rows.mean((0, 2), keepdim=True).abs() * inverse).expand_as(h)
+        slack = 2.0 ** -24 * (dz.abs() * (far + 2.0 * h.abs()).reshape(hat.shape)).sum(0)
+    return (y, *actual), (wanted_y, *wanted), slack
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("channels,groups", LAYOUTS)
+@pytest.mark.parametrize("activation", [None, "silu"])
+@pytest.mark.parametrize("said", [1, 5000, 12000, 30000])
+def test_a_sample_much_longer_than_said(said, channels, groups, activation, dtype):
+    """max_rows of ``said`` elements for a sample of 24 million: its sums stay as exact as others'."""
+    announce("longer than said", said, channels, groups, activation, dtype)
+    rows = 24_000_000 // channels
+    generator = torch.Generator(device=DEV).manual_seed(channels)
+    x = (torch.randn(rows, channels, generator=generator, device=DEV) * 1.5 + 0.5).to(dtype)
+    scale = torch.rand(channels, generator=generator, device=DEV) + 0.5
+    bias = torch.randn(channels, generator=generator, device=DEV)
+    offsets = torch.tensor([0, rows], device=DEV)
+    actual, wanted, slack = _even_gradients(x, groups, scale, bias, offsets, 0.1, activation, max(said // channels, 1))
+    for name, a, b in zip(("y", "grad_x", "grad_scale", "grad_bias"), actual, wanted):
+        if name == "grad_scale":
+            bound = 1e-5 * b.abs() + 1e-5 * b.abs().max() + slack
+            assert ((a.double() - b).abs() <= bound).all(), f"grad_scale: {((a.double() - b).abs() / bound).max()} of the bound"
+        else:
+            assert_close_scaled(a, b, rtol=_rtol(dtype) if name in ("y", "grad_x") else 1e-5, what=name)
+
+
+def test_a_far_mean_of_a_sample_much_longer_than_said():
+    rows, channels, mean = 375_000, 64, -1000.0
+    generator = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(rows, channels, generator=generator, device=DEV) * 1.5 + mean
+    y = group_norm(x, 8, offsets=torch.tensor([0, rows], device=DEV), max_rows=1)
+    part = x.double().view(rows, 8, 8)
+    centred = part - part.mean((0, 2), keepdim=True)
+    wanted = centred / torch.sqrt(centred.square().mean((0, 2), keepdim=True) + 1e-5)
+    # the rounding of the mean, 2^-24 |mean| / std on values of up to about 4
+    assert_close_scaled(y, wanted.view(rows, channels), scale=1e-5 + 2.0 ** -24 * abs(mean) * 4, what="far mean")
+
+
+@pytest.mark.parametrize("channels,groups", LAYOUTS)
+@pytest.mark.parametrize("size", [0.3, 7.7])
+def test_deviations_of_one_size_in_a_sample_much_longer_than_said(size, channels, groups):
+    """Rows of +size and -size by turns: every batch adds the same to the squared deviations."""
+    rows = 48_000_000 // channels // 2 * 2
+    sign = torch.ones(rows, 1, device=DEV)
+    sign[1::2] = -1.0
+    x = (sign * size).expand(rows, channels).contiguous()
+    y = group_norm(x, groups, offsets=torch.tensor([0, rows], device=DEV), max_rows=1)
+    value = float(x[0, 0])
+    assert_close_scaled(y, (sign.double() * (value / (value * value + 1e-5) ** 0.5)).expand(rows, channels), what="one size")
