@@ -586,6 +586,15 @@ struct Slot {
   float count, mean, squares;
 };
 
+// What two passes over a piece leave of a group.
+__device__ __forceinline__ Slot joined(const Slot& a, const Slot& b) {
+  if (!(b.count > 0.0f)) return a;
+  if (!(a.count > 0.0f)) return b;
+  const float total = a.count + b.count, delta = b.mean - a.mean;
+  const float weight = b.count * __builtin_amdgcn_rcpf(total);
+  return {total, fmaf(delta, weight, a.mean), a.squares + fmaf(delta * delta, a.count * weight, b.squares)};
+}
+
 __device__ __forceinline__ float inverse_root(double squares, double count, float eps) {
   return static_cast<float>(1.0 / sqrt(squares / count + static_cast<double>(eps)));
 }
@@ -682,7 +691,7 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_moments_kernel(const T*
   const int64_t tile = block_index();
   if (tile >= s.tiles) return;
   each_piece(s, tile, [&](int64_t sample, int64_t a, int64_t b) {
-    Slot* out = slots + (tile + sample) * columns.passes * s.groups;
+    Slot* out = slots + (tile + sample) * s.groups;
     for (int pass = 0; pass < columns.passes; ++pass) {
       const Share share = share_of<T, kTileBlock>(columns, pass, s.channels);
       const Units u = units_of<kTileBlock, kVec<T>, N>(columns, pass, s.channels, s.groups);
@@ -690,7 +699,8 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_moments_kernel(const T*
       running.add_run(x + a * s.channels, (b - a) * s.channels, share, columns.stride_vectors(),
                       split_of<T, N>(share, s.channels / s.groups));
       merge_moments<kTileBlock>(running, share.live, lds, u, s.groups, [&](int g, float count, float mean, float squares) {
-        out[pass * s.groups + g] = {count, mean, squares};
+        const Slot own = {count, mean, squares};
+        out[g] = pass == 0 ? own : joined(out[g], own);
       });
       __syncthreads();
     }
@@ -698,17 +708,15 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_moments_kernel(const T*
 }
 
 // The slots of a sample's rows [first, last): where they start and how many.
-__device__ __forceinline__ int64_t slots_of(const Shape& s, int passes, int64_t sample, int64_t first, int64_t last,
-                                            int64_t& start) {
+__device__ __forceinline__ int64_t slots_of(const Shape& s, int64_t sample, int64_t first, int64_t last, int64_t& start) {
   const int64_t tile = first / s.tile_rows;
-  start = (tile + sample) * passes;
-  return ((last - 1) / s.tile_rows - tile + 1) * passes;
+  start = tile + sample;
+  return (last - 1) / s.tile_rows - tile + 1;
 }
 
 // A wave per (sample, group) of the long samples.
-__global__ __launch_bounds__(256) void group_norm_finish_kernel(const Slot* __restrict__ slots, Shape s, int passes,
-                                                                float eps, float* __restrict__ mean,
-                                                                float* __restrict__ rstd) {
+__global__ __launch_bounds__(256) void group_norm_finish_kernel(const Slot* __restrict__ slots, Shape s, float eps,
+                                                                float* __restrict__ mean, float* __restrict__ rstd) {
   const int64_t unit = uniform_i64(block_index() * 4 + (threadIdx.x >> 6));
   if (unit >= s.samples * s.groups) return;
   const int64_t sample = unit / s.groups;
@@ -716,7 +724,7 @@ __global__ __launch_bounds__(256) void group_norm_finish_kernel(const Slot* __re
   const int lane = threadIdx.x & 63;
   if (last - first <= s.long_rows) return;
   int64_t start;
-  const int64_t n = slots_of(s, passes, sample, first, last, start);
+  const int64_t n = slots_of(s, sample, first, last, start);
   const Merged m = merge_slots(slots + start * s.groups + unit % s.groups, n, s.groups, lane, 64);
   if (lane != 0) return;
   mean[unit] = static_cast<float>(m.mean);
@@ -1072,9 +1080,11 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_sums_kernel(
                           inverse, silu);
         }
       }
-      float2* out = slots + ((tile + sample) * columns.passes + pass) * G;
-      merge_sums<kTileBlock>(sums, channels, share.live, lds, u, G,
-                             [&](int g, float sum_u, float sum_uh) { out[g] = {sum_u, sum_uh}; });
+      float2* out = slots + (tile + sample) * G;
+      merge_sums<kTileBlock>(sums, channels, share.live, lds, u, G, [&](int g, float sum_u, float sum_uh) {
+        if (pass == 0) out[g] = {sum_u, sum_uh};
+        else out[g] = {out[g].x + sum_u, out[g].y + sum_uh};
+      });
       total.add(sums);
       __syncthreads();
     });
@@ -1107,7 +1117,7 @@ __device__ __forceinline__ float2 merge_sum_slots(const float2* __restrict__ slo
 }
 
 // A wave per (sample, group): means of u, then of u h, of each sample's groups.
-__global__ __launch_bounds__(256) void group_norm_means_kernel(const float2* __restrict__ slots, Shape s, int passes,
+__global__ __launch_bounds__(256) void group_norm_means_kernel(const float2* __restrict__ slots, Shape s,
                                                                float* __restrict__ means) {
   const int64_t unit = uniform_i64(block_index() * 4 + (threadIdx.x >> 6));
   if (unit >= s.samples * s.groups) return;
@@ -1115,7 +1125,7 @@ __global__ __launch_bounds__(256) void group_norm_means_kernel(const float2* __r
   const int64_t first = clamped_offset(s, sample) * s.inner, last = clamped_offset(s, sample + 1) * s.inner;
   if (last - first <= s.long_rows) return;
   int64_t start;
-  const int64_t n = slots_of(s, passes, sample, first, last, start);
+  const int64_t n = slots_of(s, sample, first, last, start);
   const int lane = threadIdx.x & 63;
   const double count = static_cast<double>(last - first) * (s.channels / s.groups);
   const float2 m = merge_sum_slots(slots + start * s.groups + unit % s.groups, n, s.groups, lane, 64, count);
@@ -1451,7 +1461,6 @@ struct Schedule {
   Shape shape;
   int threads;            // of a direct workgroup; 0: tiles alone
   bool tiles;             // whether samples may be longer than a direct workgroup holds
-  int passes;             // of a tile
   int64_t workers;        // direct workgroups of the backward
   int64_t zero_blocks;    // direct workgroups for rows without a sample
   bool long_launch;       // whether samples of more than long_rows rows take a direct launch of their own, in the backward
@@ -1503,7 +1512,6 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
     return fail(DPA4K_EINVAL, "%s: the sample count exceeds the launch limit", what);
   const int vec = static_cast<int>(16 / type_bytes(type));
   const int period = static_cast<int>(channels) / gcd_of(static_cast<int>(channels), vec);
-  out.passes = (period + kTileBlock - 1) / kTileBlock;
   // the smallest direct workgroup that holds `sample_rows`, 0 where none does
   const auto holds = [&](int threads) { return static_cast<int64_t>(threads / period) * period * 32 / channels; };
   const auto threads_for = [&](int64_t sample_rows) {
@@ -1541,15 +1549,15 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
 }
 
 struct Workspace {
-  Slot* slots;          // per (piece, pass, group), forward
-  float2* sum_slots;    // per (piece, pass, group), backward
+  Slot* slots;          // per (piece, group), forward
+  float2* sum_slots;    // per (piece, group), backward
   float* means;         // per (sample, sum, group), backward
   float2* column_sums;  // rows of channels, backward
 };
 
 template <typename Take>
 void each_array(const Schedule& c, bool backward, Take take) {
-  const size_t pieces = c.tiles ? static_cast<size_t>(c.shape.tiles + c.shape.samples) * c.passes * c.shape.groups : 0;
+  const size_t pieces = c.tiles ? static_cast<size_t>(c.shape.tiles + c.shape.samples) * c.shape.groups : 0;
   if (!backward) {
     take(&Workspace::slots, pieces);
     return;
@@ -1607,8 +1615,7 @@ int forward_as(const T* x, const float* scale, const float* bias, T* y, float* m
   group_norm_moments_kernel<T, N><<<grid, kTileBlock, 0, stream>>>(x, s, columns, w.slots);
   if (int e = launched("group_norm_moments_kernel")) return e;
   if (s.samples > 0) {
-    group_norm_finish_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(w.slots, s, columns.passes,
-                                                                                                  eps, mean, rstd);
+    group_norm_finish_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(w.slots, s, eps, mean, rstd);
     if (int e = launched("group_norm_finish_kernel")) return e;
   }
   group_norm_apply_kernel<T, N><<<grid, kTileBlock, 0, stream>>>(x, scale, bias, silu, mean, rstd, y, s, columns);
@@ -1647,8 +1654,7 @@ int backward_as(const T* grad, const T* x, const float* scale, const float* bias
     if (int e = launched("group_norm_sums_kernel")) return e;
     if (grad_x != nullptr) {
       if (s.samples > 0) {
-        group_norm_means_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(w.sum_slots, s,
-                                                                                                     columns.passes, w.means);
+        group_norm_means_kernel<<<launch_grid((s.samples * s.groups + 3) / 4, 256), 256, 0, stream>>>(w.sum_slots, s, w.means);
         if (int e = launched("group_norm_means_kernel")) return e;
       }
       group_norm_backward_kernel<T, N><<<grid, kTileBlock, 0, stream>>>(grad, x, scale, bias, mean, rstd, w.means, silu,
