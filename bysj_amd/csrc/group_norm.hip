@@ -1474,6 +1474,11 @@ constexpr int kDirectThreads[] = {64, 256, 512, 1024};
 // whose last third finds the CUs full).
 constexpr int64_t workers_for(int threads) { return 256 * (threads > 256 ? 2 : 12 / (threads / 64)); }
 
+// No workgroup keeps its sums per channel, in 32 bits, over more samples than this:
+// 61M samples of one row, 19,900 to a workgroup, left them off by 1.7e-4 of their
+// value under gradients of one size.
+constexpr int64_t kWorkerSamples = 256;
+
 // Checks the sizes, cuts the rows into tiles, and chooses the schedule.  A
 // direct workgroup holds 32 elements a thread.  Samples of one length take the
 // smallest that holds one.  Ragged samples take the smallest that holds the
@@ -1536,7 +1541,12 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
     out.tiles = out.threads == 0 || longest > limit;
     out.shape.long_rows = out.threads == 0 ? 0 : (out.tiles ? limit : INT64_MAX);  // with no tiles any sample is streamed
   }
-  out.workers = out.threads == 0 ? 0 : (samples < workers_for(out.threads) ? samples : workers_for(out.threads));
+  if (out.threads != 0) {
+    const int64_t filled = samples < rows ? samples : rows;  // at most: the others are empty
+    const int64_t wanted = (filled + kWorkerSamples - 1) / kWorkerSamples, most = 0xFFFFFFFFLL / out.threads - 4096;
+    out.workers = wanted > workers_for(out.threads) ? (wanted < most ? wanted : most) : workers_for(out.threads);
+    if (samples < out.workers) out.workers = samples;
+  }
   const int64_t kilobytes64 = rows * row_bytes / 65536 + 1;
   out.zero_blocks = offsets == nullptr || out.tiles ? 0 : (kilobytes64 < 256 ? kilobytes64 : 256);
   out.shape.streamed_rows = kStreamed * holds(out.threads);

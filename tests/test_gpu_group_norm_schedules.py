@@ -10,6 +10,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from bysj_amd.kernels import _C
 from bysj_amd.kernels.group_norm import group_norm
 from parity import announce, assert_close_scaled
 from test_gpu_group_norm import _check, _inputs, _offsets, _rtol
@@ -156,3 +157,14 @@ def test_deviations_of_one_size_in_a_sample_much_longer_than_said(size, channels
     y = group_norm(x, groups, offsets=torch.tensor([0, rows], device=DEV), max_rows=1)
     value = float(x[0, 0])
     assert_close_scaled(y, (sign.double() * (value / (value * value + 1e-5) ** 0.5)).expand(rows, channels), what="one size")
+
+
+def test_gradients_summed_over_many_samples():
+    """61 million samples of one row under gradients of one size: what a workgroup adds up stays short."""
+    announce("many samples")
+    samples, channels = 61_000_000, 8
+    x = torch.randn(samples, channels, generator=torch.Generator(device=DEV).manual_seed(0), device=DEV)
+    grad = torch.full_like(x, 0.1)
+    _, statistics = _C.group_norm_forward(x, 1)
+    _, _, grad_bias = _C.group_norm_backward(grad, x, 1, None, None, None, statistics, want_x=False, want_scale=False)
+    assert_close_scaled(grad_bias, torch.full((channels,), samples * float(grad[0, 0]), dtype=torch.float64), what="grad_bias")
