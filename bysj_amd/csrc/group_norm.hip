@@ -1476,7 +1476,9 @@ constexpr int64_t workers_for(int threads) { return 256 * (threads > 256 ? 2 : 1
 
 // No workgroup keeps its sums per channel, in 32 bits, over more samples than this:
 // 61M samples of one row, 19,900 to a workgroup, left them off by 1.7e-4 of their
-// value under gradients of one size.
+// value under gradients of one size.  More samples take more rounds of as many
+// workgroups as are resident (a million of 8 rows of 16: 0.9 ms with 3,072 or 6,144
+// workgroups, 1.34 with 3,907, whose second round leaves most CUs idle).
 constexpr int64_t kWorkerSamples = 256;
 
 // Checks the sizes, cuts the rows into tiles, and chooses the schedule.  A
@@ -1543,8 +1545,9 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
   }
   if (out.threads != 0) {
     const int64_t filled = samples < rows ? samples : rows;  // at most: the others are empty
-    const int64_t wanted = (filled + kWorkerSamples - 1) / kWorkerSamples, most = 0xFFFFFFFFLL / out.threads - 4096;
-    out.workers = wanted > workers_for(out.threads) ? (wanted < most ? wanted : most) : workers_for(out.threads);
+    const int64_t resident = workers_for(out.threads), rounds = (filled + resident * kWorkerSamples - 1) / (resident * kWorkerSamples);
+    const int64_t most = 0xFFFFFFFFLL / out.threads / resident - 1;
+    out.workers = resident * (rounds < 1 ? 1 : (rounds < most ? rounds : most));
     if (samples < out.workers) out.workers = samples;
   }
   const int64_t kilobytes64 = rows * row_bytes / 65536 + 1;
