@@ -42,7 +42,10 @@ namespace {
 constexpr int kTileBlock = 256;
 constexpr int kMaxChannels = DPA4K_GROUP_NORM_MAX_CHANNELS;
 constexpr int64_t kTileBytes = 16384;   // least bytes of a tile
-constexpr int64_t kTiles = 1024;        // most tiles where they are larger than that: 4 workgroups per CU
+constexpr int64_t kTiles = 1024;        // most tiles of between those and kMostTileBytes: 4 workgroups to a CU, of which
+                                        // the kernels of more than 128 registers (16-bit apply, sums) keep 3 resident
+constexpr int64_t kMostTileBytes = 1 << 20;  // 256 vectors a thread: its sums in 32 bits stay short (16 GB under gradients
+                                             // of one size: grad_bias was off by 3.7e-5 of its value with 1,024 tiles)
 constexpr int kLdsGroups = 1024;        // groups of a direct workgroup, whose statistics are kept in LDS
 constexpr int64_t kStreamed = 16;       // times what it holds: the longest sample that a direct workgroup is meant for
 constexpr float kLog2e = 1.4426950408889634f;
@@ -1510,6 +1513,7 @@ int schedule_of(const char* what, int64_t samples, int64_t entries, int64_t inne
   const int64_t row_bytes = channels * type_bytes(type);
   const int64_t least = kTileBytes / row_bytes;
   int64_t tile_rows = (rows + kTiles - 1) / kTiles;
+  if (tile_rows > kMostTileBytes / row_bytes) tile_rows = kMostTileBytes / row_bytes;
   if (tile_rows < least) tile_rows = least;
   if (tile_rows < 1) tile_rows = 1;
   out = {};

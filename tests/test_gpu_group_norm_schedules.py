@@ -168,3 +168,15 @@ def test_gradients_summed_over_many_samples():
     _, statistics = _C.group_norm_forward(x, 1)
     _, _, grad_bias = _C.group_norm_backward(grad, x, 1, None, None, None, statistics, want_x=False, want_scale=False)
     assert_close_scaled(grad_bias, torch.full((channels,), samples * float(grad[0, 0]), dtype=torch.float64), what="grad_bias")
+
+
+def test_gradients_summed_over_a_large_sample():
+    """One sample of 4e9 elements (16 GB): the same for a tile's workgroup."""
+    announce("large sample")
+    rows, channels = 62_500_000, 64
+    x = torch.randn(rows, channels, generator=torch.Generator(device=DEV).manual_seed(0), device=DEV)
+    grad = torch.full_like(x, 0.1)
+    offsets = torch.tensor([0, rows], device=DEV)
+    _, statistics = _C.group_norm_forward(x, 8, None, None, offsets)
+    _, _, grad_bias = _C.group_norm_backward(grad, x, 8, None, None, offsets, statistics, want_x=False, want_scale=False)
+    assert_close_scaled(grad_bias, torch.full((channels,), rows * float(grad[0, 0]), dtype=torch.float64), what="grad_bias")
