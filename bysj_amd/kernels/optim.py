@@ -302,12 +302,17 @@ class AdamW(torch.optim.Optimizer):
     def _check_group(cls, group) -> None:
         cls._check_options(group)
         for p in group["params"]:
-            if isinstance(group["lr"], torch.Tensor) and group["lr"].device != p.device and p.device.type != "cpu":
-                raise ValueError("AdamW lr must be on the parameters' device")
+            if p.device.type != "cpu":  # on the CPU they may still be on their way
+                cls._check_place(group, p.device)
             if p.dtype not in DTYPES:
                 raise TypeError("AdamW requires float32 or bfloat16 parameters")
             if not p.is_contiguous():
                 raise ValueError("AdamW parameters must be contiguous")
+
+    @staticmethod
+    def _check_place(group, device) -> None:
+        if isinstance(group["lr"], torch.Tensor) and group["lr"].device != device:
+            raise ValueError("AdamW lr must be on the parameters' device")
 
     @staticmethod
     def _refuse_variants(groups) -> None:
@@ -392,7 +397,10 @@ class AdamW(torch.optim.Optimizer):
                 if plan is None:
                     plan = self._plans[key] = self._build(params, {})
                 index, dtype = key
-                work.append((self.param_groups[index], plan, grads, index * 2 + (dtype == torch.bfloat16)))
+                group = self.param_groups[index]
+                self._check_options(group)  # all of them before the first group's step
+                self._check_place(group, plan.device)
+                work.append((group, plan, grads, index * 2 + (dtype == torch.bfloat16)))
         self.norm = factor = None
         if self.max_norm is not None and work:
             self.norm, factor = grad_norm([g for _, _, grads, _ in work for g in grads if g is not None], self.max_norm)

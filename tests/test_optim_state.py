@@ -292,3 +292,21 @@ def test_a_learning_rate_tensor_is_on_the_parameters_device():
     assert optimiser.param_groups[0]["lr"].device == there.device
     assert checkpoint["param_groups"][0]["lr"].device.type == "cpu"
     optim.AdamW([torch.zeros(3)], lr=torch.tensor(0.1, device="meta"))    # parameters that are still to be moved
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("error,option,value", [
+    (ValueError, "lr", -1.0), (TypeError, "lr", "1"), (ValueError, "lr", torch.zeros(2)), (ValueError, "lr", torch.zeros((), device="meta")),
+    (TypeError, "betas", 0.9), (ValueError, "betas", (0.9, 1.0)), (ValueError, "eps", 0.0), (ValueError, "weight_decay", -0.1),
+])
+def test_a_step_is_refused_whole(error, option, value, bits):
+    """An option of the second group goes wrong between two steps: the first group takes no step either."""
+    optimiser, params = _trained(bits)
+    before, values = optimiser.state_dict(), [p.detach().clone() for p in params]
+    held = optimiser.param_groups[1][option]
+    optimiser.param_groups[1][option] = value
+    with pytest.raises(error):
+        optimiser.step()
+    optimiser.param_groups[1][option] = held
+    _same(optimiser.state_dict(), before)
+    _same([p.detach() for p in params], values)
