@@ -14,7 +14,8 @@
 //  - direct: a workgroup of 64 to 1,024 threads per sample holds the sample in
 //    registers between its statistics and its output, one launch and one read
 //    (16M float32 elements in samples of 8,000, forward: 23 us, 5.8 TB/s;
-//    backward 45 us, 4.5 TB/s).  Somewhat longer samples are read twice by it.
+//    backward 45 us, 4.5 TB/s).  Somewhat longer samples are read twice by it,
+//    and any longer ones, if they come in spite of max_rows, piece by piece.
 //  - tiles: samples too long for that (or of unknown length) are cut, whatever
 //    their lengths, by tiles of equal rows, a workgroup per tile that walks the
 //    pieces of samples in it.  A piece leaves its sums in slot (tile + sample),
@@ -42,10 +43,14 @@ namespace {
 constexpr int kTileBlock = 256;
 constexpr int kMaxChannels = DPA4K_GROUP_NORM_MAX_CHANNELS;
 constexpr int64_t kTileBytes = 16384;   // least bytes of a tile
-constexpr int64_t kTiles = 1024;        // most tiles of between those and kMostTileBytes: 4 workgroups to a CU, of which
-                                        // the kernels of more than 128 registers (16-bit apply, sums) keep 3 resident
-constexpr int64_t kMostTileBytes = 1 << 20;  // 256 vectors a thread: its sums in 32 bits stay short (16 GB under gradients
-                                             // of one size: grad_bias was off by 3.7e-5 of its value with 1,024 tiles)
+// Most tiles of between kTileBytes and kMostTileBytes: 4 workgroups to a CU, all of
+// them resident but in the 16-bit kernels of more than 128 registers (the apply
+// kernel where N = 1, 132, and the sums kernel where N = V, 133), which keep 3.
+constexpr int64_t kTiles = 1024;
+// Most bytes of a tile, 256 vectors a thread, so that sums in 32 bits stay short:
+// with 1,024 tiles on 16 GB grad_bias was off by 3.7e-5 of its value under
+// gradients of one size.
+constexpr int64_t kMostTileBytes = 1 << 20;
 constexpr int kLdsGroups = 1024;        // groups of a direct workgroup, whose statistics are kept in LDS
 constexpr int64_t kStreamed = 16;       // times what it holds: the longest sample that a direct workgroup is meant for
 constexpr float kLog2e = 1.4426950408889634f;
@@ -782,8 +787,9 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_apply_kernel(
 // direct, forward
 // ---------------------------------------------------------------------------
 //
-// TS threads hold 32 elements each of a sample.  A longer sample (the workgroup
-// is chosen for the mean) is streamed twice, and one that is longer than that
+// TS threads hold 32 elements each of a sample (1,024 threads with narrow 16-bit
+// groups spill 4 registers).  A longer sample (the workgroup is chosen for the
+// mean) is streamed twice, and one that is longer than that
 // allows for (max_rows was too small) piece by piece.  Blocks behind the samples
 // write the zeros of rows without a sample.
 template <typename T>
@@ -1251,10 +1257,10 @@ __global__ __launch_bounds__(kTileBlock) void group_norm_backward_kernel(
 // threads (1,024 would leave 128 registers each, half of them held).  With 16
 // elements a thread samples of 60 rows of 64 took 512 threads, of which a CU
 // holds two workgroups: 51 us for 3,000 of them (139 MB), 37 us with 32.  512
-// threads are held to 128 registers, so that a CU holds two of them (some spill:
-// 16M elements in samples of 16,000 took 58 us with one, 50 us with two; 53 and
-// 38 us in bfloat16); fewer threads are slower that way (47 and 54 us in samples
-// of 1,024).  A workgroup takes the samples b, b + workgroups, ... and keeps its
+// threads are held to 128 registers, so that a CU holds two of them (they spill 34
+// to 40 registers in float32, 10 to 46 in 16 bits: 16M elements in samples of
+// 16,000 took 58 us with one, 50 us with two; 53 and 38 us in bfloat16; with SiLU
+// 69 and 37); fewer threads are slower that way (47 and 54 us in samples of 1,024).  A workgroup takes the samples b, b + workgroups, ... and keeps its
 // sums per channel across them, one row of column sums in the end.  A longer
 // sample is streamed, two vectors of each tensor at once: four would take the
 // registers of the third wave of a SIMD from every sample (37 -> 51 us above).

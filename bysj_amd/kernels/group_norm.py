@@ -11,6 +11,10 @@ with ``groups`` = 1 a layer norm over each sample, with ``groups`` = channels
 an instance norm.  Samples are given by CSR offsets, as in ``segment_sum``, or
 are the entries of the first axis.  Gradients of the input, the scale and the
 bias.  Not part of ``kernels.__all__``, which stays the reference's list.
+
+It is a norm of invariant features.  Of spherical-harmonic components it may
+run over the l = 0 row alone: a mean over the rows of l > 0, a bias on them or a
+SiLU of them depends on the orientation of the frame.
 """
 from __future__ import annotations
 
@@ -117,8 +121,11 @@ def group_norm(x: torch.Tensor, groups: int, scale: torch.Tensor | None = None, 
     their rows; entries of no sample give 0.  Without offsets every entry is a
     sample.  ``scale``, ``bias``: float32 ``(channels,)``.  ``max_rows``: the
     entries of the longest sample where the caller knows it; it only selects
-    the schedule.  ``activation``: None or ``"silu"``.  Statistics are kept in
-    float32 or wider whatever the input's type.
+    the schedule (one that is too small costs time).  ``activation``: None or
+    ``"silu"``.  Statistics are kept in float32 or wider whatever the input's
+    type; the squared deviations of a sample's group must add up to less than
+    float32's largest number (3e38), else its rstd is 0.  The gradients have no
+    gradients of their own: a second derivative is refused.
     """
     groups, eps = _validate(x, groups, scale, bias, offsets, max_rows, eps, activation)
     require_dcu(x, scale, bias, offsets)

@@ -596,7 +596,9 @@ int dpa4k_grad_norm(const void* const* grads, const int64_t* counts,
  * exp_avg and exp_avg_sq are float[count] and the scales NULL.  With moments in
  * 8 bits they are codes, one byte per element of `count` rounded up to a
  * multiple of 32 and 8-byte aligned, and the scales one byte per 32 elements
- * (at least 16 and 32); codes of 0 stand for moments of 0. */
+ * (at least 16 and 32); codes of 0 stand for moments of 0. A block with an
+ * infinity, a NaN, a value above 1.875 * 2^127 or a second moment below 0 becomes
+ * NaN. */
 typedef struct {
   void* param;
   void* exp_avg;
