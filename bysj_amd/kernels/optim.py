@@ -256,7 +256,9 @@ class AdamW(torch.optim.Optimizer):
 
     The plans are built in the first step; later steps may be captured in a
     HIP graph (with ``lr`` a tensor where a schedule changes it between
-    replays).  Checkpoints hold each parameter's step count and moments; 8-bit
+    replays; a graph uses the plans it was captured with, which
+    ``load_state_dict`` and parameters that move, come or go replace).  What is
+    refused (a step, a group, a checkpoint) changes nothing.  Checkpoints hold each parameter's step count and moments; 8-bit
     moments are kept as their codes.  They come from ``state_dict``, and its
     hooks see them: ``state`` itself stays empty, for the moments live in the
     plans.
