@@ -1,0 +1,877 @@
+// The experts' products, forward and backward, and the sum of a token's slots (no
+// counterpart in the reference; a matrix per segment of its CSR contract):
+//
+//   place p of expert e, row i of its entry:   z[p, i] = W[e] x[entry(p), i]
+//   entry(p) = order[p] / k (x by token) or p (x by place)
+//   y = z,  or  silu(z[:F]) z[F:]  with the gated SiLU
+//   dx[entry] = sum over its places of W[e]^T dz[p],   dW[e] = sum_p dz[p] x[entry(p)]^T
+//   out[t, i] = sum_j w[t, j] y[places[t, j], i]
+//
+// One tiled product serves all three directions; they differ in which of its two
+// operands has the summed index contiguous:
+//
+//            rows of the result     columns           summed over     x or dz / W
+//   forward  a segment's rows       outputs           inputs          both contiguous
+//   dx       a segment's rows       inputs            outputs         W across
+//   dW       outputs                inputs            rows            both across
+//
+// A workgroup finds its segment by a scan of the offsets, so that nothing waits for
+// the host and the calls can be captured.  Tiles go through LDS in slices of 128
+// bytes along the summed index (or of as many rows), double-buffered: the next
+// slice is on its way from memory while this one is multiplied.  Results are held
+// in 32 bits in the matrix units' registers.
+#include <climits>
+#include <type_traits>
+
+#include "elements.h"
+
+namespace dpa4k {
+namespace {
+
+constexpr int kMaxExperts = DPA4K_EXPERTS_MAX;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+enum { kForward = 0, kGated = 1, kInput = 2, kWeight = 3 };
+
+struct ProductCall {
+  const void* a;           // x (forward), dz (dx, dW)
+  const void* b;           // W (forward, dx), x (dW)
+  void* out;               // y, dx by place or by slot, dW or its partial sums
+  float* before;           // forward, gated: z, or null
+  const int64_t* offsets;
+  const int64_t* order;    // null: x by place
+  int64_t places;
+  int experts, k, inner;   // k: slots of a token, which order is divided by
+  int k_in, n_out;         // of W[e], n_out before the gate
+  int chunk_rows;          // dW: rows of a segment that one workgroup takes
+  int chunks;              // dW: most chunks of all segments; 1 and no partial sums if every segment is one
+  int by_slot;             // dx: written at order[p] instead of p
+};
+
+// ---------------------------------------------------------------------------
+// segments and tiles
+// ---------------------------------------------------------------------------
+
+// Rows [begin, end) of segment e; segment `experts` is what lies behind the last.
+struct Span {
+  int begin, end;
+};
+
+__device__ __forceinline__ Span span_of(const ProductCall& call, int e) {
+  const int64_t all = call.places;
+  int64_t begin = call.offsets[e], end = e < call.experts ? call.offsets[e + 1] : all;
+  begin = begin < 0 ? 0 : (begin > all ? all : begin);
+  end = end < begin ? begin : (end > all ? all : end);
+  return Span{static_cast<int>(begin * call.inner), static_cast<int>(end * call.inner)};
+}
+
+// Tiles of `rows` rows of a segment; `empty`: an empty one has a tile too.
+__device__ __forceinline__ int tiles_of(const Span& span, int rows, bool empty) {
+  const int length = span.end - span.begin;
+  return length > 0 ? (length - 1) / rows + 1 : (empty ? 1 : 0);
+}
+
+// The segment that tile `tile` of tiles of `rows` rows belongs to, and the tile's
+// number in it; false behind the last.  A wave looks at 64 segments at a time.
+__device__ __forceinline__ bool find_tile(const ProductCall& call, int segments, int rows, bool empty, int tile, int& segment,
+                                          int& number, Span& span) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int first = 0; first < segments; first += 64) {
+    const int e = first + lane;
+    int count = 0;
+    Span mine{0, 0};
+    if (e < segments) {
+      mine = span_of(call, e);
+      count = tiles_of(mine, rows, empty);
+    }
+    int upto = count;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+      const int other = __shfl_up(upto, step, 64);
+      if (lane >= step) upto += other;
+    }
+    const uint64_t past = __ballot(before + upto > tile);
+    if (past != 0) {
+      const int found = __builtin_ctzll(past);
+      segment = first + found;
+      number = tile - before - __shfl(upto - count, found, 64);
+      span.begin = __shfl(mine.begin, found, 64);
+      span.end = __shfl(mine.end, found, 64);
+      segment = __builtin_amdgcn_readfirstlane(segment);
+      number = __builtin_amdgcn_readfirstlane(number);
+      span.begin = __builtin_amdgcn_readfirstlane(span.begin);
+      span.end = __builtin_amdgcn_readfirstlane(span.end);
+      return true;
+    }
+    before += __shfl(upto, 63, 64);
+  }
+  return false;
+}
+
+// The row of x that row `row` of the places is.
+__device__ __forceinline__ int64_t row_of_x(const ProductCall& call, int row) {
+  if (call.order == nullptr) return row;
+  int place = row, inside = 0;
+  if (call.inner > 1) {
+    place = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(call.inner));
+    inside = row - place * call.inner;
+  }
+  const int64_t slot = call.order[place];
+  // an order outside the slots reads row 0
+  const uint32_t token = static_cast<uint64_t>(slot) < static_cast<uint64_t>(call.places)
+                             ? static_cast<uint32_t>(slot) / static_cast<uint32_t>(call.k) : 0u;
+  return static_cast<int64_t>(token) * call.inner + inside;
+}
+
+// ---------------------------------------------------------------------------
+// operands
+// ---------------------------------------------------------------------------
+//
+// Along: LDS holds [rows][128 bytes of the summed index], a 16-byte piece c of row
+// r at c ^ (r / 2 mod 8): 16 rows' pieces of one number cover all 64 banks.
+// Across: LDS holds [slice rows][columns], 64-byte pieces of a row exchanged by
+// the row's number, so that four rows' pieces of 64 bytes lie in different banks;
+// 16-bit operands are read with the transposing LDS load.
+
+template <typename T>
+constexpr int kV = 16 / sizeof(T);           // elements of a piece
+template <typename T>
+constexpr int kSlice = 128 / sizeof(T);      // summed index of a slice
+
+__device__ __forceinline__ int along_byte(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) << 4); }
+
+template <typename T, int COLS>
+__device__ __forceinline__ int across_byte(int row, int byte) {
+  constexpr int kRow = COLS * static_cast<int>(sizeof(T));
+  if constexpr (sizeof(T) == 4) {
+    return row * kRow + (byte ^ (((row >> 2) & 1) << 7));
+  } else if constexpr (kRow >= 256) {
+    return row * kRow + (byte ^ ((row & 3) << 6));
+  } else {
+    return row * kRow + (byte ^ (((row >> 1) & 1) << 6));
+  }
+}
+
+// 16 bytes per lane as operands of the matrix unit: 32 rows (or columns) by 16
+// (16-bit) or 8 (float32) of the summed index, lane l holding row l mod 32.
+template <typename T>
+__device__ __forceinline__ f32x16 multiply(const u32x4& a, const u32x4& b, f32x16 sum) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), sum, 0, 0, 0);
+    return sum;
+  } else if constexpr (std::is_same<T, __bf16>::value) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), sum, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), sum, 0, 0, 0);
+  }
+}
+
+// Operand fragment `step` of a slice for the 32 rows from `row` on.
+template <typename T>
+__device__ __forceinline__ u32x4 along_fragment(const char* lds, int row, int step) {
+  const int lane = threadIdx.x & 63;
+  return *reinterpret_cast<const u32x4*>(lds + along_byte(row + (lane & 31), step * 2 + (lane >> 5)));
+}
+
+template <typename T, int COLS>
+__device__ __forceinline__ u32x4 across_fragment(const char* lds, int column, int step) {
+  const int lane = threadIdx.x & 63;
+  u32x4 out;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      out[j] = *reinterpret_cast<const uint32_t*>(lds + across_byte<T, COLS>(step * 8 + (lane >> 5) * 4 + j, (column + (lane & 31)) * 4));
+  } else {
+    // 16 lanes read four rows by 16 columns; lane c of them receives column c
+    const int from = column + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row = step * 16 + (lane >> 5) * 8 + half * 4 + ((lane >> 2) & 3);
+      const s16x4 part = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4*)(lds + across_byte<T, COLS>(row, from * 2)));
+      const uint64_t bits = __builtin_bit_cast(uint64_t, part);
+      out[half * 2] = static_cast<uint32_t>(bits);
+      out[half * 2 + 1] = static_cast<uint32_t>(bits >> 32);
+    }
+  }
+  return out;
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 load_piece(const T* __restrict__ p, int live, int64_t room) {
+  const Pack<T, kV<T>> raw = load_pack<T, kV<T>>(p, live, room);
+  u32x4 out;
+  __builtin_memcpy(&out, &raw, 16);
+  return out;
+}
+
+// ---------------------------------------------------------------------------
+// the tiled product
+// ---------------------------------------------------------------------------
+
+// BM by BN results by WM by WN waves.
+template <typename T, int MODE, int BM, int BN, int WM, int WN>
+struct Tile {
+  static constexpr int kThreads = WM * WN * 64;
+  static constexpr bool kAcrossA = MODE == kWeight, kAcrossB = MODE == kWeight || MODE == kInput;
+  static constexpr int kBytesA = BM * 128, kBytesB = BN * 128;   // of a slice
+  static constexpr int kPiecesA = kBytesA / 16 / kThreads, kPiecesB = kBytesB / 16 / kThreads;
+  static constexpr int kFragmentsM = BM / WM / 32, kFragmentsN = BN / WN / 32;
+  static constexpr int kSteps = 4;                               // of 32 bytes a slice
+  static_assert(kBytesA % (16 * kThreads) == 0 && kBytesB % (16 * kThreads) == 0, "whole pieces");
+};
+
+template <typename T, int MODE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductCall call, int columns, int tiles) {
+  typedef Tile<T, MODE, BM, BN, WM, WN> Z;
+  constexpr int V = kV<T>, S = kSlice<T>;
+  __shared__ __attribute__((aligned(16))) char lds[2][Z::kBytesA + Z::kBytesB];
+  const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
+
+  // which tile: neighbours share the segment's rows (and the expert's matrix), so
+  // each die takes a contiguous run of them
+  const int block = static_cast<int>(xcd_block(blockIdx.x, gridDim.x));
+  if (block >= tiles) return;
+  const int column_tile = block % columns, rest = block / columns;
+  int segment, number;
+  Span span;
+  int row_tile = 0, chunk = 0;
+  if constexpr (MODE == kWeight) {
+    const int row_tiles = (call.n_out + BM - 1) / BM;
+    row_tile = rest % row_tiles;
+    chunk = rest / row_tiles;
+    if (!find_tile(call, call.experts, call.chunk_rows, true, chunk, segment, number, span)) return;
+    span.begin += number * call.chunk_rows;
+    if (span.end - span.begin > call.chunk_rows) span.end = span.begin + call.chunk_rows;
+  } else {
+    const int segments = MODE == kInput && call.by_slot ? call.experts : call.experts + 1;
+    if (!find_tile(call, segments, BM, false, rest, segment, number, span)) return;
+  }
+  const int half = call.n_out / 2;                       // gated: where the second half starts
+  const int first_row = MODE == kWeight ? row_tile * BM : span.begin + number * BM;
+  const int live_rows = (MODE == kWeight ? call.n_out : span.end) - first_row;
+  const int first_column = column_tile * (MODE == kGated ? BN / 2 : BN);
+  const int width = MODE == kGated ? half : (MODE == kForward ? call.n_out : call.k_in);   // columns of the result
+  const int depth = MODE == kWeight ? span.end - span.begin : (MODE == kInput ? call.n_out : call.k_in);
+
+  if (MODE != kWeight && segment == call.experts) {      // rows of no expert: zeros
+    constexpr int kTileColumns = MODE == kGated ? BN / 2 : BN;
+    T* y = static_cast<T*>(call.out);
+    const int rows = live_rows < BM ? live_rows : BM;
+    for (int at = thread; at < rows * kTileColumns; at += Z::kThreads) {
+      const int c = first_column + at % kTileColumns;
+      if (c < width) y[static_cast<int64_t>(first_row + at / kTileColumns) * width + c] = static_cast<T>(0.0f);
+    }
+    return;
+  }
+
+  const T* a = static_cast<const T*>(call.a);
+  const T* b = static_cast<const T*>(call.b);
+  const int64_t matrix = static_cast<int64_t>(segment) * call.n_out * call.k_in;
+  const int64_t end_b = MODE == kWeight ? 0 : static_cast<int64_t>(call.experts) * call.n_out * call.k_in;
+
+  // this thread's pieces of a slice
+  const T* from_a[Z::kPiecesA];
+  const T* from_b[Z::kPiecesB];
+  int live_a[Z::kPiecesA], live_b[Z::kPiecesB];          // along: whether the row is there; across: elements of the piece
+  u32x4 next_a[Z::kPiecesA], next_b[Z::kPiecesB];
+  int64_t x_rows[MODE == kWeight ? Z::kPiecesB : 1];
+  const T* last_a = a;                                   // one past the last element that may be read
+  const T* last_b = b + end_b;
+  const int ld_a = MODE == kForward || MODE == kGated ? call.k_in : call.n_out;
+  if constexpr (MODE != kWeight) {
+    last_a = a + (MODE == kInput ? static_cast<int64_t>(call.places) * call.inner
+                                 : (call.order != nullptr ? call.places / call.k : call.places) * static_cast<int64_t>(call.inner)) * ld_a;
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesA; ++i) {
+      const int row = (thread + i * Z::kThreads) >> 3;
+      live_a[i] = row < live_rows;
+      from_a[i] = a;
+      if (row < live_rows) {
+        const int at = first_row + row;
+        from_a[i] = a + (MODE == kInput ? static_cast<int64_t>(at) : row_of_x(call, at)) * ld_a + (thread & 7) * V;
+      }
+    }
+  } else {
+    last_a = a + call.places * static_cast<int64_t>(call.inner) * call.n_out;
+    last_b = b + (call.order != nullptr ? call.places / call.k : call.places) * static_cast<int64_t>(call.inner) * call.k_in;
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesA; ++i) {
+      const int at = thread + i * Z::kThreads;
+      const int column = first_row + at % (BM / V) * V;
+      live_a[i] = call.n_out - column;
+      from_a[i] = a + static_cast<int64_t>(span.begin + at / (BM / V)) * call.n_out + column;
+    }
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesB; ++i) {
+      const int at = thread + i * Z::kThreads;
+      const int row = at / (BN / V);
+      live_b[i] = call.k_in - (first_column + at % (BN / V) * V);
+      x_rows[i] = row < depth ? row_of_x(call, span.begin + row) : 0;
+    }
+  }
+  if constexpr (MODE == kForward || MODE == kGated) {
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesB; ++i) {
+      const int row = (thread + i * Z::kThreads) >> 3;
+      int output = first_column + row;
+      bool there = output < call.n_out;
+      if constexpr (MODE == kGated) {                    // 32 gates, their 32 partners, 32 gates ...
+        const int column = first_column + (row >> 6) * 32 + (row & 31);
+        output = (row & 32) ? half + column : column;
+        there = column < half;
+      }
+      live_b[i] = there;
+      from_b[i] = there ? b + matrix + static_cast<int64_t>(output) * call.k_in + (thread & 7) * V : b;
+    }
+  } else if constexpr (MODE == kInput) {
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesB; ++i) {
+      const int at = thread + i * Z::kThreads;
+      const int column = first_column + at % (BN / V) * V;
+      live_b[i] = call.k_in - column;
+      from_b[i] = b + matrix + static_cast<int64_t>(at / (BN / V)) * call.k_in + column;
+    }
+  }
+
+  const auto fetch = [&](int slice) {
+    const int done = slice * S;
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesA; ++i) {
+      if constexpr (MODE != kWeight) {
+        const int left = live_a[i] ? depth - done - (thread & 7) * V : 0;
+        const T* p = from_a[i] + done;
+        next_a[i] = load_piece<T>(p, left, last_a - p);
+      } else {
+        const int row = done + (thread + i * Z::kThreads) / (BM / V);
+        const T* p = from_a[i] + static_cast<int64_t>(done) * call.n_out;
+        next_a[i] = load_piece<T>(p, row < depth ? live_a[i] : 0, last_a - p);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesB; ++i) {
+      if constexpr (MODE == kForward || MODE == kGated) {
+        const int left = live_b[i] ? depth - done - (thread & 7) * V : 0;
+        const T* p = from_b[i] + done;
+        next_b[i] = load_piece<T>(p, left, last_b - p);
+      } else if constexpr (MODE == kInput) {
+        const int row = done + (thread + i * Z::kThreads) / (BN / V);
+        const T* p = from_b[i] + static_cast<int64_t>(done) * call.k_in;
+        next_b[i] = load_piece<T>(p, row < depth ? live_b[i] : 0, last_b - p);
+      } else {
+        const int at = thread + i * Z::kThreads;
+        const int row = done + at / (BN / V);
+        const T* p = b + x_rows[i] * call.k_in + first_column + at % (BN / V) * V;
+        next_b[i] = load_piece<T>(p, row < depth ? live_b[i] : 0, last_b - p);
+        // where the next slice's rows are: a load of its own, started a slice ahead
+        x_rows[i] = row + S < depth ? row_of_x(call, span.begin + row + S) : 0;
+      }
+    }
+  };
+  const auto keep = [&](char* to) {
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesA; ++i) {
+      const int at = thread + i * Z::kThreads;
+      const int byte = Z::kAcrossA ? across_byte<T, BM>(at / (BM / V), at % (BM / V) * 16) : along_byte(at >> 3, at & 7);
+      *reinterpret_cast<u32x4*>(to + byte) = next_a[i];
+    }
+#pragma unroll
+    for (int i = 0; i < Z::kPiecesB; ++i) {
+      const int at = thread + i * Z::kThreads;
+      const int byte = Z::kAcrossB ? across_byte<T, BN>(at / (BN / V), at % (BN / V) * 16) : along_byte(at >> 3, at & 7);
+      *reinterpret_cast<u32x4*>(to + Z::kBytesA + byte) = next_b[i];
+    }
+  };
+
+  f32x16 sum[Z::kFragmentsM][Z::kFragmentsN];
+#pragma unroll
+  for (int m = 0; m < Z::kFragmentsM; ++m)
+#pragma unroll
+    for (int n = 0; n < Z::kFragmentsN; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[m][n][i] = 0.0f;
+
+  const int wave_row = (wave / WN) * (BM / WM), wave_column = (wave % WN) * (BN / WN);
+  const int slices = (depth + S - 1) / S;
+  if (slices > 0) {
+    fetch(0);
+    keep(lds[0]);
+  }
+  __syncthreads();
+  for (int slice = 0; slice < slices; ++slice) {
+    const char* at_a = lds[slice & 1];
+    const char* at_b = at_a + Z::kBytesA;
+    if (slice + 1 < slices) fetch(slice + 1);
+#pragma unroll
+    for (int step = 0; step < Z::kSteps; ++step) {
+      u32x4 fa[Z::kFragmentsM], fb[Z::kFragmentsN];
+#pragma unroll
+      for (int m = 0; m < Z::kFragmentsM; ++m) {
+        if constexpr (Z::kAcrossA) fa[m] = across_fragment<T, BM>(at_a, wave_row + m * 32, step);
+        else fa[m] = along_fragment<T>(at_a, wave_row + m * 32, step);
+      }
+#pragma unroll
+      for (int n = 0; n < Z::kFragmentsN; ++n) {
+        if constexpr (Z::kAcrossB) fb[n] = across_fragment<T, BN>(at_b, wave_column + n * 32, step);
+        else fb[n] = along_fragment<T>(at_b, wave_column + n * 32, step);
+      }
+#pragma unroll
+      for (int m = 0; m < Z::kFragmentsM; ++m)
+#pragma unroll
+        for (int n = 0; n < Z::kFragmentsN; ++n) sum[m][n] = multiply<T>(fa[m], fb[n], sum[m][n]);
+    }
+    if (slice + 1 < slices) keep(lds[(slice + 1) & 1]);
+    __syncthreads();
+  }
+
+  // register i of a lane: row 8 (i / 4) + 4 (lane / 32) + i mod 4, column lane mod 32
+  const bool partial = MODE == kWeight && call.chunks > 0;
+#pragma unroll
+  for (int m = 0; m < Z::kFragmentsM; ++m) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = wave_row + m * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+      if (row >= live_rows) continue;
+      int64_t out_row = first_row + row;
+      if constexpr (MODE == kInput) {
+        if (call.by_slot) {
+          const int place = static_cast<int>(static_cast<uint32_t>(out_row) / static_cast<uint32_t>(call.inner));
+          const int64_t slot = call.order[place];
+          if (static_cast<uint64_t>(slot) >= static_cast<uint64_t>(call.places)) continue;
+          out_row = slot * call.inner + (out_row - static_cast<int64_t>(place) * call.inner);
+        }
+      } else if constexpr (MODE == kWeight) {
+        out_row += static_cast<int64_t>(partial ? chunk : segment) * call.n_out;
+      }
+#pragma unroll
+      for (int n = 0; n < Z::kFragmentsN; ++n) {
+        if constexpr (MODE == kGated) {
+          if (n % 2 != 0) continue;
+          const int column = first_column + (wave_column >> 1) + (n / 2) * 32 + (lane & 31);
+          if (column >= half) continue;
+          const float gate = sum[m][n][i], up = sum[m][n + 1][i];
+          static_cast<T*>(call.out)[out_row * half + column] = static_cast<T>(gate * logistic(gate) * up);
+          if (call.before != nullptr) {
+            float* z = call.before + out_row * call.n_out;
+            z[column] = gate;
+            z[half + column] = up;
+          }
+        } else {
+          const int column = first_column + wave_column + n * 32 + (lane & 31);
+          if (column >= width) continue;
+          const int64_t at = out_row * width + column;
+          if (partial || (MODE == kInput && call.by_slot)) static_cast<float*>(call.out)[at] = sum[m][n][i];
+          else static_cast<T*>(call.out)[at] = static_cast<T>(sum[m][n][i]);
+        }
+      }
+    }
+  }
+}
+
+// dW[e] = the sum of its chunks' partial sums, in order, in 64 bits.
+template <typename T>
+__global__ __launch_bounds__(256) void weight_sum_kernel(ProductCall call, const float* __restrict__ partial, T* __restrict__ out,
+                                                         int blocks) {
+  const int e = blockIdx.x / blocks;
+  // the first chunk of the expert: chunks of the ones before
+  __shared__ int found[2];
+  if (threadIdx.x < 64) {
+    int before = 0, mine = 1;
+    for (int f = threadIdx.x; f <= e; f += 64) {
+      const Span span = span_of(call, f);
+      const int count = tiles_of(span, call.chunk_rows, true);
+      if (f < e) before += count;
+      else mine = count;
+    }
+    before = group_sum<64>(before);
+    if (threadIdx.x == 0) found[0] = before;
+    if (static_cast<int>(threadIdx.x) == e % 64) found[1] = mine;
+  }
+  __syncthreads();
+  const int64_t size = static_cast<int64_t>(call.n_out) * call.k_in;
+  const float* from = partial + found[0] * size;
+  const int count = found[1];
+  for (int64_t at = static_cast<int64_t>(blockIdx.x % blocks) * 256 + threadIdx.x; at < size; at += static_cast<int64_t>(blocks) * 256) {
+    double sum = 0.0;
+#pragma unroll 4
+    for (int c = 0; c < count; ++c) sum += static_cast<double>(from[c * size + at]);
+    out[e * size + at] = static_cast<T>(sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// elementwise parts
+// ---------------------------------------------------------------------------
+
+// dz of the gated SiLU; 16 bytes of dy a thread.  z comes in 32 bits: dz has to be
+// rounded to the operands' type for the products, and with z rounded as well the
+// gradients of bfloat16 were 1.8 times as far from their exact values as one
+// rounding puts them (1.4 times so).
+template <typename T>
+__global__ __launch_bounds__(256) void gate_backward_kernel(const T* __restrict__ dy, const float* __restrict__ z, T* __restrict__ dz,
+                                                            int64_t rows, int half) {
+  constexpr int V = kV<T>;
+  const int pieces = (half + V - 1) / V;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < rows * pieces; at += stride) {
+    const int64_t row = at / pieces;
+    const int column = static_cast<int>(at - row * pieces) * V;
+    const int live = half - column;
+    const float* gates = z + row * 2 * half + column;
+    const int64_t room = (rows - row) * half - column, room_z = (rows - row) * 2 * half - column;
+    const Pack<T, V> grad = load_pack<T, V>(dy + row * half + column, live, room);
+    const Pack<float, V> gate = load_pack<float, V>(gates, live, room_z);
+    const Pack<float, V> up = load_pack<float, V>(gates + half, live, room_z - half);
+    float of_gate[V], of_up[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float g = gate[j], d = static_cast<float>(grad[j]);
+      const float s = logistic(g);
+      of_gate[j] = d * up[j] * (s * fmaf(g, 1.0f - s, 1.0f));
+      of_up[j] = d * (g * s);
+    }
+    store_pack<T, V>(dz + row * 2 * half + column, of_gate, live);
+    store_pack<T, V>(dz + row * 2 * half + half + column, of_up, live);
+  }
+}
+
+// dx[t] = the sum over the token's slots that have a place, in slot order.
+template <typename T>
+__global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__ by_slot, const int64_t* __restrict__ places,
+                                                       T* __restrict__ dx, int64_t tokens, int k, int64_t size, int64_t limit) {
+  constexpr int V = kV<T>;
+  const int64_t pieces = (size + V - 1) / V;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < tokens * pieces; at += stride) {
+    const int64_t token = at / pieces;
+    const int64_t first = (at - token * pieces) * V;
+    const int live = static_cast<int>(size - first < V ? size - first : V);
+    float sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+    for (int j = 0; j < k; ++j) {
+      const int64_t slot = token * k + j;
+      if (static_cast<uint64_t>(places[slot]) >= static_cast<uint64_t>(limit)) continue;
+      const Pack<float, V> part = load_pack<float, V>(by_slot + slot * size + first, live, (tokens * k - slot) * size - first);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] += part[i];
+    }
+    store_pack<T, V>(dx + token * size + first, sum, live);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the weighted sum of a token's slots
+// ---------------------------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, const float* __restrict__ weights,
+                                                      const int64_t* __restrict__ places, T* __restrict__ out, int64_t tokens, int k,
+                                                      int64_t size, int64_t limit) {
+  constexpr int V = kV<T>;
+  const int64_t pieces = (size + V - 1) / V;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < tokens * pieces; at += stride) {
+    const int64_t token = at / pieces;
+    const int64_t first = (at - token * pieces) * V;
+    const int live = static_cast<int>(size - first < V ? size - first : V);
+    float sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+#pragma unroll 4
+    for (int j = 0; j < k; ++j) {
+      const int64_t place = places[token * k + j];
+      if (static_cast<uint64_t>(place) >= static_cast<uint64_t>(limit)) continue;
+      const float w = weights[token * k + j];
+      const Pack<T, V> part = load_pack<T, V>(y + place * size + first, live, (limit - place) * size - first);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] = fmaf(w, static_cast<float>(part[i]), sum[i]);
+    }
+    store_pack<T, V>(out + token * size + first, sum, live);
+  }
+}
+
+// dy[place] = w dout[t],  dw = the dot product of dout[t] and y[place].  L lanes a
+// token, whose slots they take in turn; behind the tokens, workgroups that clear
+// the places of no slot.
+template <typename T, int L>
+__global__ __launch_bounds__((L > 256 ? L : 256)) void combine_backward_kernel(
+    const T* __restrict__ dout, const T* __restrict__ y, const float* __restrict__ weights, const int64_t* __restrict__ places,
+    const int64_t* __restrict__ last, T* __restrict__ dy, float* __restrict__ dw, int64_t tokens, int k, int64_t size, int64_t limit,
+    int64_t token_blocks) {
+  constexpr int V = kV<T>;
+  constexpr int kGroups = 256 / L;
+  __shared__ float words[4];
+  const int64_t block = block_index();
+  const int64_t pieces = (size + V - 1) / V;
+  if (block >= token_blocks) {
+    if (dy == nullptr) return;
+    int64_t from = *last;
+    from = from < 0 ? 0 : (from > limit ? limit : from);
+    const int64_t clearing = 64, number = block - token_blocks;
+    if (number >= clearing) return;
+    for (int64_t at = from * size + number * 256 + threadIdx.x; at < limit * size; at += clearing * 256) dy[at] = static_cast<T>(0.0f);
+    return;
+  }
+  const int lane = threadIdx.x % L;
+  const int64_t token = block * kGroups + threadIdx.x / L;
+  const bool live_token = token < tokens;
+  for (int j = 0; j < k; ++j) {
+    const int64_t place = live_token ? places[token * k + j] : -1;
+    const bool held = static_cast<uint64_t>(place) < static_cast<uint64_t>(limit);
+    const float w = held ? weights[token * k + j] : 0.0f;
+    float dot = 0.0f;
+    if (held) {
+      for (int64_t piece = lane; piece < pieces; piece += L) {
+        const int64_t first = piece * V;
+        const int live = static_cast<int>(size - first < V ? size - first : V);
+        const Pack<T, V> grad = load_pack<T, V>(dout + token * size + first, live, (tokens - token) * size - first);
+        if (dw != nullptr) {
+          const Pack<T, V> row = load_pack<T, V>(y + place * size + first, live, (limit - place) * size - first);
+#pragma unroll
+          for (int i = 0; i < V; ++i) dot = fmaf(static_cast<float>(grad[i]), static_cast<float>(row[i]), dot);
+        }
+        if (dy != nullptr) {
+          float part[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) part[i] = w * static_cast<float>(grad[i]);
+          store_pack<T, V>(dy + place * size + first, part, live);
+        }
+      }
+    }
+    if (dw == nullptr) continue;
+    dot = group_sum<(L < 64 ? L : 64)>(dot);
+    if constexpr (L > 64) {
+      if ((threadIdx.x & 63) == 0) words[threadIdx.x / 64] = dot;
+      __syncthreads();
+      dot = (words[0] + words[1]) + (words[2] + words[3]);
+      __syncthreads();
+    }
+    if (lane == 0 && live_token) dw[token * k + j] = dot;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+int check_product(const char* what, int64_t places, int64_t k, int64_t inner, int64_t experts, int64_t k_in, int64_t n_out, int type) {
+  if (places < 0 || inner < 0) return fail(DPA4K_EINVAL, "%s: negative sizes", what);
+  if (experts < 1 || experts > kMaxExperts) return fail(DPA4K_EINVAL, "%s takes 1 to %d experts", what, kMaxExperts);
+  if (k < 1 || places % k != 0) return fail(DPA4K_EINVAL, "%s: the places must be k for each token", what);
+  if (k_in < 1 || n_out < 1 || k_in > (1 << 24) || n_out > (1 << 24)) return fail(DPA4K_EINVAL, "%s: channels must be 1 to 2^24", what);
+  if (!known_type(type)) return fail(DPA4K_EINVAL, "%s: unknown type", what);
+  // tiles of a row short of 2^31, whatever their number
+  if (inner > 0 && places > (INT32_MAX - 1024) / inner) return fail(DPA4K_EINVAL, "%s takes fewer than 2^31 rows", what);
+  return DPA4K_OK;
+}
+
+template <typename T, int MODE, int BM, int BN, int WM, int WN>
+int launch_product(const ProductCall& call, hipStream_t stream) {
+  typedef Tile<T, MODE, BM, BN, WM, WN> Z;
+  const int64_t rows = call.places * call.inner;
+  const int64_t width = MODE == kGated ? call.n_out / 2 : (MODE == kForward ? call.n_out : call.k_in);
+  const int64_t columns = (width + (MODE == kGated ? BN / 2 : BN) - 1) / (MODE == kGated ? BN / 2 : BN);
+  int64_t tiles;
+  if (MODE == kWeight) tiles = columns * ((call.n_out + BM - 1) / BM) * (call.chunks > 0 ? call.chunks : call.experts);
+  else tiles = columns * (rows / BM + call.experts + 1);
+  if (tiles > row_block_limit(Z::kThreads)) return fail(DPA4K_EINVAL, "expert linear: more tiles than a launch takes");
+  expert_product_kernel<T, MODE, BM, BN, WM, WN><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
+      call, static_cast<int>(columns), static_cast<int>(tiles));
+  return launched("expert_product_kernel");
+}
+
+template <typename T, int MODE>
+int run_product(const ProductCall& call, hipStream_t stream) {
+  const int64_t width = MODE == kForward || MODE == kGated ? call.n_out : call.k_in;
+  if constexpr (MODE == kWeight) {
+    if (call.n_out <= 64 || call.k_in <= 64) return launch_product<T, MODE, 64, 64, 2, 2>(call, stream);
+  } else {
+    if (width <= 64) return launch_product<T, MODE, 128, 64, 4, 1>(call, stream);
+  }
+  return launch_product<T, MODE, 128, 128, 2, 2>(call, stream);
+}
+
+// Rows of a segment that one workgroup of dW takes: all of them where the matrices
+// make tiles enough, else so few that about 1,024 workgroups have some.
+struct Chunks {
+  int rows, most;    // most == 0: no partial sums
+};
+
+Chunks weight_chunks(int64_t places, int64_t inner, int64_t experts, int64_t k_in, int64_t n_out) {
+  const int64_t rows = places * inner;
+  const int64_t edge = n_out <= 64 || k_in <= 64 ? 64 : 128;
+  const int64_t tiles = ((n_out + edge - 1) / edge) * ((k_in + edge - 1) / edge);
+  if (tiles * experts >= 512 || rows <= 512 * experts) return Chunks{INT_MAX, 0};
+  int64_t chunk = (rows * tiles + 1023) / 1024;
+  chunk = (chunk + 255) / 256 * 256;
+  return Chunks{static_cast<int>(chunk), static_cast<int>(rows / chunk + experts)};
+}
+
+int pieces_grid(int64_t pieces) {
+  const int64_t blocks = (pieces + 255) / 256;
+  return static_cast<int>(blocks < 8192 ? (blocks > 0 ? blocks : 1) : 8192);
+}
+
+}  // namespace
+}  // namespace dpa4k
+
+using namespace dpa4k;
+
+extern "C" int dpa4k_expert_linear_forward(const void* x, const void* weight, const int64_t* offsets, const int64_t* order, void* y,
+                                           float* before, int64_t places, int64_t k, int64_t inner, int64_t n_experts, int64_t k_in,
+                                           int64_t n_out, int gated, int type, dpa4k_stream_t stream) {
+  clear_error();
+  const int status = check_product("expert linear", places, k, inner, n_experts, k_in, n_out, type);
+  if (status != DPA4K_OK) return status;
+  if (gated && n_out % 2 != 0) return fail(DPA4K_EINVAL, "expert linear: a gate needs an even number of outputs");
+  if (places == 0 || inner == 0) return DPA4K_OK;
+  if (x == nullptr || weight == nullptr || offsets == nullptr || y == nullptr) return fail(DPA4K_EINVAL, "expert linear: null pointer");
+  ProductCall call{};
+  call.a = x, call.b = weight, call.out = y, call.before = before, call.offsets = offsets, call.order = order;
+  call.places = places, call.experts = static_cast<int>(n_experts), call.k = static_cast<int>(k), call.inner = static_cast<int>(inner);
+  call.k_in = static_cast<int>(k_in), call.n_out = static_cast<int>(n_out);
+  return with_type(type, DPA4K_EINVAL, [&](auto t) {
+    typedef typename decltype(t)::type T;
+    return gated ? run_product<T, kGated>(call, as_stream(stream)) : run_product<T, kForward>(call, as_stream(stream));
+  });
+}
+
+extern "C" int dpa4k_expert_gate_backward(const void* grad, const float* before, void* grad_before, int64_t rows, int64_t channels,
+                                          int type, dpa4k_stream_t stream) {
+  clear_error();
+  if (rows < 0 || channels < 1 || channels > (1 << 23)) return fail(DPA4K_EINVAL, "expert gate: bad sizes");
+  if (rows > INT32_MAX) return fail(DPA4K_EINVAL, "expert gate takes fewer than 2^31 rows");
+  if (!known_type(type)) return fail(DPA4K_EINVAL, "expert gate: unknown type");
+  if (rows == 0) return DPA4K_OK;
+  if (grad == nullptr || before == nullptr || grad_before == nullptr) return fail(DPA4K_EINVAL, "expert gate: null pointer");
+  return with_type(type, DPA4K_EINVAL, [&](auto t) {
+    typedef typename decltype(t)::type T;
+    const int grid = pieces_grid(rows * ((channels + kV<T> - 1) / kV<T>));
+    gate_backward_kernel<T><<<grid, 256, 0, as_stream(stream)>>>(static_cast<const T*>(grad), before,
+                                                                 static_cast<T*>(grad_before), rows, static_cast<int>(channels));
+    return launched("gate_backward_kernel");
+  });
+}
+
+extern "C" size_t dpa4k_expert_linear_workspace_size(int64_t places, int64_t k, int64_t inner, int64_t n_experts, int64_t k_in,
+                                                     int64_t n_out, int by_token, int want_x, int want_weight) {
+  if (places <= 0 || inner <= 0 || n_experts < 1 || k_in < 1 || n_out < 1 || places > INT32_MAX / inner) return 0;
+  size_t bytes = 0;
+  if (want_x && by_token) bytes = round_up_256(static_cast<size_t>(places * inner) * k_in * sizeof(float));
+  if (want_weight) {
+    const Chunks chunks = weight_chunks(places, inner, n_experts, k_in, n_out);
+    const size_t partial = round_up_256(static_cast<size_t>(chunks.most) * n_out * k_in * sizeof(float));
+    bytes = partial > bytes ? partial : bytes;    // one after the other
+  }
+  return bytes;
+}
+
+extern "C" int dpa4k_expert_linear_backward(const void* grad, const void* x, const void* weight, const int64_t* offsets,
+                                            const int64_t* order, const int64_t* slots, void* grad_x, void* grad_weight,
+                                            int64_t places, int64_t k, int64_t inner, int64_t n_experts, int64_t k_in, int64_t n_out,
+                                            int type, void* workspace, size_t workspace_bytes, dpa4k_stream_t stream) {
+  clear_error();
+  const int status = check_product("expert linear", places, k, inner, n_experts, k_in, n_out, type);
+  if (status != DPA4K_OK) return status;
+  const hipStream_t on = as_stream(stream);
+  const bool by_token = order != nullptr;
+  const bool nothing = places == 0 || inner == 0;
+  if (nothing) grad_x = nullptr;
+  if (grad_x == nullptr && grad_weight == nullptr) return DPA4K_OK;
+  if (offsets == nullptr || (!nothing && grad == nullptr) || (grad_x != nullptr && (weight == nullptr || (by_token && slots == nullptr))) ||
+      (grad_weight != nullptr && !nothing && x == nullptr))
+    return fail(DPA4K_EINVAL, "expert linear: null pointer");
+  const size_t needed = dpa4k_expert_linear_workspace_size(places, k, inner, n_experts, k_in, n_out, by_token, grad_x != nullptr,
+                                                           grad_weight != nullptr);
+  if (needed > 0 && (workspace == nullptr || workspace_bytes < needed))
+    return fail(DPA4K_EWORKSPACE, "expert linear: workspace too small");
+  ProductCall call{};
+  call.offsets = offsets, call.order = order;
+  call.places = places, call.experts = static_cast<int>(n_experts), call.k = static_cast<int>(k), call.inner = static_cast<int>(inner);
+  call.k_in = static_cast<int>(k_in), call.n_out = static_cast<int>(n_out);
+  return with_type(type, DPA4K_EINVAL, [&](auto t) {
+    typedef typename decltype(t)::type T;
+    if (grad_x != nullptr) {
+      ProductCall of_x = call;
+      of_x.a = grad, of_x.b = weight, of_x.out = by_token ? workspace : grad_x, of_x.by_slot = by_token;
+      int ran = run_product<T, kInput>(of_x, on);
+      if (ran != DPA4K_OK) return ran;
+      if (by_token) {
+        const int64_t tokens = places / k, size = inner * k_in;
+        slot_sum_kernel<T><<<pieces_grid(tokens * ((size + kV<T> - 1) / kV<T>)), 256, 0, on>>>(
+            static_cast<const float*>(workspace), slots, static_cast<T*>(grad_x), tokens, static_cast<int>(k), size, places);
+        ran = launched("slot_sum_kernel");
+        if (ran != DPA4K_OK) return ran;
+      }
+    }
+    if (grad_weight != nullptr) {
+      ProductCall of_w = call;
+      const Chunks chunks = weight_chunks(places, inner, n_experts, k_in, n_out);
+      of_w.a = grad, of_w.b = x, of_w.chunk_rows = chunks.rows, of_w.chunks = chunks.most;
+      of_w.out = chunks.most > 0 ? workspace : grad_weight;
+      int ran = run_product<T, kWeight>(of_w, on);
+      if (ran != DPA4K_OK || chunks.most == 0) return ran;
+      const int64_t size = k_in * n_out;
+      const int64_t blocks = (size + 255) / 256 < 64 ? (size + 255) / 256 : 64;
+      weight_sum_kernel<T><<<static_cast<unsigned int>(blocks * n_experts), 256, 0, on>>>(
+          of_w, static_cast<const float*>(workspace), static_cast<T*>(grad_weight), static_cast<int>(blocks));
+      return launched("weight_sum_kernel");
+    }
+    return static_cast<int>(DPA4K_OK);
+  });
+}
+
+extern "C" int dpa4k_expert_combine_forward(const void* y, const float* weights, const int64_t* slots, void* out, int64_t tokens,
+                                            int64_t k, int64_t size, int type, dpa4k_stream_t stream) {
+  clear_error();
+  if (tokens < 0 || k < 1 || size < 0) return fail(DPA4K_EINVAL, "expert combine: bad sizes");
+  if (!known_type(type)) return fail(DPA4K_EINVAL, "expert combine: unknown type");
+  if (tokens > INT32_MAX / k) return fail(DPA4K_EINVAL, "expert combine takes fewer than 2^31 slots");
+  if (size > INT32_MAX) return fail(DPA4K_EINVAL, "expert combine: an entry has fewer than 2^31 elements");
+  if (tokens == 0 || size == 0) return DPA4K_OK;
+  if (y == nullptr || weights == nullptr || slots == nullptr || out == nullptr) return fail(DPA4K_EINVAL, "expert combine: null pointer");
+  return with_type(type, DPA4K_EINVAL, [&](auto t) {
+    typedef typename decltype(t)::type T;
+    combine_kernel<T><<<pieces_grid(tokens * ((size + kV<T> - 1) / kV<T>)), 256, 0, as_stream(stream)>>>(
+        static_cast<const T*>(y), weights, slots, static_cast<T*>(out), tokens, static_cast<int>(k), size, tokens * k);
+    return launched("combine_kernel");
+  });
+}
+
+extern "C" int dpa4k_expert_combine_backward(const void* grad, const void* y, const float* weights, const int64_t* slots,
+                                             const int64_t* last_offset, void* grad_y, float* grad_weights, int64_t tokens, int64_t k,
+                                             int64_t size, int type, dpa4k_stream_t stream) {
+  clear_error();
+  if (tokens < 0 || k < 1 || size < 0) return fail(DPA4K_EINVAL, "expert combine: bad sizes");
+  if (!known_type(type)) return fail(DPA4K_EINVAL, "expert combine: unknown type");
+  if (tokens > INT32_MAX / k) return fail(DPA4K_EINVAL, "expert combine takes fewer than 2^31 slots");
+  if (size > INT32_MAX) return fail(DPA4K_EINVAL, "expert combine: an entry has fewer than 2^31 elements");
+  if (tokens == 0) return DPA4K_OK;
+  if (slots == nullptr || weights == nullptr || (size > 0 && (grad == nullptr || y == nullptr)) ||
+      (grad_y != nullptr && last_offset == nullptr))
+    return fail(DPA4K_EINVAL, "expert combine: null pointer");
+  return with_type(type, DPA4K_EINVAL, [&](auto t) {
+    typedef typename decltype(t)::type T;
+    const int64_t pieces = (size + kV<T> - 1) / kV<T>;
+    const auto run = [&](auto l) {
+      constexpr int L = l.value;
+      const int64_t blocks = (tokens + 256 / L - 1) / (256 / L);
+      combine_backward_kernel<T, L><<<launch_grid(blocks + 64, 256), 256, 0, as_stream(stream)>>>(
+          static_cast<const T*>(grad), static_cast<const T*>(y), weights, slots, last_offset, static_cast<T*>(grad_y), grad_weights,
+          tokens, static_cast<int>(k), size, tokens * k, blocks);
+      return launched("combine_backward_kernel");
+    };
+    if (pieces <= 16) return run(std::integral_constant<int, 16>{});
+    if (pieces <= 256) return run(std::integral_constant<int, 64>{});
+    return run(std::integral_constant<int, 256>{});
+  });
+}

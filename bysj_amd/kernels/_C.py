@@ -19,11 +19,13 @@ inputs; ``segment_offsets``, ``group_by_key``, ``gie_group`` and the
 ``gie_rmsnorm_forward_csr`` is the fused GIE -> RMSNorm forward;
 ``edge_stream_combine`` is the fused edge-stream elementwise chain;
 ``group_norm_forward/backward``, ``grad_norm`` and the ``adamw_*`` entry
-points are the operators of a training step.
+points are the operators of a training step; ``residual_norm_*`` and
+``expert_*`` those of a feed-forward block with experts.
 """
 from __future__ import annotations
 
 import ctypes
+import math
 import operator
 import weakref
 from array import array
@@ -941,6 +943,158 @@ def group_norm_backward(grad_output, x, groups, scale, bias, offsets, statistics
             code, _ptr(workspace), nbytes, stream)
     _lib.check(status)
     return grad_x, grad_scale, grad_bias
+
+
+# ---------------------------------------------------------------------------
+# a feed-forward block with experts (no reference implementation)
+# ---------------------------------------------------------------------------
+
+# The callers (kernels.block_norm, kernels.experts) have checked dtypes, shapes and devices.
+
+def residual_norm_forward(x, residual, gate, post_scale, residual_scale, pre_scale, options, keep: bool):
+    """``(h, y, post_rstd, pre_rstd)``; y is None without the second norm, the rstds where not kept.
+
+    ``options``: ``(rows, channels, factor, eps, post_norm, pre_norm, gate_kind, gate_activation)``.
+    """
+    rows, channels, factor, eps, post_norm, pre_norm, gate_kind, activation = options
+    device = x.device
+    h = torch.empty_like(residual)
+    y = torch.empty_like(x) if pre_norm else None
+    rstd = torch.empty((2, rows), dtype=torch.float32, device=device) if keep else None
+    at = rstd.data_ptr() if keep else 0
+    with _on(device) as stream:
+        status = _LIB.dpa4k_residual_norm_forward(
+            _ptr(x), _ptr(residual), _ptr(gate), _ptr(post_scale), _ptr(residual_scale), _ptr(pre_scale), _ptr(h), _ptr(y),
+            at or None, at + 4 * rows if keep else None, rows, channels, factor, eps, post_norm, pre_norm, gate_kind, activation,
+            ELEMENT_TYPES[x.dtype], ELEMENT_TYPES[residual.dtype], stream)
+    _lib.check(status)
+    return h, y, rstd
+
+
+def residual_norm_backward(grad_h, grad_y, x, residual, gate, post_scale, residual_scale, pre_scale, rstd, options, want):
+    """Gradients of ``(x, residual, gate, post_scale, residual_scale, pre_scale)``, None where ``want`` is false."""
+    rows, channels, factor, _, post_norm, pre_norm, gate_kind, activation = options
+    device = x.device
+    grads = [torch.empty_like(t) if t is not None and wanted else None
+             for t, wanted in zip((x, residual, gate, post_scale, residual_scale, pre_scale), want)]
+    dx, dresidual, dgate, dpost, dscale, dpre = grads
+    nbytes = 0
+    if dpost is not None or dscale is not None or dpre is not None:
+        nbytes = _LIB.dpa4k_residual_norm_workspace_size(rows, channels)
+    workspace = _workspace(nbytes, device) if nbytes else None
+    at = rstd.data_ptr()
+    with _on(device) as stream:
+        status = _LIB.dpa4k_residual_norm_backward(
+            _ptr(grad_h), _ptr(grad_y), _ptr(x), _ptr(residual), _ptr(gate), _ptr(post_scale), _ptr(residual_scale),
+            _ptr(pre_scale), at or None, at + 4 * rows if rows else None, _ptr(dx), _ptr(dresidual), _ptr(dgate), _ptr(dpost),
+            _ptr(dpre), _ptr(dscale), rows, channels, factor, post_norm, pre_norm, gate_kind, activation, ELEMENT_TYPES[x.dtype],
+            ELEMENT_TYPES[residual.dtype], _ptr(workspace), nbytes, stream)
+    _lib.check(status)
+    return grads
+
+
+def expert_route_forward(logits, bias, options, keep: bool):
+    """``(weights, experts, statistics)``; ``options``: ``(k, groups, top_groups, scores, normalize, scale)``."""
+    k, groups, top_groups, scores, normalize, scale = options
+    tokens, n_experts = logits.shape
+    device = logits.device
+    weights = torch.empty((tokens, k), dtype=torch.float32, device=device)
+    experts = torch.empty((tokens, k), dtype=torch.int64, device=device)
+    statistics = torch.empty((2, tokens), dtype=torch.float32, device=device) if keep else None
+    with _on(device) as stream:
+        status = _LIB.dpa4k_expert_route_forward(
+            _ptr(logits), _ptr(bias), _ptr(weights), _ptr(experts), _ptr(statistics), tokens, n_experts, k, groups, top_groups,
+            scores, normalize, scale, ELEMENT_TYPES[logits.dtype], stream)
+    _lib.check(status)
+    return weights, experts, statistics
+
+
+def expert_route_backward(grad_weights, logits, experts, statistics, options):
+    k, _, _, scores, normalize, scale = options
+    tokens, n_experts = logits.shape
+    grad_logits = torch.empty_like(logits)
+    with _on(logits.device) as stream:
+        status = _LIB.dpa4k_expert_route_backward(
+            _ptr(grad_weights), _ptr(logits), _ptr(experts), _ptr(statistics), _ptr(grad_logits), tokens, n_experts, k, scores,
+            normalize, scale, ELEMENT_TYPES[logits.dtype], stream)
+    _lib.check(status)
+    return grad_logits
+
+
+def expert_dispatch(experts, n_experts: int):
+    """``(offsets, order, slots)`` of ``experts`` (tokens, k); never synchronises."""
+    slots, device = experts.numel(), experts.device
+    offsets = torch.empty((n_experts + 1,), dtype=torch.int64, device=device)
+    order = torch.empty((slots,), dtype=torch.int64, device=device)
+    places = torch.empty_like(experts)
+    nbytes = _LIB.dpa4k_expert_dispatch_workspace_size(slots, n_experts)
+    workspace = _workspace(nbytes, device) if nbytes else None
+    with _on(device) as stream:
+        status = _LIB.dpa4k_expert_dispatch(_ptr(experts), slots, n_experts, offsets.data_ptr(), _ptr(order), _ptr(places),
+                                            _ptr(workspace), nbytes, stream)
+    _lib.check(status)
+    return offsets, order, places
+
+
+def expert_linear_forward(x, weight, offsets, order, sizes, gated: bool, keep: bool):
+    """``(y, before)``; ``sizes``: ``(places, k, inner)``; ``order`` None: x by place.  ``before`` (float32) is kept with a gate."""
+    places, k, inner = sizes
+    n_experts, n_out, k_in = weight.shape
+    device, middle = x.device, x.shape[1:-1]
+    y = torch.empty((places, *middle, n_out // 2 if gated else n_out), dtype=x.dtype, device=device)
+    before = torch.empty((places, *middle, n_out), dtype=torch.float32, device=device) if gated and keep else None
+    with _on(device) as stream:
+        status = _LIB.dpa4k_expert_linear_forward(
+            _ptr(x), _ptr(weight), offsets.data_ptr(), _ptr(order), _ptr(y), _ptr(before), places, k, inner, n_experts, k_in,
+            n_out, gated, ELEMENT_TYPES[x.dtype], stream)
+    _lib.check(status)
+    return y, before
+
+
+def expert_linear_backward(grad, x, weight, before, offsets, order, slots, sizes, want_x: bool, want_weight: bool):
+    """``(grad_x, grad_weight)``, None where not wanted; ``before``: what a gated forward kept, else None."""
+    places, k, inner = sizes
+    n_experts, n_out, k_in = weight.shape
+    device, code = x.device, ELEMENT_TYPES[x.dtype]
+    grad_x = torch.empty_like(x) if want_x else None
+    grad_weight = torch.empty_like(weight) if want_weight else None
+    nbytes = _LIB.dpa4k_expert_linear_workspace_size(places, k, inner, n_experts, k_in, n_out, order is not None, want_x, want_weight)
+    workspace = _workspace(nbytes, device) if nbytes else None
+    with _on(device) as stream:
+        if before is not None:
+            grad_before = torch.empty(before.shape, dtype=x.dtype, device=device)
+            _lib.check(_LIB.dpa4k_expert_gate_backward(_ptr(grad), _ptr(before), _ptr(grad_before), places * inner, n_out // 2, code,
+                                                       stream))
+            grad = grad_before
+        status = _LIB.dpa4k_expert_linear_backward(
+            _ptr(grad), _ptr(x), _ptr(weight), offsets.data_ptr(), _ptr(order), _ptr(slots), _ptr(grad_x), _ptr(grad_weight),
+            places, k, inner, n_experts, k_in, n_out, code, _ptr(workspace), nbytes, stream)
+    _lib.check(status)
+    return grad_x, grad_weight
+
+
+def expert_combine_forward(y, weights, slots):
+    tokens, k = weights.shape
+    size = math.prod(y.shape[1:])
+    out = torch.empty((tokens, *y.shape[1:]), dtype=y.dtype, device=y.device)
+    with _on(y.device) as stream:
+        status = _LIB.dpa4k_expert_combine_forward(_ptr(y), _ptr(weights), _ptr(slots), _ptr(out), tokens, k, size,
+                                                   ELEMENT_TYPES[y.dtype], stream)
+    _lib.check(status)
+    return out
+
+
+def expert_combine_backward(grad, y, weights, offsets, slots, want_y: bool, want_weights: bool):
+    tokens, k = weights.shape
+    size = math.prod(y.shape[1:])
+    grad_y = torch.empty_like(y) if want_y else None
+    grad_weights = torch.empty_like(weights) if want_weights else None
+    with _on(y.device) as stream:
+        status = _LIB.dpa4k_expert_combine_backward(
+            _ptr(grad), _ptr(y), _ptr(weights), _ptr(slots), offsets.data_ptr() + 8 * (offsets.numel() - 1), _ptr(grad_y),
+            _ptr(grad_weights), tokens, k, size, ELEMENT_TYPES[y.dtype], stream)
+    _lib.check(status)
+    return grad_y, grad_weights
 
 
 # ---------------------------------------------------------------------------

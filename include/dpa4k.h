@@ -61,7 +61,7 @@ const char* dpa4k_last_error(void);
 
 /* ABI version of this header (bumped on any signature change). */
 int dpa4k_abi_version(void);
-#define DPA4K_ABI_VERSION 11
+#define DPA4K_ABI_VERSION 12
 
 /* ------------------------------------------------------------------------
  * CSR construction
@@ -575,6 +575,151 @@ int dpa4k_group_norm_backward(const void* grad, const void* x,
                               int64_t max_entries, int silu, int type,
                               void* workspace, size_t workspace_bytes,
                               dpa4k_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Norms around a block, gate and residual sum (no reference counterpart)
+ * ---------------------------------------------------------------------- */
+
+/* x, y, gate[rows, C] of `type`, residual, h[rows, C] of `residual_type` (the
+ * same or DPA4K_TYPE_F32).  Over each row
+ *   a = x post_scale / sqrt(mean x^2 + eps)   (a = x without post_norm)
+ *   h = residual + s act(gate) a
+ *   y = h pre_scale / sqrt(mean h^2 + eps)    (not written without pre_norm)
+ * gate_kind: 0 no gate, 1 gate[rows, C], 2 gate[rows]; gate_activation: 0 none,
+ * 1 sigmoid, 2 SiLU.  s is residual_scale[C] where given, else residual_factor.
+ * The scales are float[C] or NULL (1).  post_rstd, pre_rstd[rows] are kept for
+ * the backward (NULL: not kept).  Sums in 32 bits; y is of the unrounded h.
+ * 1 <= C <= DPA4K_RESIDUAL_NORM_MAX_CHANNELS; eps finite and > 0.  Tensors may
+ * start at any element. */
+#define DPA4K_RESIDUAL_NORM_MAX_CHANNELS 8192
+int dpa4k_residual_norm_forward(const void* x, const void* residual,
+                                const void* gate, const float* post_scale,
+                                const float* residual_scale,
+                                const float* pre_scale, void* h, void* y,
+                                float* post_rstd, float* pre_rstd, int64_t rows,
+                                int64_t channels, float residual_factor,
+                                float eps, int post_norm, int pre_norm,
+                                int gate_kind, int gate_activation, int type,
+                                int residual_type, dpa4k_stream_t stream);
+
+/* Gradients of every input from grad_h (like h) and grad_y (like y); either may
+ * be NULL, and so may any output.  The gradients of the scales are float[C],
+ * summed over all rows in a fixed order, in 64 bits past 256 rows a workgroup;
+ * they alone need the workspace. */
+size_t dpa4k_residual_norm_workspace_size(int64_t rows, int64_t channels);
+int dpa4k_residual_norm_backward(const void* grad_h, const void* grad_y,
+                                 const void* x, const void* residual,
+                                 const void* gate, const float* post_scale,
+                                 const float* residual_scale,
+                                 const float* pre_scale, const float* post_rstd,
+                                 const float* pre_rstd, void* grad_x,
+                                 void* grad_residual, void* grad_gate,
+                                 float* grad_post_scale, float* grad_pre_scale,
+                                 float* grad_residual_scale, int64_t rows,
+                                 int64_t channels, float residual_factor,
+                                 int post_norm, int pre_norm, int gate_kind,
+                                 int gate_activation, int type,
+                                 int residual_type, void* workspace,
+                                 size_t workspace_bytes, dpa4k_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Experts (no reference counterpart)
+ * ---------------------------------------------------------------------- */
+
+/* The k best of a token's experts and their weights.  logits[T, E] of `type`,
+ * bias[E] or NULL, weights float[T, k], experts[T, k].
+ *   s = softmax(l) (scores 0) or 1 / (1 + exp(-l)) (scores 1), in 32 bits
+ *   ranked by s + bias, in 64 bits; without a bias and groups by l
+ *   groups of E / groups neighbours: the top_groups groups with the largest sum
+ *   of their two best keys take part (one key where a group has one)
+ *   weights = scale s / (sum of the chosen s + 1e-20), or scale s
+ * Equal keys go to the lowest index, and the chosen are in the order of their
+ * keys.  A logit of -inf (or a bias of -inf) takes an expert out; where fewer
+ * than k are left, the last entries are expert -1 with weight 0.  A NaN ranks
+ * behind every other key.  statistics float[2, T] are kept for the backward of
+ * softmax scores (NULL: not kept).  E <= DPA4K_EXPERTS_MAX, groups <=
+ * DPA4K_EXPERT_GROUPS_MAX, T k < 2^31. */
+#define DPA4K_EXPERTS_MAX 1024
+#define DPA4K_EXPERT_GROUPS_MAX 64
+int dpa4k_expert_route_forward(const void* logits, const float* bias,
+                               float* weights, int64_t* experts,
+                               float* statistics, int64_t tokens,
+                               int64_t n_experts, int64_t k, int64_t groups,
+                               int64_t top_groups, int scores, int normalize,
+                               float scale, int type, dpa4k_stream_t stream);
+
+/* grad_logits[T, E] of `type` from grad_weights float[T, k]; the choice itself
+ * has no gradient, nor has the bias. */
+int dpa4k_expert_route_backward(const float* grad_weights, const void* logits,
+                                const int64_t* experts, const float* statistics,
+                                void* grad_logits, int64_t tokens,
+                                int64_t n_experts, int64_t k, int scores,
+                                int normalize, float scale, int type,
+                                dpa4k_stream_t stream);
+
+/* The CSR of slots by expert: experts[slots] -> offsets[E + 1], order[slots]
+ * (the slot at each place, in slot order inside an expert), places[slots] (its
+ * inverse).  Slots whose expert is outside [0, E) have place -1; there are
+ * offsets[E] places, and order is -1 behind them.  Never synchronises. */
+size_t dpa4k_expert_dispatch_workspace_size(int64_t slots, int64_t n_experts);
+int dpa4k_expert_dispatch(const int64_t* experts, int64_t slots,
+                          int64_t n_experts, int64_t* offsets, int64_t* order,
+                          int64_t* places, void* workspace,
+                          size_t workspace_bytes, dpa4k_stream_t stream);
+
+/* z[p, i] = weight[e] x[entry(p), i] for the places p of expert e and the rows
+ * 0 <= i < inner of an entry; entry(p) is order[p] / k, or p where order is
+ * NULL.  x[places / k or places, inner, k_in], weight[E, n_out, k_in],
+ * y[places, inner, n_out].  gated: y[places, inner, n_out / 2] =
+ * silu(z[.., :n_out / 2]) z[.., n_out / 2:], and z itself to float
+ * `before`[places, inner, n_out] unless that is NULL.  Rows behind
+ * offsets[E] become 0 in y and are not written in `before`.  Products are
+ * summed in 32 bits.  places * inner < 2^31 - 1024. */
+int dpa4k_expert_linear_forward(const void* x, const void* weight,
+                                const int64_t* offsets, const int64_t* order,
+                                void* y, float* before, int64_t places, int64_t k,
+                                int64_t inner, int64_t n_experts, int64_t k_in,
+                                int64_t n_out, int gated, int type,
+                                dpa4k_stream_t stream);
+
+/* dz of the gated SiLU: grad[rows, C] and grad_before[rows, 2 C] of `type`,
+ * before float[rows, 2 C]. */
+int dpa4k_expert_gate_backward(const void* grad, const float* before,
+                               void* grad_before, int64_t rows, int64_t channels,
+                               int type, dpa4k_stream_t stream);
+
+/* grad[places, inner, n_out] is that of z.  grad_x like x: with order, the sum
+ * in 32 bits over the places of a token (slots[places] as places of
+ * dpa4k_expert_dispatch); without, rows behind offsets[E] become 0.
+ * grad_weight like weight, 0 for an expert without places.  Either may be NULL. */
+size_t dpa4k_expert_linear_workspace_size(int64_t places, int64_t k,
+                                          int64_t inner, int64_t n_experts,
+                                          int64_t k_in, int64_t n_out,
+                                          int by_token, int want_x,
+                                          int want_weight);
+int dpa4k_expert_linear_backward(const void* grad, const void* x,
+                                 const void* weight, const int64_t* offsets,
+                                 const int64_t* order, const int64_t* slots,
+                                 void* grad_x, void* grad_weight, int64_t places,
+                                 int64_t k, int64_t inner, int64_t n_experts,
+                                 int64_t k_in, int64_t n_out, int type,
+                                 void* workspace, size_t workspace_bytes,
+                                 dpa4k_stream_t stream);
+
+/* out[t] = sum_j weights[t, j] y[slots[t, j]] over entries of `size` elements of
+ * `type`, summed in 32 bits in order; a slot of -1 adds nothing.  y has T k
+ * entries.  backward: grad_y[slots[t, j]] = weights[t, j] grad[t], entries from
+ * *last_offset (device, offsets[E]) on become 0; grad_weights[t, j] = the dot
+ * product of grad[t] and y[slots[t, j]], 0 without a place.  Either may be NULL. */
+int dpa4k_expert_combine_forward(const void* y, const float* weights,
+                                 const int64_t* slots, void* out, int64_t tokens,
+                                 int64_t k, int64_t size, int type,
+                                 dpa4k_stream_t stream);
+int dpa4k_expert_combine_backward(const void* grad, const void* y,
+                                  const float* weights, const int64_t* slots,
+                                  const int64_t* last_offset, void* grad_y,
+                                  float* grad_weights, int64_t tokens, int64_t k,
+                                  int64_t size, int type, dpa4k_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Optimiser step (no reference counterpart)
