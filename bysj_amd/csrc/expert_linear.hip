@@ -25,6 +25,13 @@
 
 #include "elements.h"
 
+#ifndef BIG_WM
+#define BIG_WM 2
+#define BIG_WN 4
+#endif
+#ifndef USE_BIG
+#define USE_BIG 1
+#endif
 namespace dpa4k {
 namespace {
 
@@ -115,30 +122,40 @@ __device__ __forceinline__ bool find_tile(const ProductCall& call, int segments,
   return false;
 }
 
-// The row of x that row `row` of the places is.
-__device__ __forceinline__ int64_t row_of_x(const ProductCall& call, int row) {
-  if (call.order == nullptr) return row;
-  int place = row, inside = 0;
-  if (call.inner > 1) {
-    place = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(call.inner));
-    inside = row - place * call.inner;
-  }
-  const int64_t slot = call.order[place];
-  // an order outside the slots reads row 0
-  const uint32_t token = static_cast<uint64_t>(slot) < static_cast<uint64_t>(call.places)
-                             ? static_cast<uint32_t>(slot) / static_cast<uint32_t>(call.k) : 0u;
-  return static_cast<int64_t>(token) * call.inner + inside;
+// The row of x that row `row` of the places is, in two halves, so that a loop can
+// start the load of the slot long before it needs the row.
+struct PlaceRow {
+  int64_t slot;
+  int inside;    // the row of the entry; without an order `slot` is the row itself
+};
+
+__device__ __forceinline__ PlaceRow place_row(const ProductCall& call, int row) {
+  if (call.order == nullptr) return PlaceRow{row, 0};
+  if (call.inner == 1) return PlaceRow{call.order[row], 0};
+  const int place = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(call.inner));
+  return PlaceRow{call.order[place], row - place * call.inner};
+}
+
+__device__ __forceinline__ int64_t row_of_x(const ProductCall& call, const PlaceRow& at) {
+  if (call.order == nullptr) return at.slot;
+  // an order outside the slots reads token 0
+  const uint32_t token = static_cast<uint64_t>(at.slot) < static_cast<uint64_t>(call.places)
+                             ? static_cast<uint32_t>(at.slot) / static_cast<uint32_t>(call.k) : 0u;
+  return static_cast<int64_t>(token) * call.inner + at.inside;
 }
 
 // ---------------------------------------------------------------------------
 // operands
 // ---------------------------------------------------------------------------
 //
-// Along: LDS holds [rows][128 bytes of the summed index], a 16-byte piece c of row
-// r at c ^ (r / 2 mod 8): 16 rows' pieces of one number cover all 64 banks.
-// Across: LDS holds [slice rows][columns], 64-byte pieces of a row exchanged by
-// the row's number, so that four rows' pieces of 64 bytes lie in different banks;
-// 16-bit operands are read with the transposing LDS load.
+// Along: LDS holds [rows][128 bytes of the summed index], piece c of 16 bytes of row
+// r at place c ^ (r / 2 mod 8): 16 rows' pieces of one number cover all 64 banks.
+// Across: LDS holds [slice rows][columns], with the 64-byte (float32: 128-byte) parts
+// of a row exchanged by the row's number, so that the rows that are read together
+// lie in different banks; 16-bit operands are read with the transposing LDS load.
+// Thread t of a workgroup fills the 16 bytes t, t + threads, ... of a slice in
+// order, as loads that go to LDS without registers do; what is exchanged is which
+// piece it loads.
 
 template <typename T>
 constexpr int kV = 16 / sizeof(T);           // elements of a piece
@@ -157,6 +174,14 @@ __device__ __forceinline__ int across_byte(int row, int byte) {
   } else {
     return row * kRow + (byte ^ (((row >> 1) & 1) << 6));
   }
+}
+
+// The piece of its row that lies at 16 bytes number `at` of a slice.
+template <typename T, int COLS>
+__device__ __forceinline__ int across_piece(int at) {
+  constexpr int kPerRow = COLS / kV<T>;
+  const int row = at / kPerRow;
+  return (across_byte<T, COLS>(row, (at % kPerRow) * 16) - row * kPerRow * 16) / 16;
 }
 
 // 16 bytes per lane as operands of the matrix unit: 32 rows (or columns) by 16
@@ -205,6 +230,15 @@ __device__ __forceinline__ u32x4 across_fragment(const char* lds, int column, in
   return out;
 }
 
+// 64 lanes' 16 bytes of a buffer view to 1,024 consecutive bytes of LDS from `to` (the
+// same in every lane) on; zeros from offsets past the end of the view.
+__device__ __forceinline__ void load_to_lds(BufferView view, uint32_t offset, char* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(view, (__attribute__((address_space(3))) void*)to, 16, static_cast<int>(offset), 0, 0, 0);
+}
+
+// s_waitcnt vmcnt(0), any number of other operations left.
+constexpr int kNoLoadsLeft = 0x0f70;
+
 template <typename T>
 __device__ __forceinline__ u32x4 load_piece(const T* __restrict__ p, int live, int64_t room) {
   const Pack<T, kV<T>> raw = load_pack<T, kV<T>>(p, live, room);
@@ -229,11 +263,16 @@ struct Tile {
   static_assert(kBytesA % (16 * kThreads) == 0 && kBytesB % (16 * kThreads) == 0, "whole pieces");
 };
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, bool WHOLE>
 __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductCall call, int columns, int tiles) {
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   constexpr int V = kV<T>, S = kSlice<T>;
-  __shared__ __attribute__((aligned(16))) char lds[2][Z::kBytesA + Z::kBytesB];
+  __shared__ __attribute__((aligned(1024))) char lds_a0[Z::kBytesA];
+  __shared__ __attribute__((aligned(1024))) char lds_b0[Z::kBytesB];
+  __shared__ __attribute__((aligned(1024))) char lds_a1[Z::kBytesA];
+  __shared__ __attribute__((aligned(1024))) char lds_b1[Z::kBytesB];
+  // dW: the rows of x of the slices around the present one, found by one thread a row
+  __shared__ int rows_of_x[MODE == kWeight ? 4 : 1][MODE == kWeight ? S : 1];
   const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
 
   // which tile: neighbours share the segment's rows (and the expert's matrix), so
@@ -273,55 +312,76 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     return;
   }
 
+  // This thread's pieces of a slice.  WHOLE: as 32-bit offsets from bases that are the
+  // same for the workgroup, kNoRow where there is none; loads past the end of an
+  // operand give zeros.  Otherwise as pointers with the elements that are there.
   const T* a = static_cast<const T*>(call.a);
   const T* b = static_cast<const T*>(call.b);
-  const int64_t matrix = static_cast<int64_t>(segment) * call.n_out * call.k_in;
-  const int64_t end_b = MODE == kWeight ? 0 : static_cast<int64_t>(call.experts) * call.n_out * call.k_in;
-
-  // this thread's pieces of a slice
-  const T* from_a[Z::kPiecesA];
-  const T* from_b[Z::kPiecesB];
-  int live_a[Z::kPiecesA], live_b[Z::kPiecesB];          // along: whether the row is there; across: elements of the piece
-  u32x4 next_a[Z::kPiecesA], next_b[Z::kPiecesB];
-  int64_t x_rows[MODE == kWeight ? Z::kPiecesB : 1];
-  const T* last_a = a;                                   // one past the last element that may be read
-  const T* last_b = b + end_b;
+  const int64_t inner = call.inner;
+  const int64_t rows_x = (call.order != nullptr ? call.places / call.k : call.places) * inner;
   const int ld_a = MODE == kForward || MODE == kGated ? call.k_in : call.n_out;
-  if constexpr (MODE != kWeight) {
-    last_a = a + (MODE == kInput ? static_cast<int64_t>(call.places) * call.inner
-                                 : (call.order != nullptr ? call.places / call.k : call.places) * static_cast<int64_t>(call.inner)) * ld_a;
-#pragma unroll
-    for (int i = 0; i < Z::kPiecesA; ++i) {
-      const int row = (thread + i * Z::kThreads) >> 3;
-      live_a[i] = row < live_rows;
-      from_a[i] = a;
-      if (row < live_rows) {
-        const int at = first_row + row;
-        from_a[i] = a + (MODE == kInput ? static_cast<int64_t>(at) : row_of_x(call, at)) * ld_a + (thread & 7) * V;
-      }
-    }
+  const int64_t matrix = static_cast<int64_t>(call.n_out) * call.k_in;
+  int64_t elements_a, elements_b;                        // from the bases to the ends
+  if constexpr (MODE == kForward || MODE == kGated) {
+    elements_a = rows_x * call.k_in;
+  } else if constexpr (MODE == kInput) {
+    elements_a = (WHOLE ? static_cast<int64_t>(live_rows) : call.places * inner - first_row) * call.n_out;
+    a += static_cast<int64_t>(first_row) * call.n_out;
   } else {
-    last_a = a + call.places * static_cast<int64_t>(call.inner) * call.n_out;
-    last_b = b + (call.order != nullptr ? call.places / call.k : call.places) * static_cast<int64_t>(call.inner) * call.k_in;
-#pragma unroll
-    for (int i = 0; i < Z::kPiecesA; ++i) {
-      const int at = thread + i * Z::kThreads;
-      const int column = first_row + at % (BM / V) * V;
-      live_a[i] = call.n_out - column;
-      from_a[i] = a + static_cast<int64_t>(span.begin + at / (BM / V)) * call.n_out + column;
-    }
-#pragma unroll
-    for (int i = 0; i < Z::kPiecesB; ++i) {
-      const int at = thread + i * Z::kThreads;
-      const int row = at / (BN / V);
-      live_b[i] = call.k_in - (first_column + at % (BN / V) * V);
-      x_rows[i] = row < depth ? row_of_x(call, span.begin + row) : 0;
-    }
+    elements_a = (WHOLE ? static_cast<int64_t>(depth) : call.places * inner - span.begin) * call.n_out;
+    a += static_cast<int64_t>(span.begin) * call.n_out;
   }
+  if constexpr (MODE == kWeight) {
+    elements_b = rows_x * call.k_in;
+  } else {
+    elements_b = (WHOLE ? 1 : static_cast<int64_t>(call.experts - segment)) * matrix;
+    b += segment * matrix;
+  }
+  // the piece of its row that lies where this thread's 16 bytes go (rows of this
+  // thread's other pieces have the same place in the pattern)
+  const int along_piece = (thread & 7) ^ ((thread >> 4) & 7);
+  typedef typename std::conditional<WHOLE, uint32_t, int64_t>::type Offset;
+  Offset from_a[Z::kPiecesA], from_b[Z::kPiecesB];       // WHOLE: bytes, else elements
+  int live_a[Z::kPiecesA], live_b[Z::kPiecesB];          // else; along: whether the row is there, across: elements
+  constexpr int kUnit = WHOLE ? static_cast<int>(sizeof(T)) : 1;
+  const auto offset_of = [&](bool there, int64_t element) {
+    if constexpr (WHOLE) return there ? static_cast<uint32_t>(element * kUnit) : kNoRow;
+    else return element;
+  };
+  PlaceRow of_places[Z::kPiecesA];                       // all loads before the first use
   if constexpr (MODE == kForward || MODE == kGated) {
 #pragma unroll
-    for (int i = 0; i < Z::kPiecesB; ++i) {
+    for (int i = 0; i < Z::kPiecesA; ++i) {
       const int row = (thread + i * Z::kThreads) >> 3;
+      of_places[i] = place_row(call, first_row + (row < live_rows ? row : 0));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < Z::kPiecesA; ++i) {
+    const int at = thread + i * Z::kThreads;
+    if constexpr (Z::kAcrossA) {
+      const int column = first_row + across_piece<T, BM>(at) * V;
+      live_a[i] = call.n_out - column;
+      from_a[i] = offset_of(live_a[i] > 0, static_cast<int64_t>(at / (BM / V)) * call.n_out + column);
+    } else {
+      const int row = at >> 3;
+      live_a[i] = row < live_rows;
+      const int64_t of_row = MODE == kInput ? row : row_of_x(call, of_places[i]);
+      from_a[i] = offset_of(row < live_rows, of_row * ld_a + along_piece * V);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < Z::kPiecesB; ++i) {
+    const int at = thread + i * Z::kThreads;
+    if constexpr (MODE == kWeight) {
+      live_b[i] = call.k_in - (first_column + across_piece<T, BN>(at) * V);
+      from_b[i] = 0;
+    } else if constexpr (MODE == kInput) {
+      const int column = first_column + across_piece<T, BN>(at) * V;
+      live_b[i] = call.k_in - column;
+      from_b[i] = offset_of(live_b[i] > 0, static_cast<int64_t>(at / (BN / V)) * call.k_in + column);
+    } else {
+      const int row = at >> 3;
       int output = first_column + row;
       bool there = output < call.n_out;
       if constexpr (MODE == kGated) {                    // 32 gates, their 32 partners, 32 gates ...
@@ -330,64 +390,63 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
         there = column < half;
       }
       live_b[i] = there;
-      from_b[i] = there ? b + matrix + static_cast<int64_t>(output) * call.k_in + (thread & 7) * V : b;
-    }
-  } else if constexpr (MODE == kInput) {
-#pragma unroll
-    for (int i = 0; i < Z::kPiecesB; ++i) {
-      const int at = thread + i * Z::kThreads;
-      const int column = first_column + at % (BN / V) * V;
-      live_b[i] = call.k_in - column;
-      from_b[i] = b + matrix + static_cast<int64_t>(at / (BN / V)) * call.k_in + column;
+      from_b[i] = offset_of(there, there ? static_cast<int64_t>(output) * call.k_in + along_piece * V : 0);
     }
   }
 
-  const auto fetch = [&](int slice) {
+  // kNoRow for this thread's pieces behind the summed index, else 0; from the sign, as
+  // the compiler turns a choice of offsets into branches around two loads.
+  const auto past_depth = [&](int done) { return static_cast<uint32_t>(depth - 1 - (done + along_piece * V)) & kNoRow; };
+  // Starts the loads of slice `slice`.  WHOLE: straight to LDS, whose 16 bytes of a
+  // wave are consecutive; zeros where there is nothing.  Else to registers.
+  u32x4 piece_a[WHOLE ? 1 : Z::kPiecesA], piece_b[WHOLE ? 1 : Z::kPiecesB];
+  const auto fetch = [&](int slice, char* to_a, char* to_b) {
     const int done = slice * S;
+    const uint32_t past = past_depth(done);
+    const int64_t moved_a = Z::kAcrossA ? static_cast<int64_t>(done) * call.n_out : done;
+    const int64_t moved_b = MODE == kWeight ? 0 : Z::kAcrossB ? static_cast<int64_t>(done) * call.k_in : done;
+    if constexpr (MODE == kWeight) {
 #pragma unroll
-    for (int i = 0; i < Z::kPiecesA; ++i) {
-      if constexpr (MODE != kWeight) {
-        const int left = live_a[i] ? depth - done - (thread & 7) * V : 0;
-        const T* p = from_a[i] + done;
-        next_a[i] = load_piece<T>(p, left, last_a - p);
-      } else {
-        const int row = done + (thread + i * Z::kThreads) / (BM / V);
-        const T* p = from_a[i] + static_cast<int64_t>(done) * call.n_out;
-        next_a[i] = load_piece<T>(p, row < depth ? live_a[i] : 0, last_a - p);
+      for (int i = 0; i < Z::kPiecesB; ++i) {
+        const int at = thread + i * Z::kThreads, row = at / (BN / V);
+        from_b[i] = offset_of(done + row < depth && live_b[i] > 0, rows_of_x[slice & 3][row] * static_cast<int64_t>(call.k_in) +
+                                                                       first_column + across_piece<T, BN>(at) * V);
       }
     }
+    if constexpr (WHOLE) {
+      const BufferView view_a = buffer_view(a + moved_a, (elements_a - moved_a) * static_cast<int64_t>(sizeof(T)));
+      const BufferView view_b = buffer_view(b + moved_b, (elements_b - moved_b) * static_cast<int64_t>(sizeof(T)));
 #pragma unroll
-    for (int i = 0; i < Z::kPiecesB; ++i) {
-      if constexpr (MODE == kForward || MODE == kGated) {
-        const int left = live_b[i] ? depth - done - (thread & 7) * V : 0;
-        const T* p = from_b[i] + done;
-        next_b[i] = load_piece<T>(p, left, last_b - p);
-      } else if constexpr (MODE == kInput) {
-        const int row = done + (thread + i * Z::kThreads) / (BN / V);
-        const T* p = from_b[i] + static_cast<int64_t>(done) * call.k_in;
-        next_b[i] = load_piece<T>(p, row < depth ? live_b[i] : 0, last_b - p);
-      } else {
-        const int at = thread + i * Z::kThreads;
-        const int row = done + at / (BN / V);
-        const T* p = b + x_rows[i] * call.k_in + first_column + at % (BN / V) * V;
-        next_b[i] = load_piece<T>(p, row < depth ? live_b[i] : 0, last_b - p);
-        // where the next slice's rows are: a load of its own, started a slice ahead
-        x_rows[i] = row + S < depth ? row_of_x(call, span.begin + row + S) : 0;
+      for (int i = 0; i < Z::kPiecesA; ++i)
+        load_to_lds(view_a, Z::kAcrossA ? from_a[i] : from_a[i] | past, to_a + (wave * 64 + i * Z::kThreads) * 16);
+#pragma unroll
+      for (int i = 0; i < Z::kPiecesB; ++i)
+        load_to_lds(view_b, Z::kAcrossB ? from_b[i] : from_b[i] | past, to_b + (wave * 64 + i * Z::kThreads) * 16);
+    } else {
+      const int along_left = depth - done - along_piece * V;
+#pragma unroll
+      for (int i = 0; i < Z::kPiecesA; ++i) {
+        const bool there = Z::kAcrossA ? done + (thread + i * Z::kThreads) / (BM / V) < depth : live_a[i] != 0;
+        const int left = there ? (Z::kAcrossA ? live_a[i] : along_left) : 0;
+        piece_a[i] = load_piece<T>(a + from_a[i] + moved_a, left, elements_a - from_a[i] - moved_a);
+      }
+#pragma unroll
+      for (int i = 0; i < Z::kPiecesB; ++i) {
+        const bool there = Z::kAcrossB ? done + (thread + i * Z::kThreads) / (BN / V) < depth : live_b[i] != 0;
+        const int left = there ? (Z::kAcrossB ? live_b[i] : along_left) : 0;
+        piece_b[i] = load_piece<T>(b + from_b[i] + moved_b, left, elements_b - from_b[i] - moved_b);
       }
     }
   };
-  const auto keep = [&](char* to) {
+  // The slice that was fetched is in LDS behind the next barrier.
+  const auto land = [&](char* to_a, char* to_b) {
+    if constexpr (WHOLE) {
+      __builtin_amdgcn_s_waitcnt(kNoLoadsLeft);
+    } else {
 #pragma unroll
-    for (int i = 0; i < Z::kPiecesA; ++i) {
-      const int at = thread + i * Z::kThreads;
-      const int byte = Z::kAcrossA ? across_byte<T, BM>(at / (BM / V), at % (BM / V) * 16) : along_byte(at >> 3, at & 7);
-      *reinterpret_cast<u32x4*>(to + byte) = next_a[i];
-    }
+      for (int i = 0; i < Z::kPiecesA; ++i) *reinterpret_cast<u32x4*>(to_a + (thread + i * Z::kThreads) * 16) = piece_a[i];
 #pragma unroll
-    for (int i = 0; i < Z::kPiecesB; ++i) {
-      const int at = thread + i * Z::kThreads;
-      const int byte = Z::kAcrossB ? across_byte<T, BN>(at / (BN / V), at % (BN / V) * 16) : along_byte(at >> 3, at & 7);
-      *reinterpret_cast<u32x4*>(to + Z::kBytesA + byte) = next_b[i];
+      for (int i = 0; i < Z::kPiecesB; ++i) *reinterpret_cast<u32x4*>(to_b + (thread + i * Z::kThreads) * 16) = piece_b[i];
     }
   };
 
@@ -399,38 +458,61 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum[m][n][i] = 0.0f;
 
+  // Slice s is multiplied from one half of LDS while s + 1 is on its way to the other;
+  // inside a slice, the operands of the next step are read while one step's
+  // products run.
   const int wave_row = (wave / WN) * (BM / WM), wave_column = (wave % WN) * (BN / WN);
   const int slices = (depth + S - 1) / S;
-  if (slices > 0) {
-    fetch(0);
-    keep(lds[0]);
+  u32x4 fa[2][Z::kFragmentsM], fb[2][Z::kFragmentsN];
+  const auto read = [&](const char* at_a, const char* at_b, int step, u32x4 (&a_to)[Z::kFragmentsM], u32x4 (&b_to)[Z::kFragmentsN]) {
+#pragma unroll
+    for (int n = 0; n < Z::kFragmentsN; ++n) {
+      if constexpr (Z::kAcrossB) b_to[n] = across_fragment<T, BN>(at_b, wave_column + n * 32, step);
+      else b_to[n] = along_fragment<T>(at_b, wave_column + n * 32, step);
+    }
+#pragma unroll
+    for (int m = 0; m < Z::kFragmentsM; ++m) {
+      if constexpr (Z::kAcrossA) a_to[m] = across_fragment<T, BM>(at_a, wave_row + m * 32, step);
+      else a_to[m] = along_fragment<T>(at_a, wave_row + m * 32, step);
+    }
+  };
+  if constexpr (MODE == kWeight) {
+    for (int row = thread; row < 2 * S && row < depth; row += Z::kThreads)
+      rows_of_x[row / S][row % S] = static_cast<int>(row_of_x(call, place_row(call, span.begin + row)));
+    __syncthreads();
   }
-  __syncthreads();
-  for (int slice = 0; slice < slices; ++slice) {
-    const char* at_a = lds[slice & 1];
-    const char* at_b = at_a + Z::kBytesA;
-    if (slice + 1 < slices) fetch(slice + 1);
+  if (slices > 0) {
+    fetch(0, lds_a0, lds_b0);
+    land(lds_a0, lds_b0);
+  }
+  const auto turn = [&](int slice, const char* at_a, const char* at_b, char* to_a, char* to_b) {
+    __syncthreads();
+    fetch(slice + 1, to_a, to_b);
+    PlaceRow ahead{0, 0};
+    const bool finds = MODE == kWeight && thread < S && (slice + 2) * S + thread < depth;
+    if (finds) ahead = place_row(call, span.begin + (slice + 2) * S + thread);
+    read(at_a, at_b, 0, fa[0], fb[0]);
 #pragma unroll
     for (int step = 0; step < Z::kSteps; ++step) {
-      u32x4 fa[Z::kFragmentsM], fb[Z::kFragmentsN];
-#pragma unroll
-      for (int m = 0; m < Z::kFragmentsM; ++m) {
-        if constexpr (Z::kAcrossA) fa[m] = across_fragment<T, BM>(at_a, wave_row + m * 32, step);
-        else fa[m] = along_fragment<T>(at_a, wave_row + m * 32, step);
-      }
-#pragma unroll
-      for (int n = 0; n < Z::kFragmentsN; ++n) {
-        if constexpr (Z::kAcrossB) fb[n] = across_fragment<T, BN>(at_b, wave_column + n * 32, step);
-        else fb[n] = along_fragment<T>(at_b, wave_column + n * 32, step);
-      }
+      if (step + 1 < Z::kSteps) read(at_a, at_b, step + 1, fa[(step + 1) & 1], fb[(step + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);   // loads and reads start here, not where their values are used
 #pragma unroll
       for (int m = 0; m < Z::kFragmentsM; ++m)
 #pragma unroll
-        for (int n = 0; n < Z::kFragmentsN; ++n) sum[m][n] = multiply<T>(fa[m], fb[n], sum[m][n]);
+        for (int n = 0; n < Z::kFragmentsN; ++n) sum[m][n] = multiply<T>(fa[step & 1][m], fb[step & 1][n], sum[m][n]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (slice + 1 < slices) keep(lds[(slice + 1) & 1]);
-    __syncthreads();
+    land(to_a, to_b);
+    if (finds) rows_of_x[(slice + 2) & 3][thread] = static_cast<int>(row_of_x(call, ahead));
+  };
+  // the two halves by name: the compiler then sees that reads of one need not wait
+  // for loads to the other
+  int slice = 0;
+  for (; slice + 1 < slices; slice += 2) {
+    turn(slice, lds_a0, lds_b0, lds_a1, lds_b1);
+    turn(slice + 1, lds_a1, lds_b1, lds_a0, lds_b0);
   }
+  if (slice < slices) turn(slice, lds_a0, lds_b0, lds_a1, lds_b1);
 
   // register i of a lane: row 8 (i / 4) + 4 (lane / 32) + i mod 4, column lane mod 32
   const bool partial = MODE == kWeight && call.chunks > 0;
@@ -674,7 +756,7 @@ int check_product(const char* what, int64_t places, int64_t k, int64_t inner, in
   return DPA4K_OK;
 }
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, bool WHOLE>
 int launch_product(const ProductCall& call, hipStream_t stream) {
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   const int64_t rows = call.places * call.inner;
@@ -684,20 +766,36 @@ int launch_product(const ProductCall& call, hipStream_t stream) {
   if (MODE == kWeight) tiles = columns * ((call.n_out + BM - 1) / BM) * (call.chunks > 0 ? call.chunks : call.experts);
   else tiles = columns * (rows / BM + call.experts + 1);
   if (tiles > row_block_limit(Z::kThreads)) return fail(DPA4K_EINVAL, "expert linear: more tiles than a launch takes");
-  expert_product_kernel<T, MODE, BM, BN, WM, WN><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
+  expert_product_kernel<T, MODE, BM, BN, WM, WN, WHOLE><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
       call, static_cast<int>(columns), static_cast<int>(tiles));
   return launched("expert_product_kernel");
 }
 
-template <typename T, int MODE>
-int run_product(const ProductCall& call, hipStream_t stream) {
+template <typename T, int MODE, bool WHOLE>
+int run_tiles(const ProductCall& call, hipStream_t stream) {
   const int64_t width = MODE == kForward || MODE == kGated ? call.n_out : call.k_in;
   if constexpr (MODE == kWeight) {
-    if (call.n_out <= 64 || call.k_in <= 64) return launch_product<T, MODE, 64, 64, 2, 2>(call, stream);
+    if (call.n_out <= 64 || call.k_in <= 64) return launch_product<T, MODE, 64, 64, 2, 2, WHOLE>(call, stream);
   } else {
-    if (width <= 64) return launch_product<T, MODE, 128, 64, 4, 1>(call, stream);
+    if (width <= 64) return launch_product<T, MODE, 128, 64, 4, 1, WHOLE>(call, stream);
   }
-  return launch_product<T, MODE, 128, 128, 2, 2>(call, stream);
+  if constexpr (WHOLE && sizeof(T) == 2 && USE_BIG) {
+    if (width >= 256 && (MODE == kWeight ? call.n_out : call.places * call.inner / call.experts) >= 256)
+      return launch_product<T, MODE, 256, 256, BIG_WM, BIG_WN, WHOLE>(call, stream);
+  }
+  return launch_product<T, MODE, 128, 128, 2, 2, WHOLE>(call, stream);
+}
+
+template <typename T, int MODE>
+int run_product(const ProductCall& call, hipStream_t stream) {
+  // Pieces of 16 bytes are whole and aligned, and x and a tile of dz lie within 32-bit
+  // offsets; other calls load each piece through its own address.
+  const int64_t rows_x = (call.order != nullptr ? call.places / call.k : call.places) * call.inner;
+  const int64_t limit = int64_t(kNoRow) / static_cast<int64_t>(sizeof(T));
+  const bool whole = call.k_in % kV<T> == 0 && call.n_out % kV<T> == 0 && aligned16(call.a) && aligned16(call.b) &&
+                     rows_x * call.k_in < limit && static_cast<int64_t>(call.n_out) * call.k_in < limit &&
+                     static_cast<int64_t>(call.n_out) * 256 < limit && static_cast<int64_t>(call.k_in) * 256 < limit;
+  return whole ? run_tiles<T, MODE, true>(call, stream) : run_tiles<T, MODE, false>(call, stream);
 }
 
 // Rows of a segment that one workgroup of dW takes: all of them where the matrices
