@@ -78,6 +78,17 @@ __device__ __forceinline__ Span span_of(const ProductCall& call, int e) {
   return Span{static_cast<int>(begin * call.inner), static_cast<int>(end * call.inner)};
 }
 
+// Workgroups go to the 8 dies in turn.  Each die takes groups of `group` neighbouring
+// tiles, which share rows and matrices in its cache; the groups are dealt in turn,
+// as tiles of long segments and the unused ones at the end would otherwise all
+// fall to one die.
+__device__ __forceinline__ int tile_of_block(int block, int tiles, int group) {
+  const int round = group * static_cast<int>(kXcds);
+  if (block >= tiles / round * round) return block;
+  const int die = block % static_cast<int>(kXcds), index = block / static_cast<int>(kXcds);
+  return (index / group * static_cast<int>(kXcds) + die) * group + index % group;
+}
+
 // Tiles of `rows` rows of a segment; `empty`: an empty one has a tile too.
 __device__ __forceinline__ int tiles_of(const Span& span, int rows, bool empty) {
   const int length = span.end - span.begin;
@@ -264,7 +275,7 @@ struct Tile {
 };
 
 template <typename T, int MODE, int BM, int BN, int WM, int WN, bool WHOLE>
-__global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductCall call, int columns, int tiles) {
+__global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductCall call, int columns, int tiles, int group) {
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   constexpr int V = kV<T>, S = kSlice<T>;
   __shared__ __attribute__((aligned(1024))) char lds_a0[Z::kBytesA];
@@ -275,10 +286,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   __shared__ int rows_of_x[MODE == kWeight ? 4 : 1][MODE == kWeight ? S : 1];
   const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
 
-  // which tile: neighbours share the segment's rows (and the expert's matrix), so
-  // each die takes a contiguous run of them
-  const int block = static_cast<int>(xcd_block(blockIdx.x, gridDim.x));
-  if (block >= tiles) return;
+  const int block = tile_of_block(blockIdx.x, tiles, group);
   const int column_tile = block % columns, rest = block / columns;
   int segment, number;
   Span span;
@@ -310,6 +318,18 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       if (c < width) y[static_cast<int64_t>(first_row + at / kTileColumns) * width + c] = static_cast<T>(0.0f);
     }
     return;
+  }
+
+  // dx by slot: where the tile's rows go, -1 for a slot that is none
+  __shared__ int out_rows[MODE == kInput ? BM : 1];
+  if constexpr (MODE == kInput) {
+    if (call.by_slot && thread < BM && thread < live_rows) {
+      const int row = first_row + thread;
+      const int place = call.inner == 1 ? row : static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(call.inner));
+      const int64_t slot = call.order[place];
+      out_rows[thread] = static_cast<uint64_t>(slot) < static_cast<uint64_t>(call.places)
+                             ? static_cast<int>(slot) * call.inner + (row - place * call.inner) : -1;
+    }
   }
 
   // This thread's pieces of a slice.  WHOLE: as 32-bit offsets from bases that are the
@@ -476,34 +496,48 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       else a_to[m] = along_fragment<T>(at_a, wave_row + m * 32, step);
     }
   };
+  PlaceRow ahead{0, 0};                                  // dW: of the slice behind the next two
+  const auto look_ahead = [&](int slice) {
+    if (MODE == kWeight && thread < S && slice * S + thread < depth) ahead = place_row(call, span.begin + slice * S + thread);
+  };
   if constexpr (MODE == kWeight) {
     for (int row = thread; row < 2 * S && row < depth; row += Z::kThreads)
       rows_of_x[row / S][row % S] = static_cast<int>(row_of_x(call, place_row(call, span.begin + row)));
+    look_ahead(2);
     __syncthreads();
   }
   if (slices > 0) {
     fetch(0, lds_a0, lds_b0);
     land(lds_a0, lds_b0);
   }
-  const auto turn = [&](int slice, const char* at_a, const char* at_b, char* to_a, char* to_b) {
-    __syncthreads();
-    fetch(slice + 1, to_a, to_b);
-    PlaceRow ahead{0, 0};
-    const bool finds = MODE == kWeight && thread < S && (slice + 2) * S + thread < depth;
-    if (finds) ahead = place_row(call, span.begin + (slice + 2) * S + thread);
-    read(at_a, at_b, 0, fa[0], fb[0]);
+  __syncthreads();
+  if (slices > 0) {
+    fetch(1, lds_a1, lds_b1);
+    read(lds_a0, lds_b0, 0, fa[0], fb[0]);
+  }
+  // The half at `at` is read for the last time in front of the third step's products;
+  // behind them every wave has read it and the next slice has landed, so that the
+  // last step's products hide the next slice's first reads.
+  const auto turn = [&](int slice, char* at_a, char* at_b, char* next_a, char* next_b) {
 #pragma unroll
     for (int step = 0; step < Z::kSteps; ++step) {
-      if (step + 1 < Z::kSteps) read(at_a, at_b, step + 1, fa[(step + 1) & 1], fb[(step + 1) & 1]);
+      const int to = (step + 1) & 1;
+      if (step + 1 < Z::kSteps) read(at_a, at_b, step + 1, fa[to], fb[to]);
+      else read(next_a, next_b, 0, fa[to], fb[to]);
       __builtin_amdgcn_sched_barrier(0);   // loads and reads start here, not where their values are used
 #pragma unroll
       for (int m = 0; m < Z::kFragmentsM; ++m)
 #pragma unroll
         for (int n = 0; n < Z::kFragmentsN; ++n) sum[m][n] = multiply<T>(fa[step & 1][m], fb[step & 1][n], sum[m][n]);
       __builtin_amdgcn_sched_barrier(0);
+      if (step == Z::kSteps - 2) {
+        land(next_a, next_b);
+        if (MODE == kWeight && thread < S) rows_of_x[(slice + 2) & 3][thread] = static_cast<int>(row_of_x(call, ahead));
+        __syncthreads();
+        fetch(slice + 2, at_a, at_b);
+        look_ahead(slice + 3);
+      }
     }
-    land(to_a, to_b);
-    if (finds) rows_of_x[(slice + 2) & 3][thread] = static_cast<int>(row_of_x(call, ahead));
   };
   // the two halves by name: the compiler then sees that reads of one need not wait
   // for loads to the other
@@ -513,6 +547,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     turn(slice + 1, lds_a1, lds_b1, lds_a0, lds_b0);
   }
   if (slice < slices) turn(slice, lds_a0, lds_b0, lds_a1, lds_b1);
+  __builtin_amdgcn_s_waitcnt(kNoLoadsLeft);              // the workgroup's LDS is not given away while loads to it are under way
 
   // register i of a lane: row 8 (i / 4) + 4 (lane / 32) + i mod 4, column lane mod 32
   const bool partial = MODE == kWeight && call.chunks > 0;
@@ -524,12 +559,8 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       if (row >= live_rows) continue;
       int64_t out_row = first_row + row;
       if constexpr (MODE == kInput) {
-        if (call.by_slot) {
-          const int place = static_cast<int>(static_cast<uint32_t>(out_row) / static_cast<uint32_t>(call.inner));
-          const int64_t slot = call.order[place];
-          if (static_cast<uint64_t>(slot) >= static_cast<uint64_t>(call.places)) continue;
-          out_row = slot * call.inner + (out_row - static_cast<int64_t>(place) * call.inner);
-        }
+        if (call.by_slot) out_row = out_rows[row];
+        if (out_row < 0) continue;
       } else if constexpr (MODE == kWeight) {
         out_row += static_cast<int64_t>(partial ? chunk : segment) * call.n_out;
       }
@@ -767,7 +798,7 @@ int launch_product(const ProductCall& call, hipStream_t stream) {
   else tiles = columns * (rows / BM + call.experts + 1);
   if (tiles > row_block_limit(Z::kThreads)) return fail(DPA4K_EINVAL, "expert linear: more tiles than a launch takes");
   expert_product_kernel<T, MODE, BM, BN, WM, WN, WHOLE><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
-      call, static_cast<int>(columns), static_cast<int>(tiles));
+      call, static_cast<int>(columns), static_cast<int>(tiles), static_cast<int>(tiles >= columns * 128 ? columns * 4 : columns));
   return launched("expert_product_kernel");
 }
 
