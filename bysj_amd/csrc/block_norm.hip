@@ -12,15 +12,22 @@
 //
 // Bound by its streams: each input is read once and each output written once,
 // because a row stays in the registers of the lanes that share it, L of them with
-// E elements each: 8 to 64 lanes of a wave for rows of up to 1,024, a workgroup
-// beyond.  h is not kept in 32 bits between the two passes; the backward computes
+// E elements each: 8 to 64 lanes of a wave for rows of up to 1,024 (two waves of
+// half the elements were as fast forward and slower backward, 126 -> 170 us for
+// 30,011 rows of 810, as their sums need a barrier each), a workgroup beyond.  h is not kept in 32 bits between the two passes; the backward computes
 // it again from the residual, which is as many bytes as reading h, and y and the
 // gradients see the unrounded h.
 //
 // The gradients of post, pre and scale are sums over all rows.  A workgroup walks
-// its rows with a column's sum in a register, for at most kRunRows rows (sums in
-// 32 bits stay short), and leaves one row of partial sums; a second launch adds
-// these in 64 bits in a fixed order.
+// its rows with the columns' sums in LDS, for at most kRunRows rows (sums in 32
+// bits stay short), and leaves one row of partial sums; a second launch adds these
+// in 64 bits in a fixed order.
+//
+// Measured: 24,576 rows of 1,024 in float32 with a gate, forward 90 us (5.6 TB/s of
+// its five streams), backward 155 us (5.2 TB/s of eight); 30,011 rows of 810 in
+// bfloat16 on a float32 residual, forward 52 us (5.6 TB/s), backward 118 us
+// (3.7 TB/s; rows that start anywhere, four tenths of the second chunk's lanes idle).
+// Outputs are stored past the caches (through them: 90, 160, 61 and 123 us).
 #include "elements.h"
 
 namespace dpa4k {
@@ -77,12 +84,12 @@ __device__ __forceinline__ float row_sum(float value, float (*words)[16], int sl
     return group_sum<L>(value);
   } else {
     value = group_sum<64>(value);
-    const int wave = threadIdx.x / 64;
-    if ((threadIdx.x & 63) == 0) words[slot][wave] = value;
+    if ((threadIdx.x & 63) == 0) words[slot][threadIdx.x / 64] = value;
     __syncthreads();
+    const int first = threadIdx.x / L * (L / 64);
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < L / 64; ++w) sum += words[slot][w];
+    for (int w = 0; w < L / 64; ++w) sum += words[slot][first + w];
     return sum;
   }
 }
@@ -98,18 +105,46 @@ struct Row {
   static __device__ __forceinline__ int column(int n, int lane) { return (n * L + lane) * V; }
 };
 
-// Values of one stream at this lane's columns of `row`.
-template <typename T, typename S, typename R, int L, int E>
-__device__ __forceinline__ void load_row(const S* __restrict__ p, int64_t row, int lane, int width, int64_t total, bool live,
-                                         float (&out)[E]) {
+// Whether a chunk of the workgroup's rows from `first` on may reach past the tensor.
+template <typename T, typename R, int L, int E>
+__device__ __forceinline__ bool near_end(int64_t first, int64_t rows, int width) {
+  typedef Row<T, R, L, E> Z;
+  return (rows - first - Z::kGroups) * width < Z::V;
+}
+
+// One stream at this lane's columns of `row`, as it is in memory.  A ragged chunk is
+// read with the start of the next row and masked by `values_of`, or, where the
+// workgroup has the last row, behind which nothing may be read, piece by piece.
+// All streams of a row are loaded in one block of code and masked behind it: what
+// uses a value in between waits for it, and what follows is loaded no sooner.
+template <typename T, typename S, int E>
+struct Stream {
+  static constexpr int V = 16 / sizeof(T);
+  Pack<S, V> chunk[E / V];
+};
+
+template <bool LAST, typename T, typename R, int L, int E, typename S>
+__device__ __forceinline__ void load_stream(const S* __restrict__ p, int64_t row, int lane, int width, int64_t total, bool live,
+                                            Stream<T, S, E>& to) {
   typedef Row<T, R, L, E> Z;
 #pragma unroll
   for (int n = 0; n < Z::N; ++n) {
     const int c = Z::column(n, lane);
     const int64_t at = row * width + c;
-    const Pack<S, Z::V> raw = load_pack<S, Z::V>(p + at, live ? width - c : 0, total - at);
+    if constexpr (LAST) to.chunk[n] = load_pack<S, Z::V>(p + at, live ? width - c : 0, total - at);
+    else to.chunk[n] = *reinterpret_cast<const Pack<S, Z::V>*>(p + row * width + (c < width ? c : 0));
+  }
+}
+
+// The values of a stream, zeros behind the row.
+template <typename T, typename R, int L, int E, typename S>
+__device__ __forceinline__ void values_of(const Stream<T, S, E>& from, int lane, int width, float (&out)[E]) {
+  typedef Row<T, R, L, E> Z;
 #pragma unroll
-    for (int j = 0; j < Z::V; ++j) out[n * Z::V + j] = static_cast<float>(raw[j]);
+  for (int n = 0; n < Z::N; ++n) {
+    const int here = width - Z::column(n, lane);
+#pragma unroll
+    for (int j = 0; j < Z::V; ++j) out[n * Z::V + j] = j < here ? static_cast<float>(from.chunk[n][j]) : 0.0f;
   }
 }
 
@@ -123,14 +158,16 @@ __device__ __forceinline__ void store_row(S* __restrict__ p, int64_t row, int la
     float part[Z::V];
 #pragma unroll
     for (int j = 0; j < Z::V; ++j) part[j] = value[n * Z::V + j];
-    if (c < width) store_pack<S, Z::V>(p + row * width + c, part, width - c);
+    if (c < width) store_pack<true, S, Z::V>(p + row * width + c, part, width - c);
   }
 }
 
 template <typename T, typename R, int L, int E>
 __device__ __forceinline__ void load_weight(const float* __restrict__ p, float otherwise, int lane, int width, float (&out)[E]) {
   if (p != nullptr) {
-    load_row<T, float, R, L, E>(p, 0, lane, width, width, true, out);
+    Stream<T, float, E> raw;
+    load_stream<true, T, R, L, E>(p, 0, lane, width, width, true, raw);
+    values_of<T, R, L, E>(raw, lane, width, out);
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i) out[i] = otherwise;
@@ -145,7 +182,7 @@ __device__ __forceinline__ void residual_sum(const float (&x)[E], const float (&
   for (int i = 0; i < E; ++i) h[i] = fmaf(scale[i] * act[i], x[i] * r * post[i], residual[i]);
 }
 
-template <typename T, typename R, int L, int E>
+template <typename T, typename R, int L, int E, bool FULL_GATE>
 __global__ __launch_bounds__((L > 256 ? L : 256)) void residual_norm_forward_kernel(NormCall call) {
   typedef Row<T, R, L, E> Z;
   __shared__ float words[2][16];
@@ -158,13 +195,25 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void residual_norm_forward_ker
   const int64_t row = block_index() * Z::kGroups + group;
   if (block_index() * Z::kGroups >= call.rows) return;
   const bool live = row < call.rows;
+  const bool last = near_end<T, R, L, E>(block_index() * Z::kGroups, call.rows, width);
   float x[E], residual[E], act[E], post[E], scale[E], h[E];
-  load_row<T, T, R, L, E>(x_at, row, lane, width, total, live, x);
-  load_row<T, R, R, L, E>(residual_at, row, lane, width, total, live, residual);
-  if (call.gate_kind == kGateFull) {
-    load_row<T, T, R, L, E>(gate_at, row, lane, width, total, live, act);
+  Stream<T, T, E> raw_x, raw_gate;
+  Stream<T, R, E> raw_residual;
+  const auto load = [&](auto at_end) {
+    constexpr bool LAST = decltype(at_end)::value;
+    load_stream<LAST, T, R, L, E>(x_at, row, lane, width, total, live, raw_x);
+    load_stream<LAST, T, R, L, E>(residual_at, row, lane, width, total, live, raw_residual);
+    if constexpr (FULL_GATE) load_stream<LAST, T, R, L, E>(gate_at, row, lane, width, total, live, raw_gate);
+  };
+  if (last) load(std::true_type{});
+  else load(std::false_type{});
+  values_of<T, R, L, E>(raw_x, lane, width, x);
+  values_of<T, R, L, E>(raw_residual, lane, width, residual);
+  if constexpr (FULL_GATE) {
+    values_of<T, R, L, E>(raw_gate, lane, width, act);
   } else {
-    const float one = call.gate_kind == kGateRow && live ? static_cast<float>(gate_at[row]) : 1.0f;
+    float one = 1.0f, slope;
+    if (call.gate_kind == kGateRow) one = gate_value(live ? static_cast<float>(gate_at[row]) : 0.0f, call.act, slope);
 #pragma unroll
     for (int i = 0; i < E; ++i) act[i] = one;
   }
@@ -177,7 +226,7 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void residual_norm_forward_ker
     for (int i = 0; i < E; ++i) sum = fmaf(x[i], x[i], sum);
     r = 1.0f / sqrtf(row_sum<L>(sum, words, 0) / static_cast<float>(width) + call.eps);
   }
-  if (call.gate_kind != kGateNone) {
+  if constexpr (FULL_GATE) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       float slope;
@@ -200,34 +249,45 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void residual_norm_forward_ker
   if (call.post_norm && call.r != nullptr && live && lane == 0) call.r[row] = r;
 }
 
-// One sum of columns: over the row groups of the workgroup, then to its row of
-// partial sums.
+// A workgroup's sums of columns lie in LDS, [3][chunks][threads][V], each thread's
+// own: registers for them (48 of 250 with 16 elements a lane) would halve the waves
+// that are resident, or leave no room to load all streams of a row at once.
 template <typename T, typename R, int L, int E>
-__device__ __forceinline__ void leave_sums(const float (&sum)[E], float* words, float* __restrict__ to, int lane, int group, int width) {
+__device__ __forceinline__ void add_to(float* words, const float (&value)[E]) {
   typedef Row<T, R, L, E> Z;
-  if constexpr (Z::kGroups == 1) {
-    store_row<T, float, R, L, E>(to, 0, lane, width, true, sum);
-  } else {
-    // words[group][E][L]; the first L lanes' worth of threads add the groups in order
 #pragma unroll
-    for (int i = 0; i < E; ++i) words[(group * E + i) * L + lane] = sum[i];
-    __syncthreads();
-    for (int at = threadIdx.x; at < E * L; at += Z::kBlock) {
-      float all = 0.0f;
-      for (int g = 0; g < Z::kGroups; ++g) all += words[g * E * L + at];
-      const int i = at / L, l = at % L;
-      const int c = Z::column(i / Z::V, l) + i % Z::V;
-      if (c < width) to[c] = all;
+  for (int n = 0; n < Z::N; ++n) {
+    float* at = words + (n * Z::kBlock + static_cast<int>(threadIdx.x)) * Z::V;
+#pragma unroll
+    for (int j = 0; j < Z::V; j += 4) {
+      f32x4* four = reinterpret_cast<f32x4*>(at + j);
+      f32x4 sum = *four;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += value[n * Z::V + j + i];
+      *four = sum;
     }
-    __syncthreads();
   }
 }
 
+// One sum of columns over the row groups of the workgroup, in order, to its row of
+// partial sums.
 template <typename T, typename R, int L, int E>
+__device__ __forceinline__ void leave_sums(const float* words, float* __restrict__ to, int width) {
+  typedef Row<T, R, L, E> Z;
+  for (int c = threadIdx.x; c < width; c += Z::kBlock) {
+    const int chunk = c / Z::V;
+    const float* at = words + (chunk / L * Z::kBlock + chunk % L) * Z::V + c % Z::V;
+    float all = 0.0f;
+    for (int g = 0; g < Z::kGroups; ++g) all += at[g * L * Z::V];
+    to[c] = all;
+  }
+}
+
+template <typename T, typename R, int L, int E, bool FULL_GATE>
 __global__ __launch_bounds__((L > 256 ? L : 256)) void residual_norm_backward_kernel(NormCall call, int64_t blocks) {
   typedef Row<T, R, L, E> Z;
   __shared__ float words[3][16];
-  __shared__ float column_words[Z::kGroups > 1 ? Z::kBlock * E : 1];
+  __shared__ __attribute__((aligned(16))) float sums[3][Z::kBlock * E];
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
   const int width = call.width;
   const float inverse_width = 1.0f / static_cast<float>(width);
@@ -235,41 +295,56 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void residual_norm_backward_ke
   const int64_t block = block_index();
   if (block >= blocks) return;
   const T* x_at = static_cast<const T*>(call.x);
-  const R* residual_at = static_cast<const R*>(call.residual);
+  const R* residual_at = static_cast<const R*>(call.residual != nullptr ? call.residual : call.dh);
   const T* gate_at = static_cast<const T*>(call.gate);
-  float sum_post[E], sum_pre[E], sum_scale[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) sum_post[i] = sum_pre[i] = sum_scale[i] = 0.0f;
+  const T* dy_at = call.dy != nullptr ? static_cast<const T*>(call.dy) : x_at;
+  const R* dh_at = static_cast<const R*>(call.dh != nullptr ? call.dh : call.residual);
+  for (int i = threadIdx.x; i < 3 * Z::kBlock * E; i += Z::kBlock) (&sums[0][0])[i] = 0.0f;
+  __syncthreads();
 
   for (int64_t first = block * Z::kGroups; first < call.rows; first += blocks * Z::kGroups) {
     const int64_t row = first + group;
     const bool live = row < call.rows;
+    const bool last = near_end<T, R, L, E>(first, call.rows, width);
     float x[E], act[E], slope[E], post[E], scale[E], g[E];
-    load_row<T, T, R, L, E>(x_at, row, lane, width, total, live, x);
-    if (call.gate_kind == kGateFull) {
-      load_row<T, T, R, L, E>(gate_at, row, lane, width, total, live, act);
+    // in the place of a stream that is not there another one is read again, which costs no bytes
+    Stream<T, T, E> raw_x, raw_gate, raw_dy;
+    Stream<T, R, E> raw_residual, raw_dh;
+    const auto load = [&](auto at_end) {
+      constexpr bool LAST = decltype(at_end)::value;
+      load_stream<LAST, T, R, L, E>(x_at, row, lane, width, total, live, raw_x);
+      load_stream<LAST, T, R, L, E>(residual_at, row, lane, width, total, live, raw_residual);
+      if constexpr (FULL_GATE) load_stream<LAST, T, R, L, E>(gate_at, row, lane, width, total, live, raw_gate);
+      load_stream<LAST, T, R, L, E>(dh_at, row, lane, width, total, live, raw_dh);
+      load_stream<LAST, T, R, L, E>(dy_at, row, lane, width, total, live, raw_dy);
+    };
+    if (last) load(std::true_type{});
+    else load(std::false_type{});
+    values_of<T, R, L, E>(raw_x, lane, width, x);
+    if constexpr (FULL_GATE) {
+      values_of<T, R, L, E>(raw_gate, lane, width, act);
     } else {
-      const float one = call.gate_kind == kGateRow && live ? static_cast<float>(gate_at[row]) : 1.0f;
+      float one = 1.0f, its_slope = 0.0f;
+      if (call.gate_kind == kGateRow) one = gate_value(live ? static_cast<float>(gate_at[row]) : 0.0f, call.act, its_slope);
 #pragma unroll
-      for (int i = 0; i < E; ++i) act[i] = one;
+      for (int i = 0; i < E; ++i) act[i] = one, slope[i] = its_slope;
     }
-    if (call.dh != nullptr) {
-      load_row<T, R, R, L, E>(static_cast<const R*>(call.dh), row, lane, width, total, live, g);
-    } else {
+    values_of<T, R, L, E>(raw_dh, lane, width, g);
+    if (call.dh == nullptr) {
 #pragma unroll
       for (int i = 0; i < E; ++i) g[i] = 0.0f;
     }
     load_weight<T, R, L, E>(call.post, 1.0f, lane, width, post);
     load_weight<T, R, L, E>(call.scale, call.scale_value, lane, width, scale);
     const float r = call.post_norm && live ? call.r[row] : 1.0f;
-    if (call.gate_kind != kGateNone) {
+    if constexpr (FULL_GATE) {
 #pragma unroll
       for (int i = 0; i < E; ++i) act[i] = gate_value(act[i], call.act, slope[i]);
     }
     if (call.dy != nullptr) {
       float residual[E], dy[E], pre[E], h[E];
-      load_row<T, R, R, L, E>(residual_at, row, lane, width, total, live, residual);
-      load_row<T, T, R, L, E>(static_cast<const T*>(call.dy), row, lane, width, total, live, dy);
+      values_of<T, R, L, E>(raw_residual, lane, width, residual);
+      values_of<T, R, L, E>(raw_dy, lane, width, dy);
       load_weight<T, R, L, E>(call.pre, 1.0f, lane, width, pre);
       const float q = live ? call.q[row] : 0.0f;
       residual_sum<E>(x, residual, act, post, scale, r, h);
@@ -277,29 +352,32 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void residual_norm_backward_ke
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         h[i] *= q;
-        sum_pre[i] = fmaf(dy[i], h[i], sum_pre[i]);
-        dy[i] *= pre[i];
-        dot = fmaf(dy[i], h[i], dot);
+        pre[i] *= dy[i];
+        dy[i] *= h[i];
+        dot = fmaf(pre[i], h[i], dot);
       }
+      add_to<T, R, L, E>(sums[1], dy);
       dot = row_sum<L>(dot, words, 0) * inverse_width;
 #pragma unroll
-      for (int i = 0; i < E; ++i) g[i] = fmaf(q, fmaf(-h[i], dot, dy[i]), g[i]);
+      for (int i = 0; i < E; ++i) g[i] = fmaf(q, fmaf(-h[i], dot, pre[i]), g[i]);
     }
     if (call.dresidual != nullptr) store_row<T, R, R, L, E>(static_cast<R*>(call.dresidual), row, lane, width, live, g);
     // x from here on is x r, the normed row
-    float dot = 0.0f, row_gate = 0.0f;
+    float dot = 0.0f, row_gate = 0.0f, of_scale[E], of_post[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       x[i] *= r;
       const float a = x[i] * post[i];
-      sum_scale[i] = fmaf(g[i], act[i] * a, sum_scale[i]);
+      of_scale[i] = g[i] * (act[i] * a);
       const float b = g[i] * scale[i];
-      if (call.gate_kind != kGateNone) slope[i] *= b * a;   // the gate's gradient
+      slope[i] *= b * a;   // the gate's gradient
       g[i] = b * act[i];
-      sum_post[i] = fmaf(g[i], x[i], sum_post[i]);
+      of_post[i] = g[i] * x[i];
       g[i] *= post[i];
       dot = fmaf(g[i], x[i], dot);
     }
+    add_to<T, R, L, E>(sums[2], of_scale);
+    add_to<T, R, L, E>(sums[0], of_post);
     if (call.dgate != nullptr) {
       if (call.gate_kind == kGateFull) {
         store_row<T, T, R, L, E>(static_cast<T*>(call.dgate), row, lane, width, live, slope);
@@ -319,11 +397,9 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void residual_norm_backward_ke
     if constexpr (L > 64) __syncthreads();   // before the words of the next row
   }
   if (!call.want_sums) return;
-  const int64_t stride = blocks * width;
-  float* to = call.partial + block * width;
-  leave_sums<T, R, L, E>(sum_post, column_words, to, lane, group, width);
-  leave_sums<T, R, L, E>(sum_pre, column_words, to + stride, lane, group, width);
-  leave_sums<T, R, L, E>(sum_scale, column_words, to + 2 * stride, lane, group, width);
+  __syncthreads();
+  for (int sum = 0; sum < 3; ++sum)
+    leave_sums<T, R, L, E>(sums[sum], call.partial + (sum * blocks + block) * width, width);
 }
 
 // out[c] = sum over the workgroups of partial[.][c], 32 columns a workgroup, eight
@@ -433,8 +509,13 @@ extern "C" int dpa4k_residual_norm_forward(const void* x, const void* residual, 
     return with_layout(call.width, [&](auto l, auto e) {
       typedef Row<typename decltype(t)::type, typename decltype(s)::type, l.value, e.value> Z;
       const int64_t blocks = (rows + Z::kGroups - 1) / Z::kGroups;
-      residual_norm_forward_kernel<typename decltype(t)::type, typename decltype(s)::type, l.value, e.value>
-          <<<launch_grid(blocks, Z::kBlock), Z::kBlock, 0, as_stream(stream)>>>(call);
+      const dim3 grid = launch_grid(blocks, Z::kBlock);
+      if (gate_kind == kGateFull)
+        residual_norm_forward_kernel<typename decltype(t)::type, typename decltype(s)::type, l.value, e.value, true>
+            <<<grid, Z::kBlock, 0, as_stream(stream)>>>(call);
+      else
+        residual_norm_forward_kernel<typename decltype(t)::type, typename decltype(s)::type, l.value, e.value, false>
+            <<<grid, Z::kBlock, 0, as_stream(stream)>>>(call);
       return launched("residual_norm_forward_kernel");
     });
   });
@@ -466,7 +547,7 @@ extern "C" int dpa4k_residual_norm_backward(const void* grad_h, const void* grad
     }
     return DPA4K_OK;
   }
-  if (x == nullptr || (post_norm && post_rstd == nullptr) || (gate_kind != kGateNone && gate == nullptr) ||
+  if ((grad_h == nullptr && grad_y == nullptr) || x == nullptr || (post_norm && post_rstd == nullptr) || (gate_kind != kGateNone && gate == nullptr) ||
       (grad_y != nullptr && (!pre_norm || residual == nullptr || pre_rstd == nullptr)))
     return fail(DPA4K_EINVAL, "residual norm: null pointer");
   const int64_t blocks = backward_blocks(rows, width);
@@ -485,8 +566,13 @@ extern "C" int dpa4k_residual_norm_backward(const void* grad_h, const void* grad
   const int ran = with_types(type, residual_type, [&](auto t, auto s) {
     return with_layout(width, [&](auto l, auto e) {
       typedef Row<typename decltype(t)::type, typename decltype(s)::type, l.value, e.value> Z;
-      residual_norm_backward_kernel<typename decltype(t)::type, typename decltype(s)::type, l.value, e.value>
-          <<<launch_grid(blocks, Z::kBlock), Z::kBlock, 0, on>>>(call, blocks);
+      const dim3 grid = launch_grid(blocks, Z::kBlock);
+      if (gate_kind == kGateFull)
+        residual_norm_backward_kernel<typename decltype(t)::type, typename decltype(s)::type, l.value, e.value, true>
+            <<<grid, Z::kBlock, 0, on>>>(call, blocks);
+      else
+        residual_norm_backward_kernel<typename decltype(t)::type, typename decltype(s)::type, l.value, e.value, false>
+            <<<grid, Z::kBlock, 0, on>>>(call, blocks);
       return launched("residual_norm_backward_kernel");
     });
   });

@@ -67,14 +67,16 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T* __restrict__ p, int liv
   return out;
 }
 
-// N floats, of which the first `live` are stored.
-template <typename T, int N>
+// N floats, of which the first `live` are stored.  STREAM: past the caches, for
+// outputs that the same kernel's loads would otherwise be displaced by.
+template <bool STREAM, typename T, int N>
 __device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&value)[N], int live) {
   Pack<T, N> out;
 #pragma unroll
   for (int j = 0; j < N; ++j) out[j] = static_cast<T>(value[j]);
   if (live >= N) {
-    *reinterpret_cast<Pack<T, N>*>(p) = out;
+    if constexpr (STREAM) __builtin_nontemporal_store(out, reinterpret_cast<Pack<T, N>*>(p));
+    else *reinterpret_cast<Pack<T, N>*>(p) = out;
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -82,7 +84,29 @@ __device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&valu
   }
 }
 
-// 1 / (1 + exp(-x)) to about two roundings; 0 and 1 at the infinities.
-__device__ __forceinline__ float logistic(float x) { return 1.0f / (1.0f + expf(-x)); }
+// Row and piece of piece `at` of rows of `pieces`: divided in 32 bits where `short_`,
+// the same for the launch, says that all numbers fit.
+__device__ __forceinline__ void split_piece(int64_t at, int64_t pieces, bool short_, int64_t& row, int64_t& piece) {
+  if (short_) {
+    const uint32_t quotient = static_cast<uint32_t>(at) / static_cast<uint32_t>(pieces);
+    row = quotient;
+    piece = static_cast<uint32_t>(at) - quotient * static_cast<uint32_t>(pieces);
+  } else {
+    row = at / pieces;
+    piece = at - row * pieces;
+  }
+}
+
+// 1 / (1 + exp(-x)) to about two roundings, NaN for NaN.  The product x log2(e) is
+// carried with its rounding error; past +-90 the result is 0 and 1 to float32.
+__device__ __forceinline__ float logistic(float x) {
+  constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147182f;
+  x = x < -90.0f ? -90.0f : x;
+  x = x > 90.0f ? 90.0f : x;
+  const float t = -x * kLog2e;
+  const float rest = fmaf(-x, kLog2eRest, fmaf(-x, kLog2e, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_amdgcn_rcpf(1.0f + fmaf(e, rest * kLn2, e));
+}
 
 }  // namespace dpa4k

@@ -612,11 +612,24 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(ProductCall call, const
   const int64_t size = static_cast<int64_t>(call.n_out) * call.k_in;
   const float* from = partial + found[0] * size;
   const int count = found[1];
-  for (int64_t at = static_cast<int64_t>(blockIdx.x % blocks) * 256 + threadIdx.x; at < size; at += static_cast<int64_t>(blocks) * 256) {
+  // 32 elements at a time, eight threads each
+  __shared__ double words[8][32];
+  const int part = threadIdx.x / 32, element = threadIdx.x % 32;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x % blocks) * 32; first < size; first += static_cast<int64_t>(blocks) * 32) {
+    const int64_t at = first + element;
     double sum = 0.0;
-#pragma unroll 4
-    for (int c = 0; c < count; ++c) sum += static_cast<double>(from[c * size + at]);
-    out[e * size + at] = static_cast<T>(sum);
+    if (at < size) {
+#pragma unroll 8
+      for (int c = part; c < count; c += 8) sum += static_cast<double>(from[c * size + at]);
+    }
+    words[part][element] = sum;
+    __syncthreads();
+    if (part == 0 && at < size) {
+#pragma unroll
+      for (int p = 1; p < 8; ++p) sum += words[p][element];
+      out[e * size + at] = static_cast<T>(sum);
+    }
+    __syncthreads();
   }
 }
 
@@ -633,10 +646,12 @@ __global__ __launch_bounds__(256) void gate_backward_kernel(const T* __restrict_
                                                             int64_t rows, int half) {
   constexpr int V = kV<T>;
   const int pieces = (half + V - 1) / V;
+  const bool short_ = rows * pieces <= UINT32_MAX;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < rows * pieces; at += stride) {
-    const int64_t row = at / pieces;
-    const int column = static_cast<int>(at - row * pieces) * V;
+    int64_t row, piece;
+    split_piece(at, pieces, short_, row, piece);
+    const int column = static_cast<int>(piece) * V;
     const int live = half - column;
     const float* gates = z + row * 2 * half + column;
     const int64_t room = (rows - row) * half - column, room_z = (rows - row) * 2 * half - column;
@@ -651,8 +666,8 @@ __global__ __launch_bounds__(256) void gate_backward_kernel(const T* __restrict_
       of_gate[j] = d * up[j] * (s * fmaf(g, 1.0f - s, 1.0f));
       of_up[j] = d * (g * s);
     }
-    store_pack<T, V>(dz + row * 2 * half + column, of_gate, live);
-    store_pack<T, V>(dz + row * 2 * half + half + column, of_up, live);
+    store_pack<false, T, V>(dz + row * 2 * half + column, of_gate, live);
+    store_pack<false, T, V>(dz + row * 2 * half + half + column, of_up, live);
   }
 }
 
@@ -662,10 +677,12 @@ __global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__
                                                        T* __restrict__ dx, int64_t tokens, int k, int64_t size, int64_t limit) {
   constexpr int V = kV<T>;
   const int64_t pieces = (size + V - 1) / V;
+  const bool short_ = tokens * pieces <= UINT32_MAX;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < tokens * pieces; at += stride) {
-    const int64_t token = at / pieces;
-    const int64_t first = (at - token * pieces) * V;
+    int64_t token, piece;
+    split_piece(at, pieces, short_, token, piece);
+    const int64_t first = piece * V;
     const int live = static_cast<int>(size - first < V ? size - first : V);
     float sum[V];
 #pragma unroll
@@ -677,7 +694,7 @@ __global__ __launch_bounds__(256) void slot_sum_kernel(const float* __restrict__
 #pragma unroll
       for (int i = 0; i < V; ++i) sum[i] += part[i];
     }
-    store_pack<T, V>(dx + token * size + first, sum, live);
+    store_pack<false, T, V>(dx + token * size + first, sum, live);
   }
 }
 
@@ -691,10 +708,12 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, c
                                                       int64_t size, int64_t limit) {
   constexpr int V = kV<T>;
   const int64_t pieces = (size + V - 1) / V;
+  const bool short_ = tokens * pieces <= UINT32_MAX;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < tokens * pieces; at += stride) {
-    const int64_t token = at / pieces;
-    const int64_t first = (at - token * pieces) * V;
+    int64_t token, piece;
+    split_piece(at, pieces, short_, token, piece);
+    const int64_t first = piece * V;
     const int live = static_cast<int>(size - first < V ? size - first : V);
     float sum[V];
 #pragma unroll
@@ -708,7 +727,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, c
 #pragma unroll
       for (int i = 0; i < V; ++i) sum[i] = fmaf(w, static_cast<float>(part[i]), sum[i]);
     }
-    store_pack<T, V>(out + token * size + first, sum, live);
+    store_pack<true, T, V>(out + token * size + first, sum, live);
   }
 }
 
@@ -756,7 +775,7 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void combine_backward_kernel(
           float part[V];
 #pragma unroll
           for (int i = 0; i < V; ++i) part[i] = w * static_cast<float>(grad[i]);
-          store_pack<T, V>(dy + place * size + first, part, live);
+          store_pack<true, T, V>(dy + place * size + first, part, live);
         }
       }
     }
@@ -950,7 +969,7 @@ extern "C" int dpa4k_expert_linear_backward(const void* grad, const void* x, con
       int ran = run_product<T, kWeight>(of_w, on);
       if (ran != DPA4K_OK || chunks.most == 0) return ran;
       const int64_t size = k_in * n_out;
-      const int64_t blocks = (size + 255) / 256 < 64 ? (size + 255) / 256 : 64;
+      const int64_t blocks = (size + 31) / 32 < 512 ? (size + 31) / 32 : 512;
       weight_sum_kernel<T><<<static_cast<unsigned int>(blocks * n_experts), 256, 0, on>>>(
           of_w, static_cast<const float*>(workspace), static_cast<T*>(grad_weight), static_cast<int>(blocks));
       return launched("weight_sum_kernel");

@@ -335,7 +335,7 @@ __global__ __launch_bounds__(kBlock) void expert_route_backward_kernel(RouteCall
       if (call.scores == kSoftmax) part[j] = logit[i * Z::V + j] == -INFINITY ? 0.0f : s * (d - inner);
       else part[j] = d == 0.0f ? 0.0f : d * s * (1.0f - s);
     }
-    if (at < n) store_pack<T, Z::V>(out + row * n + at, part, n - at);
+    if (at < n) store_pack<false, T, Z::V>(out + row * n + at, part, n - at);
   }
 }
 

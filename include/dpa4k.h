@@ -602,8 +602,8 @@ int dpa4k_residual_norm_forward(const void* x, const void* residual,
                                 int gate_kind, int gate_activation, int type,
                                 int residual_type, dpa4k_stream_t stream);
 
-/* Gradients of every input from grad_h (like h) and grad_y (like y); either may
- * be NULL, and so may any output.  The gradients of the scales are float[C],
+/* Gradients of every input from grad_h (like h) and grad_y (like y); one of them
+ * may be NULL, and so may any output.  The gradients of the scales are float[C],
  * summed over all rows in a fixed order, in 64 bits past 256 rows a workgroup;
  * they alone need the workspace. */
 size_t dpa4k_residual_norm_workspace_size(int64_t rows, int64_t channels);
