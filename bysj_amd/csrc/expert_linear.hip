@@ -25,12 +25,8 @@
 
 #include "elements.h"
 
-#ifndef BIG_WM
-#define BIG_WM 2
-#define BIG_WN 4
-#endif
-#ifndef USE_BIG
-#define USE_BIG 1
+#ifndef NARROW
+#define NARROW 128, 64, 4, 1
 #endif
 namespace dpa4k {
 namespace {
@@ -45,6 +41,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 enum { kForward = 0, kGated = 1, kInput = 2, kWeight = 3 };
+// how pieces are loaded: each through its own address and registers, or straight to
+// LDS with ragged last pieces of rows, or without any
+enum { kByPiece = 0, kRagged = 1, kWhole = 2 };
 
 struct ProductCall {
   const void* a;           // x (forward), dz (dx, dW)
@@ -274,7 +273,7 @@ struct Tile {
   static_assert(kBytesA % (16 * kThreads) == 0 && kBytesB % (16 * kThreads) == 0, "whole pieces");
 };
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN, bool WHOLE>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST>
 __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductCall call, int columns, int tiles, int group) {
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   constexpr int V = kV<T>, S = kSlice<T>;
@@ -332,9 +331,12 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     }
   }
 
-  // This thread's pieces of a slice.  WHOLE: as 32-bit offsets from bases that are the
+  // This thread's pieces of a slice.  FAST: as 32-bit offsets from bases that are the
   // same for the workgroup, kNoRow where there is none; loads past the end of an
-  // operand give zeros.  Otherwise as pointers with the elements that are there.
+  // operand give zeros.  A ragged last piece of a row is the row's last 16 bytes, so
+  // that no load leaves its row: along the summed index, what it repeats is shifted
+  // out in LDS; across it, its columns of the result are stored a little further left,
+  // where its neighbour stores the same.  Otherwise as elements of which some are there.
   const T* a = static_cast<const T*>(call.a);
   const T* b = static_cast<const T*>(call.b);
   const int64_t inner = call.inner;
@@ -345,29 +347,31 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   if constexpr (MODE == kForward || MODE == kGated) {
     elements_a = rows_x * call.k_in;
   } else if constexpr (MODE == kInput) {
-    elements_a = (WHOLE ? static_cast<int64_t>(live_rows) : call.places * inner - first_row) * call.n_out;
+    elements_a = (FAST ? static_cast<int64_t>(live_rows) : call.places * inner - first_row) * call.n_out;
     a += static_cast<int64_t>(first_row) * call.n_out;
   } else {
-    elements_a = (WHOLE ? static_cast<int64_t>(depth) : call.places * inner - span.begin) * call.n_out;
+    elements_a = (FAST ? static_cast<int64_t>(depth) : call.places * inner - span.begin) * call.n_out;
     a += static_cast<int64_t>(span.begin) * call.n_out;
   }
   if constexpr (MODE == kWeight) {
     elements_b = rows_x * call.k_in;
   } else {
-    elements_b = (WHOLE ? 1 : static_cast<int64_t>(call.experts - segment)) * matrix;
+    elements_b = (FAST ? 1 : static_cast<int64_t>(call.experts - segment)) * matrix;
     b += segment * matrix;
   }
   // the piece of its row that lies where this thread's 16 bytes go (rows of this
   // thread's other pieces have the same place in the pattern)
   const int along_piece = (thread & 7) ^ ((thread >> 4) & 7);
-  typedef typename std::conditional<WHOLE, uint32_t, int64_t>::type Offset;
-  Offset from_a[Z::kPiecesA], from_b[Z::kPiecesB];       // WHOLE: bytes, else elements
+  typedef typename std::conditional<(FAST != kByPiece), uint32_t, int64_t>::type Offset;
+  Offset from_a[Z::kPiecesA], from_b[Z::kPiecesB];       // FAST: bytes, else elements
   int live_a[Z::kPiecesA], live_b[Z::kPiecesB];          // else; along: whether the row is there, across: elements
-  constexpr int kUnit = WHOLE ? static_cast<int>(sizeof(T)) : 1;
+  constexpr int kUnit = FAST ? static_cast<int>(sizeof(T)) : 1;
   const auto offset_of = [&](bool there, int64_t element) {
-    if constexpr (WHOLE) return there ? static_cast<uint32_t>(element * kUnit) : kNoRow;
+    if constexpr (FAST != kByPiece) return there ? static_cast<uint32_t>(element * kUnit) : kNoRow;
     else return element;
   };
+  // what a piece with `live` elements left in its row repeats of the one before
+  const auto repeated = [&](int live) { return FAST == kRagged && live > 0 && live < V ? V - live : 0; };
   PlaceRow of_places[Z::kPiecesA];                       // all loads before the first use
   if constexpr (MODE == kForward || MODE == kGated) {
 #pragma unroll
@@ -382,7 +386,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     if constexpr (Z::kAcrossA) {
       const int column = first_row + across_piece<T, BM>(at) * V;
       live_a[i] = call.n_out - column;
-      from_a[i] = offset_of(live_a[i] > 0, static_cast<int64_t>(at / (BM / V)) * call.n_out + column);
+      from_a[i] = offset_of(live_a[i] > 0, static_cast<int64_t>(at / (BM / V)) * call.n_out + column - repeated(live_a[i]));
     } else {
       const int row = at >> 3;
       live_a[i] = row < live_rows;
@@ -399,7 +403,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     } else if constexpr (MODE == kInput) {
       const int column = first_column + across_piece<T, BN>(at) * V;
       live_b[i] = call.k_in - column;
-      from_b[i] = offset_of(live_b[i] > 0, static_cast<int64_t>(at / (BN / V)) * call.k_in + column);
+      from_b[i] = offset_of(live_b[i] > 0, static_cast<int64_t>(at / (BN / V)) * call.k_in + column - repeated(live_b[i]));
     } else {
       const int row = at >> 3;
       int output = first_column + row;
@@ -414,36 +418,36 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     }
   }
 
-  // kNoRow for this thread's pieces behind the summed index, else 0; from the sign, as
-  // the compiler turns a choice of offsets into branches around two loads.
-  const auto past_depth = [&](int done) { return static_cast<uint32_t>(depth - 1 - (done + along_piece * V)) & kNoRow; };
-  // Starts the loads of slice `slice`.  WHOLE: straight to LDS, whose 16 bytes of a
+  // Starts the loads of slice `slice`.  FAST: straight to LDS, whose 16 bytes of a
   // wave are consecutive; zeros where there is nothing.  Else to registers.
-  u32x4 piece_a[WHOLE ? 1 : Z::kPiecesA], piece_b[WHOLE ? 1 : Z::kPiecesB];
+  u32x4 piece_a[FAST ? 1 : Z::kPiecesA], piece_b[FAST ? 1 : Z::kPiecesB];
   const auto fetch = [&](int slice, char* to_a, char* to_b) {
     const int done = slice * S;
-    const uint32_t past = past_depth(done);
-    const int64_t moved_a = Z::kAcrossA ? static_cast<int64_t>(done) * call.n_out : done;
-    const int64_t moved_b = MODE == kWeight ? 0 : Z::kAcrossB ? static_cast<int64_t>(done) * call.k_in : done;
+    const int along_left = depth - done - along_piece * V;
+    // across, the base moves; along, the offset (to before it, in a ragged last piece)
+    const int64_t moved_a = Z::kAcrossA ? static_cast<int64_t>(done) * call.n_out : FAST ? 0 : done;
+    const int64_t moved_b = MODE == kWeight ? 0 : Z::kAcrossB ? static_cast<int64_t>(done) * call.k_in : FAST ? 0 : done;
     if constexpr (MODE == kWeight) {
 #pragma unroll
       for (int i = 0; i < Z::kPiecesB; ++i) {
         const int at = thread + i * Z::kThreads, row = at / (BN / V);
         from_b[i] = offset_of(done + row < depth && live_b[i] > 0, rows_of_x[slice & 3][row] * static_cast<int64_t>(call.k_in) +
-                                                                       first_column + across_piece<T, BN>(at) * V);
+                                                                       call.k_in - live_b[i] - repeated(live_b[i]));
       }
     }
-    if constexpr (WHOLE) {
+    if constexpr (FAST != kByPiece) {
       const BufferView view_a = buffer_view(a + moved_a, (elements_a - moved_a) * static_cast<int64_t>(sizeof(T)));
       const BufferView view_b = buffer_view(b + moved_b, (elements_b - moved_b) * static_cast<int64_t>(sizeof(T)));
+      // by arithmetic, as the compiler makes branches around two loads of a choice
+      const uint32_t past = static_cast<uint32_t>(along_left - 1) & kNoRow;
+      const uint32_t further = static_cast<uint32_t>((done - repeated(along_left)) * kUnit);
 #pragma unroll
       for (int i = 0; i < Z::kPiecesA; ++i)
-        load_to_lds(view_a, Z::kAcrossA ? from_a[i] : from_a[i] | past, to_a + (wave * 64 + i * Z::kThreads) * 16);
+        load_to_lds(view_a, Z::kAcrossA ? from_a[i] : (from_a[i] + further) | past, to_a + (wave * 64 + i * Z::kThreads) * 16);
 #pragma unroll
       for (int i = 0; i < Z::kPiecesB; ++i)
-        load_to_lds(view_b, Z::kAcrossB ? from_b[i] : from_b[i] | past, to_b + (wave * 64 + i * Z::kThreads) * 16);
+        load_to_lds(view_b, Z::kAcrossB ? from_b[i] : (from_b[i] + further) | past, to_b + (wave * 64 + i * Z::kThreads) * 16);
     } else {
-      const int along_left = depth - done - along_piece * V;
 #pragma unroll
       for (int i = 0; i < Z::kPiecesA; ++i) {
         const bool there = Z::kAcrossA ? done + (thread + i * Z::kThreads) / (BM / V) < depth : live_a[i] != 0;
@@ -459,9 +463,27 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     }
   };
   // The slice that was fetched is in LDS behind the next barrier.
-  const auto land = [&](char* to_a, char* to_b) {
-    if constexpr (WHOLE) {
+  const auto land = [&](int slice, char* to_a, char* to_b) {
+    if constexpr (FAST != kByPiece) {
       __builtin_amdgcn_s_waitcnt(kNoLoadsLeft);
+      const int repeats = repeated(depth - slice * S - along_piece * V);
+      if (MODE != kWeight && repeats > 0) {
+        const int words = repeats * static_cast<int>(sizeof(T)) / 4;
+        const auto align = [&](char* piece) {
+          u32x4 w = *reinterpret_cast<u32x4*>(piece);
+          if (words & 1) w = u32x4{w[1], w[2], w[3], 0u};
+          if (words & 2) w = u32x4{w[2], w[3], 0u, 0u};
+          *reinterpret_cast<u32x4*>(piece) = w;
+        };
+        if constexpr (!Z::kAcrossA) {
+#pragma unroll
+          for (int i = 0; i < Z::kPiecesA; ++i) align(to_a + (thread + i * Z::kThreads) * 16);
+        }
+        if constexpr (!Z::kAcrossB) {
+#pragma unroll
+          for (int i = 0; i < Z::kPiecesB; ++i) align(to_b + (thread + i * Z::kThreads) * 16);
+        }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < Z::kPiecesA; ++i) *reinterpret_cast<u32x4*>(to_a + (thread + i * Z::kThreads) * 16) = piece_a[i];
@@ -508,7 +530,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   }
   if (slices > 0) {
     fetch(0, lds_a0, lds_b0);
-    land(lds_a0, lds_b0);
+    land(0, lds_a0, lds_b0);
   }
   __syncthreads();
   if (slices > 0) {
@@ -531,7 +553,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
         for (int n = 0; n < Z::kFragmentsN; ++n) sum[m][n] = multiply<T>(fa[step & 1][m], fb[step & 1][n], sum[m][n]);
       __builtin_amdgcn_sched_barrier(0);
       if (step == Z::kSteps - 2) {
-        land(next_a, next_b);
+        land(slice + 1, next_a, next_b);
         if (MODE == kWeight && thread < S) rows_of_x[(slice + 2) & 3][thread] = static_cast<int>(row_of_x(call, ahead));
         __syncthreads();
         fetch(slice + 2, at_a, at_b);
@@ -551,11 +573,13 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
 
   // register i of a lane: row 8 (i / 4) + 4 (lane / 32) + i mod 4, column lane mod 32
   const bool partial = MODE == kWeight && call.chunks > 0;
+  const auto shifted = [&](int index, int size) { return FAST == kRagged && index >= size / V * V ? (V - size % V) % V : 0; };
 #pragma unroll
   for (int m = 0; m < Z::kFragmentsM; ++m) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int row = wave_row + m * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+      int row = wave_row + m * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+      if (Z::kAcrossA) row -= shifted(first_row + row, call.n_out);
       if (row >= live_rows) continue;
       int64_t out_row = first_row + row;
       if constexpr (MODE == kInput) {
@@ -578,7 +602,8 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
             z[half + column] = up;
           }
         } else {
-          const int column = first_column + wave_column + n * 32 + (lane & 31);
+          int column = first_column + wave_column + n * 32 + (lane & 31);
+          if (Z::kAcrossB) column -= shifted(column, call.k_in);
           if (column >= width) continue;
           const int64_t at = out_row * width + column;
           if (partial || (MODE == kInput && call.by_slot)) static_cast<float*>(call.out)[at] = sum[m][n][i];
@@ -806,7 +831,7 @@ int check_product(const char* what, int64_t places, int64_t k, int64_t inner, in
   return DPA4K_OK;
 }
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN, bool WHOLE>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST>
 int launch_product(const ProductCall& call, hipStream_t stream) {
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   const int64_t rows = call.places * call.inner;
@@ -816,36 +841,40 @@ int launch_product(const ProductCall& call, hipStream_t stream) {
   if (MODE == kWeight) tiles = columns * ((call.n_out + BM - 1) / BM) * (call.chunks > 0 ? call.chunks : call.experts);
   else tiles = columns * (rows / BM + call.experts + 1);
   if (tiles > row_block_limit(Z::kThreads)) return fail(DPA4K_EINVAL, "expert linear: more tiles than a launch takes");
-  expert_product_kernel<T, MODE, BM, BN, WM, WN, WHOLE><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
+  expert_product_kernel<T, MODE, BM, BN, WM, WN, FAST><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
       call, static_cast<int>(columns), static_cast<int>(tiles), static_cast<int>(tiles >= columns * 128 ? columns * 4 : columns));
   return launched("expert_product_kernel");
 }
 
-template <typename T, int MODE, bool WHOLE>
+template <typename T, int MODE, int FAST>
 int run_tiles(const ProductCall& call, hipStream_t stream) {
   const int64_t width = MODE == kForward || MODE == kGated ? call.n_out : call.k_in;
   if constexpr (MODE == kWeight) {
-    if (call.n_out <= 64 || call.k_in <= 64) return launch_product<T, MODE, 64, 64, 2, 2, WHOLE>(call, stream);
+    if (call.n_out <= 64 || call.k_in <= 64) return launch_product<T, MODE, 64, 64, 2, 2, FAST>(call, stream);
   } else {
-    if (width <= 64) return launch_product<T, MODE, 128, 64, 4, 1, WHOLE>(call, stream);
+    if (width <= 64) return launch_product<T, MODE, NARROW, FAST>(call, stream);
   }
-  if constexpr (WHOLE && sizeof(T) == 2 && USE_BIG) {
-    if (width >= 256 && (MODE == kWeight ? call.n_out : call.places * call.inner / call.experts) >= 256)
-      return launch_product<T, MODE, 256, 256, BIG_WM, BIG_WN, WHOLE>(call, stream);
+  if constexpr (FAST == kRagged && sizeof(T) == 2) {
+    if (call.k_in % kV<T> == 0 && call.n_out % kV<T> == 0 && width >= 256 && (MODE == kWeight ? call.n_out : call.places * call.inner / call.experts) >= 256)
+      return launch_product<T, MODE, 256, 256, 2, 4, kWhole>(call, stream);
   }
-  return launch_product<T, MODE, 128, 128, 2, 2, WHOLE>(call, stream);
+  return launch_product<T, MODE, 128, 128, 2, 2, FAST>(call, stream);
 }
 
 template <typename T, int MODE>
 int run_product(const ProductCall& call, hipStream_t stream) {
-  // Pieces of 16 bytes are whole and aligned, and x and a tile of dz lie within 32-bit
-  // offsets; other calls load each piece through its own address.
+  // Rows are whole 4-byte words and hold a piece of 16 bytes at least, and x, a matrix
+  // and a tile of dz lie within 32-bit offsets (with some to spare, which a ragged
+  // piece's offset moves back by); other calls load each piece through its own
+  // address and registers.
   const int64_t rows_x = (call.order != nullptr ? call.places / call.k : call.places) * call.inner;
-  const int64_t limit = int64_t(kNoRow) / static_cast<int64_t>(sizeof(T));
-  const bool whole = call.k_in % kV<T> == 0 && call.n_out % kV<T> == 0 && aligned16(call.a) && aligned16(call.b) &&
-                     rows_x * call.k_in < limit && static_cast<int64_t>(call.n_out) * call.k_in < limit &&
-                     static_cast<int64_t>(call.n_out) * 256 < limit && static_cast<int64_t>(call.k_in) * 256 < limit;
-  return whole ? run_tiles<T, MODE, true>(call, stream) : run_tiles<T, MODE, false>(call, stream);
+  const int64_t limit = (int64_t(kNoRow) - 4096) / static_cast<int64_t>(sizeof(T));
+  const auto words = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
+  const bool fast = call.k_in * sizeof(T) % 4 == 0 && call.n_out * sizeof(T) % 4 == 0 && call.k_in >= kV<T> && call.n_out >= kV<T> &&
+                    words(call.a) && words(call.b) && rows_x * call.k_in < limit &&
+                    static_cast<int64_t>(call.n_out) * call.k_in < limit && static_cast<int64_t>(call.n_out) * 256 < limit &&
+                    static_cast<int64_t>(call.k_in) * 256 < limit;
+  return fast ? run_tiles<T, MODE, kRagged>(call, stream) : run_tiles<T, MODE, kByPiece>(call, stream);
 }
 
 // Rows of a segment that one workgroup of dW takes: all of them where the matrices
@@ -860,7 +889,7 @@ Chunks weight_chunks(int64_t places, int64_t inner, int64_t experts, int64_t k_i
   const int64_t tiles = ((n_out + edge - 1) / edge) * ((k_in + edge - 1) / edge);
   if (tiles * experts >= 512 || rows <= 512 * experts) return Chunks{INT_MAX, 0};
   int64_t chunk = (rows * tiles + 1023) / 1024;
-  chunk = (chunk + 255) / 256 * 256;
+  chunk = (chunk + 511) / 512 * 512;
   return Chunks{static_cast<int>(chunk), static_cast<int>(rows / chunk + experts)};
 }
 
