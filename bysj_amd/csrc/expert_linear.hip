@@ -25,9 +25,6 @@
 
 #include "elements.h"
 
-#ifndef NARROW
-#define NARROW 128, 64, 4, 1
-#endif
 namespace dpa4k {
 namespace {
 
@@ -44,6 +41,7 @@ enum { kForward = 0, kGated = 1, kInput = 2, kWeight = 3 };
 // how pieces are loaded: each through its own address and registers, or straight to
 // LDS with ragged last pieces of rows, or without any
 enum { kByPiece = 0, kRagged = 1, kWhole = 2 };
+constexpr int kMostRun = 8;
 
 struct ProductCall {
   const void* a;           // x (forward), dz (dx, dW)
@@ -58,6 +56,7 @@ struct ProductCall {
   int chunk_rows;          // dW: rows of a segment that one workgroup takes
   int chunks;              // dW: most chunks of all segments; 1 and no partial sums if every segment is one
   int by_slot;             // dx: written at order[p] instead of p
+  int run;                 // row tiles that one workgroup takes, up to kMostRun
 };
 
 // ---------------------------------------------------------------------------
@@ -273,7 +272,7 @@ struct Tile {
   static_assert(kBytesA % (16 * kThreads) == 0 && kBytesB % (16 * kThreads) == 0, "whole pieces");
 };
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST, bool RUN>
 __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductCall call, int columns, int tiles, int group) {
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   constexpr int V = kV<T>, S = kSlice<T>;
@@ -287,6 +286,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
 
   const int block = tile_of_block(blockIdx.x, tiles, group);
   const int column_tile = block % columns, rest = block / columns;
+  const int tile_rows = RUN ? call.run * BM : BM;
   int segment, number;
   Span span;
   int row_tile = 0, chunk = 0;
@@ -299,11 +299,12 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     if (span.end - span.begin > call.chunk_rows) span.end = span.begin + call.chunk_rows;
   } else {
     const int segments = MODE == kInput && call.by_slot ? call.experts : call.experts + 1;
-    if (!find_tile(call, segments, BM, false, rest, segment, number, span)) return;
+    if (!find_tile(call, segments, tile_rows, false, rest, segment, number, span)) return;
   }
   const int half = call.n_out / 2;                       // gated: where the second half starts
-  const int first_row = MODE == kWeight ? row_tile * BM : span.begin + number * BM;
-  const int live_rows = (MODE == kWeight ? call.n_out : span.end) - first_row;
+  const int first_row = MODE == kWeight ? row_tile * BM : span.begin + number * tile_rows;
+  const int rows_left = (MODE == kWeight ? call.n_out : span.end) - first_row;
+  const int live_rows = rows_left < tile_rows ? rows_left : tile_rows;
   const int first_column = column_tile * (MODE == kGated ? BN / 2 : BN);
   const int width = MODE == kGated ? half : (MODE == kForward ? call.n_out : call.k_in);   // columns of the result
   const int depth = MODE == kWeight ? span.end - span.begin : (MODE == kInput ? call.n_out : call.k_in);
@@ -311,24 +312,27 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   if (MODE != kWeight && segment == call.experts) {      // rows of no expert: zeros
     constexpr int kTileColumns = MODE == kGated ? BN / 2 : BN;
     T* y = static_cast<T*>(call.out);
-    const int rows = live_rows < BM ? live_rows : BM;
-    for (int at = thread; at < rows * kTileColumns; at += Z::kThreads) {
+    for (int at = thread; at < live_rows * kTileColumns; at += Z::kThreads) {
       const int c = first_column + at % kTileColumns;
       if (c < width) y[static_cast<int64_t>(first_row + at / kTileColumns) * width + c] = static_cast<T>(0.0f);
     }
     return;
   }
 
-  // dx by slot: where the tile's rows go, -1 for a slot that is none
-  __shared__ int out_rows[MODE == kInput ? BM : 1];
+  // dx by slot: where the rows go, -1 for a slot that is none; forward, in runs:
+  // the rows of x
+  constexpr int kRows = RUN ? kMostRun * BM : BM;
+  __shared__ int row_words[MODE == kInput || (RUN && MODE != kWeight) ? kRows : 1];
   if constexpr (MODE == kInput) {
-    if (call.by_slot && thread < BM && thread < live_rows) {
-      const int row = first_row + thread;
-      const int place = call.inner == 1 ? row : static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(call.inner));
-      const int64_t slot = call.order[place];
-      out_rows[thread] = static_cast<uint64_t>(slot) < static_cast<uint64_t>(call.places)
-                             ? static_cast<int>(slot) * call.inner + (row - place * call.inner) : -1;
+    for (int row = thread; call.by_slot && row < live_rows; row += Z::kThreads) {
+      const PlaceRow at = place_row(call, first_row + row);
+      row_words[row] = static_cast<uint64_t>(at.slot) < static_cast<uint64_t>(call.places)
+                           ? static_cast<int>(at.slot) * call.inner + at.inside : -1;
     }
+  } else if constexpr (RUN && MODE != kWeight) {
+    for (int row = thread; row < live_rows; row += Z::kThreads)
+      row_words[row] = static_cast<int>(row_of_x(call, place_row(call, first_row + row)));
+    __syncthreads();
   }
 
   // This thread's pieces of a slice.  FAST: as 32-bit offsets from bases that are the
@@ -373,7 +377,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   // what a piece with `live` elements left in its row repeats of the one before
   const auto repeated = [&](int live) { return FAST == kRagged && live > 0 && live < V ? V - live : 0; };
   PlaceRow of_places[Z::kPiecesA];                       // all loads before the first use
-  if constexpr (MODE == kForward || MODE == kGated) {
+  if constexpr (!RUN && (MODE == kForward || MODE == kGated)) {
 #pragma unroll
     for (int i = 0; i < Z::kPiecesA; ++i) {
       const int row = (thread + i * Z::kThreads) >> 3;
@@ -387,7 +391,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       const int column = first_row + across_piece<T, BM>(at) * V;
       live_a[i] = call.n_out - column;
       from_a[i] = offset_of(live_a[i] > 0, static_cast<int64_t>(at / (BM / V)) * call.n_out + column - repeated(live_a[i]));
-    } else {
+    } else if constexpr (!RUN) {
       const int row = at >> 3;
       live_a[i] = row < live_rows;
       const int64_t of_row = MODE == kInput ? row : row_of_x(call, of_places[i]);
@@ -418,10 +422,10 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     }
   }
 
-  // Starts the loads of slice `slice`.  FAST: straight to LDS, whose 16 bytes of a
+  // Starts the loads of slice `slice` of row tile `tile` of the run.  FAST: straight to LDS, whose 16 bytes of a
   // wave are consecutive; zeros where there is nothing.  Else to registers.
   u32x4 piece_a[FAST ? 1 : Z::kPiecesA], piece_b[FAST ? 1 : Z::kPiecesB];
-  const auto fetch = [&](int slice, char* to_a, char* to_b) {
+  const auto fetch = [&](int tile, int slice, char* to_a, char* to_b) {
     const int done = slice * S;
     const int along_left = depth - done - along_piece * V;
     // across, the base moves; along, the offset (to before it, in a ragged last piece)
@@ -441,6 +445,15 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       // by arithmetic, as the compiler makes branches around two loads of a choice
       const uint32_t past = static_cast<uint32_t>(along_left - 1) & kNoRow;
       const uint32_t further = static_cast<uint32_t>((done - repeated(along_left)) * kUnit);
+      if constexpr (RUN && !Z::kAcrossA) {
+#pragma unroll
+        for (int i = 0; i < Z::kPiecesA; ++i) {
+          const int row = tile * BM + ((thread + i * Z::kThreads) >> 3);
+          int of_row = row;
+          if constexpr (MODE != kInput) of_row = row_words[row < live_rows ? row : 0];
+          from_a[i] = offset_of(row < live_rows, static_cast<int64_t>(of_row) * ld_a + along_piece * V);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < Z::kPiecesA; ++i)
         load_to_lds(view_a, Z::kAcrossA ? from_a[i] : (from_a[i] + further) | past, to_a + (wave * 64 + i * Z::kThreads) * 16);
@@ -493,12 +506,14 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   };
 
   f32x16 sum[Z::kFragmentsM][Z::kFragmentsN];
+  const auto clear = [&] {
 #pragma unroll
-  for (int m = 0; m < Z::kFragmentsM; ++m)
+    for (int m = 0; m < Z::kFragmentsM; ++m)
 #pragma unroll
-    for (int n = 0; n < Z::kFragmentsN; ++n)
+      for (int n = 0; n < Z::kFragmentsN; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum[m][n][i] = 0.0f;
+        for (int i = 0; i < 16; ++i) sum[m][n][i] = 0.0f;
+  };
 
   // Slice s is multiplied from one half of LDS while s + 1 is on its way to the other;
   // inside a slice, the operands of the next step are read while one step's
@@ -529,18 +544,19 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     __syncthreads();
   }
   if (slices > 0) {
-    fetch(0, lds_a0, lds_b0);
+    fetch(0, 0, lds_a0, lds_b0);
     land(0, lds_a0, lds_b0);
   }
   __syncthreads();
   if (slices > 0) {
-    fetch(1, lds_a1, lds_b1);
+    fetch(0, 1, lds_a1, lds_b1);
     read(lds_a0, lds_b0, 0, fa[0], fb[0]);
   }
   // The half at `at` is read for the last time in front of the third step's products;
   // behind them every wave has read it and the next slice has landed, so that the
   // last step's products hide the next slice's first reads.
-  const auto turn = [&](int slice, char* at_a, char* at_b, char* next_a, char* next_b) {
+  // `slice` is multiplied, `landing` lands in the other half, `coming` of `tile` starts.
+  const auto turn = [&](int slice, int landing, int tile, int coming, char* at_a, char* at_b, char* next_a, char* next_b) {
 #pragma unroll
     for (int step = 0; step < Z::kSteps; ++step) {
       const int to = (step + 1) & 1;
@@ -553,65 +569,224 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
         for (int n = 0; n < Z::kFragmentsN; ++n) sum[m][n] = multiply<T>(fa[step & 1][m], fb[step & 1][n], sum[m][n]);
       __builtin_amdgcn_sched_barrier(0);
       if (step == Z::kSteps - 2) {
-        land(slice + 1, next_a, next_b);
+        land(landing, next_a, next_b);
         if (MODE == kWeight && thread < S) rows_of_x[(slice + 2) & 3][thread] = static_cast<int>(row_of_x(call, ahead));
         __syncthreads();
-        fetch(slice + 2, at_a, at_b);
+        fetch(tile, coming, at_a, at_b);
         look_ahead(slice + 3);
       }
     }
   };
-  // the two halves by name: the compiler then sees that reads of one need not wait
-  // for loads to the other
-  int slice = 0;
-  for (; slice + 1 < slices; slice += 2) {
-    turn(slice, lds_a0, lds_b0, lds_a1, lds_b1);
-    turn(slice + 1, lds_a1, lds_b1, lds_a0, lds_b0);
-  }
-  if (slice < slices) turn(slice, lds_a0, lds_b0, lds_a1, lds_b1);
-  __builtin_amdgcn_s_waitcnt(kNoLoadsLeft);              // the workgroup's LDS is not given away while loads to it are under way
-
-  // register i of a lane: row 8 (i / 4) + 4 (lane / 32) + i mod 4, column lane mod 32
+  // Register i of a lane: row 8 (i / 4) + 4 (lane / 32) + i mod 4, column lane mod 32
   const bool partial = MODE == kWeight && call.chunks > 0;
   const auto shifted = [&](int index, int size) { return FAST == kRagged && index >= size / V * V ? (V - size % V) % V : 0; };
+  const auto store = [&](int tile) {
+    const int above = tile * BM;                           // rows of the run above this tile
 #pragma unroll
-  for (int m = 0; m < Z::kFragmentsM; ++m) {
+    for (int m = 0; m < Z::kFragmentsM; ++m) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      int row = wave_row + m * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
-      if (Z::kAcrossA) row -= shifted(first_row + row, call.n_out);
-      if (row >= live_rows) continue;
-      int64_t out_row = first_row + row;
-      if constexpr (MODE == kInput) {
-        if (call.by_slot) out_row = out_rows[row];
-        if (out_row < 0) continue;
-      } else if constexpr (MODE == kWeight) {
-        out_row += static_cast<int64_t>(partial ? chunk : segment) * call.n_out;
-      }
+      for (int i = 0; i < 16; ++i) {
+        int row = above + wave_row + m * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+        if (Z::kAcrossA) row -= shifted(first_row + row, call.n_out);
+        if (row >= live_rows) continue;
+        int64_t out_row = first_row + row;
+        if constexpr (MODE == kInput) {
+          if (call.by_slot) out_row = row_words[row];
+          if (out_row < 0) continue;
+        } else if constexpr (MODE == kWeight) {
+          out_row += static_cast<int64_t>(partial ? chunk : segment) * call.n_out;
+        }
 #pragma unroll
-      for (int n = 0; n < Z::kFragmentsN; ++n) {
-        if constexpr (MODE == kGated) {
-          if (n % 2 != 0) continue;
-          const int column = first_column + (wave_column >> 1) + (n / 2) * 32 + (lane & 31);
-          if (column >= half) continue;
-          const float gate = sum[m][n][i], up = sum[m][n + 1][i];
-          static_cast<T*>(call.out)[out_row * half + column] = static_cast<T>(gate * logistic(gate) * up);
-          if (call.before != nullptr) {
-            float* z = call.before + out_row * call.n_out;
-            z[column] = gate;
-            z[half + column] = up;
+        for (int n = 0; n < Z::kFragmentsN; ++n) {
+          if constexpr (MODE == kGated) {
+            if (n % 2 != 0) continue;
+            const int column = first_column + (wave_column >> 1) + (n / 2) * 32 + (lane & 31);
+            if (column >= half) continue;
+            const float gate = sum[m][n][i], up = sum[m][n + 1][i];
+            static_cast<T*>(call.out)[out_row * half + column] = static_cast<T>(gate * logistic(gate) * up);
+            if (call.before != nullptr) {
+              float* z = call.before + out_row * call.n_out;
+              z[column] = gate;
+              z[half + column] = up;
+            }
+          } else {
+            int column = first_column + wave_column + n * 32 + (lane & 31);
+            if (Z::kAcrossB) column -= shifted(column, call.k_in);
+            if (column >= width) continue;
+            const int64_t at = out_row * width + column;
+            if (partial || (MODE == kInput && call.by_slot)) static_cast<float*>(call.out)[at] = sum[m][n][i];
+            else static_cast<T*>(call.out)[at] = static_cast<T>(sum[m][n][i]);
           }
-        } else {
-          int column = first_column + wave_column + n * 32 + (lane & 31);
-          if (Z::kAcrossB) column -= shifted(column, call.k_in);
-          if (column >= width) continue;
-          const int64_t at = out_row * width + column;
-          if (partial || (MODE == kInput && call.by_slot)) static_cast<float*>(call.out)[at] = sum[m][n][i];
-          else static_cast<T*>(call.out)[at] = static_cast<T>(sum[m][n][i]);
         }
       }
     }
+  };
+
+  // the two halves by name: the compiler then sees that reads of one need not wait
+  // for loads to the other
+  if constexpr (RUN) {
+    // every tile takes an even number of slices, so that the halves do not change
+    // places: a last odd one is followed by zeros
+    const int padded = slices + (slices & 1);
+    for (int tile = 0; tile * BM < live_rows; ++tile) {
+      clear();
+      for (int slice = 0; slice < padded; slice += 2) {
+        const bool wraps = slice + 2 >= padded;
+        const int coming = wraps ? 0 : slice + 2;
+        turn(slice, slice + 1, wraps ? tile + 1 : tile, coming, lds_a0, lds_b0, lds_a1, lds_b1);
+        turn(slice + 1, coming, wraps ? tile + 1 : tile, coming + 1, lds_a1, lds_b1, lds_a0, lds_b0);
+      }
+      store(tile);
+    }
+  } else {
+    clear();
+    int slice = 0;
+    for (; slice + 1 < slices; slice += 2) {
+      turn(slice, slice + 1, 0, slice + 2, lds_a0, lds_b0, lds_a1, lds_b1);
+      turn(slice + 1, slice + 2, 0, slice + 3, lds_a1, lds_b1, lds_a0, lds_b0);
+    }
+    if (slice < slices) turn(slice, slice + 1, 0, slice + 2, lds_a0, lds_b0, lds_a1, lds_b1);
+    store(0);
   }
+  __builtin_amdgcn_s_waitcnt(kNoLoadsLeft);              // the workgroup's LDS is not given away while loads to it are under way
+}
+
+// ---------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------
+
+// Forward for a few rows an expert, as when single tokens are served: bound by reading
+// the matrices once.  A workgroup takes 16 rows and 64 rows of W (gated: 32 gates
+// and their partners); its four waves take every fourth 64 bytes of the summed index,
+// each lane 16 of them, straight into the operands of the matrix unit, and add up
+// in LDS.  WHOLE: rows of whole 16-byte pieces.
+typedef float f32x4m __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ f32x4m multiply16(const u32x4& a, const u32x4& b, f32x4m sum) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), sum, 0, 0, 0);
+    return sum;
+  } else if constexpr (std::is_same<T, __bf16>::value) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), sum, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), sum, 0, 0, 0);
+  }
+}
+
+template <typename T, bool GATED, bool WHOLE>
+__global__ __launch_bounds__(256) void expert_few_rows_kernel(ProductCall call, int columns) {
+  constexpr int V = kV<T>, kRows = 16, kColumns = 64, kGroups = kColumns / 16, kStep = 4 * V, kAhead = 4;
+  __shared__ float words[4][kRows][kColumns + 4];
+  const int thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
+  const int column_tile = static_cast<int>(blockIdx.x) % columns;
+  int segment, number;
+  Span span;
+  if (!find_tile(call, call.experts + 1, kRows, false, static_cast<int>(blockIdx.x) / columns, segment, number, span)) return;
+  const int half = call.n_out / 2;
+  const int width = GATED ? half : call.n_out;
+  constexpr int kOut = GATED ? kColumns / 2 : kColumns;
+  const int first_row = span.begin + number * kRows, first_column = column_tile * kOut;
+  const int live_rows = span.end - first_row < kRows ? span.end - first_row : kRows;
+  T* y = static_cast<T*>(call.out);
+  if (segment == call.experts) {
+    for (int at = thread; at < live_rows * kOut; at += 256) {
+      const int c = first_column + at % kOut;
+      if (c < width) y[static_cast<int64_t>(first_row + at / kOut) * width + c] = static_cast<T>(0.0f);
+    }
+    return;
+  }
+  // lane l: row (of x and of W) l mod 16, piece l / 16 of a step
+  const int piece = (lane >> 4) * V;
+  const T* x = static_cast<const T*>(call.a);
+  const T* w = static_cast<const T*>(call.b);
+  const int64_t end_x = (call.order != nullptr ? call.places / call.k : call.places) * static_cast<int64_t>(call.inner) * call.k_in;
+  const int64_t end_w = static_cast<int64_t>(call.experts) * call.n_out * call.k_in;
+  const bool row_there = (lane & 15) < live_rows;
+  const int64_t from_x = row_of_x(call, place_row(call, first_row + (row_there ? lane & 15 : 0))) * call.k_in;
+  int64_t from_w[kGroups];
+  bool there[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    int output = first_column + g * 16 + (lane & 15);
+    there[g] = output < width;
+    if constexpr (GATED) {
+      output = first_column + (g & 1) * 16 + (lane & 15);
+      there[g] = output < half;
+      if (g >= 2) output += half;
+    }
+    from_w[g] = (static_cast<int64_t>(segment) * call.n_out + (there[g] ? output : 0)) * call.k_in;
+  }
+  f32x4m sum[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) sum[g] = f32x4m{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto load = [&](const T* p, int64_t from, int64_t end, int k, bool is_there) {
+    const int left = is_there ? call.k_in - k : 0;
+    if constexpr (WHOLE) {
+      const Pack<T, V> raw = *reinterpret_cast<const Pack<T, V>*>(p + from + (left > 0 ? k : 0));
+      u32x4 out;
+      __builtin_memcpy(&out, &raw, 16);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) out[d] = left > 0 ? out[d] : 0u;
+      return out;
+    } else {
+      return load_piece<T>(p + from + k, left, end - from - k);
+    }
+  };
+  const int steps = (call.k_in + kStep - 1) / kStep;
+  for (int first = wave; first < steps; first += 4 * kAhead) {
+    u32x4 px[kAhead], pw[kAhead][kGroups];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k = (first + 4 * i) * kStep + piece;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) pw[i][g] = load(w, from_w[g], end_w, k, there[g]);
+      px[i] = load(x, from_x, end_x, k, row_there);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) sum[g] = multiply16<T>(px[i], pw[i][g], sum[g]);
+  }
+  // register i of a lane: row 4 (lane / 16) + i, column lane mod 16
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) words[wave][4 * (lane >> 4) + i][g * 16 + (lane & 15)] = sum[g][i];
+  __syncthreads();
+  for (int at = thread; at < live_rows * kOut; at += 256) {
+    const int row = at / kOut, c = at % kOut, column = first_column + c;
+    if (column >= width) continue;
+    const auto total = [&](int place) {
+      return (words[0][row][place] + words[1][row][place]) + (words[2][row][place] + words[3][row][place]);
+    };
+    const int64_t out_row = first_row + row;
+    if constexpr (GATED) {
+      const float gate = total(c), up = total(c + 32);
+      y[out_row * half + column] = static_cast<T>(gate * logistic(gate) * up);
+      if (call.before != nullptr) {
+        call.before[out_row * call.n_out + column] = gate;
+        call.before[out_row * call.n_out + half + column] = up;
+      }
+    } else {
+      y[out_row * width + column] = static_cast<T>(total(c));
+    }
+  }
+}
+
+template <typename T, bool GATED>
+int run_few_rows(const ProductCall& call, hipStream_t stream) {
+  const int width = GATED ? call.n_out / 2 : call.n_out;
+  const int64_t columns = (width + (GATED ? 31 : 63)) / (GATED ? 32 : 64);
+  const int64_t tiles = columns * (call.places * call.inner / 16 + call.experts + 1);
+  if (tiles > row_block_limit(256)) return fail(DPA4K_EINVAL, "expert linear: more tiles than a launch takes");
+  const unsigned int grid = static_cast<unsigned int>(tiles);
+  if (call.k_in % kV<T> == 0)
+    expert_few_rows_kernel<T, GATED, true><<<grid, 256, 0, stream>>>(call, static_cast<int>(columns));
+  else
+    expert_few_rows_kernel<T, GATED, false><<<grid, 256, 0, stream>>>(call, static_cast<int>(columns));
+  return launched("expert_few_rows_kernel");
 }
 
 // dW[e] = the sum of its chunks' partial sums, in order, in 64 bits.
@@ -831,17 +1006,17 @@ int check_product(const char* what, int64_t places, int64_t k, int64_t inner, in
   return DPA4K_OK;
 }
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST>
-int launch_product(const ProductCall& call, hipStream_t stream) {
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST, bool RUN = false>
+int launch_product(ProductCall call, hipStream_t stream) {
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   const int64_t rows = call.places * call.inner;
   const int64_t width = MODE == kGated ? call.n_out / 2 : (MODE == kForward ? call.n_out : call.k_in);
   const int64_t columns = (width + (MODE == kGated ? BN / 2 : BN) - 1) / (MODE == kGated ? BN / 2 : BN);
   int64_t tiles;
   if (MODE == kWeight) tiles = columns * ((call.n_out + BM - 1) / BM) * (call.chunks > 0 ? call.chunks : call.experts);
-  else tiles = columns * (rows / BM + call.experts + 1);
+  else tiles = columns * (rows / (RUN ? call.run * BM : BM) + call.experts + 1);
   if (tiles > row_block_limit(Z::kThreads)) return fail(DPA4K_EINVAL, "expert linear: more tiles than a launch takes");
-  expert_product_kernel<T, MODE, BM, BN, WM, WN, FAST><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
+  expert_product_kernel<T, MODE, BM, BN, WM, WN, FAST, RUN><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
       call, static_cast<int>(columns), static_cast<int>(tiles), static_cast<int>(tiles >= columns * 128 ? columns * 4 : columns));
   return launched("expert_product_kernel");
 }
@@ -852,10 +1027,33 @@ int run_tiles(const ProductCall& call, hipStream_t stream) {
   if constexpr (MODE == kWeight) {
     if (call.n_out <= 64 || call.k_in <= 64) return launch_product<T, MODE, 64, 64, 2, 2, FAST>(call, stream);
   } else {
-    if (width <= 64) return launch_product<T, MODE, NARROW, FAST>(call, stream);
+    // Short sums over many rows: the workgroups' starts (the segment, the rows of x, the
+    // first loads) take longer than their products, so each takes a run of tiles
+    // and loads the next one while it multiplies and stores (786,432 rows of 64 by
+    // 64 in float32: forward 114 -> 104 us, dx 127 -> 116 us; in two rounds 107 and 119).
+    if constexpr (FAST == kRagged) {
+      const int64_t depth = MODE == kInput ? call.n_out : call.k_in;
+      const int64_t rows = call.places * call.inner, columns = width <= 64 ? 1 : (width + 127) / 128;
+      const int64_t tiles = rows / 128 * columns, resident = width <= 64 ? 768 : 512;
+      constexpr int64_t kRounds = 4;   // of workgroups, so that short runs at the segments' ends even out
+      if (depth <= 4 * kSlice<T> && tiles >= 2 * kRounds * resident) {
+        ProductCall runs = call;
+        runs.run = static_cast<int>(tiles / (kRounds * resident) < kMostRun ? tiles / (kRounds * resident) : kMostRun);
+        if (width <= 64) return launch_product<T, MODE, 128, 64, 4, 1, FAST, true>(runs, stream);
+        return launch_product<T, MODE, 128, 128, 2, 2, FAST, true>(runs, stream);
+      }
+    }
+    // Float32 is bound by its products: where segments are short, tiles of 32 rows
+    // multiply fewer rows that are not there (64 rows an expert, 1,024 to 2 x 2,048:
+    // 327 -> 237 us; bfloat16 81 -> 103 us).
+    if constexpr (sizeof(T) == 4) {
+      if (call.places * call.inner < 96 * call.experts) return launch_product<T, MODE, 32, 128, 1, 2, FAST>(call, stream);
+    }
+    if (width <= 64) return launch_product<T, MODE, 128, 64, 4, 1, FAST>(call, stream);
   }
   if constexpr (FAST == kRagged && sizeof(T) == 2) {
-    if (call.k_in % kV<T> == 0 && call.n_out % kV<T> == 0 && width >= 256 && (MODE == kWeight ? call.n_out : call.places * call.inner / call.experts) >= 256)
+    if (call.k_in % kV<T> == 0 && call.n_out % kV<T> == 0 && width >= 256 &&
+        (MODE == kWeight ? call.n_out : call.places * call.inner / call.experts) >= 256)
       return launch_product<T, MODE, 256, 256, 2, 4, kWhole>(call, stream);
   }
   return launch_product<T, MODE, 128, 128, 2, 2, FAST>(call, stream);
@@ -918,6 +1116,11 @@ extern "C" int dpa4k_expert_linear_forward(const void* x, const void* weight, co
   call.k_in = static_cast<int>(k_in), call.n_out = static_cast<int>(n_out);
   return with_type(type, DPA4K_EINVAL, [&](auto t) {
     typedef typename decltype(t)::type T;
+    // Rows an expert up to which the matrices' bytes bound it (1,024 to 2 x 2,048, 32
+    // experts, us, this way and in tiles: bfloat16 34 and 45 at one row, 56 and 55 at
+    // eight, 70 and 58 at 16; float32 143 and 188 at 16 rows, 213 and 178 at 32).
+    if (places * inner <= (sizeof(T) == 4 ? 24 : 8) * n_experts)
+      return gated ? run_few_rows<T, true>(call, as_stream(stream)) : run_few_rows<T, false>(call, as_stream(stream));
     return gated ? run_product<T, kGated>(call, as_stream(stream)) : run_product<T, kForward>(call, as_stream(stream));
   });
 }

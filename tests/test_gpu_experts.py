@@ -268,6 +268,32 @@ def test_linear_long_segments(dtype):
     _check_linear(_plan(2500, 2, 3, seed=8), 3, (), 136, 200, dtype, from_tokens=False, gated=True, what="long")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("k_in,n_out,gated", [(264, 304, False), (256, 264, True), (520, 272, False), (266, 300, False)])
+def test_linear_large_matrices(k_in, n_out, gated, dtype):
+    """Several hundred rows an expert through matrices of more than 256 by 256 (tiles of 256 by 256, or of 128 where a
+    row is no whole pieces of 16 bytes), one segment far longer than the others, one of a single row."""
+    generator = torch.Generator().manual_seed(k_in)
+    chosen = torch.randint(0, 4, (900, 2), generator=generator)
+    chosen[torch.rand(900, generator=generator) < 0.6] = 1
+    chosen[0, 0] = 4
+    plan = expert_dispatch_reference(chosen, 5)
+    for from_tokens in (True, False):
+        _check_linear(plan, 5, (), k_in, n_out, dtype, from_tokens=from_tokens, gated=gated, seed=k_in, what="large")
+
+
+@pytest.mark.parametrize("dtype,k_in,n_out,gated", [(F32, 8, 12, False), (BF16, 16, 10, False), (BF16, 8, 6, True), (F16, 10, 72, False)])
+def test_linear_many_rows(dtype, k_in, n_out, gated):
+    """So many rows that a workgroup takes a run of tiles: segments of any length, one without rows, places of none."""
+    generator = torch.Generator().manual_seed(n_out)
+    chosen = torch.multinomial(torch.tensor([0.5, 0.0, 0.3, 0.01, 0.19]), 26_000, replacement=True, generator=generator)[:, None]
+    chosen[torch.rand(26_000, generator=generator) < 0.02] = -1
+    plan = expert_dispatch(chosen.to(DEV), 5)
+    plan = tuple(t.cpu() for t in plan)
+    for from_tokens in (True, False):
+        _check_linear(plan, 5, (33,), k_in, n_out, dtype, from_tokens=from_tokens, gated=gated, seed=1, what="many rows")
+
+
 def test_linear_only_what_is_wanted():
     plan = ExpertPlan(*(t.to(DEV) for t in _plan(50, 2, 4, seed=3)))
     x, weight = torch.randn(50, 32, device=DEV), torch.randn(4, 16, 32, device=DEV)
