@@ -566,7 +566,11 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
 #pragma unroll
       for (int m = 0; m < Z::kFragmentsM; ++m)
 #pragma unroll
-        for (int n = 0; n < Z::kFragmentsN; ++n) sum[m][n] = multiply<T>(fa[step & 1][m], fb[step & 1][n], sum[m][n]);
+        for (int n = 0; n < Z::kFragmentsN; ++n) {
+          // gated: rows of the result are the matrix unit's rows, else its columns
+          if constexpr (MODE == kGated) sum[m][n] = multiply<T>(fa[step & 1][m], fb[step & 1][n], sum[m][n]);
+          else sum[m][n] = multiply<T>(fb[step & 1][n], fa[step & 1][m], sum[m][n]);
+        }
       __builtin_amdgcn_sched_barrier(0);
       if (step == Z::kSteps - 2) {
         land(landing, next_a, next_b);
@@ -577,29 +581,25 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       }
     }
   };
-  // Register i of a lane: row 8 (i / 4) + 4 (lane / 32) + i mod 4, column lane mod 32
+  // Register i of a lane is row 8 (i / 4) + 4 (lane / 32) + i mod 4 and column lane mod 32
+  // of the matrix unit's result.  Its rows are the columns here: four values are
+  // stored at once and a lane has few rows to find (dx of the largest case 378 -> 354
+  // us).  Gated, its rows are the rows, so that z is stored in whole lines of 128 bytes
+  // (516 -> 458 us forward).
   const bool partial = MODE == kWeight && call.chunks > 0;
   const auto shifted = [&](int index, int size) { return FAST == kRagged && index >= size / V * V ? (V - size % V) % V : 0; };
   const auto store = [&](int tile) {
-    const int above = tile * BM;                           // rows of the run above this tile
+    const int above = tile * BM;                         // rows of the run above this tile
+    if constexpr (MODE == kGated) {
 #pragma unroll
-    for (int m = 0; m < Z::kFragmentsM; ++m) {
+      for (int m = 0; m < Z::kFragmentsM; ++m) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        int row = above + wave_row + m * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
-        if (Z::kAcrossA) row -= shifted(first_row + row, call.n_out);
-        if (row >= live_rows) continue;
-        int64_t out_row = first_row + row;
-        if constexpr (MODE == kInput) {
-          if (call.by_slot) out_row = row_words[row];
-          if (out_row < 0) continue;
-        } else if constexpr (MODE == kWeight) {
-          out_row += static_cast<int64_t>(partial ? chunk : segment) * call.n_out;
-        }
+        for (int i = 0; i < 16; ++i) {
+          const int row = above + wave_row + m * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
+          if (row >= live_rows) continue;
+          const int64_t out_row = first_row + row;
 #pragma unroll
-        for (int n = 0; n < Z::kFragmentsN; ++n) {
-          if constexpr (MODE == kGated) {
-            if (n % 2 != 0) continue;
+          for (int n = 0; n < Z::kFragmentsN; n += 2) {
             const int column = first_column + (wave_column >> 1) + (n / 2) * 32 + (lane & 31);
             if (column >= half) continue;
             const float gate = sum[m][n][i], up = sum[m][n + 1][i];
@@ -609,14 +609,37 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
               z[column] = gate;
               z[half + column] = up;
             }
-          } else {
-            int column = first_column + wave_column + n * 32 + (lane & 31);
-            if (Z::kAcrossB) column -= shifted(column, call.k_in);
-            if (column >= width) continue;
-            const int64_t at = out_row * width + column;
-            if (partial || (MODE == kInput && call.by_slot)) static_cast<float*>(call.out)[at] = sum[m][n][i];
-            else static_cast<T*>(call.out)[at] = static_cast<T>(sum[m][n][i]);
           }
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int m = 0; m < Z::kFragmentsM; ++m) {
+      int row = above + wave_row + m * 32 + (lane & 31);
+      if (Z::kAcrossA) row -= shifted(first_row + row, call.n_out);
+      if (row >= live_rows) continue;
+      int64_t out_row = first_row + row;
+      if constexpr (MODE == kInput) {
+        if (call.by_slot) out_row = row_words[row];
+        if (out_row < 0) continue;
+      } else if constexpr (MODE == kWeight) {
+        out_row += static_cast<int64_t>(partial ? chunk : segment) * call.n_out;
+      }
+#pragma unroll
+      for (int n = 0; n < Z::kFragmentsN; ++n) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int inside = 8 * g + 4 * (lane >> 5);
+          int column = first_column + wave_column + n * 32 + inside;
+          if (Z::kAcrossB) column -= shifted(column, call.k_in);
+          if (column >= width) continue;
+          const int64_t at = out_row * width + column;
+          float four[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) four[i] = sum[m][n][4 * g + i];
+          if (partial || (MODE == kInput && call.by_slot)) store_pack<false, float, 4>(static_cast<float*>(call.out) + at, four, width - column);
+          else store_pack<false, T, 4>(static_cast<T*>(call.out) + at, four, width - column);
         }
       }
     }
