@@ -87,10 +87,15 @@ __device__ __forceinline__ int tile_of_block(int block, int tiles, int group) {
   return (index / group * static_cast<int>(kXcds) + die) * group + index % group;
 }
 
-// Tiles of `rows` rows of a segment; `empty`: an empty one has a tile too.
+// Tiles of `rows` rows of a segment; `empty`: an empty one has a tile too.  At most
+// kMostTiles, which is more than a launch has, so that the sums over 64 segments fit
+// 32 bits whatever the offsets (those of a malformed plan may overlap).
+constexpr int kMostTiles = 1 << 24;
+
 __device__ __forceinline__ int tiles_of(const Span& span, int rows, bool empty) {
   const int length = span.end - span.begin;
-  return length > 0 ? (length - 1) / rows + 1 : (empty ? 1 : 0);
+  const int tiles = length > 0 ? (length - 1) / rows + 1 : (empty ? 1 : 0);
+  return tiles < kMostTiles ? tiles : kMostTiles;
 }
 
 // The segment that tile `tile` of tiles of `rows` rows belongs to, and the tile's
@@ -819,22 +824,24 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(ProductCall call, const
   const int e = blockIdx.x / blocks;
   // the first chunk of the expert: chunks of the ones before
   __shared__ int found[2];
+  // not past the chunks there are: segments of a malformed plan may overlap
+  const auto there = [&](int chunk) { return chunk < call.chunks ? chunk : call.chunks; };
   if (threadIdx.x < 64) {
     int before = 0, mine = 1;
     for (int f = threadIdx.x; f <= e; f += 64) {
       const Span span = span_of(call, f);
       const int count = tiles_of(span, call.chunk_rows, true);
-      if (f < e) before += count;
-      else mine = count;
+      if (f < e) before = there(before + there(count));
+      else mine = there(count);
     }
-    before = group_sum<64>(before);
+    before = there(group_sum<64>(before));
     if (threadIdx.x == 0) found[0] = before;
     if (static_cast<int>(threadIdx.x) == e % 64) found[1] = mine;
   }
   __syncthreads();
   const int64_t size = static_cast<int64_t>(call.n_out) * call.k_in;
   const float* from = partial + found[0] * size;
-  const int count = found[1];
+  const int count = there(found[0] + found[1]) - found[0];
   // 32 elements at a time, eight threads each
   __shared__ double words[8][32];
   const int part = threadIdx.x / 32, element = threadIdx.x % 32;
@@ -1039,8 +1046,11 @@ int launch_product(ProductCall call, hipStream_t stream) {
   if (MODE == kWeight) tiles = columns * ((call.n_out + BM - 1) / BM) * (call.chunks > 0 ? call.chunks : call.experts);
   else tiles = columns * (rows / (RUN ? call.run * BM : BM) + call.experts + 1);
   if (tiles > row_block_limit(Z::kThreads)) return fail(DPA4K_EINVAL, "expert linear: more tiles than a launch takes");
+  // two row tiles with all their columns; of dW, one (the largest case: forward 459 ->
+  // 420 us against four, dW 439 -> 418 us, as dies then get more equal shares)
+  const int64_t group = MODE != kWeight && tiles >= columns * 64 ? columns * 2 : columns;
   expert_product_kernel<T, MODE, BM, BN, WM, WN, FAST, RUN><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
-      call, static_cast<int>(columns), static_cast<int>(tiles), static_cast<int>(tiles >= columns * 128 ? columns * 4 : columns));
+      call, static_cast<int>(columns), static_cast<int>(tiles), static_cast<int>(group));
   return launched("expert_product_kernel");
 }
 

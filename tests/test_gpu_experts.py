@@ -354,7 +354,41 @@ def test_malformed_plans_stay_in_bounds():
             z = torch.randn(6, 32, device=DEV).to(dtype).requires_grad_(True)
             out = expert_combine(z, w, plan)
             torch.autograd.grad(out, (z, w), torch.ones_like(out))
+    # segments that overlap, longer together than all places: more tiles and chunks than there is room for
+    places = 4000
+    order = torch.arange(places, device=DEV)
+    plan = ExpertPlan(torch.tensor([0, places, 0, places, 0, places, places], device=DEV), order, order.view(-1, 2))
+    for dtype in (F32, BF16):
+        x = torch.randn(places // 2, 4, 32, device=DEV).to(dtype).requires_grad_(True)
+        weight = torch.randn(6, 32, 32, device=DEV).to(dtype).requires_grad_(True)
+        y = expert_linear(x, weight, plan)
+        torch.autograd.grad(y, (x, weight), torch.ones_like(y))
     torch.cuda.synchronize()
+
+
+def test_linear_past_32_bits():
+    """x of more than 2^31 bytes: rows behind that border, their gradients, and matrices' gradients that sum over all."""
+    announce("expert linear, x of 2.3 GB")
+    tokens, k_in, n_out = 4_500_000, 128, 24
+    x = torch.randn(tokens, k_in, device=DEV).requires_grad_(True)
+    weight = (torch.randn(2, n_out, k_in, device=DEV) * k_in ** -0.5).requires_grad_(True)
+    chosen = (torch.arange(tokens, device=DEV) % 2)[:, None].contiguous()
+    plan = expert_dispatch(chosen, 2)
+    y = expert_linear(x, weight, plan)
+    dy = torch.randn_like(y)
+    dx, dw = torch.autograd.grad(y, (x, weight), dy)
+    for token in (0, 1, 4_194_302, 4_194_304, tokens - 2, tokens - 1):
+        place, e = int(plan.slots[token, 0]), token % 2
+        row, matrix = x[token].detach().cpu().double(), weight[e].detach().cpu().double()
+        assert_close_scaled(y[place], matrix @ row, what=f"y of token {token}")
+        assert_close_scaled(dx[token], dy[place].cpu().double() @ matrix, what=f"dx of token {token}")
+    for e in range(2):
+        wanted = torch.zeros(n_out, k_in, dtype=torch.float64, device=DEV)
+        rows, grads = x.detach()[e::2], dy[int(plan.offsets[e]): int(plan.offsets[e + 1])]
+        for first in range(0, rows.shape[0], 500_000):
+            wanted += grads[first: first + 500_000].double().t() @ rows[first: first + 500_000].double()
+        # 2.25M products of either sign; 512 and more in sequence in 32 bits, the rest in 64
+        assert_close_scaled(dw[e], wanted.cpu(), what=f"dweight {e}")
 
 
 # ---------------------------------------------------------------------------
