@@ -511,6 +511,24 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   };
 
   f32x16 sum[Z::kFragmentsM][Z::kFragmentsN];
+  // dW in float32: the sum over the rows in two levels, 512 rows (256 additions, the
+  // matrix unit takes two rows at a time) and their sums, as additions of one size
+  // do not average their roundings out.  16-bit operands go 16 rows an addition and
+  // end in 16 bits.
+  constexpr bool kFolds = MODE == kWeight && sizeof(T) == 4;
+  constexpr int kFoldSlices = 16;
+  f32x16 folded[kFolds ? Z::kFragmentsM : 1][kFolds ? Z::kFragmentsN : 1];
+  const auto fold = [&] {
+#pragma unroll
+    for (int m = 0; m < Z::kFragmentsM; ++m)
+#pragma unroll
+      for (int n = 0; n < Z::kFragmentsN; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          folded[m][n][i] += sum[m][n][i];
+          sum[m][n][i] = 0.0f;
+        }
+  };
   const auto clear = [&] {
 #pragma unroll
     for (int m = 0; m < Z::kFragmentsM; ++m)
@@ -668,12 +686,28 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     }
   } else {
     clear();
+    if constexpr (kFolds) {
+#pragma unroll
+      for (int m = 0; m < Z::kFragmentsM; ++m)
+#pragma unroll
+        for (int n = 0; n < Z::kFragmentsN; ++n) folded[m][n] = sum[m][n];
+    }
     int slice = 0;
     for (; slice + 1 < slices; slice += 2) {
       turn(slice, slice + 1, 0, slice + 2, lds_a0, lds_b0, lds_a1, lds_b1);
       turn(slice + 1, slice + 2, 0, slice + 3, lds_a1, lds_b1, lds_a0, lds_b0);
+      if constexpr (kFolds) {
+        if (slice % kFoldSlices == kFoldSlices - 2) fold();
+      }
     }
     if (slice < slices) turn(slice, slice + 1, 0, slice + 2, lds_a0, lds_b0, lds_a1, lds_b1);
+    if constexpr (kFolds) {
+      fold();
+#pragma unroll
+      for (int m = 0; m < Z::kFragmentsM; ++m)
+#pragma unroll
+        for (int n = 0; n < Z::kFragmentsN; ++n) sum[m][n] = folded[m][n];
+    }
     store(0);
   }
   __builtin_amdgcn_s_waitcnt(kNoLoadsLeft);              // the workgroup's LDS is not given away while loads to it are under way
@@ -1109,7 +1143,11 @@ int run_product(const ProductCall& call, hipStream_t stream) {
 }
 
 // Rows of a segment that one workgroup of dW takes: all of them where the matrices
-// make tiles enough, else so few that about 1,024 workgroups have some.
+// make tiles enough, else so few that about 1,024 workgroups have some; and no more
+// than kLongest, 1,024 additions of 16-bit operands, where segments are longer than
+// that in the mean.
+constexpr int64_t kLongest = 16384;
+
 struct Chunks {
   int rows, most;    // most == 0: no partial sums
 };
@@ -1118,8 +1156,10 @@ Chunks weight_chunks(int64_t places, int64_t inner, int64_t experts, int64_t k_i
   const int64_t rows = places * inner;
   const int64_t edge = n_out <= 64 || k_in <= 64 ? 64 : 128;
   const int64_t tiles = ((n_out + edge - 1) / edge) * ((k_in + edge - 1) / edge);
-  if (tiles * experts >= 512 || rows <= 512 * experts) return Chunks{INT_MAX, 0};
-  int64_t chunk = (rows * tiles + 1023) / 1024;
+  const bool many = tiles * experts >= 512;
+  if ((many && rows <= kLongest * experts) || rows <= 512 * experts) return Chunks{INT_MAX, 0};
+  int64_t chunk = many ? kLongest : (rows * tiles + 1023) / 1024;
+  if (chunk > kLongest) chunk = kLongest;
   chunk = (chunk + 511) / 512 * 512;
   return Chunks{static_cast<int>(chunk), static_cast<int>(rows / chunk + experts)};
 }

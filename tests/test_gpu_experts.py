@@ -366,6 +366,22 @@ def test_malformed_plans_stay_in_bounds():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_long_sums_of_one_size(dtype):
+    """dW over 4.8M equal rows a matrix: additions of one size do not average their roundings out."""
+    announce("expert linear, long sums", dtype)
+    tokens, inner = 600_000, 8
+    plan = expert_dispatch(torch.zeros(tokens, 1, dtype=torch.int64, device=DEV), 1)
+    x = torch.full((tokens, inner, 8), 0.7, device=DEV, dtype=dtype)
+    weight = torch.zeros(1, 8, 8, device=DEV, dtype=dtype, requires_grad=True)
+    y = expert_linear(x, weight, plan)
+    scale = 2.0 ** -12 if dtype == F16 else 1.0
+    dy = torch.full_like(y, 0.3 * scale)
+    (dw,) = torch.autograd.grad(y, weight, dy)
+    wanted = torch.full((1, 8, 8), tokens * inner * float(x[0, 0, 0]) * float(dy[0, 0, 0]), dtype=torch.float64)
+    assert_close_scaled(dw, wanted, rtol=1e-5 + _half(dtype), what="dweight")
+
+
 def test_linear_past_32_bits():
     """x of more than 2^31 bytes: rows behind that border, their gradients, and matrices' gradients that sum over all."""
     announce("expert linear, x of 2.3 GB")
