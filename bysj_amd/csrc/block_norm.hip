@@ -14,8 +14,9 @@
 // because a row stays in the registers of the lanes that share it, L of them with
 // E elements each: 8 to 64 lanes of a wave for rows of up to 1,024 (two waves of
 // half the elements were as fast forward and slower backward, 126 -> 170 us for
-// 30,011 rows of 810, as their sums need a barrier each), a workgroup beyond.  h is not kept in 32 bits between the two passes; the backward computes
-// it again from the residual, which is as many bytes as reading h, and y and the
+// 30,011 rows of 810, as their sums need a barrier each), a workgroup
+// beyond.  h is not kept in 32 bits between the two passes; the backward computes it
+// again from the residual, which is as many bytes as reading h, and y and the
 // gradients see the unrounded h.
 //
 // The gradients of post, pre and scale are sums over all rows.  A workgroup walks
@@ -23,9 +24,9 @@
 // bits stay short), and leaves one row of partial sums; a second launch adds these
 // in 64 bits in a fixed order.
 //
-// Measured: 24,576 rows of 1,024 in float32 with a gate, forward 90 us (5.6 TB/s of
-// its five streams), backward 155 us (5.2 TB/s of eight); 30,011 rows of 810 in
-// bfloat16 on a float32 residual, forward 52 us (5.6 TB/s), backward 118 us
+// Measured: 24,576 rows of 1,024 in float32 with a gate, forward 92 us (5.5 TB/s of
+// its five streams), backward 158 us (5.1 TB/s of eight); 30,011 rows of 810 in
+// bfloat16 on a float32 residual, forward 54 us (5.4 TB/s), backward 117 us
 // (3.7 TB/s; rows that start anywhere, four tenths of the second chunk's lanes idle).
 // Outputs are stored past the caches (through them: 90, 160, 61 and 123 us).
 #include "elements.h"

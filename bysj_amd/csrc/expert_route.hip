@@ -27,6 +27,12 @@
 // The CSR is a stable counting sort of tokens * k slots into experts + 1 bins, the
 // last for slots without an expert: counts per run of kRunSlots slots, a scan, and
 // ranks inside a wave from ballots; a single workgroup up to kSmallSlots slots.
+//
+// Bound by the k dependent steps of a row (a reduction over its lanes each), not by
+// the logits' bytes.  Measured: 24,576 rows of 64 in float32, sigmoid, bias, 4 of 8
+// groups, k 6: route 19.4 us, backward 6.5, the CSR of 147,456 slots 16; 65,536 rows
+// of 256 in bfloat16, softmax, k 8: route 35 us (1 TB/s), backward 26 (2.7 TB/s), the
+// CSR of 524,288 slots 24; 192 rows of 8: route 3.1 us, the CSR 2.8 in one launch.
 #include <climits>
 #include <type_traits>
 

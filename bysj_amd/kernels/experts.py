@@ -34,6 +34,7 @@ ACTIVATIONS = (None, "silu_gate")
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_EXPERTS = 1024
 MAX_GROUPS = 64
+MAX_CHANNELS = 65536   # of a product, whose sum over them is one chain in float32
 _MOST = 2**31 - 1
 
 
@@ -222,8 +223,8 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, fr
     ``(tokens * k, ..., inputs)`` by place, in float32, bfloat16 or float16.
     ``weight``: ``(E, outputs, inputs)`` of its dtype, one matrix for each of
     the plan's experts.  ``activation="silu_gate"``: the first half of the outputs
-    is a gate, ``silu(gate) * rest``, and the result has half of them.  Sums
-    are kept in float32.  Places behind ``plan.offsets[-1]`` give 0 and take no
+    is a gate, ``silu(gate) * rest``, and the result has half of them.  At most
+    65,536 inputs and outputs, whose sums are kept in float32.  Places behind ``plan.offsets[-1]`` give 0 and take no
     part in a gradient.  Gradients of ``x`` (summed in float32 over a
     token's slots) and ``weight``, once.
     """
@@ -242,8 +243,8 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, fr
         raise ValueError("expert linear weight must have shape (experts, outputs, inputs) for the plan's experts")
     if weight.shape[2] != x.shape[-1]:
         raise ValueError("expert linear weight does not fit the input's last dimension")
-    if not 1 <= weight.shape[1] <= 2**24 or not 1 <= weight.shape[2] <= 2**24:
-        raise ValueError("expert linear takes 1 to 2^24 inputs and outputs")
+    if not 1 <= weight.shape[1] <= MAX_CHANNELS or not 1 <= weight.shape[2] <= MAX_CHANNELS:
+        raise ValueError(f"expert linear takes 1 to {MAX_CHANNELS} inputs and outputs")
     if activation is not None and weight.shape[1] % 2 != 0:
         raise ValueError("expert linear: a gate needs an even number of outputs")
     entries = tokens if from_tokens else tokens * k
@@ -304,4 +305,4 @@ def expert_combine(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) -> 
 
 
 __all__ = ["ExpertPlan", "expert_route", "expert_dispatch", "expert_linear", "expert_combine", "ACTIVATIONS", "DTYPES",
-           "MAX_EXPERTS", "MAX_GROUPS", "SCORES"]
+           "MAX_CHANNELS", "MAX_EXPERTS", "MAX_GROUPS", "SCORES"]

@@ -674,7 +674,7 @@ int dpa4k_expert_dispatch(const int64_t* experts, int64_t slots,
  * silu(z[.., :n_out / 2]) z[.., n_out / 2:], and z itself to float
  * `before`[places, inner, n_out] unless that is NULL.  Rows behind
  * offsets[E] become 0 in y and are not written in `before`.  Products are
- * summed in 32 bits.  places * inner < 2^31 - 1024. */
+ * summed in 32 bits.  places * inner < 2^31 - 1024, k_in and n_out <= 65536. */
 int dpa4k_expert_linear_forward(const void* x, const void* weight,
                                 const int64_t* offsets, const int64_t* order,
                                 void* y, float* before, int64_t places, int64_t k,
