@@ -1157,9 +1157,11 @@ int run_product(const ProductCall& call, hipStream_t stream) {
 
 // Rows of a segment that one workgroup of dW takes: all of them where the matrices
 // make tiles enough, else so few that about 1,024 workgroups have some; and no more
-// than kLongest, 1,024 additions of 16-bit operands, where segments are longer than
-// that in the mean.
-constexpr int64_t kLongest = 16384;
+// than kLongest, 2,048 additions of 16-bit operands (6e-5 of equal terms at worst) and
+// 256 and 64 of float32, where segments are longer than that in the mean.  Shorter
+// cuts would cost partial sums: at 4,096 by 4,096 these are an eighth of the
+// operands' bytes.
+constexpr int64_t kLongest = 32768;
 
 struct Chunks {
   int rows, most;    // most == 0: no partial sums

@@ -382,6 +382,24 @@ def test_long_sums_of_one_size(dtype):
     assert_close_scaled(dw, wanted, rtol=1e-5 + _half(dtype), what="dweight")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long_sums_of_wide_matrices(dtype):
+    """dW of segments of over 32,768 rows whose matrices have tiles enough to fill the card uncut."""
+    announce("expert linear, long sums of wide matrices", dtype)
+    tokens, experts, k_in, n_out = 140_003, 4, 1024, 2048
+    plan = expert_dispatch((torch.arange(tokens, device=DEV) ** 2 % 4)[:, None].contiguous(), experts)   # 0 and 1 alone
+    counts = (plan.offsets[1:] - plan.offsets[:-1]).cpu().double()
+    x = torch.full((tokens, k_in), 0.7, device=DEV, dtype=dtype)
+    x[:, 1::2] = -0.35
+    weight = torch.zeros(experts, n_out, k_in, device=DEV, dtype=dtype, requires_grad=True)
+    y = expert_linear(x, weight, plan)
+    dy = torch.full_like(y, 0.3)
+    (dw,) = torch.autograd.grad(y, weight, dy)
+    wanted = (counts[:, None] * (x[0].cpu().double() * float(dy[0, 0])))[:, None, :].expand(experts, n_out, k_in)
+    # equal terms, n of them in sequence: at most n 2^-25 off; 256 and 64 in float32, 2,048 in bfloat16
+    assert_close_scaled(dw, wanted, rtol=(320 if dtype == F32 else 2048) * 2.0 ** -25 + 2.0 ** -24 + _half(dtype), what="dweight")
+
+
 def test_linear_past_32_bits():
     """x of more than 2^31 bytes: rows behind that border, their gradients, and matrices' gradients that sum over all."""
     announce("expert linear, x of 2.3 GB")
