@@ -165,6 +165,19 @@ def test_unaligned_tensors_and_another_stream():
             assert_bitwise(a, b)
 
 
+def test_gradient_of_gates_near_one():
+    """Sigmoid gates up to 1 - 1e-13: their slopes keep their digits."""
+    announce("residual norm, gates near one")
+    gate = torch.linspace(-30.0, 30.0, 512, device=DEV).view(8, 64).contiguous().requires_grad_(True)
+    x, dh = torch.randn(8, 64, device=DEV), torch.randn(8, 64, device=DEV)
+    h, _ = residual_norm(x, torch.zeros_like(x), gate=gate, gate_activation="sigmoid", post_norm=False, pre_norm=False)
+    (grad,) = torch.autograd.grad(h, gate, dh)
+    exact = gate.detach().cpu().double()
+    wanted = dh.cpu().double() * x.cpu().double() * torch.sigmoid(exact) * torch.sigmoid(-exact)
+    # two sigmoids and three products, each a few steps of 2^-24 off
+    assert_close_scaled(grad, wanted, rtol=2e-6, scale=0.0, what="dgate")
+
+
 def test_second_derivative_is_refused():
     x = torch.randn(4, 8, device=DEV, requires_grad=True)
     h, y = residual_norm(x, torch.zeros_like(x))

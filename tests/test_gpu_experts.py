@@ -157,6 +157,17 @@ def test_route_grad_of_a_column_of_weights():
     assert_bitwise(torch.autograd.grad(weights, logits, seed.contiguous())[0], first)
 
 
+def test_route_gradient_of_scores_near_one():
+    """Sigmoid scores up to 1 - 1e-13: their slopes keep their digits."""
+    announce("expert route, scores near one")
+    logits = torch.linspace(-30.0, 30.0, 512, device=DEV)[:, None].contiguous().requires_grad_(True)
+    weights, _, _ = expert_route(logits, 1, scores="sigmoid", normalize=False)
+    (grad,) = torch.autograd.grad(weights.sum(), logits)
+    exact = logits.detach().cpu().double()
+    # two sigmoids and a product, each a few steps of 2^-24 off
+    assert_close_scaled(grad, torch.sigmoid(exact) * torch.sigmoid(-exact), rtol=1e-6, scale=0.0, what="dlogits")
+
+
 @pytest.mark.parametrize("slots,experts", [(1, 1), (64, 3), (8192, 1024), (8193, 1), (100_003, 5), (70_000, 1024), (300_000, 64)])
 def test_dispatch(slots, experts):
     announce("expert dispatch", slots, experts)
