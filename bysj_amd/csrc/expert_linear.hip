@@ -617,8 +617,10 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   // Register i of a lane is row 8 (i / 4) + 4 (lane / 32) + i mod 4 and column lane mod 32
   // of the matrix unit's result.  Its rows are the columns here: four values are
   // stored at once and a lane has few rows to find (dx of 32,768 rows, 2 x 2,048 to
-  // 1,024 in bfloat16, 378 -> 354 us).  Gated, its rows are the rows, so that z is stored in whole lines of 128 bytes
-  // (516 -> 458 us forward).
+  // 1,024 in bfloat16, 378 -> 354 us).  Gated, its rows are the
+  // rows, so that z is stored in whole lines of 128 bytes (516 -> 458 us forward), past
+  // the caches, which its 537 MB would empty of rows and matrices (forward alone 391 ->
+  // 371 us, the gate's backward behind it 189 -> 164; no change where z fits them).
   const bool partial = MODE == kWeight && call.chunks > 0;
   const auto shifted = [&](int index, int size) { return FAST == kRagged && index >= size / V * V ? (V - size % V) % V : 0; };
   const auto store = [&](int tile) {
@@ -639,8 +641,8 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
             static_cast<T*>(call.out)[out_row * half + column] = static_cast<T>(gate * logistic(gate) * up);
             if (call.before != nullptr) {
               float* z = call.before + out_row * call.n_out;
-              z[column] = gate;
-              z[half + column] = up;
+              __builtin_nontemporal_store(gate, z + column);
+              __builtin_nontemporal_store(up, z + half + column);
             }
           }
         }
@@ -912,7 +914,7 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(ProductCall call, const
 // ---------------------------------------------------------------------------
 
 // dz of the gated SiLU; 16 bytes of dy a thread (32,768 rows of 2,048 in bfloat16: 938
-// MB in 189 us, 5.0 TB/s).  z comes in 32 bits: dz has to be
+// MB in 164 us, 5.7 TB/s).  z comes in 32 bits: dz has to be
 // rounded to the operands' type for the products, and with z rounded as well the
 // gradients of bfloat16 were 1.8 times as far from their exact values as one
 // rounding puts them (1.4 times so).
