@@ -25,7 +25,7 @@
 // in 64 bits in a fixed order.
 //
 // Measured: 24,576 rows of 1,024 in float32 with a gate, forward 92 us (5.5 TB/s of
-// its five streams), backward 161 us (5.0 TB/s of eight); 30,011 rows of 810 in
+// its five streams), backward 160 us (5.0 TB/s of eight); 30,011 rows of 810 in
 // bfloat16 on a float32 residual, forward 54 us (5.4 TB/s), backward 117 us
 // (3.7 TB/s; rows that start anywhere, four tenths of the second chunk's lanes idle).
 // Outputs are stored past the caches (through them: 90, 160, 61 and 123 us).
@@ -66,12 +66,13 @@ struct NormCall {
 __device__ __forceinline__ float gate_value(float gate, int act, float& slope) {
   slope = 1.0f;
   if (act == kActNone) return gate;
-  const float s = logistic(gate);
+  float other;
+  const float s = logistic(gate, other);
   if (act == kActSigmoid) {
-    slope = s * logistic(-gate);     // 1 - s has no digits left where s is near 1
+    slope = s * other;
     return s;
   }
-  slope = s * fmaf(gate, 1.0f - s, 1.0f);
+  slope = s * fmaf(gate, other, 1.0f);
   return gate * s;
 }
 

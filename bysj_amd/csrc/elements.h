@@ -98,15 +98,25 @@ __device__ __forceinline__ void split_piece(int64_t at, int64_t pieces, bool sho
 }
 
 // 1 / (1 + exp(-x)) to about two roundings, NaN for NaN.  The product x log2(e) is
-// carried with its rounding error; past +-90 the result is 0 and 1 to float32.
-__device__ __forceinline__ float logistic(float x) {
+// carried with its rounding error; past +-88 the result is 0 (6e-39) and 1;
+// exp(90) would be infinite and its rounding error NaN.
+// `other`: 1 minus it, with all its digits where the result is near 1.
+__device__ __forceinline__ float logistic(float x, float& other) {
   constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147182f;
-  x = x < -90.0f ? -90.0f : x;
-  x = x > 90.0f ? 90.0f : x;
+  x = x < -88.0f ? -88.0f : x;
+  x = x > 88.0f ? 88.0f : x;
   const float t = -x * kLog2e;
   const float rest = fmaf(-x, kLog2eRest, fmaf(-x, kLog2e, -t));
-  const float e = __builtin_amdgcn_exp2f(t);
-  return __builtin_amdgcn_rcpf(1.0f + fmaf(e, rest * kLn2, e));
+  float e = __builtin_amdgcn_exp2f(t);
+  e = fmaf(e, rest * kLn2, e);
+  const float s = __builtin_amdgcn_rcpf(1.0f + e);
+  other = x < -80.0f ? 1.0f : e * s;   // s may be 0 there
+  return s;
+}
+
+__device__ __forceinline__ float logistic(float x) {
+  float other;
+  return logistic(x, other);
 }
 
 }  // namespace dpa4k

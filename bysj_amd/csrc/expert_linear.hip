@@ -939,8 +939,9 @@ __global__ __launch_bounds__(256) void gate_backward_kernel(const T* __restrict_
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float g = gate[j], d = static_cast<float>(grad[j]);
-      const float s = logistic(g);
-      of_gate[j] = d * up[j] * (s * fmaf(g, 1.0f - s, 1.0f));
+      float other;
+      const float s = logistic(g, other);
+      of_gate[j] = d * up[j] * (s * fmaf(g, other, 1.0f));
       of_up[j] = d * (g * s);
     }
     store_pack<false, T, V>(dz + row * 2 * half + column, of_gate, live);

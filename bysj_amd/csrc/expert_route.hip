@@ -30,7 +30,7 @@
 //
 // Bound by the k dependent steps of a row (a reduction over its lanes each), not by
 // the logits' bytes.  Measured: 24,576 rows of 64 in float32, sigmoid, bias, 4 of 8
-// groups, k 6: route 19.4 us, backward 6.9, the CSR of 147,456 slots 16; 65,536 rows
+// groups, k 6: route 19.4 us, backward 6.3, the CSR of 147,456 slots 16; 65,536 rows
 // of 256 in bfloat16, softmax, k 8: route 35 us (1 TB/s), backward 26 (2.7 TB/s), the
 // CSR of 524,288 slots 24; 192 rows of 8: route 3.1 us, the CSR 2.8 in one launch.
 #include <climits>
@@ -337,9 +337,14 @@ __global__ __launch_bounds__(kBlock) void expert_route_backward_kernel(RouteCall
 #pragma unroll
     for (int j = 0; j < Z::V; ++j) {
       const float d = at + j < n ? ds[group][at + j] : 0.0f;
-      const float s = score_of(logit[i * Z::V + j], call.scores, top, sum);
-      if (call.scores == kSoftmax) part[j] = logit[i * Z::V + j] == -INFINITY ? 0.0f : s * (d - inner);
-      else part[j] = d == 0.0f ? 0.0f : d * s * logistic(-logit[i * Z::V + j]);   // 1 - s where s is near 1
+      const float l = logit[i * Z::V + j];
+      if (call.scores == kSoftmax) {
+        part[j] = l == -INFINITY ? 0.0f : score_of(l, kSoftmax, top, sum) * (d - inner);
+      } else {
+        float other;
+        const float s = logistic(l, other);
+        part[j] = d == 0.0f ? 0.0f : d * s * other;
+      }
     }
     if (at < n) store_pack<false, T, Z::V>(out + row * n + at, part, n - at);
   }

@@ -178,6 +178,22 @@ def test_gradient_of_gates_near_one():
     assert_close_scaled(grad, wanted, rtol=2e-6, scale=0.0, what="dgate")
 
 
+@pytest.mark.parametrize("activation", ["sigmoid", "silu"])
+def test_gates_near_zero(activation):
+    """Gates of -120 to -80, whose exponential passes float32."""
+    announce("residual norm, gates near zero", activation)
+    gate = torch.linspace(-120.0, -80.0, 4096, device=DEV).view(64, 64).contiguous().requires_grad_(True)
+    x = torch.ones(64, 64, device=DEV)
+    h, _ = residual_norm(x, torch.zeros_like(x), gate=gate, gate_activation=activation, post_norm=False, pre_norm=False)
+    (grad,) = torch.autograd.grad(h, gate, torch.ones_like(h))
+    exact = gate.detach().cpu().double()
+    s = torch.sigmoid(exact)
+    value, slope = (s, s * (1.0 - s)) if activation == "sigmoid" else (exact * s, s * (1.0 + exact * (1.0 - s)))
+    # where s is below float32's smallest normal number, 1.2e-38, it may be 0
+    for got, wanted in ((h, value), (grad, slope)):
+        assert ((got.detach().cpu().double() - wanted).abs() <= 1e-5 * wanted.abs() + 1.2e-38 * 121.0).all()
+
+
 def test_second_derivative_is_refused():
     x = torch.randn(4, 8, device=DEV, requires_grad=True)
     h, y = residual_norm(x, torch.zeros_like(x))

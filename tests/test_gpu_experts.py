@@ -168,6 +168,18 @@ def test_route_gradient_of_scores_near_one():
     assert_close_scaled(grad, torch.sigmoid(exact) * torch.sigmoid(-exact), rtol=1e-6, scale=0.0, what="dlogits")
 
 
+def test_route_scores_near_zero():
+    """Sigmoid scores whose exponential passes float32: weights and gradients are finite, and the tiny numbers that they are."""
+    announce("expert route, scores near zero")
+    logits = torch.linspace(-120.0, -80.0, 4096, device=DEV)[:, None].contiguous().requires_grad_(True)
+    weights, _, _ = expert_route(logits, 1, scores="sigmoid", normalize=False)
+    (grad,) = torch.autograd.grad(weights.sum(), logits)
+    exact = torch.sigmoid(logits.detach().cpu().double())
+    # below float32's smallest normal number, 1.2e-38, either may be 0
+    for got in (weights, grad):
+        assert ((got.detach().cpu().double() - exact).abs() <= 1e-6 * exact + 1.2e-38).all()
+
+
 @pytest.mark.parametrize("slots,experts", [(1, 1), (64, 3), (8192, 1024), (8193, 1), (100_003, 5), (70_000, 1024), (300_000, 64)])
 def test_dispatch(slots, experts):
     announce("expert dispatch", slots, experts)
@@ -303,6 +315,24 @@ def test_linear_many_rows(dtype, k_in, n_out, gated):
     plan = tuple(t.cpu() for t in plan)
     for from_tokens in (True, False):
         _check_linear(plan, 5, (33,), k_in, n_out, dtype, from_tokens=from_tokens, gated=gated, seed=1, what="many rows")
+
+
+@pytest.mark.parametrize("tokens", [40, 4096])
+def test_linear_gates_near_zero(tokens):
+    """Gates of -120 to -80, whose exponential passes float32."""
+    announce("expert linear, gates near zero", tokens)
+    plan = expert_dispatch(torch.zeros(tokens, 1, dtype=torch.int64, device=DEV), 1)
+    x = torch.linspace(-120.0, -80.0, tokens, device=DEV)[:, None].contiguous().requires_grad_(True)
+    weight = torch.ones(1, 2, 1, device=DEV, requires_grad=True)     # z = (x, x)
+    y = expert_linear(x, weight, plan, activation="silu_gate")
+    dx, dw = torch.autograd.grad(y, (x, weight), torch.ones_like(y))
+    exact = x.detach().cpu().double()
+    s = torch.sigmoid(exact)
+    slope = 2.0 * exact * s + exact * exact * s * (1.0 - s)           # of x silu(x)
+    # where s is below float32's smallest normal number, 1.2e-38, it may be 0
+    assert ((y.detach().cpu().double() - exact * exact * s).abs() <= 1e-5 * (exact * exact * s) + 1.2e-38 * 120.0 ** 2).all()
+    assert ((dx.cpu().double() - slope).abs() <= 1e-5 * slope.abs() + 1.2e-38 * 2.0 * 120.0 ** 2).all()
+    assert torch.isfinite(dw).all()
 
 
 def test_linear_only_what_is_wanted():
