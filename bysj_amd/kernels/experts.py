@@ -34,7 +34,7 @@ ACTIVATIONS = (None, "silu_gate")
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_EXPERTS = 1024
 MAX_GROUPS = 64
-MAX_CHANNELS = 65536   # of a product, whose sum over them is one chain in float32
+MAX_CHANNELS = 65536   # of a product, whose sum over them is held in float32
 _MOST = 2**31 - 1
 
 

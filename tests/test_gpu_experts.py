@@ -423,6 +423,22 @@ def test_long_sums_of_one_size(dtype):
     assert_close_scaled(dw, wanted, rtol=1e-5 + _half(dtype), what="dweight")
 
 
+def test_long_sums_over_channels():
+    """The forward over 65,536 inputs and dx over as many outputs, all products equal, in float32."""
+    announce("expert linear, long sums over channels")
+    plan = expert_dispatch(torch.zeros(300, 1, dtype=torch.int64, device=DEV), 1)
+    for k_in, n_out in ((65536, 48), (48, 65536)):
+        x = torch.full((300, k_in), 0.7, device=DEV, requires_grad=True)
+        weight = torch.full((1, n_out, k_in), 0.3, device=DEV)
+        y = expert_linear(x, weight, plan)
+        (dx,) = torch.autograd.grad(y, x, torch.full_like(y, 0.7))
+        product = float(x[0, 0].detach()) * float(weight[0, 0, 0])
+        # equal terms, n of them in sequence: at most n 2^-25 off; 256 and 128 here
+        for got, terms in ((y, k_in), (dx, n_out)):
+            wanted = torch.full(tuple(got.shape), terms * product, dtype=torch.float64)
+            assert_close_scaled(got, wanted, rtol=384 * 2.0 ** -25 + 2.0 ** -24, scale=0.0, what=f"sum of {terms}")
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_long_sums_of_wide_matrices(dtype):
     """dW of segments of over 32,768 rows whose matrices have tiles enough to fill the card uncut."""
