@@ -24,7 +24,8 @@
 //
 // Measured: 32,768 slots through 32 matrices of 1,024 to 2 x 2,048 in bfloat16 (8,192
 // tokens, four slots each), forward with the gate 399 us (690 TFLOP/s), dW 393 (700),
-// dx 347 (790), where a library's one product of that size reaches 1,090 to 1,300:
+// dx 347 (790), with the gate's dz in two parts 694 and 667 (the operations twice),
+// where a library's one product of that size reaches 1,090 to 1,300:
 // one workgroup fits a CU with its 256 by 256 tile, so nothing multiplies while it
 // starts and stores, and unequal segments leave a last round half filled.  786,432
 // rows of 64 by 64 in float32: forward 107 us, dW 104, dx 115 (2 to 4 TB/s over rows
@@ -55,6 +56,7 @@ constexpr int kMostRun = 8;
 
 struct ProductCall {
   const void* a;           // x (forward), dz (dx, dW)
+  const void* a_low;       // dx, dW: what dz has below `a`, or null (two_parts)
   const void* b;           // W (forward, dx), x (dW)
   void* out;               // y, dx by place or by slot, dW or its partial sums
   float* before;           // forward, gated: z, or null
@@ -186,6 +188,19 @@ constexpr int kV = 16 / sizeof(T);           // elements of a piece
 template <typename T>
 constexpr int kSlice = 128 / sizeof(T);      // summed index of a slice
 
+// dz in 16 bits is held in two parts, unit * high + low, as one of them would round
+// every product (and overflow float16 where dx and dW do not).  bfloat16: 2^-18 of the
+// value is lost.  float16: 2^-24 of it or 2^-25, up to 1.3e8; a unit of 2048 is the most
+// that what the high part leaves, half a step of it, fits the low one for.
+template <typename T>
+constexpr float kPartUnit = std::is_same<T, _Float16>::value ? 2048.0f : 1.0f;
+
+template <typename T>
+__device__ __forceinline__ void two_parts(float value, float& high, float& low) {
+  high = static_cast<float>(static_cast<T>(value * (1.0f / kPartUnit<T>)));
+  low = __builtin_fabsf(high) < INFINITY ? fmaf(-kPartUnit<T>, high, value) : 0.0f;
+}
+
 __device__ __forceinline__ int along_byte(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) << 4); }
 
 template <typename T, int COLS>
@@ -287,7 +302,7 @@ struct Tile {
   static_assert(kBytesA % (16 * kThreads) == 0 && kBytesB % (16 * kThreads) == 0, "whole pieces");
 };
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST, bool RUN>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST, bool RUN, bool TWO>
 __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductCall call, int columns, int tiles, int group) {
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   constexpr int V = kV<T>, S = kSlice<T>;
@@ -356,7 +371,9 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   // that no load leaves its row: along the summed index, what it repeats is shifted
   // out in LDS; across it, its columns of the result are stored a little further left,
   // where its neighbour stores the same.  Otherwise as elements of which some are there.
-  const T* a = static_cast<const T*>(call.a);
+  const int64_t skipped_a = (MODE == kInput ? first_row : MODE == kWeight ? span.begin : 0) * static_cast<int64_t>(call.n_out);
+  const T* a = static_cast<const T*>(call.a) + skipped_a;
+  const T* a_low = TWO ? static_cast<const T*>(call.a_low) + skipped_a : a;
   const T* b = static_cast<const T*>(call.b);
   const int64_t inner = call.inner;
   const int64_t rows_x = (call.order != nullptr ? call.places / call.k : call.places) * inner;
@@ -367,10 +384,8 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     elements_a = rows_x * call.k_in;
   } else if constexpr (MODE == kInput) {
     elements_a = (FAST ? static_cast<int64_t>(live_rows) : call.places * inner - first_row) * call.n_out;
-    a += static_cast<int64_t>(first_row) * call.n_out;
   } else {
     elements_a = (FAST ? static_cast<int64_t>(depth) : call.places * inner - span.begin) * call.n_out;
-    a += static_cast<int64_t>(span.begin) * call.n_out;
   }
   if constexpr (MODE == kWeight) {
     elements_b = rows_x * call.k_in;
@@ -437,11 +452,19 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     }
   }
 
+  // Slices of the first part of dz come first, those of what it leaves behind them.
+  const int slices_of_part = (depth + S - 1) / S;
+  const int slices = TWO ? 2 * slices_of_part : slices_of_part;
+  const auto is_low = [&](int slice) { return TWO && slice >= slices_of_part; };
+  // summed index where a slice starts; past `depth` for slices behind the last
+  const auto start_of = [&](int slice) { return (is_low(slice) ? slice - slices_of_part : slice) * S; };
+
   // Starts the loads of slice `slice` of row tile `tile` of the run.  FAST: straight to LDS, whose 16 bytes of a
   // wave are consecutive; zeros where there is nothing.  Else to registers.
   u32x4 piece_a[FAST ? 1 : Z::kPiecesA], piece_b[FAST ? 1 : Z::kPiecesB];
   const auto fetch = [&](int tile, int slice, char* to_a, char* to_b) {
-    const int done = slice * S;
+    const int done = start_of(slice);
+    const T* a_here = is_low(slice) ? a_low : a;
     const int along_left = depth - done - along_piece * V;
     // across, the base moves; along, the offset (to before it, in a ragged last piece)
     const int64_t moved_a = Z::kAcrossA ? static_cast<int64_t>(done) * call.n_out : FAST ? 0 : done;
@@ -455,7 +478,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       }
     }
     if constexpr (FAST != kByPiece) {
-      const BufferView view_a = buffer_view(a + moved_a, (elements_a - moved_a) * static_cast<int64_t>(sizeof(T)));
+      const BufferView view_a = buffer_view(a_here + moved_a, (elements_a - moved_a) * static_cast<int64_t>(sizeof(T)));
       const BufferView view_b = buffer_view(b + moved_b, (elements_b - moved_b) * static_cast<int64_t>(sizeof(T)));
       // by arithmetic, as the compiler makes branches around two loads of a choice
       const uint32_t past = static_cast<uint32_t>(along_left - 1) & kNoRow;
@@ -480,7 +503,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       for (int i = 0; i < Z::kPiecesA; ++i) {
         const bool there = Z::kAcrossA ? done + (thread + i * Z::kThreads) / (BM / V) < depth : live_a[i] != 0;
         const int left = there ? (Z::kAcrossA ? live_a[i] : along_left) : 0;
-        piece_a[i] = load_piece<T>(a + from_a[i] + moved_a, left, elements_a - from_a[i] - moved_a);
+        piece_a[i] = load_piece<T>(a_here + from_a[i] + moved_a, left, elements_a - from_a[i] - moved_a);
       }
 #pragma unroll
       for (int i = 0; i < Z::kPiecesB; ++i) {
@@ -494,7 +517,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   const auto land = [&](int slice, char* to_a, char* to_b) {
     if constexpr (FAST != kByPiece) {
       __builtin_amdgcn_s_waitcnt(kNoLoadsLeft);
-      const int repeats = repeated(depth - slice * S - along_piece * V);
+      const int repeats = repeated(depth - start_of(slice) - along_piece * V);
       if (MODE != kWeight && repeats > 0) {
         const int words = repeats * static_cast<int>(sizeof(T)) / 4;
         const auto align = [&](char* piece) {
@@ -540,6 +563,16 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
           sum[m][n][i] = 0.0f;
         }
   };
+  // The first part of dz comes in units of kPartUnit.
+  const auto raise = [&](int slice) {
+    if (!TWO || kPartUnit<T> == 1.0f || slice != slices_of_part) return;
+#pragma unroll
+    for (int m = 0; m < Z::kFragmentsM; ++m)
+#pragma unroll
+      for (int n = 0; n < Z::kFragmentsN; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[m][n][i] *= kPartUnit<T>;
+  };
   const auto clear = [&] {
 #pragma unroll
     for (int m = 0; m < Z::kFragmentsM; ++m)
@@ -553,7 +586,6 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   // inside a slice, the operands of the next step are read while one step's
   // products run.
   const int wave_row = (wave / WN) * (BM / WM), wave_column = (wave % WN) * (BN / WN);
-  const int slices = (depth + S - 1) / S;
   u32x4 fa[2][Z::kFragmentsM], fb[2][Z::kFragmentsN];
   const auto read = [&](const char* at_a, const char* at_b, int step, u32x4 (&a_to)[Z::kFragmentsM], u32x4 (&b_to)[Z::kFragmentsN]) {
 #pragma unroll
@@ -569,11 +601,14 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   };
   PlaceRow ahead{0, 0};                                  // dW: of the slice behind the next two
   const auto look_ahead = [&](int slice) {
-    if (MODE == kWeight && thread < S && slice * S + thread < depth) ahead = place_row(call, span.begin + slice * S + thread);
+    const int at = start_of(slice) + thread;
+    if (MODE == kWeight && thread < S && at < depth) ahead = place_row(call, span.begin + at);
   };
   if constexpr (MODE == kWeight) {
-    for (int row = thread; row < 2 * S && row < depth; row += Z::kThreads)
-      rows_of_x[row / S][row % S] = static_cast<int>(row_of_x(call, place_row(call, span.begin + row)));
+    for (int row = thread; row < 2 * S; row += Z::kThreads) {
+      const int at = start_of(row / S) + row % S;
+      if (at < depth) rows_of_x[row / S][row % S] = static_cast<int>(row_of_x(call, place_row(call, span.begin + at)));
+    }
     look_ahead(2);
     __syncthreads();
   }
@@ -692,7 +727,9 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
       for (int slice = 0; slice < padded; slice += 2) {
         const bool wraps = slice + 2 >= padded;
         const int coming = wraps ? 0 : slice + 2;
+        raise(slice);
         turn(slice, slice + 1, wraps ? tile + 1 : tile, coming, lds_a0, lds_b0, lds_a1, lds_b1);
+        raise(slice + 1);
         turn(slice + 1, coming, wraps ? tile + 1 : tile, coming + 1, lds_a1, lds_b1, lds_a0, lds_b0);
       }
       store(tile);
@@ -707,7 +744,9 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
     }
     int slice = 0;
     for (; slice + 1 < slices; slice += 2) {
+      raise(slice);
       turn(slice, slice + 1, 0, slice + 2, lds_a0, lds_b0, lds_a1, lds_b1);
+      raise(slice + 1);
       turn(slice + 1, slice + 2, 0, slice + 3, lds_a1, lds_b1, lds_a0, lds_b0);
       if constexpr (kFolds) {
         if (slice % kFoldSlices == kFoldSlices - 2) fold();
@@ -914,14 +953,13 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(ProductCall call, const
 // elementwise parts
 // ---------------------------------------------------------------------------
 
-// dz of the gated SiLU; 16 bytes of dy a thread (32,768 rows of 2,048 in bfloat16: 938
-// MB in 164 us, 5.7 TB/s).  z comes in 32 bits: dz has to be
-// rounded to the operands' type for the products, and with z rounded as well the
-// gradients of bfloat16 were 1.8 times as far from their exact values as one
-// rounding puts them (1.4 times so).
+// dz of the gated SiLU; 16 bytes of dy a thread (32,768 rows of 2,048 in bfloat16: 1.2 GB
+// in 207 us, 5.8 TB/s).  z comes in 32 bits and dz goes to the products in two parts of
+// 16 bits: with one, the gradients were 1.4 times as far from their exact values as
+// one rounding puts them, and with z rounded as well 1.8 times.
 template <typename T>
 __global__ __launch_bounds__(256) void gate_backward_kernel(const T* __restrict__ dy, const float* __restrict__ z, T* __restrict__ dz,
-                                                            int64_t rows, int half) {
+                                                            T* __restrict__ dz_low, int64_t rows, int half) {
   constexpr int V = kV<T>;
   const int pieces = (half + V - 1) / V;
   const bool short_ = rows * pieces <= UINT32_MAX;
@@ -945,8 +983,19 @@ __global__ __launch_bounds__(256) void gate_backward_kernel(const T* __restrict_
       of_gate[j] = d * up[j] * (s * fmaf(g, other, 1.0f));
       of_up[j] = d * (g * s);
     }
-    store_pack<false, T, V>(dz + row * 2 * half + column, of_gate, live);
-    store_pack<false, T, V>(dz + row * 2 * half + half + column, of_up, live);
+    const int64_t to = row * 2 * half + column;
+    if constexpr (sizeof(T) == 2) {
+      float low_gate[V], low_up[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        two_parts<T>(of_gate[j], of_gate[j], low_gate[j]);
+        two_parts<T>(of_up[j], of_up[j], low_up[j]);
+      }
+      store_pack<false, T, V>(dz_low + to, low_gate, live);
+      store_pack<false, T, V>(dz_low + to + half, low_up, live);
+    }
+    store_pack<false, T, V>(dz + to, of_gate, live);
+    store_pack<false, T, V>(dz + to + half, of_up, live);
   }
 }
 
@@ -1087,8 +1136,11 @@ int check_product(const char* what, int64_t places, int64_t k, int64_t inner, in
   return DPA4K_OK;
 }
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST, bool RUN = false>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int FAST, bool RUN = false, bool TWO = false>
 int launch_product(ProductCall call, hipStream_t stream) {
+  if constexpr (!TWO && sizeof(T) == 2 && (MODE == kInput || MODE == kWeight)) {
+    if (call.a_low != nullptr) return launch_product<T, MODE, BM, BN, WM, WN, FAST, RUN, true>(call, stream);
+  }
   typedef Tile<T, MODE, BM, BN, WM, WN> Z;
   const int64_t rows = call.places * call.inner;
   const int64_t width = MODE == kGated ? call.n_out / 2 : (MODE == kForward ? call.n_out : call.k_in);
@@ -1100,7 +1152,7 @@ int launch_product(ProductCall call, hipStream_t stream) {
   // two row tiles with all their columns; of dW, one (32,768 rows, 1,024 to 2 x 2,048 in
   // bfloat16: forward 459 -> 420 us against four, dW 439 -> 418 us, as dies then get more equal shares)
   const int64_t group = MODE != kWeight && tiles >= columns * 64 ? columns * 2 : columns;
-  expert_product_kernel<T, MODE, BM, BN, WM, WN, FAST, RUN><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
+  expert_product_kernel<T, MODE, BM, BN, WM, WN, FAST, RUN, TWO><<<static_cast<unsigned int>(tiles), Z::kThreads, 0, stream>>>(
       call, static_cast<int>(columns), static_cast<int>(tiles), static_cast<int>(group));
   return launched("expert_product_kernel");
 }
@@ -1153,7 +1205,7 @@ int run_product(const ProductCall& call, hipStream_t stream) {
   const int64_t limit = (int64_t(kNoRow) - 4096) / static_cast<int64_t>(sizeof(T));
   const auto words = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
   const bool fast = call.k_in * sizeof(T) % 4 == 0 && call.n_out * sizeof(T) % 4 == 0 && call.k_in >= kV<T> && call.n_out >= kV<T> &&
-                    words(call.a) && words(call.b) && rows_x * call.k_in < limit &&
+                    words(call.a) && words(call.a_low) && words(call.b) && rows_x * call.k_in < limit &&
                     static_cast<int64_t>(call.n_out) * call.k_in < limit && static_cast<int64_t>(call.n_out) * 256 < limit &&
                     static_cast<int64_t>(call.k_in) * 256 < limit;
   return fast ? run_tiles<T, MODE, kRagged>(call, stream) : run_tiles<T, MODE, kByPiece>(call, stream);
@@ -1217,23 +1269,6 @@ extern "C" int dpa4k_expert_linear_forward(const void* x, const void* weight, co
   });
 }
 
-extern "C" int dpa4k_expert_gate_backward(const void* grad, const float* before, void* grad_before, int64_t rows, int64_t channels,
-                                          int type, dpa4k_stream_t stream) {
-  clear_error();
-  if (rows < 0 || channels < 1 || channels > (1 << 23)) return fail(DPA4K_EINVAL, "expert gate: bad sizes");
-  if (rows > INT32_MAX) return fail(DPA4K_EINVAL, "expert gate takes fewer than 2^31 rows");
-  if (!known_type(type)) return fail(DPA4K_EINVAL, "expert gate: unknown type");
-  if (rows == 0) return DPA4K_OK;
-  if (grad == nullptr || before == nullptr || grad_before == nullptr) return fail(DPA4K_EINVAL, "expert gate: null pointer");
-  return with_type(type, DPA4K_EINVAL, [&](auto t) {
-    typedef typename decltype(t)::type T;
-    const int grid = pieces_grid(rows * ((channels + kV<T> - 1) / kV<T>));
-    gate_backward_kernel<T><<<grid, 256, 0, as_stream(stream)>>>(static_cast<const T*>(grad), before,
-                                                                 static_cast<T*>(grad_before), rows, static_cast<int>(channels));
-    return launched("gate_backward_kernel");
-  });
-}
-
 extern "C" size_t dpa4k_expert_linear_workspace_size(int64_t places, int64_t k, int64_t inner, int64_t n_experts, int64_t k_in,
                                                      int64_t n_out, int by_token, int want_x, int want_weight) {
   if (places <= 0 || inner <= 0 || n_experts < 1 || k_in < 1 || n_out < 1 || places > INT32_MAX / inner) return 0;
@@ -1247,34 +1282,23 @@ extern "C" size_t dpa4k_expert_linear_workspace_size(int64_t places, int64_t k, 
   return bytes;
 }
 
-extern "C" int dpa4k_expert_linear_backward(const void* grad, const void* x, const void* weight, const int64_t* offsets,
-                                            const int64_t* order, const int64_t* slots, void* grad_x, void* grad_weight,
-                                            int64_t places, int64_t k, int64_t inner, int64_t n_experts, int64_t k_in, int64_t n_out,
-                                            int type, void* workspace, size_t workspace_bytes, dpa4k_stream_t stream) {
-  clear_error();
-  const int status = check_product("expert linear", places, k, inner, n_experts, k_in, n_out, type);
-  if (status != DPA4K_OK) return status;
-  const hipStream_t on = as_stream(stream);
+namespace {
+
+// What both backwards do: dx and dW from dz, whose second part is `grad_low` (or null).
+int linear_backward(const void* grad, const void* grad_low, const void* x, const void* weight, const int64_t* offsets,
+                    const int64_t* order, const int64_t* slots, void* grad_x, void* grad_weight, int64_t places, int64_t k,
+                    int64_t inner, int64_t n_experts, int64_t k_in, int64_t n_out, int type, void* workspace, hipStream_t on) {
   const bool by_token = order != nullptr;
-  const bool nothing = places == 0 || inner == 0;
-  if (nothing) grad_x = nullptr;
-  if (grad_x == nullptr && grad_weight == nullptr) return DPA4K_OK;
-  if (offsets == nullptr || (!nothing && grad == nullptr) || (grad_x != nullptr && (weight == nullptr || (by_token && slots == nullptr))) ||
-      (grad_weight != nullptr && !nothing && x == nullptr))
-    return fail(DPA4K_EINVAL, "expert linear: null pointer");
-  const size_t needed = dpa4k_expert_linear_workspace_size(places, k, inner, n_experts, k_in, n_out, by_token, grad_x != nullptr,
-                                                           grad_weight != nullptr);
-  if (needed > 0 && (workspace == nullptr || workspace_bytes < needed))
-    return fail(DPA4K_EWORKSPACE, "expert linear: workspace too small");
   ProductCall call{};
   call.offsets = offsets, call.order = order;
   call.places = places, call.experts = static_cast<int>(n_experts), call.k = static_cast<int>(k), call.inner = static_cast<int>(inner);
   call.k_in = static_cast<int>(k_in), call.n_out = static_cast<int>(n_out);
+  call.a = grad, call.a_low = grad_low;
   return with_type(type, DPA4K_EINVAL, [&](auto t) {
     typedef typename decltype(t)::type T;
     if (grad_x != nullptr) {
       ProductCall of_x = call;
-      of_x.a = grad, of_x.b = weight, of_x.out = by_token ? workspace : grad_x, of_x.by_slot = by_token;
+      of_x.b = weight, of_x.out = by_token ? workspace : grad_x, of_x.by_slot = by_token;
       int ran = run_product<T, kInput>(of_x, on);
       if (ran != DPA4K_OK) return ran;
       if (by_token) {
@@ -1288,7 +1312,7 @@ extern "C" int dpa4k_expert_linear_backward(const void* grad, const void* x, con
     if (grad_weight != nullptr) {
       ProductCall of_w = call;
       const Chunks chunks = weight_chunks(places, inner, n_experts, k_in, n_out);
-      of_w.a = grad, of_w.b = x, of_w.chunk_rows = chunks.rows, of_w.chunks = chunks.most;
+      of_w.b = x, of_w.chunk_rows = chunks.rows, of_w.chunks = chunks.most;
       of_w.out = chunks.most > 0 ? workspace : grad_weight;
       int ran = run_product<T, kWeight>(of_w, on);
       if (ran != DPA4K_OK || chunks.most == 0) return ran;
@@ -1300,6 +1324,80 @@ extern "C" int dpa4k_expert_linear_backward(const void* grad, const void* x, con
     }
     return static_cast<int>(DPA4K_OK);
   });
+}
+
+// One part of dz, in bytes; a 16-bit dz has two.
+size_t part_bytes(int64_t places, int64_t inner, int64_t n_out, int type) {
+  return round_up_256(static_cast<size_t>(places * inner) * n_out * size_of_type(type));
+}
+
+}  // namespace
+
+extern "C" int dpa4k_expert_linear_backward(const void* grad, const void* x, const void* weight, const int64_t* offsets,
+                                            const int64_t* order, const int64_t* slots, void* grad_x, void* grad_weight,
+                                            int64_t places, int64_t k, int64_t inner, int64_t n_experts, int64_t k_in, int64_t n_out,
+                                            int type, void* workspace, size_t workspace_bytes, dpa4k_stream_t stream) {
+  clear_error();
+  const int status = check_product("expert linear", places, k, inner, n_experts, k_in, n_out, type);
+  if (status != DPA4K_OK) return status;
+  const bool by_token = order != nullptr;
+  const bool nothing = places == 0 || inner == 0;
+  if (nothing) grad_x = nullptr;
+  if (grad_x == nullptr && grad_weight == nullptr) return DPA4K_OK;
+  if (offsets == nullptr || (!nothing && grad == nullptr) || (grad_x != nullptr && (weight == nullptr || (by_token && slots == nullptr))) ||
+      (grad_weight != nullptr && !nothing && x == nullptr))
+    return fail(DPA4K_EINVAL, "expert linear: null pointer");
+  const size_t needed = dpa4k_expert_linear_workspace_size(places, k, inner, n_experts, k_in, n_out, by_token, grad_x != nullptr,
+                                                           grad_weight != nullptr);
+  if (needed > 0 && (workspace == nullptr || workspace_bytes < needed))
+    return fail(DPA4K_EWORKSPACE, "expert linear: workspace too small");
+  return linear_backward(grad, nullptr, x, weight, offsets, order, slots, grad_x, grad_weight, places, k, inner, n_experts, k_in, n_out,
+                         type, workspace, as_stream(stream));
+}
+
+extern "C" size_t dpa4k_expert_gated_workspace_size(int64_t places, int64_t k, int64_t inner, int64_t n_experts, int64_t k_in,
+                                                    int64_t n_out, int by_token, int want_x, int want_weight, int type) {
+  if (places <= 0 || inner <= 0 || n_experts < 1 || k_in < 1 || n_out < 1 || places > INT32_MAX / inner || !known_type(type)) return 0;
+  return part_bytes(places, inner, n_out, type) * (size_of_type(type) == 2 ? 2 : 1) +
+         dpa4k_expert_linear_workspace_size(places, k, inner, n_experts, k_in, n_out, by_token, want_x, want_weight);
+}
+
+extern "C" int dpa4k_expert_gated_backward(const void* grad, const float* before, const void* x, const void* weight,
+                                           const int64_t* offsets, const int64_t* order, const int64_t* slots, void* grad_x,
+                                           void* grad_weight, int64_t places, int64_t k, int64_t inner, int64_t n_experts, int64_t k_in,
+                                           int64_t n_out, int type, void* workspace, size_t workspace_bytes, dpa4k_stream_t stream) {
+  clear_error();
+  const int status = check_product("expert linear", places, k, inner, n_experts, k_in, n_out, type);
+  if (status != DPA4K_OK) return status;
+  if (n_out % 2 != 0) return fail(DPA4K_EINVAL, "expert linear: a gate needs an even number of outputs");
+  const hipStream_t on = as_stream(stream);
+  const bool by_token = order != nullptr;
+  const bool nothing = places == 0 || inner == 0;
+  if (nothing) grad_x = nullptr;
+  if (grad_x == nullptr && grad_weight == nullptr) return DPA4K_OK;
+  if (offsets == nullptr || (!nothing && (grad == nullptr || before == nullptr)) ||
+      (grad_x != nullptr && (weight == nullptr || (by_token && slots == nullptr))) || (grad_weight != nullptr && !nothing && x == nullptr))
+    return fail(DPA4K_EINVAL, "expert linear: null pointer");
+  const size_t needed = dpa4k_expert_gated_workspace_size(places, k, inner, n_experts, k_in, n_out, by_token, grad_x != nullptr,
+                                                          grad_weight != nullptr, type);
+  if (needed > 0 && (workspace == nullptr || workspace_bytes < needed))
+    return fail(DPA4K_EWORKSPACE, "expert linear: workspace too small");
+  const size_t part = nothing ? 0 : part_bytes(places, inner, n_out, type);
+  char* high = static_cast<char*>(workspace);
+  char* low = size_of_type(type) == 2 && !nothing ? high + part : nullptr;
+  char* rest = low != nullptr ? low + part : high + part;
+  if (!nothing) {
+    const int ran = with_type(type, DPA4K_EINVAL, [&](auto t) {
+      typedef typename decltype(t)::type T;
+      const int64_t rows = places * inner, half = n_out / 2;
+      gate_backward_kernel<T><<<pieces_grid(rows * ((half + kV<T> - 1) / kV<T>)), 256, 0, on>>>(
+          static_cast<const T*>(grad), before, reinterpret_cast<T*>(high), reinterpret_cast<T*>(low), rows, static_cast<int>(half));
+      return launched("gate_backward_kernel");
+    });
+    if (ran != DPA4K_OK) return ran;
+  }
+  return linear_backward(high, low, x, weight, offsets, order, slots, grad_x, grad_weight, places, k, inner, n_experts, k_in, n_out,
+                         type, rest, on);
 }
 
 extern "C" int dpa4k_expert_combine_forward(const void* y, const float* weights, const int64_t* slots, void* out, int64_t tokens,

@@ -1058,17 +1058,19 @@ def expert_linear_backward(grad, x, weight, before, offsets, order, slots, sizes
     device, code = x.device, ELEMENT_TYPES[x.dtype]
     grad_x = torch.empty_like(x) if want_x else None
     grad_weight = torch.empty_like(weight) if want_weight else None
-    nbytes = _LIB.dpa4k_expert_linear_workspace_size(places, k, inner, n_experts, k_in, n_out, order is not None, want_x, want_weight)
+    extents = places, k, inner, n_experts, k_in, n_out
+    if before is None:
+        nbytes = _LIB.dpa4k_expert_linear_workspace_size(*extents, order is not None, want_x, want_weight)
+    else:
+        nbytes = _LIB.dpa4k_expert_gated_workspace_size(*extents, order is not None, want_x, want_weight, code)
     workspace = _workspace(nbytes, device) if nbytes else None
+    rest = (_ptr(x), _ptr(weight), offsets.data_ptr(), _ptr(order), _ptr(slots), _ptr(grad_x), _ptr(grad_weight), *extents, code,
+            _ptr(workspace), nbytes)
     with _on(device) as stream:
-        if before is not None:
-            grad_before = torch.empty(before.shape, dtype=x.dtype, device=device)
-            _lib.check(_LIB.dpa4k_expert_gate_backward(_ptr(grad), _ptr(before), _ptr(grad_before), places * inner, n_out // 2, code,
-                                                       stream))
-            grad = grad_before
-        status = _LIB.dpa4k_expert_linear_backward(
-            _ptr(grad), _ptr(x), _ptr(weight), offsets.data_ptr(), _ptr(order), _ptr(slots), _ptr(grad_x), _ptr(grad_weight),
-            places, k, inner, n_experts, k_in, n_out, code, _ptr(workspace), nbytes, stream)
+        if before is None:
+            status = _LIB.dpa4k_expert_linear_backward(_ptr(grad), *rest, stream)
+        else:
+            status = _LIB.dpa4k_expert_gated_backward(_ptr(grad), _ptr(before), *rest, stream)
     _lib.check(status)
     return grad_x, grad_weight
 

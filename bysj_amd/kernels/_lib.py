@@ -15,7 +15,7 @@ from pathlib import Path
 LIBRARY_PATH = Path(__file__).resolve().parent.parent / "libdpa4k.so"
 
 OK, EINVAL, EHIP, EWORKSPACE = 0, 1, 2, 3
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -113,9 +113,10 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "dpa4k_expert_dispatch_workspace_size": (_SZ, [_I64] * 2),
     "dpa4k_expert_dispatch": (_INT, [_P, _I64, _I64, _P, _P, _P, _P, _SZ, _P]),
     "dpa4k_expert_linear_forward": (_INT, [_P] * 6 + [_I64] * 6 + [_INT] * 2 + [_P]),
-    "dpa4k_expert_gate_backward": (_INT, [_P] * 3 + [_I64] * 2 + [_INT, _P]),
     "dpa4k_expert_linear_workspace_size": (_SZ, [_I64] * 6 + [_INT] * 3),
     "dpa4k_expert_linear_backward": (_INT, [_P] * 8 + [_I64] * 6 + [_INT, _P, _SZ, _P]),
+    "dpa4k_expert_gated_workspace_size": (_SZ, [_I64] * 6 + [_INT] * 4),
+    "dpa4k_expert_gated_backward": (_INT, [_P] * 9 + [_I64] * 6 + [_INT, _P, _SZ, _P]),
     "dpa4k_expert_combine_forward": (_INT, [_P] * 4 + [_I64] * 3 + [_INT, _P]),
     "dpa4k_expert_combine_backward": (_INT, [_P] * 7 + [_I64] * 3 + [_INT, _P]),
     "dpa4k_grad_norm_workspace_size": (_SZ, [_P, _I64]),

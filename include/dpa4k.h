@@ -61,7 +61,7 @@ const char* dpa4k_last_error(void);
 
 /* ABI version of this header (bumped on any signature change). */
 int dpa4k_abi_version(void);
-#define DPA4K_ABI_VERSION 12
+#define DPA4K_ABI_VERSION 13
 
 /* ------------------------------------------------------------------------
  * CSR construction
@@ -682,12 +682,6 @@ int dpa4k_expert_linear_forward(const void* x, const void* weight,
                                 int64_t n_out, int gated, int type,
                                 dpa4k_stream_t stream);
 
-/* dz of the gated SiLU: grad[rows, C] and grad_before[rows, 2 C] of `type`,
- * before float[rows, 2 C]. */
-int dpa4k_expert_gate_backward(const void* grad, const float* before,
-                               void* grad_before, int64_t rows, int64_t channels,
-                               int type, dpa4k_stream_t stream);
-
 /* grad[places, inner, n_out] is that of z.  grad_x like x: with order, the sum
  * in 32 bits over the places of a token (slots[places] as places of
  * dpa4k_expert_dispatch); without, rows behind offsets[E] become 0.
@@ -705,6 +699,24 @@ int dpa4k_expert_linear_backward(const void* grad, const void* x,
                                  int64_t k_in, int64_t n_out, int type,
                                  void* workspace, size_t workspace_bytes,
                                  dpa4k_stream_t stream);
+
+/* The same for a gated forward: grad[places, inner, n_out / 2] is that of y, before
+ * float[places, inner, n_out] what the forward kept.  The gradient of z lies in the
+ * workspace, in 16-bit types in two parts whose products are added (2^-18 of
+ * it is lost in bfloat16; in float16 2^-24 or 2^-25, and it goes up to 1.3e8). */
+size_t dpa4k_expert_gated_workspace_size(int64_t places, int64_t k,
+                                         int64_t inner, int64_t n_experts,
+                                         int64_t k_in, int64_t n_out,
+                                         int by_token, int want_x,
+                                         int want_weight, int type);
+int dpa4k_expert_gated_backward(const void* grad, const float* before,
+                                const void* x, const void* weight,
+                                const int64_t* offsets, const int64_t* order,
+                                const int64_t* slots, void* grad_x,
+                                void* grad_weight, int64_t places, int64_t k,
+                                int64_t inner, int64_t n_experts, int64_t k_in,
+                                int64_t n_out, int type, void* workspace,
+                                size_t workspace_bytes, dpa4k_stream_t stream);
 
 /* out[t] = sum_j weights[t, j] y[slots[t, j]] over entries of `size` elements of
  * `type`, summed in 32 bits in order; a slot of -1 adds nothing.  y has T k

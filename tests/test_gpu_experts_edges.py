@@ -1,0 +1,103 @@
+"""GPU tests of the expert operators where a sum is long, a value extreme or a segment far from the mean.
+
+Sums of n equal terms in sequence: each addition is off by at most half a step of the running sum, so together at most
+n 2^-25 of the result, here with every second-level addition counted too.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from bysj_amd.kernels.block_norm import residual_norm
+from bysj_amd.kernels.experts import ExpertPlan, expert_dispatch, expert_linear, expert_route
+from oracle.experts import expert_dispatch_reference, expert_linear_reference, expert_route_reference
+from parity import announce, assert_bitwise, assert_close_scaled
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _half(dtype):
+    return 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+
+
+# ---------------------------------------------------------------------------
+# the gated SiLU's gradient between the products
+# ---------------------------------------------------------------------------
+
+def _gated_gradients(plan, experts, inner, k_in, n_out, dtype, *, from_tokens, seed):
+    announce("expert linear, gated gradients", tuple(plan[2].shape), experts, inner, k_in, n_out, dtype, from_tokens)
+    generator = torch.Generator().manual_seed(seed)
+    entries = plan[2].shape[0] if from_tokens else plan[2].numel()
+    x = torch.randn(entries, *inner, k_in, generator=generator).to(dtype)
+    weight = (torch.randn(experts, 2 * n_out, k_in, generator=generator) * k_in ** -0.5).to(dtype)
+    dy = torch.randn(plan[2].numel(), *inner, n_out, generator=generator).to(dtype)
+    leaves = x.to(DEV).requires_grad_(True), weight.to(DEV).requires_grad_(True)
+    y = expert_linear(*leaves, ExpertPlan(*(t.to(DEV) for t in plan)), from_tokens=from_tokens, activation="silu_gate")
+    grads = torch.autograd.grad(y, leaves, dy.to(DEV))
+    _, *wanted = expert_linear_reference(x, weight, plan, from_tokens=from_tokens, activation="silu_gate", grad=dy)
+    # dz in two parts: bfloat16 2^-18 of each product, float16 2^-24, or 2^-25 of the other operand
+    operands = (weight.double().abs().sum((0, 1)), x.double().abs().reshape(-1, k_in).sum(0))
+    for got, value, products, operand, what in zip(grads, wanted[:2], wanted[2:], operands, ("dx", "dweight")):
+        budget = (1e-5 + _half(dtype)) * value.abs() + 1e-5 * value.abs().max()
+        budget = budget + (2.0 ** -18 * products if dtype == BF16 else 2.0 ** -24 * products + 2.0 ** -25 * (1.0 + operand))
+        error = (got.detach().cpu().double() - value).abs()
+        assert bool((error <= budget).all()), (what, float((error - budget).max()), float(value.abs().max()))
+
+
+def _random_plan(tokens, k, experts, seed):
+    generator = torch.Generator().manual_seed(seed)
+    chosen = torch.randint(0, experts, (tokens, k), generator=generator)
+    chosen[torch.rand(tokens, generator=generator) < 0.1] = -1
+    return expert_dispatch_reference(chosen, experts)
+
+
+# loads by piece and straight to LDS, ragged and whole rows, every tile; sums of one slice, of several, of an odd number
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("k_in,n_out", [(1, 1), (3, 5), (16, 20), (32, 32), (33, 31), (64, 64), (90, 65), (128, 96), (130, 200), (264, 33)])
+def test_gated_gradients_round_once(k_in, n_out, dtype):
+    for from_tokens in (True, False):
+        _gated_gradients(_random_plan(61, 3, 5, seed=k_in), 5, (), k_in, n_out, dtype, from_tokens=from_tokens, seed=n_out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens,k,experts,inner,k_in,n_out", [(900, 2, 3, (), 256, 264), (900, 2, 3, (), 266, 130), (1, 1, 1, (), 48, 40),
+                                                               (3000, 1, 2, (3,), 64, 48), (40, 2, 200, (), 48, 70)])
+def test_gated_gradients_of_plans(tokens, k, experts, inner, k_in, n_out, dtype):
+    """Tiles of 256 by 256 and of 128, one token, segments that dW cuts, more experts than rows."""
+    for from_tokens in (True, False):
+        _gated_gradients(_random_plan(tokens, k, experts, seed=tokens), experts, inner, k_in, n_out, dtype, from_tokens=from_tokens, seed=k)
+
+
+@pytest.mark.parametrize("dtype,k_in,n_out", [(BF16, 8, 6), (F16, 10, 48), (BF16, 16, 96)])
+def test_gated_gradients_of_many_rows(dtype, k_in, n_out):
+    """So many rows that a workgroup takes a run of tiles; sums of one, two and three slices a part."""
+    generator = torch.Generator().manual_seed(n_out)
+    chosen = torch.multinomial(torch.tensor([0.5, 0.0, 0.3, 0.01, 0.19]), 26_000, replacement=True, generator=generator)[:, None]
+    chosen[torch.rand(26_000, generator=generator) < 0.02] = -1
+    plan = tuple(t.cpu() for t in expert_dispatch(chosen.to(DEV), 5))
+    for from_tokens in (True, False):
+        _gated_gradients(plan, 5, (33,), k_in, n_out, dtype, from_tokens=from_tokens, seed=1)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 700])
+def test_gated_gradients_past_float16(rows):
+    """dy * up * slope of 1.8e5: past float16, while the gradients of x and of the matrix fit."""
+    announce("expert linear, gated gradients past float16", rows)
+    k_in = 256
+    x = torch.full((rows, k_in), 0.3, dtype=F16)
+    weight = torch.full((1, 2, k_in), 0.53, dtype=F16)
+    weight[0, 0] = 0.026
+    dy = torch.zeros(rows, 1, dtype=F16)
+    dy[rows // 2] = 4000.0
+    plan = expert_dispatch_reference(torch.zeros(rows, 1, dtype=torch.int64), 1)
+    leaves = x.to(DEV).requires_grad_(True), weight.to(DEV).requires_grad_(True)
+    y = expert_linear(*leaves, ExpertPlan(*(t.to(DEV) for t in plan)), activation="silu_gate")
+    grads = torch.autograd.grad(y, leaves, dy.to(DEV))
+    _, want_x, want_w, _, _ = expert_linear_reference(x, weight, plan, activation="silu_gate", grad=dy)
+    assert float(want_x.abs().max()) < 65504.0 and float(want_w.abs().max()) < 65504.0
+    for got, wanted in zip(grads, (want_x, want_w)):
+        assert_close_scaled(got, wanted, rtol=1e-5 + _half(F16), what="gradient")
