@@ -58,15 +58,16 @@ struct ProductCall {
   const void* a;           // x (forward), dz (dx, dW)
   const void* a_low;       // dx, dW: what dz has below `a`, or null (two_parts)
   const void* b;           // W (forward, dx), x (dW)
-  void* out;               // y, dx by place or by slot, dW or its partial sums
+  void* out;               // y, dx by place or by slot, dW
+  float* partial;          // dW: [chunks][n_out][k_in], the sums of the cut segments' chunks
   float* before;           // forward, gated: z, or null
   const int64_t* offsets;
   const int64_t* order;    // null: x by place
   int64_t places;
   int experts, k, inner;   // k: slots of a token, which order is divided by
   int k_in, n_out;         // of W[e], n_out before the gate
-  int chunk_rows;          // dW: rows of a segment that one workgroup takes
-  int chunks;              // dW: most chunks of all segments; 1 and no partial sums if every segment is one
+  int chunk_rows;          // dW: rows that one workgroup takes; longer segments are cut
+  int chunks;              // dW: most chunks of all cut segments; 0 if none can be longer
   int by_slot;             // dx: written at order[p] instead of p
   int run;                 // row tiles that one workgroup takes, up to kMostRun
 };
@@ -144,6 +145,48 @@ __device__ __forceinline__ bool find_tile(const ProductCall& call, int segments,
       return true;
     }
     before += __shfl(upto, 63, 64);
+  }
+  return false;
+}
+
+// dW: chunks of a segment that is cut, 0 for one that a workgroup takes whole.  At most
+// the chunks there are, as segments of a malformed plan may overlap.
+__device__ __forceinline__ int chunks_of(const ProductCall& call, const Span& span) {
+  const int count = tiles_of(span, call.chunk_rows, true);
+  return count < 2 ? 0 : (count < call.chunks ? count : call.chunks);
+}
+
+// Chunks of the cut segments in front of `segment`, by a wave.
+__device__ __forceinline__ int chunks_before(const ProductCall& call, int segment) {
+  int sum = 0;
+  for (int e = threadIdx.x & 63; e < segment; e += 64) {
+    sum += chunks_of(call, span_of(call, e));
+    sum = sum < call.chunks ? sum : call.chunks;
+  }
+  sum = group_sum<64>(sum);
+  return __builtin_amdgcn_readfirstlane(sum < call.chunks ? sum : call.chunks);
+}
+
+// The cut segment number `number`, the chunks of those in front of it and its own, by a
+// wave; false behind the last.
+__device__ __forceinline__ bool cut_segment(const ProductCall& call, int number, int& segment, int& before, int& count) {
+  const int lane = threadIdx.x & 63;
+  before = 0;
+  for (int first = 0; first < call.experts; first += 64) {
+    const int mine = first + lane < call.experts ? chunks_of(call, span_of(call, first + lane)) : 0;
+    const uint64_t cut = __ballot(mine > 0);
+    const uint64_t in_front = cut & ((uint64_t(1) << lane) - 1);
+    const uint64_t found = __ballot(mine > 0 && __popcll(in_front) == number);
+    const int there = found != 0 ? __builtin_ctzll(found) : 64;
+    before += group_sum<64>(lane < there ? mine : 0);
+    before = before < call.chunks ? before : call.chunks;
+    if (found != 0) {
+      segment = first + there;
+      count = __shfl(mine, there, 64);
+      count = count < call.chunks - before ? count : call.chunks - before;
+      return true;
+    }
+    number -= __popcll(cut);
   }
   return false;
 }
@@ -319,12 +362,15 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   const int tile_rows = RUN ? call.run * BM : BM;
   int segment, number;
   Span span;
-  int row_tile = 0, chunk = 0;
+  int row_tile = 0, chunk = -1;                          // dW: the chunk of a cut segment
   if constexpr (MODE == kWeight) {
     const int row_tiles = (call.n_out + BM - 1) / BM;
     row_tile = rest % row_tiles;
-    chunk = rest / row_tiles;
-    if (!find_tile(call, call.experts, call.chunk_rows, true, chunk, segment, number, span)) return;
+    if (!find_tile(call, call.experts, call.chunk_rows, true, rest / row_tiles, segment, number, span)) return;
+    if (call.chunks > 0 && chunks_of(call, span) > 0) {
+      chunk = chunks_before(call, segment) + number;
+      if (chunk >= call.chunks) return;                  // of a malformed plan
+    }
     span.begin += number * call.chunk_rows;
     if (span.end - span.begin > call.chunk_rows) span.end = span.begin + call.chunk_rows;
   } else {
@@ -657,7 +703,7 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
   // rows, so that z is stored in whole lines of 128 bytes (516 -> 458 us forward), past
   // the caches, which its 537 MB would empty of rows and matrices (forward alone 391 ->
   // 371 us, the gate's backward behind it 189 -> 164; no change where z fits them).
-  const bool partial = MODE == kWeight && call.chunks > 0;
+  const bool partial = MODE == kWeight && chunk >= 0;
   const auto shifted = [&](int index, int size) { return FAST == kRagged && index >= size / V * V ? (V - size % V) % V : 0; };
   const auto store = [&](int tile) {
     const int above = tile * BM;                         // rows of the run above this tile
@@ -709,7 +755,8 @@ __global__ __launch_bounds__((WM * WN * 64)) void expert_product_kernel(ProductC
           float four[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) four[i] = sum[m][n][4 * g + i];
-          if (partial || (MODE == kInput && call.by_slot)) store_pack<false, float, 4>(static_cast<float*>(call.out) + at, four, width - column);
+          if (partial) store_pack<false, float, 4>(call.partial + at, four, width - column);
+          else if (MODE == kInput && call.by_slot) store_pack<false, float, 4>(static_cast<float*>(call.out) + at, four, width - column);
           else store_pack<false, T, 4>(static_cast<T*>(call.out) + at, four, width - column);
         }
       }
@@ -903,31 +950,14 @@ int run_few_rows(const ProductCall& call, hipStream_t stream) {
   return launched("expert_few_rows_kernel");
 }
 
-// dW[e] = the sum of its chunks' partial sums, in order, in 64 bits.
+// dW[e] of the cut segments: the sum of their chunks' partial sums, in order, in 64 bits.
 template <typename T>
-__global__ __launch_bounds__(256) void weight_sum_kernel(ProductCall call, const float* __restrict__ partial, T* __restrict__ out,
-                                                         int blocks) {
-  const int e = blockIdx.x / blocks;
-  // the first chunk of the expert: chunks of the ones before
-  __shared__ int found[2];
-  // not past the chunks there are: segments of a malformed plan may overlap
-  const auto there = [&](int chunk) { return chunk < call.chunks ? chunk : call.chunks; };
-  if (threadIdx.x < 64) {
-    int before = 0, mine = 1;
-    for (int f = threadIdx.x; f <= e; f += 64) {
-      const Span span = span_of(call, f);
-      const int count = tiles_of(span, call.chunk_rows, true);
-      if (f < e) before = there(before + there(count));
-      else mine = there(count);
-    }
-    before = there(group_sum<64>(before));
-    if (threadIdx.x == 0) found[0] = before;
-    if (static_cast<int>(threadIdx.x) == e % 64) found[1] = mine;
-  }
-  __syncthreads();
+__global__ __launch_bounds__(256) void weight_sum_kernel(ProductCall call, int blocks) {
+  int e, before, count;
+  if (!cut_segment(call, blockIdx.x / blocks, e, before, count)) return;
   const int64_t size = static_cast<int64_t>(call.n_out) * call.k_in;
-  const float* from = partial + found[0] * size;
-  const int count = there(found[0] + found[1]) - found[0];
+  const float* from = call.partial + before * size;
+  T* out = static_cast<T*>(call.out) + e * size;
   // 32 elements at a time, eight threads each
   __shared__ double words[8][32];
   const int part = threadIdx.x / 32, element = threadIdx.x % 32;
@@ -943,7 +973,7 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(ProductCall call, const
     if (part == 0 && at < size) {
 #pragma unroll
       for (int p = 1; p < 8; ++p) sum += words[p][element];
-      out[e * size + at] = static_cast<T>(sum);
+      out[at] = static_cast<T>(sum);
     }
     __syncthreads();
   }
@@ -1146,7 +1176,7 @@ int launch_product(ProductCall call, hipStream_t stream) {
   const int64_t width = MODE == kGated ? call.n_out / 2 : (MODE == kForward ? call.n_out : call.k_in);
   const int64_t columns = (width + (MODE == kGated ? BN / 2 : BN) - 1) / (MODE == kGated ? BN / 2 : BN);
   int64_t tiles;
-  if (MODE == kWeight) tiles = columns * ((call.n_out + BM - 1) / BM) * (call.chunks > 0 ? call.chunks : call.experts);
+  if (MODE == kWeight) tiles = columns * ((call.n_out + BM - 1) / BM) * (call.experts + (call.chunks > 0 ? rows / call.chunk_rows : 0));
   else tiles = columns * (rows / (RUN ? call.run * BM : BM) + call.experts + 1);
   if (tiles > row_block_limit(Z::kThreads)) return fail(DPA4K_EINVAL, "expert linear: more tiles than a launch takes");
   // two row tiles with all their columns; of dW, one (32,768 rows, 1,024 to 2 x 2,048 in
@@ -1211,28 +1241,32 @@ int run_product(const ProductCall& call, hipStream_t stream) {
   return fast ? run_tiles<T, MODE, kRagged>(call, stream) : run_tiles<T, MODE, kByPiece>(call, stream);
 }
 
-// Rows of a segment that one workgroup of dW takes: all of them where the matrices
-// make tiles enough, else so few that about 1,024 workgroups have some; and no more
-// than kLongest, 2,048 additions of 16-bit operands (6e-5 of equal terms at worst) and
-// 256 and 64 of float32, where segments are longer than that in the mean.  Shorter
-// cuts would cost partial sums: at 4,096 by 4,096 these are an eighth of the
-// operands' bytes.
+// Rows of a segment that one workgroup of dW takes: at most kLongest, 2,048 additions
+// of 16-bit operands (6e-5 of equal terms at worst) and 256 and 64 of float32, and where
+// the matrices alone do not make tiles enough, so few that about 1,024 workgroups have
+// some.  What is longer is cut, by its own length: routing may collapse to one of many
+// experts (1,000,000 rows, 32 matrices of 1,024 to 2,048 in bfloat16: 4.4 ms for equal
+// segments, 4.8 for a single one, 27.9 uncut).  Shorter cuts would cost partial sums: at
+// 4,096 by 4,096 these are an eighth of the operands' bytes, with room for twice as many.
 constexpr int64_t kLongest = 32768;
 
 struct Chunks {
-  int rows, most;    // most == 0: no partial sums
+  int rows, most;    // most == 0: no segment is longer than that
+  int segments;      // that can be longer
 };
 
 Chunks weight_chunks(int64_t places, int64_t inner, int64_t experts, int64_t k_in, int64_t n_out) {
   const int64_t rows = places * inner;
   const int64_t edge = n_out <= 64 || k_in <= 64 ? 64 : 128;
   const int64_t tiles = ((n_out + edge - 1) / edge) * ((k_in + edge - 1) / edge);
-  const bool many = tiles * experts >= 512;
-  if ((many && rows <= kLongest * experts) || rows <= 512 * experts) return Chunks{INT_MAX, 0};
-  int64_t chunk = many ? kLongest : (rows * tiles + 1023) / 1024;
-  if (chunk > kLongest) chunk = kLongest;
-  chunk = (chunk + 511) / 512 * 512;
-  return Chunks{static_cast<int>(chunk), static_cast<int>(rows / chunk + experts)};
+  int64_t chunk = kLongest;
+  if (tiles * experts < 512 && rows > 512 * experts) {
+    const int64_t share = ((rows * tiles + 1023) / 1024 + 511) / 512 * 512;
+    chunk = share < kLongest ? share : kLongest;
+  }
+  if (rows <= chunk) return Chunks{static_cast<int>(chunk), 0, 0};
+  const int64_t segments = rows / (chunk + 1) < experts ? rows / (chunk + 1) : experts;
+  return Chunks{static_cast<int>(chunk), static_cast<int>(rows / chunk + segments), static_cast<int>(segments)};
 }
 
 int pieces_grid(int64_t pieces) {
@@ -1313,13 +1347,12 @@ int linear_backward(const void* grad, const void* grad_low, const void* x, const
       ProductCall of_w = call;
       const Chunks chunks = weight_chunks(places, inner, n_experts, k_in, n_out);
       of_w.b = x, of_w.chunk_rows = chunks.rows, of_w.chunks = chunks.most;
-      of_w.out = chunks.most > 0 ? workspace : grad_weight;
+      of_w.out = grad_weight, of_w.partial = static_cast<float*>(workspace);
       int ran = run_product<T, kWeight>(of_w, on);
       if (ran != DPA4K_OK || chunks.most == 0) return ran;
       const int64_t size = k_in * n_out;
       const int64_t blocks = (size + 31) / 32 < 512 ? (size + 31) / 32 : 512;
-      weight_sum_kernel<T><<<static_cast<unsigned int>(blocks * n_experts), 256, 0, on>>>(
-          of_w, static_cast<const float*>(workspace), static_cast<T*>(grad_weight), static_cast<int>(blocks));
+      weight_sum_kernel<T><<<static_cast<unsigned int>(blocks * chunks.segments), 256, 0, on>>>(of_w, static_cast<int>(blocks));
       return launched("weight_sum_kernel");
     }
     return static_cast<int>(DPA4K_OK);

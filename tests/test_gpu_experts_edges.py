@@ -101,3 +101,54 @@ def test_gated_gradients_past_float16(rows):
     assert float(want_x.abs().max()) < 65504.0 and float(want_w.abs().max()) < 65504.0
     for got, wanted in zip(grads, (want_x, want_w)):
         assert_close_scaled(got, wanted, rtol=1e-5 + _half(F16), what="gradient")
+
+
+# ---------------------------------------------------------------------------
+# sums of long segments among short ones
+# ---------------------------------------------------------------------------
+
+def _one_segment(rows, experts, k_in, n_out, dtype, only):
+    """dW where one expert has every row and all terms are equal."""
+    announce("expert linear, one segment of many", rows, experts, k_in, n_out, dtype)
+    plan = expert_dispatch(torch.full((rows, 1), only, device=DEV), experts)
+    x = torch.full((rows, k_in), 0.7, device=DEV, dtype=dtype)
+    x[:, 1::2] = -0.35
+    weight = torch.zeros(experts, n_out, k_in, device=DEV, dtype=dtype, requires_grad=True)
+    y = expert_linear(x, weight, plan, from_tokens=False)
+    dy = torch.full_like(y, 0.3)
+    (dw,) = torch.autograd.grad(y, weight, dy)
+    row = rows * x[0].cpu().double() * float(dy[0, 0])
+    assert int(dw[:only].count_nonzero()) == 0 and int(dw[only + 1:].count_nonzero()) == 0
+    # at most 32,768 rows in sequence: 2,048 additions of 16-bit operands, 256 and 64 of float32
+    assert_close_scaled(dw[only], row.expand(n_out, k_in), rtol=(320 if dtype == F32 else 2048) * 2.0 ** -25 + 2.0 ** -24 + _half(dtype),
+                        scale=0.0, what="dweight")
+
+
+@pytest.mark.parametrize("dtype,rows,experts,k_in,n_out", [(F32, 131_000, 4, 1024, 2048), (BF16, 4_190_000, 128, 256, 256), (F32, 1_000_000, 32, 256, 512),
+                                                           (F32, 520_000, 1024, 64, 40), (F32, 256_000, 500, 64, 40), (BF16, 256_000, 500, 24, 40),
+                                                           (F16, 256_001, 501, 25, 40)])
+def test_one_segment_of_many_experts(dtype, rows, experts, k_in, n_out):
+    """Cuts go by a segment's own length: the mean is below 32,768 rows here, or below 512."""
+    _one_segment(rows, experts, k_in, n_out, dtype, experts // 2)
+
+
+@pytest.mark.parametrize("k_in,n_out", [(24, 40), (1024, 1032)])
+def test_segments_around_the_cut(k_in, n_out):
+    """Segments of 0, 1, 32,767 to 32,769, 65,536 and 65,537 rows, cut and uncut side by side, gradients against 64 bits."""
+    lengths = [32_769, 0, 65_537, 1, 32_768, 65_536, 32_767, 300, 0]
+    announce("expert linear, segments around the cut", k_in, n_out)
+    chosen = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
+    chosen = chosen[torch.randperm(chosen.numel(), generator=torch.Generator().manual_seed(1))]
+    plan = expert_dispatch(chosen[:, None].to(DEV), len(lengths))
+    for dtype in (F32, BF16):
+        generator = torch.Generator().manual_seed(2)
+        x = torch.randn(chosen.numel(), k_in, generator=generator).to(dtype).to(DEV)
+        weight = torch.randn(len(lengths), n_out, k_in, generator=generator).to(dtype).to(DEV).requires_grad_(True)
+        y = expert_linear(x, weight, plan)
+        dy = torch.randn(y.shape, generator=generator).to(dtype).to(DEV)
+        (dw,) = torch.autograd.grad(y, weight, dy)
+        offsets = plan.offsets.tolist()
+        for e in range(len(lengths)):
+            a, b = offsets[e], offsets[e + 1]
+            wanted = dy[a:b].double().t() @ x[plan.order[a:b]].double()
+            assert_close_scaled(dw[e], wanted, rtol=1e-5 + _half(dtype), what=f"dweight {e} {dtype}")
