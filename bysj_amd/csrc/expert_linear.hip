@@ -882,6 +882,29 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ProductCall call, 
   f32x4m sum[kGroups];
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) sum[g] = f32x4m{0.0f, 0.0f, 0.0f, 0.0f};
+  // Register i of a lane: row 4 (lane / 16) + i, column lane mod 16.  float32: sums in two
+  // levels, as in tiles, of 512 products of a wave and these in LDS (65,536 inputs of one
+  // size: 2e-4 off in one level; 32 rows, 32 experts, 1,024 to 2 x 2,048: 114 -> 118 us, with
+  // 16 more registers in place of LDS 128).
+  constexpr bool kFolds = sizeof(T) == 4;
+  constexpr int kFoldRounds = 512 / (kAhead * kStep);
+  const auto word = [&](int g, int i) -> float& { return words[wave][4 * (lane >> 4) + i][g * 16 + (lane & 15)]; };
+  if constexpr (kFolds) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word(g, i) = 0.0f;
+  }
+  const auto fold = [&] {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        word(g, i) = kFolds ? word(g, i) + sum[g][i] : sum[g][i];
+        sum[g][i] = 0.0f;
+      }
+    }
+  };
   const auto load = [&](const T* p, int64_t from, int64_t end, int k, bool is_there) {
     const int left = is_there ? call.k_in - k : 0;
     if constexpr (WHOLE) {
@@ -896,25 +919,26 @@ __global__ __launch_bounds__(256) void expert_few_rows_kernel(ProductCall call, 
     }
   };
   const int steps = (call.k_in + kStep - 1) / kStep;
-  for (int first = wave; first < steps; first += 4 * kAhead) {
-    u32x4 px[kAhead], pw[kAhead][kGroups];
+  const int fold_steps = kFolds ? 4 * kAhead * kFoldRounds : steps;
+  for (int from = wave; from < steps; from += fold_steps) {
+    const int upto = from + fold_steps < steps ? from + fold_steps : steps;
+    for (int first = from; first < upto; first += 4 * kAhead) {
+      u32x4 px[kAhead], pw[kAhead][kGroups];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int k = (first + 4 * i) * kStep + piece;
+      for (int i = 0; i < kAhead; ++i) {
+        const int k = (first + 4 * i) * kStep + piece;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) pw[i][g] = load(w, from_w[g], end_w, k, there[g]);
-      px[i] = load(x, from_x, end_x, k, row_there);
+        for (int g = 0; g < kGroups; ++g) pw[i][g] = load(w, from_w[g], end_w, k, there[g]);
+        px[i] = load(x, from_x, end_x, k, row_there);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) sum[g] = multiply16<T>(px[i], pw[i][g], sum[g]);
     }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) sum[g] = multiply16<T>(px[i], pw[i][g], sum[g]);
+    if constexpr (kFolds) fold();
   }
-  // register i of a lane: row 4 (lane / 16) + i, column lane mod 16
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) words[wave][4 * (lane >> 4) + i][g * 16 + (lane & 15)] = sum[g][i];
+  if constexpr (!kFolds) fold();
   __syncthreads();
   for (int at = thread; at < live_rows * kOut; at += 256) {
     const int row = at / kOut, c = at % kOut, column = first_column + c;

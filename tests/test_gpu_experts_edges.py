@@ -152,3 +152,22 @@ def test_segments_around_the_cut(k_in, n_out):
             a, b = offsets[e], offsets[e + 1]
             wanted = dy[a:b].double().t() @ x[plan.order[a:b]].double()
             assert_close_scaled(dw[e], wanted, rtol=1e-5 + _half(dtype), what=f"dweight {e} {dtype}")
+
+
+@pytest.mark.parametrize("rows", [1, 16, 24])
+@pytest.mark.parametrize("gated", [False, True])
+def test_long_sums_of_few_rows(rows, gated):
+    """65,536 inputs in float32 for a few rows: as exact as in tiles."""
+    announce("expert linear, long sums of few rows", rows, gated)
+    plan = expert_dispatch(torch.zeros(rows, 1, dtype=torch.int64, device=DEV), 1)
+    x = torch.full((rows, 65536), 0.7, device=DEV)
+    weight = (torch.arange(1, 71, device=DEV, dtype=F32) * 0.0137)[None, :, None].expand(1, 70, 65536).contiguous()
+    product = float(x[0, 0]) * weight[0, :, 0].cpu().double()
+    z = (product * 65536).expand(rows, 70)
+    # four waves' sums, each of 512 products and 32 of these in sequence
+    rtol = (512 + 32 + 4) * 2.0 ** -25 + 2.0 ** -24
+    if gated:
+        y = expert_linear(x, weight, plan, activation="silu_gate")
+        assert_close_scaled(y, z[:, :35] * torch.sigmoid(z[:, :35]) * z[:, 35:], rtol=2 * rtol + 2.0 ** -22, scale=0.0, what="y")
+    else:
+        assert_close_scaled(expert_linear(x, weight, plan), z, rtol=rtol, scale=0.0, what="y")
