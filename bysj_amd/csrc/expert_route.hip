@@ -14,8 +14,10 @@
 // with d = dw_0, so that the gradient of one expert's weight, which is about 1
 // whatever its score, is not the rounding error of a difference.
 //
-// Equal keys go to the lowest index.  A logit of -inf takes an expert out; NaN
-// ranks behind every other one, and shows in the weights.
+// Equal keys go to the lowest index.  A logit or a bias of -inf takes an expert out.
+// NaN ranks behind every other one, as does a group with a NaN among its two best
+// behind the others, and shows in the weights of a softmax's row, of a sigmoid
+// where it is chosen.
 //
 // A row is held by L lanes, C logits each.  The k best are taken one by one: the
 // largest key of a lane's C, of the row's L lanes (DPP steps inside 16 lanes), the
@@ -113,11 +115,12 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return x == -INFINITY ? 0u : key;
 }
 
-// The key of an expert with a score in 64 bits; -inf is out, NaN behind all others.
+// The key of an expert with a score in 64 bits; -inf is out.  NaN is behind all others,
+// which are above -4e38, and two of them together still in front of -inf.
 __device__ __forceinline__ double biased(float logit, double score, double bias) {
   const double key = score + bias;
-  if (logit == -INFINITY) return -INFINITY;
-  return key != key ? -1.7976931348623157e308 : key;
+  if (logit == -INFINITY || bias == -INFINITY) return -INFINITY;
+  return key != key ? -1.0e300 : key;
 }
 
 template <bool WIDE>
@@ -204,8 +207,9 @@ __global__ __launch_bounds__(kBlock) void expert_route_kernel(RouteCall call) {
       double wide = 0.0;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        score[c] = exp(static_cast<double>(logit[c]) - static_cast<double>(top));
-        wide += score[c];
+        // of the largest 1, also of an infinite one; a NaN takes its own key alone
+        score[c] = exp(logit[c] == top ? 0.0 : static_cast<double>(logit[c]) - static_cast<double>(top));
+        wide += score[c] == score[c] ? score[c] : 0.0;
       }
       inverse = over_row<L>(wide, [](double a, double b) { return a + b; });
 #pragma unroll

@@ -123,9 +123,11 @@ def expert_route(logits: torch.Tensor, k: int, *, scores: str = "softmax", bias:
     Equal keys go to the lowest index.  ``weights`` (float32 ``(tokens, k)``) are
     ``scale * score / (sum of the chosen scores + 1e-20)``, or with
     ``normalize=False`` ``scale * score``; ``experts`` (int64) is in the order of
-    the keys.  A logit of -inf takes an expert out for that token: where fewer
-    than k are left, the last entries are expert -1 with weight 0 and no place
-    in the plan.  A NaN ranks behind every other logit.
+    the keys.  A logit of -inf takes an expert out for that token (a bias of -inf
+    for all): where fewer than k are left, the last entries are expert -1 with
+    weight 0 and no place in the plan.  A NaN ranks behind every other logit, and
+    a group with one among its two best behind the others; it makes the weights of
+    its token NaN, with a sigmoid where it is chosen.
 
     Gradients of ``logits``, once; the bias has none (it only chooses).
     """

@@ -636,7 +636,8 @@ int dpa4k_residual_norm_backward(const void* grad_h, const void* grad_y,
  * Equal keys go to the lowest index, and the chosen are in the order of their
  * keys.  A logit of -inf (or a bias of -inf) takes an expert out; where fewer
  * than k are left, the last entries are expert -1 with weight 0.  A NaN ranks
- * behind every other key.  statistics float[2, T] are kept for the backward of
+ * behind every other key, and a group with one among its two best behind the
+ * others.  statistics float[2, T] are kept for the backward of
  * softmax scores (NULL: not kept).  E <= DPA4K_EXPERTS_MAX, groups <=
  * DPA4K_EXPERT_GROUPS_MAX, T k < 2^31. */
 #define DPA4K_EXPERTS_MAX 1024

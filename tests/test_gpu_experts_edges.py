@@ -171,3 +171,58 @@ def test_long_sums_of_few_rows(rows, gated):
         assert_close_scaled(y, z[:, :35] * torch.sigmoid(z[:, :35]) * z[:, 35:], rtol=2 * rtol + 2.0 ** -22, scale=0.0, what="y")
     else:
         assert_close_scaled(expert_linear(x, weight, plan), z, rtol=rtol, scale=0.0, what="y")
+
+
+# ---------------------------------------------------------------------------
+# NaN, infinities and the lowest values
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_route_nan_with_groups(scores, bias):
+    """A NaN ranks behind every other logit and in front of what is masked, in its group and among the groups."""
+    announce("expert route, NaN with groups", scores, bias)
+    nan, out = math.nan, -math.inf
+    rows = [
+        # logits of three groups of three, the experts chosen of two groups
+        ([out, out, out, nan, nan, nan, out, out, out], [3, 4, 5]),     # NaN before empty groups
+        ([out, out, out, nan, nan, nan, 1.0, 2.0, 0.5], [7, 6, 8]),     # behind a group without it
+        ([nan, 3.0, 1.0, 0.0, -1.0, -2.0, -3.0, -4.0, -5.0], [1, 2, 3]),
+        ([nan, 3.0, nan, 0.0, -1.0, -2.0, -3.0, -4.0, -5.0], [3, 4, 5]),  # its two best keys hold a NaN
+        ([nan] * 9, [0, 1, 2]),
+        ([out] * 9, [-1, -1, -1]),
+        ([out, nan, out, out, out, out, out, out, out], [1, -1, -1]),
+    ]
+    logits = torch.tensor([r for r, _ in rows], device=DEV)
+    weights, experts, plan = expert_route(logits, 3, scores=scores, groups=3, top_groups=2, bias=torch.zeros(9, device=DEV) if bias else None)
+    assert experts.tolist() == [e for _, e in rows]
+    held = torch.tensor([[e >= 0 for e in chosen] for _, chosen in rows])
+    weights = weights.cpu()
+    assert bool((weights[~held] == 0.0).all())
+    for row in (0, 4, 6):
+        assert bool(torch.isnan(weights[row][held[row]]).all())
+    if scores == "softmax":    # one NaN is in every score of its row
+        assert bool(torch.isnan(weights[:5]).all())
+    assert plan.slots.cpu().ge(0).equal(held)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_route_nan_ranks_last_with_a_bias(scores):
+    announce("expert route, NaN with a bias", scores)
+    logits = torch.tensor([[math.nan, 1.0, 3.0, 2.0], [1.0, math.nan, -50.0, math.nan], [math.nan, -math.inf, 0.0, -math.inf],
+                           [0.0, math.nan, 1.0, 2.0]], device=DEV)
+    _, experts, _ = expert_route(logits, 3, scores=scores, bias=torch.zeros(4, device=DEV))
+    assert experts.tolist() == [[2, 3, 1], [0, 2, 1], [2, 0, -1], [3, 2, 0]]
+    # a bias of -inf takes an expert out, whatever its logit
+    _, experts, _ = expert_route(logits, 4, scores=scores, bias=torch.tensor([0.0, -math.inf, 0.0, 0.0], device=DEV))
+    assert experts.tolist() == [[2, 3, 0, -1], [0, 2, 3, -1], [2, 0, -1, -1], [3, 2, 0, -1]]
+
+
+@pytest.mark.parametrize("kwargs", [{}, {"bias": torch.zeros(6)}, {"groups": 2}])
+def test_route_infinite_logits_rank_first(kwargs):
+    announce("expert route, +inf")
+    logits = torch.tensor([[0.0, 1.0, math.inf, 2.0, -1.0, 5.0], [0.0, math.inf, 1.0, -math.inf, math.nan, math.inf]], device=DEV)
+    on = {n: v.to(DEV) if isinstance(v, torch.Tensor) else v for n, v in kwargs.items()}
+    weights, experts, _ = expert_route(logits, 2, **on)
+    assert experts[:, 0].tolist() == [2, 1] and int(experts[1, 1]) == 5
+    assert bool(torch.isnan(weights).all())
