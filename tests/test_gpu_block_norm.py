@@ -232,3 +232,10 @@ def test_captured_step_replays():
         got = [t.clone() for t in outputs]
         for a, b in zip(got, step()):
             assert_bitwise(a, b)
+
+
+@pytest.mark.parametrize("dtype,stream", [(F32, F32), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("width", [1, 2, 7, 8, 9, 63, 64, 65, 90, 128, 129, 250, 256, 257, 511, 512, 513, 810, 1024])
+def test_whole_and_last_workgroups(width, dtype, stream):
+    """70 rows: workgroups with rows behind them, whose loads need no guard, and the last one, whose do."""
+    _check(*_case((70, width), dtype, stream, gate="full", activation="silu", seed=width), "workgroups")

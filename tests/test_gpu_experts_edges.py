@@ -226,3 +226,92 @@ def test_route_infinite_logits_rank_first(kwargs):
     weights, experts, _ = expert_route(logits, 2, **on)
     assert experts[:, 0].tolist() == [2, 1] and int(experts[1, 1]) == 5
     assert bool(torch.isnan(weights).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_gates_of_the_largest_size(dtype):
+    """Gates of the type's lowest and largest value, as a mask leaves them: off and on, with slopes of 0 and 1."""
+    announce("gates of the largest size", dtype)
+    most = torch.finfo(dtype).max
+    gate = torch.tensor([[-most, most, -1e4, 1e4, -200.0, 200.0, -most / 3, most / 3]], dtype=dtype, device=DEV).requires_grad_(True)
+    x = torch.full_like(gate, 2.0 ** -20)
+    for activation, value, slope in (("sigmoid", (gate > 0).double(), torch.zeros_like(gate).double()),
+                                     ("silu", torch.where(gate > 0, gate, 0.0).double(), (gate > 0).double())):
+        h, _ = residual_norm(x.detach(), torch.zeros_like(x), gate=gate, gate_activation=activation, post_norm=False, pre_norm=False)
+        (grad,) = torch.autograd.grad(h, gate, torch.ones_like(h))
+        for got, wanted in ((h, value), (grad, slope)):
+            wanted = wanted.detach().cpu() * 2.0 ** -20
+            error = (got.detach().cpu().double() - wanted).abs()
+            assert bool((error <= (1e-5 + _half(dtype)) * wanted.abs() + 1e-30 + (2.0 ** -25 if dtype == F16 else 0.0)).all()), (activation, error)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_gated_product_of_the_largest_gates(rows):
+    """z of (+-3e38, 2^-20): silu(-3e38) is 0, and so is its slope."""
+    announce("expert linear, gates of the largest size", rows)
+    plan = expert_dispatch(torch.zeros(rows, 1, dtype=torch.int64, device=DEV), 1)
+    for sign in (-1.0, 1.0):
+        x = torch.ones(rows, 1, device=DEV, requires_grad=True)
+        weight = torch.tensor([[[sign * 3e38], [2.0 ** -20]]], device=DEV, requires_grad=True)
+        y = expert_linear(x, weight, plan, activation="silu_gate")
+        (dw,) = torch.autograd.grad(y, weight, torch.full_like(y, 2.0 ** -10))
+        on = 0.0 if sign < 0 else 1.0
+        assert_close_scaled(y, torch.full((rows, 1), on * 3e38 * 2.0 ** -20, dtype=torch.float64), scale=0.0, what="y")
+        wanted = torch.tensor([[[on * 2.0 ** -30], [on * 3e38 * 2.0 ** -10]]], dtype=torch.float64) * rows
+        assert_close_scaled(dw, wanted, scale=0.0, what="dweight")
+
+
+# ---------------------------------------------------------------------------
+# runs of tiles
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,tokens,k_in,n_out,gated", [
+    (F32, 64_003, 70, 128, False),      # 3 slices forward, 4 in dx; runs of 8
+    (F32, 97_003, 100, 40, False),      # narrow columns; 4 slices forward, 2 in dx
+    (BF16, 32_803, 150, 256, False),    # two columns of tiles; 3 and 4 slices
+    (F16, 66_003, 256, 128, False),
+    (BF16, 64_003, 140, 48, True),      # 3 slices forward, 2 of each part in dx
+])
+def test_runs_of_eight_tiles(dtype, tokens, k_in, n_out, gated):
+    """Sums of up to four slices over so many rows that a workgroup takes eight tiles; an odd number of slices is padded."""
+    announce("expert linear, runs of eight", tokens, k_in, n_out, dtype, gated)
+    inner, experts = 33, 5
+    generator = torch.Generator().manual_seed(k_in)
+    chosen = torch.multinomial(torch.tensor([0.4, 0.0, 0.35, 0.01, 0.24]), tokens, replacement=True, generator=generator)[:, None]
+    chosen[torch.rand(tokens, generator=generator) < 0.02] = -1
+    plan = expert_dispatch(chosen.to(DEV), experts)
+    offsets = plan.offsets.tolist()
+    torch.manual_seed(n_out)
+    for from_tokens in (True, False):
+        x = torch.randn(tokens, inner, k_in, device=DEV).to(dtype).requires_grad_(True)
+        weight = (torch.randn(experts, n_out * (2 if gated else 1), k_in, device=DEV) * k_in ** -0.5).to(dtype).requires_grad_(True)
+        y = expert_linear(x, weight, plan, from_tokens=from_tokens, activation="silu_gate" if gated else None)
+        dy = torch.randn_like(y)
+        dx, dw = torch.autograd.grad(y, (x, weight), dy)
+        rule = 1e-5 + _half(dtype)
+        for e in range(experts):
+            a, b = offsets[e], offsets[e + 1]
+            at = plan.order[a:b] if from_tokens else slice(a, b)
+            rows, matrix = x.detach()[at].double().view(-1, k_in), weight.detach()[e].double()
+            dz = dy[a:b].double().view(-1, n_out)
+            z = rows @ matrix.t()
+            if gated:
+                gate, up = z[:, :n_out], z[:, n_out:]
+                s = torch.sigmoid(gate)
+                dz = torch.cat([dz * up * s * (1.0 + gate * (1.0 - s)), dz * gate * s], 1)
+                z = gate * s * up
+            for got, wanted, what in ((y[a:b].reshape(-1, n_out), z, "y"), (dx[at].reshape(-1, k_in), dz @ matrix, "dx"), (dw[e], dz.t() @ rows, "dweight")):
+                if wanted.numel() == 0:
+                    continue
+                # a gated dz loses 2^-18 of each of its products, at random signs as these have: 2^-18 of the root of the
+                # sum of their squares, which the largest value is past; 16 deviations
+                budget = rule * wanted.abs() + (1e-5 + (2.0 ** -14 if gated else 0.0)) * wanted.abs().max() + 2.0 ** -25
+                error = (got.detach().double() - wanted).abs()
+                assert bool((error <= budget).all()), (what, e, float((error - budget).max()))
+        held = offsets[-1]
+        assert int(y[held:].count_nonzero()) == 0
+        if from_tokens:
+            assert int(dx[(plan.slots[:, 0] < 0)].count_nonzero()) == 0
+        else:
+            assert int(dx[held:].count_nonzero()) == 0
+        del x, y, dy, dx
