@@ -318,3 +318,50 @@ def test_expert_products_oracles_against_autograd(activation, from_tokens):
     got = expert_combine_reference(y, weights, plan, dout)
     for actual, expected in zip(got, (out.detach(), *torch.autograd.grad(out, (y, weights), dout))):
         torch.testing.assert_close(actual, expected, rtol=1e-10, atol=1e-10)
+
+
+@BUILT
+def test_gated_backward_refuses_bad_sizes_before_any_device_call():
+    lib = _lib.load()
+    null, some, f32, bf16 = None, ctypes.c_void_p(256), _lib.TYPE_F32, _lib.TYPE_BF16   # never dereferenced
+
+    def gated(grad=some, before=some, x=some, weight=some, offsets=some, order=some, slots=some, dx=some, dw=some, places=4, k=2, inner=1,
+              n=3, k_in=8, n_out=8, type_=bf16, workspace=some, nbytes=1 << 30):
+        return lib.dpa4k_expert_gated_backward(grad, before, x, weight, offsets, order, slots, dx, dw, places, k, inner, n, k_in, n_out,
+                                               type_, workspace, nbytes, null)
+
+    for call, fragment in [
+        (lambda: gated(places=-2), "negative"), (lambda: gated(places=3), "k for each token"), (lambda: gated(n=0), "experts"),
+        (lambda: gated(k_in=0), "channels"), (lambda: gated(n_out=7), "even"), (lambda: gated(type_=5), "unknown type"),
+        (lambda: gated(places=2**30, inner=4), "2^31"), (lambda: gated(grad=null), "null pointer"), (lambda: gated(before=null), "null pointer"),
+        (lambda: gated(x=null), "null pointer"), (lambda: gated(weight=null), "null pointer"), (lambda: gated(offsets=null), "null pointer"),
+        (lambda: gated(slots=null), "null pointer"),
+    ]:
+        assert call() == _lib.EINVAL, fragment
+        assert fragment in lib.dpa4k_last_error().decode(), (fragment, lib.dpa4k_last_error())
+    sizes = 4, 2, 1, 3, 8, 8
+    assert gated(workspace=null) == _lib.EWORKSPACE
+    assert gated(nbytes=lib.dpa4k_expert_gated_workspace_size(*sizes, 1, 1, 1, bf16) - 1) == _lib.EWORKSPACE
+    # dz lies in front of what the products need: two parts in 16 bits, one in 32
+    rest = lib.dpa4k_expert_linear_workspace_size(*sizes, 1, 1, 1)
+    assert lib.dpa4k_expert_gated_workspace_size(*sizes, 1, 1, 1, bf16) == rest + 2 * 256
+    assert lib.dpa4k_expert_gated_workspace_size(*sizes, 1, 1, 1, f32) == rest + 256
+    assert lib.dpa4k_expert_gated_workspace_size(0, *sizes[1:], 1, 1, 1, bf16) == 0
+    assert gated(dx=null, dw=null, workspace=null) == gated(places=0, dw=null, workspace=null) == _lib.OK
+
+
+@BUILT
+def test_workspace_of_the_matrices_gradient():
+    """Partial sums for as many chunks as segments of any lengths can have, none where no segment can be cut."""
+    lib = _lib.load()
+
+    def chunks(rows, experts, k_in=256, n_out=256):
+        return lib.dpa4k_expert_linear_workspace_size(rows, 1, 1, experts, k_in, n_out, 0, 0, 1) // (4 * k_in * n_out)
+
+    assert chunks(32768, 128) == 0                 # 32,768 rows are one chunk
+    for rows, experts in ((32769, 128), (65536, 128), (65538, 128), (1_000_000, 128), (5_000_000, 128)):
+        most = 0
+        for cut in range(1, min(experts, rows // 32769) + 1):    # segments of one row more than a chunk, the last takes the rest
+            lengths = [32769] * (cut - 1) + [rows - 32769 * (cut - 1)]
+            most = max(most, sum(math.ceil(n / 32768) for n in lengths))
+        assert most <= chunks(rows, experts) <= 2 * rows // 32768, (rows, most)
