@@ -1144,7 +1144,7 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void combine_backward_kernel(
     const int64_t place = live_token ? places[token * k + j] : -1;
     const bool held = static_cast<uint64_t>(place) < static_cast<uint64_t>(limit);
     const float w = held ? weights[token * k + j] : 0.0f;
-    float dot = 0.0f;
+    double lane_dot = 0.0;   // of pieces' sums in 32 bits; all in 32: 1e-4 off over 4M equal elements
     if (held) {
       for (int64_t piece = lane; piece < pieces; piece += L) {
         const int64_t first = piece * V;
@@ -1152,8 +1152,10 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void combine_backward_kernel(
         const Pack<T, V> grad = load_pack<T, V>(dout + token * size + first, live, (tokens - token) * size - first);
         if (dw != nullptr) {
           const Pack<T, V> row = load_pack<T, V>(y + place * size + first, live, (limit - place) * size - first);
+          float of_piece = 0.0f;
 #pragma unroll
-          for (int i = 0; i < V; ++i) dot = fmaf(static_cast<float>(grad[i]), static_cast<float>(row[i]), dot);
+          for (int i = 0; i < V; ++i) of_piece = fmaf(static_cast<float>(grad[i]), static_cast<float>(row[i]), of_piece);
+          lane_dot += static_cast<double>(of_piece);
         }
         if (dy != nullptr) {
           float part[V];
@@ -1164,7 +1166,7 @@ __global__ __launch_bounds__((L > 256 ? L : 256)) void combine_backward_kernel(
       }
     }
     if (dw == nullptr) continue;
-    dot = group_sum<(L < 64 ? L : 64)>(dot);
+    float dot = group_sum<(L < 64 ? L : 64)>(static_cast<float>(lane_dot));
     if constexpr (L > 64) {
       if ((threadIdx.x & 63) == 0) words[threadIdx.x / 64] = dot;
       __syncthreads();

@@ -11,9 +11,9 @@ import pytest
 import torch
 
 from bysj_amd.kernels.block_norm import residual_norm
-from bysj_amd.kernels.experts import ExpertPlan, expert_dispatch, expert_linear, expert_route
-from oracle.experts import expert_dispatch_reference, expert_linear_reference, expert_route_reference
-from parity import announce, assert_bitwise, assert_close_scaled
+from bysj_amd.kernels.experts import ExpertPlan, expert_combine, expert_dispatch, expert_linear, expert_route
+from oracle.experts import expert_dispatch_reference, expert_linear_reference
+from parity import announce, assert_close_scaled
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -315,3 +315,37 @@ def test_runs_of_eight_tiles(dtype, tokens, k_in, n_out, gated):
         else:
             assert int(dx[held:].count_nonzero()) == 0
         del x, y, dy, dx
+
+
+# ---------------------------------------------------------------------------
+# the weighted sum
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [40_000, 1_000_003, 4_194_304])
+def test_long_sums_of_weights_gradients(dtype, size):
+    """The gradient of a weight, a dot product of entries of up to 4M equal elements, at the rule of float32."""
+    announce("expert combine, long sums", size, dtype)
+    plan = expert_dispatch(torch.tensor([[0], [1], [0]], device=DEV), 2)
+    y = torch.full((3, size), 0.7, device=DEV, dtype=dtype)
+    weights = torch.ones(3, 1, device=DEV, requires_grad=True)
+    out = expert_combine(y, weights, plan)
+    dout = torch.full_like(out, 0.3)
+    (grad,) = torch.autograd.grad(out, weights, dout)
+    wanted = torch.full((3, 1), size * float(y[0, 0]) * float(dout[0, 0]), dtype=torch.float64)
+    assert_close_scaled(grad, wanted, scale=0.0, what="dweights")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("tokens,inner", [(0, ()), (4, (0,))])
+def test_gated_products_of_nothing(tokens, inner, dtype):
+    """No tokens, and entries without rows: empty results, matrices' gradients of 0."""
+    announce("expert linear, gated, empty", tokens, inner, dtype)
+    plan = expert_dispatch(torch.zeros(tokens, 2, dtype=torch.int64, device=DEV), 3)
+    for from_tokens in (True, False):
+        x = torch.zeros(tokens if from_tokens else 2 * tokens, *inner, 5, device=DEV, dtype=dtype, requires_grad=True)
+        weight = torch.ones(3, 14, 5, device=DEV, dtype=dtype, requires_grad=True)
+        y = expert_linear(x, weight, plan, from_tokens=from_tokens, activation="silu_gate")
+        assert y.shape == (2 * tokens, *inner, 7)
+        dx, dw = torch.autograd.grad(y, (x, weight), torch.zeros_like(y))
+        assert dx.shape == x.shape and dw.shape == weight.shape and int(dw.count_nonzero()) == 0
