@@ -13,7 +13,7 @@ import torch
 from bysj_amd.kernels.block_norm import residual_norm
 from bysj_amd.kernels.experts import ExpertPlan, expert_combine, expert_dispatch, expert_linear, expert_route
 from oracle.experts import expert_dispatch_reference, expert_linear_reference
-from parity import announce, assert_close_scaled
+from parity import announce, assert_bitwise, assert_close_scaled
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -349,3 +349,70 @@ def test_gated_products_of_nothing(tokens, inner, dtype):
         assert y.shape == (2 * tokens, *inner, 7)
         dx, dw = torch.autograd.grad(y, (x, weight), torch.zeros_like(y))
         assert dx.shape == x.shape and dw.shape == weight.shape and int(dw.count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("tokens,k_in,n_out", [(60, 40, 24), (900, 256, 264)])
+def test_gated_gradients_keep_to_their_places(tokens, k_in, n_out, dtype):
+    """NaN and infinities of rows of no place reach no gradient, and one gradient alone is that of both."""
+    announce("expert linear, gated, NaN, single gradients", tokens, k_in, n_out, dtype)
+    generator = torch.Generator().manual_seed(tokens)
+    chosen = torch.randint(0, 3, (tokens, 2), generator=generator)
+    chosen[torch.rand(tokens, generator=generator) < 0.3] = -1
+    plan = expert_dispatch(chosen.to(DEV), 3)
+    held, out = int(plan.offsets[-1]), (chosen < 0).all(1)
+    weight = (torch.randn(3, 2 * n_out, k_in, generator=generator) * k_in ** -0.5).to(dtype).to(DEV)
+    dy = torch.randn(2 * tokens, n_out, generator=generator).to(dtype)
+    dirty_dy = dy.clone()
+    dirty_dy[held:] = math.inf
+    for from_tokens in (True, False):
+        x = torch.randn(tokens if from_tokens else 2 * tokens, k_in, generator=generator).to(dtype)
+        dirty = x.clone()
+        dirty[out if from_tokens else slice(held, None)] = math.nan
+        results = []
+        for rows, seed, wanted in ((x, dy, (True, True)), (dirty, dirty_dy, (True, True)), (x, dy, (True, False)), (x, dy, (False, True))):
+            leaves = [t.clone().requires_grad_(w) for t, w in zip((rows.to(DEV), weight), wanted)]
+            y = expert_linear(*leaves, plan, from_tokens=from_tokens, activation="silu_gate")
+            grads = torch.autograd.grad(y, [t for t, w in zip(leaves, wanted) if w], seed.to(DEV))
+            results.append((y.detach(), *grads))
+        for a, b in zip(results[0], results[1]):
+            assert_bitwise(a, b)
+        assert_bitwise(results[0][1], results[2][1])
+        assert_bitwise(results[0][2], results[3][1])
+
+
+def test_gated_gradients_past_32_bits():
+    """A dz whose parts are of 4.9 GB each: rows on both sides of 2^31 and 2^32 bytes, and sums over all."""
+    tokens, k_in, n_out = 600_003, 16, 2048
+    announce("expert linear, gated, dz of twice 4.9 GB", tokens, k_in, n_out)
+    torch.manual_seed(0)
+    x = torch.randn(tokens, k_in, device=DEV).to(BF16).requires_grad_(True)
+    weight = (torch.randn(2, 2 * n_out, k_in, device=DEV) * k_in ** -0.5).to(BF16).requires_grad_(True)
+    plan = expert_dispatch((torch.arange(tokens, device=DEV) % 2)[:, None].contiguous(), 2)
+    y = expert_linear(x, weight, plan, activation="silu_gate")
+    dy = torch.randn_like(y)
+    dx, dw = torch.autograd.grad(y, (x, weight), dy)
+
+    def dz_of(rows, matrix, grad):
+        z = rows @ matrix.t()
+        gate, up = z[:, :n_out], z[:, n_out:]
+        s = torch.sigmoid(gate)
+        return torch.cat([grad * up * s * (1.0 + gate * (1.0 - s)), grad * gate * s], 1)
+
+    rule = 1e-5 + _half(BF16)
+    for e in range(2):
+        matrix, begin, end = weight.detach()[e].double(), int(plan.offsets[e]), int(plan.offsets[e + 1])
+        wanted = torch.zeros(2 * n_out, k_in, dtype=torch.float64, device=DEV)
+        for first in range(begin, end, 50_000):
+            places = slice(first, min(first + 50_000, end))
+            at = plan.order[places]
+            rows = x.detach()[at].double()
+            dz = dz_of(rows, matrix, dy[places].double())
+            wanted += dz.t() @ rows
+            want_x = dz @ matrix
+            # 2^-18 of each product, at most 2^-18 of their magnitudes
+            budget = rule * want_x.abs() + 1e-5 * want_x.abs().max() + 2.0 ** -18 * (dz.abs() @ matrix.abs())
+            assert bool(((dx[at].double() - want_x).abs() <= budget).all()), f"dx of places from {first}"
+        error = (dw[e].double() - wanted).abs()
+        # roundings of 2^-18 at random signs over 300,000 products of random sign: 16 deviations
+        assert bool((error <= rule * wanted.abs() + (1e-5 + 2.0 ** -14) * wanted.abs().max()).all()), float(error.max())
