@@ -24,7 +24,7 @@
 //
 // Measured: 32,768 slots through 32 matrices of 1,024 to 2 x 2,048 in bfloat16 (8,192
 // tokens, four slots each), forward with the gate 399 us (690 TFLOP/s), dW 393 (700),
-// dx 347 (790), with the gate's dz in two parts 694 and 667 (the operations twice),
+// dx 347 (790), with the gate's dz in two parts 684 and 654 (the operations twice),
 // where a library's one product of that size reaches 1,090 to 1,300:
 // one workgroup fits a CU with its 256 by 256 tile, so nothing multiplies while it
 // starts and stores, and unequal segments leave a last round half filled.  786,432

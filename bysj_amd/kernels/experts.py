@@ -226,9 +226,11 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, fr
     ``weight``: ``(E, outputs, inputs)`` of its dtype, one matrix for each of
     the plan's experts.  ``activation="silu_gate"``: the first half of the outputs
     is a gate, ``silu(gate) * rest``, and the result has half of them.  At most
-    65,536 inputs and outputs, whose sums are kept in float32.  Places behind ``plan.offsets[-1]`` give 0 and take no
-    part in a gradient.  Gradients of ``x`` (summed in float32 over a
-    token's slots) and ``weight``, once.
+    65,536 inputs and outputs, whose sums are kept in float32.  Places behind
+    ``plan.offsets[-1]`` give 0 and take no part in a gradient.  Gradients of ``x``
+    (summed in float32 over a token's slots) and ``weight``, once; the gradient in
+    front of the gate is held in float32 or two 16-bit parts (in float16 up to
+    1.3e8), so that they are rounded once.
     """
     tokens, k = _check_plan(plan)
     _floats(x, "expert linear input")

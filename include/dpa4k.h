@@ -604,8 +604,9 @@ int dpa4k_residual_norm_forward(const void* x, const void* residual,
 
 /* Gradients of every input from grad_h (like h) and grad_y (like y); one of them
  * may be NULL, and so may any output.  The gradients of the scales are float[C],
- * summed over all rows in a fixed order, in 64 bits past 256 rows a workgroup;
- * they alone need the workspace. */
+ * summed over all rows in a fixed order, in 32 bits over at most 256 rows of the
+ * lanes that share one and over those of a workgroup, then in 64; they alone need
+ * the workspace. */
 size_t dpa4k_residual_norm_workspace_size(int64_t rows, int64_t channels);
 int dpa4k_residual_norm_backward(const void* grad_h, const void* grad_y,
                                  const void* x, const void* residual,
